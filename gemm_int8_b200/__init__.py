@@ -41,6 +41,14 @@ _libdef.define("quantize_token(Tensor a) -> (Tensor, Tensor)")
 _libdef.define("hadamard_quantize_token_block(Tensor a, int block) -> (Tensor, Tensor)")
 _libdef.define("int8_linear(Tensor x, Tensor weight_q, Tensor weight_scale, Tensor? bias, bool blockwise, int? hadamard) -> Tensor")
 
+_libdef.define("route_experts(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int groups, int top_groups, bool group_top2, bool renormalize, "
+               "float scale) -> (Tensor, Tensor)")
+_libdef.define("group_by_expert(Tensor experts, int num_experts, int first_expert) -> (Tensor, Tensor, Tensor)")
+_libdef.define("int8_matmul_experts(Tensor x, Tensor weight_q, Tensor x_scale, Tensor weight_scale, Tensor offsets, Tensor? slots, int top_k, bool swiglu) -> Tensor")
+_libdef.define("combine_experts(Tensor y, Tensor weights, Tensor places, Tensor? add) -> Tensor")
+_libdef.define("int8_experts(Tensor x, Tensor logits, Tensor? bias, Tensor gate_up_q, Tensor gate_up_scale, Tensor down_q, Tensor down_scale, int top_k, "
+               "bool sigmoid, int groups, int top_groups, bool group_top2, bool renormalize, float scale, int first_expert, Tensor? add) -> Tensor")
+
 
 def _stream_ptr(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
@@ -278,7 +286,9 @@ if _os.environ.get("GEMM_INT8_KERNEL"):
 
 
 from .linear import Int8Linear  # noqa: E402
+from .experts import Int8Experts, combine_experts, group_by_expert, matmul_experts, matmul_experts_swiglu, route_experts  # noqa: E402
 
 __all__ = ["matmul", "matmul_i32", "matmul_scaled", "matmul_blockwise", "matmul_blockwise_f32", "sum_parts_bf16",
            "quantize_per_token_block",
-           "quantize_per_token", "Int8Linear", "force_variant", "pick_variant", "device_status", "check_device", "reload_env"]
+           "quantize_per_token", "Int8Linear", "route_experts", "group_by_expert", "matmul_experts", "matmul_experts_swiglu", "combine_experts", "Int8Experts",
+           "force_variant", "pick_variant", "device_status", "check_device", "reload_env"]

@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -1584,3 +1585,5 @@ int gi8_peer_release(void* ptr)
 }
 
 }  // extern "C"
+
+#include "experts/host.cuh"

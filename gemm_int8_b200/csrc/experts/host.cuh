@@ -1,0 +1,283 @@
+// C ABI of the experts' operators: argument checks, the choice of a tile, launches.  Included at the end of api.cu, whose helpers it
+// uses.
+#pragma once
+
+#include "k_combine.cuh"
+#include "k_experts_gemm.cuh"
+#include "k_group.cuh"
+#include "k_route.cuh"
+
+namespace {
+
+// Kernels whose shared-memory limit has been raised, a bit each (DeviceState::attr_set is full).
+std::atomic<uint64_t> g_experts_attr[kMaxDevices];
+
+template <typename Kernel>
+int experts_smem(int slot, Kernel kernel, size_t bytes)
+{
+    int dev = 0;
+    GI8_CUDA(cudaGetDevice(&dev));
+    if (!((g_experts_attr[dev].load() >> slot) & 1)) {
+        GI8_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+        g_experts_attr[dev].fetch_or(uint64_t(1) << slot);
+    }
+    return GI8_OK;
+}
+
+template <typename T, int V>
+int launch_route(const RouteParams& p, cudaStream_t s)
+{
+    // Groups that are not whole runs of a power of two of lanes have their values looked up through shared memory.
+    int use_scratch = 0;
+    if (p.groups > 1) {
+        const int size = p.E / p.groups, span = size / V;
+        use_scratch = size % V != 0 || (span & (span - 1)) != 0;
+    }
+    const size_t smem = use_scratch ? static_cast<size_t>(kRouteWarps) * p.E * sizeof(double) : 0;
+    return launch(route_experts_kernel<T, V>, dim3((p.T + kRouteWarps - 1) / kRouteWarps), kRouteWarps * 32, smem, s, dim3(1), knobs().pdl, p, use_scratch);
+}
+
+template <typename T>
+int launch_route_for(RouteParams p, cudaStream_t s)
+{
+    const int per_lane = (p.E + 31) / 32;
+    auto vec = [&](int v) { return p.E % v == 0 && reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && (v * static_cast<int>(sizeof(T))) % 16 == 0; };
+#define GI8_ROUTE(V_)                                   \
+    if (per_lane <= V_) {                               \
+        p.vec = vec(V_);                                \
+        return launch_route<T, V_>(p, s);               \
+    }
+    GI8_ROUTE(1)
+    GI8_ROUTE(2)
+    GI8_ROUTE(4)
+    GI8_ROUTE(5)
+    GI8_ROUTE(8)
+    GI8_ROUTE(16)
+    GI8_ROUTE(32)
+#undef GI8_ROUTE
+    return fail(GI8_ERR_UNSUPPORTED_SHAPE, "too many experts");
+}
+
+template <int BT, int STAGES, bool SWIGLU>
+int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, const ExpertsParams& p, cudaStream_t s)
+{
+    constexpr size_t smem = static_cast<size_t>(STAGES) * (kBM + BT) * kBK + 1024;
+    auto kernel = experts_gemm_kernel<BT, STAGES, SWIGLU>;
+    if (int rc = experts_smem(slot, kernel, smem)) return rc;
+    CUtensorMap mw, mx;
+    const int64_t rows_w = static_cast<int64_t>(p.E) * p.N * (SWIGLU ? 2 : 1);
+    if (int rc = make_operand_map(&mw, w, rows_w, p.K, SWIGLU ? 16 : kBM)) return rc;
+    if (int rc = make_operand_map(&mx, x, p.tokens, p.K, p.slots ? 1 : 32)) return rc;
+    const int channels = SWIGLU ? kBM / 2 : kBM;
+    const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
+    const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
+    const int grid = static_cast<int>(std::min<int64_t>(tiles, st->sm_count));
+    return launch(kernel, dim3(grid), kExpertsThreads, smem, s, dim3(1), knobs().pdl, mw, mx, p);
+}
+
+template <bool SWIGLU>
+int dispatch_experts(DeviceState* st, const int8_t* x, const int8_t* w, const ExpertsParams& p, cudaStream_t s)
+{
+    const int64_t most = p.slots ? p.tokens : p.rows;                     // rows of one expert, if no token names it twice
+    const int64_t want = std::min(most, (3 * p.rows / 2 + p.E - 1) / p.E);  // half as many again as there are on average
+    constexpr int slot = SWIGLU ? 4 : 0;
+    if (want <= 32) return launch_experts<32, 10, SWIGLU>(st, slot, x, w, p, s);
+    if (want <= 64) return launch_experts<64, 8, SWIGLU>(st, slot + 1, x, w, p, s);
+    if (want <= 128) return launch_experts<128, 6, SWIGLU>(st, slot + 2, x, w, p, s);
+    return launch_experts<256, 4, SWIGLU>(st, slot + 3, x, w, p, s);
+}
+
+bool misaligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+}  // namespace
+
+extern "C" {
+
+int gi8_route_experts(const void* logits, int logits_dtype, const float* bias, float* weights, int32_t* experts, int64_t T, int64_t E,
+                      int64_t top_k, int sigmoid, int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale,
+                      void* stream)
+{
+    if (T < 0 || T > INT32_MAX) return fail(GI8_ERR_INVALID_ARGUMENT, "T=%lld must be in [0, 2^31)", (long long)T);
+    if (logits_dtype != 0 && logits_dtype != 1) return fail(GI8_ERR_INVALID_ARGUMENT, "logits_dtype must be 0 (fp32) or 1 (bf16)");
+    if (E < 1 || E > kRouteMaxExperts) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts: 1 to %d are supported", (long long)E, kRouteMaxExperts);
+    if (top_k < 1 || top_k > kRouteMaxTopK || top_k > E)
+        return fail(GI8_ERR_UNSUPPORTED_SHAPE, "top_k=%lld must be in [1, min(%d, experts)]", (long long)top_k, kRouteMaxTopK);
+    if (groups < 1 || groups > kRouteMaxGroups || E % groups)
+        return fail(GI8_ERR_UNSUPPORTED_SHAPE, "groups=%lld must divide the %lld experts and be at most %d", (long long)groups, (long long)E, kRouteMaxGroups);
+    if (top_groups < 1 || top_groups > groups || top_k > top_groups * (E / groups))
+        return fail(GI8_ERR_UNSUPPORTED_SHAPE, "top_groups=%lld must be in [1, groups] and hold top_k experts", (long long)top_groups);
+    if (T == 0) return GI8_OK;
+    if (!logits || !weights || !experts) return fail(GI8_ERR_INVALID_ARGUMENT, "null pointer");
+    if (misaligned(logits, logits_dtype == 0 ? 4 : 2) || misaligned(bias, 4) || misaligned(weights, 4) || misaligned(experts, 4))
+        return fail(GI8_ERR_MISALIGNED, "a pointer is not aligned to its elements");
+    DeviceState* st;
+    if (int rc = get_device_state(&st)) return rc;
+    RouteParams p{};
+    p.logits = logits, p.bias = bias, p.weights = weights, p.experts = experts;
+    p.T = (int)T, p.E = (int)E, p.top_k = (int)top_k, p.sigmoid = sigmoid != 0;
+    p.groups = top_groups == groups ? 1 : (int)groups, p.top_groups = (int)top_groups;  // where all groups are kept there are none
+    p.group_top2 = group_top2 != 0, p.renormalize = renormalize != 0, p.scale = scale;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return logits_dtype == 0 ? launch_route_for<float>(p, s) : launch_route_for<__nv_bfloat16>(p, s);
+}
+
+int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t first, int32_t* offsets, int32_t* slots, int32_t* places, void* stream)
+{
+    if (S < 0 || S > (int64_t(1) << 28)) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "S=%lld must be in [0, 2^28]", (long long)S);
+    if (E < 1 || E > kGroupMaxExperts) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts: 1 to %d are supported", (long long)E, kGroupMaxExperts);
+    if (first < 0 || first > INT32_MAX - E) return fail(GI8_ERR_INVALID_ARGUMENT, "first expert %lld out of range", (long long)first);
+    if (!offsets || (S > 0 && (!experts || !slots || !places))) return fail(GI8_ERR_INVALID_ARGUMENT, "null pointer");
+    if (misaligned(experts, 4) || misaligned(offsets, 4) || misaligned(slots, 4) || misaligned(places, 4))
+        return fail(GI8_ERR_MISALIGNED, "a pointer is not 4-byte aligned");
+    DeviceState* st;
+    if (int rc = get_device_state(&st)) return rc;
+    GroupParams p{};
+    p.experts = experts, p.offsets = offsets, p.slots = slots, p.places = places;
+    p.S = (int)S, p.E = (int)E, p.first = (int)first;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (S <= 2048) {
+        constexpr int W = 8;
+        p.per_warp = (int)((S + W * 32 - 1) / (W * 32)) * 32;
+        const size_t smem = static_cast<size_t>(W + 1) * E * 4;
+        return launch(group_by_expert_kernel<W>, dim3(1), W * 32, smem, s, dim3(1), knobs().pdl, p, 1);
+    }
+    constexpr int W = 32;
+    const int ctas = S <= 4096 ? 2 : S <= 8192 ? 4 : 8;
+    p.per_warp = (int)((S + ctas * W * 32 - 1) / (ctas * W * 32)) * 32;
+    const size_t smem = static_cast<size_t>(W + 1) * E * 4;
+    if (int rc = experts_smem(8, group_by_expert_kernel<W>, static_cast<size_t>(W + 1) * kGroupMaxExperts * 4)) return rc;
+    return launch(group_by_expert_kernel<W>, dim3(ctas), W * 32, smem, s, dim3(ctas), knobs().pdl, p, ctas);
+}
+
+int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
+                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* stream)
+{
+    if (E < 1 || E > kExpertsMaxExperts) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts: 1 to %d are supported", (long long)E, kExpertsMaxExperts);
+    if (rows < 0 || tokens < 0 || N < 0) return fail(GI8_ERR_INVALID_ARGUMENT, "negative dimension");
+    if (top_k < 1 || top_k > INT32_MAX) return fail(GI8_ERR_INVALID_ARGUMENT, "top_k=%lld must be positive", (long long)top_k);
+    if (!slots && tokens < rows) return fail(GI8_ERR_INVALID_ARGUMENT, "%lld rows of x for %lld rows of the result", (long long)tokens, (long long)rows);
+    if (tokens > INT32_MAX - 256 || rows > INT32_MAX - 256) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "rows must be below 2^31 - 256");
+    if (N > (int64_t(1) << 30) || E * N * (swiglu ? 2 : 1) > INT32_MAX - 256)
+        return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts of %lld channels: together below 2^31 - 256", (long long)E, (long long)N);
+    if (int rc = check_common(x, w, out, rows, N, K, 2)) return rc;
+    if (rows == 0 || N == 0) return GI8_OK;
+    DeviceState* st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (K == 0 || tokens == 0) {
+        if (int rc = get_device_state(&st)) return rc;
+        return zero_output(out, rows * N * 2, s);
+    }
+    if (int rc = check_scale_pointers(sx, sw)) return rc;
+    if (!offsets) return fail(GI8_ERR_INVALID_ARGUMENT, "null offsets");
+    if (misaligned(offsets, 4) || misaligned(slots, 4)) return fail(GI8_ERR_MISALIGNED, "offsets and slots must be 4-byte aligned");
+    if (int rc = get_device_state(&st)) return rc;
+    ExpertsParams p{};
+    p.out = static_cast<uint16_t*>(out), p.sx = sx, p.sw = sw, p.offsets = offsets, p.slots = slots, p.status = st->status;
+    p.rows = rows, p.tokens = (int)tokens, p.E = (int)E, p.N = (int)N, p.K = (int)K, p.top_k = (int)top_k;
+    p.vec_zero = !misaligned(out, 16) && N % 8 == 0;
+    p.weight_policy_first = rows <= 32 * E;
+    return swiglu ? dispatch_experts<true>(st, x, w, p, s) : dispatch_experts<false>(st, x, w, p, s);
+}
+
+int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
+                        int64_t rows, int64_t N, void* stream)
+{
+    if (T < 0 || T > INT32_MAX || rows < 0 || rows > INT32_MAX || N < 0 || N > INT32_MAX - 4096) return fail(GI8_ERR_INVALID_ARGUMENT, "a dimension is out of range");
+    if (top_k < 1 || top_k > kCombineMaxTopK) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "top_k=%lld must be in [1, %d]", (long long)top_k, kCombineMaxTopK);
+    if (T == 0 || N == 0) return GI8_OK;
+    if ((!y && rows > 0) || !weights || !places || !out) return fail(GI8_ERR_INVALID_ARGUMENT, "null pointer");
+    if (misaligned(y, 2) || misaligned(add, 2) || misaligned(out, 2) || misaligned(weights, 4) || misaligned(places, 4))
+        return fail(GI8_ERR_MISALIGNED, "a pointer is not aligned to its elements");
+    DeviceState* st;
+    if (int rc = get_device_state(&st)) return rc;
+    CombineParams p{};
+    p.y = static_cast<const uint16_t*>(y), p.weights = weights, p.places = places, p.add = static_cast<const uint16_t*>(add), p.out = static_cast<uint16_t*>(out);
+    p.rows = rows, p.T = (int)T, p.N = (int)N, p.top_k = (int)top_k;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool vec = N % 8 == 0 && !misaligned(y, 16) && !misaligned(add, 16) && !misaligned(out, 16);
+    const int64_t per_block = kCombineThreads * (vec ? 8 : 1);
+    const int64_t blocks_y = (N + per_block - 1) / per_block;
+    if (blocks_y > 65535) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "N=%lld is too large", (long long)N);
+    const dim3 grid((unsigned)T, (unsigned)blocks_y);
+    if (vec) return launch(combine_experts_kernel<8>, grid, kCombineThreads, 0, s, dim3(1), knobs().pdl, p);
+    return launch(combine_experts_kernel<1>, grid, kCombineThreads, 0, s, dim3(1), knobs().pdl, p);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------
+// The whole layer.  Its intermediates lie one behind the other in the caller's scratch.
+// ---------------------------------------------------------------------------------------------------
+namespace {
+
+struct ExpertsScratch {
+    int64_t weights, experts, offsets, slots, places, x_q, x_scale, h, h_q, h_scale, y, bytes;
+};
+
+ExpertsScratch experts_scratch(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k)
+{
+    ExpertsScratch s{};
+    const int64_t S = T * top_k;
+    auto take = [&](int64_t bytes) {
+        const int64_t at = s.bytes;
+        s.bytes += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    s.weights = take(4 * S), s.experts = take(4 * S), s.offsets = take(4 * (E + 1)), s.slots = take(4 * S), s.places = take(4 * S);
+    s.x_q = take(T * H), s.x_scale = take(4 * T);
+    s.h = take(2 * S * I), s.h_q = take(S * I), s.h_scale = take(4 * S);
+    s.y = take(2 * S * H);
+    return s;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t gi8_experts_scratch_bytes(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k)
+{
+    if (T < 0 || H < 0 || I < 0 || E < 0 || top_k < 0 || top_k > kRouteMaxTopK || T > INT32_MAX || H > INT32_MAX || I > INT32_MAX || E > INT32_MAX) return 0;
+    return experts_scratch(T, H, I, E, top_k).bytes;
+}
+
+int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,
+                const float* gate_up_scale, const int8_t* down, const float* down_scale, const void* add, void* out, void* scratch,
+                int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
+                int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream)
+{
+    // What any step refuses is refused before the first launch: an empty batch goes through the checks of the router, and the limits of
+    // the others are looked at here.
+    if (int rc = gi8_route_experts(logits, logits_dtype, bias, nullptr, nullptr, 0, E_router, top_k, sigmoid, groups, top_groups, group_top2, renormalize,
+                                   scale, stream))
+        return rc;
+    if (T < 0 || T > INT32_MAX || T * top_k > (int64_t(1) << 28)) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "T=%lld with top_k=%lld is out of range", (long long)T, (long long)top_k);
+    if (E < 1 || first < 0 || first + E > E_router)
+        return fail(GI8_ERR_INVALID_ARGUMENT, "experts %lld .. %lld of a router over %lld", (long long)first, (long long)(first + E - 1), (long long)E_router);
+    if (H < 1 || I < 1 || H % 16 || I % 16) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "hidden size %lld and inner size %lld must be positive multiples of 16", (long long)H, (long long)I);
+    if (H >= kMaxK || I >= kMaxK) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "hidden and inner size must be below %lld", (long long)kMaxK);
+    if (E * 2 * I > INT32_MAX - 256 || E * H > INT32_MAX - 256) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "experts times channels must be below 2^31 - 256");
+    if (x_dtype != 0 && x_dtype != 1) return fail(GI8_ERR_INVALID_ARGUMENT, "x_dtype must be 0 (fp32) or 1 (bf16)");
+    if (T == 0) return GI8_OK;
+    if (!x || !logits || !gate_up || !gate_up_scale || !down || !down_scale || !out || !scratch) return fail(GI8_ERR_INVALID_ARGUMENT, "null pointer");
+    if (misaligned(x, 16) || misaligned(gate_up, 16) || misaligned(down, 16) || misaligned(scratch, 256) || misaligned(gate_up_scale, 4) || misaligned(down_scale, 4) ||
+        misaligned(logits, logits_dtype == 0 ? 4 : 2) || misaligned(bias, 4) || misaligned(add, 2) || misaligned(out, 2))
+        return fail(GI8_ERR_MISALIGNED, "x and weights must be 16-byte aligned, scratch 256-byte aligned, the rest to its elements");
+    const ExpertsScratch m = experts_scratch(T, H, I, E, top_k);
+    if (scratch_bytes < m.bytes) return fail(GI8_ERR_WORKSPACE, "the layer needs %lld bytes of scratch, got %lld", (long long)m.bytes, (long long)scratch_bytes);
+    uint8_t* b = static_cast<uint8_t*>(scratch);
+    auto f32 = [&](int64_t at) { return reinterpret_cast<float*>(b + at); };
+    auto i32 = [&](int64_t at) { return reinterpret_cast<int32_t*>(b + at); };
+    auto i8 = [&](int64_t at) { return reinterpret_cast<int8_t*>(b + at); };
+    const int64_t S = T * top_k;
+    if (int rc = gi8_route_experts(logits, logits_dtype, bias, f32(m.weights), i32(m.experts), T, E_router, top_k, sigmoid, groups, top_groups, group_top2, renormalize,
+                                   scale, stream))
+        return rc;
+    if (int rc = gi8_group_by_expert(i32(m.experts), S, E, first, i32(m.offsets), i32(m.slots), i32(m.places), stream)) return rc;
+    if (int rc = gi8_quantize_token(x, x_dtype, i8(m.x_q), f32(m.x_scale), T, H, stream)) return rc;
+    if (int rc = gi8_matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, stream)) return rc;
+    if (int rc = gi8_quantize_token(b + m.h, 1, i8(m.h_q), f32(m.h_scale), S, I, stream)) return rc;
+    if (int rc = gi8_matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, stream)) return rc;
+    return gi8_combine_experts(b + m.y, f32(m.weights), i32(m.places), add, out, T, top_k, S, H, stream);
+}
+
+}  // extern "C"

@@ -164,6 +164,16 @@ GI8_DEVICE void tma_load_2d_hint(void* smem_dst, const CUtensorMap* map, uint64_
         : "memory");
 }
 
+// Four rows of a matrix, wherever they lie, into 4 x 128 consecutive bytes of shared memory (swizzled as a tile at that address would
+// be).  The tensor map's box is one row high; c0 as above.
+GI8_DEVICE void tma_gather4(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t r0, int32_t r1, int32_t r2, int32_t r3)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
+        : "memory");
+}
+
 // shared -> global tile store (bulk async-group completion).  Never issued at a negative coordinate.
 GI8_DEVICE void tma_store_2d(const CUtensorMap* map, const void* smem_src, int32_t c0, int32_t c1)
 {
@@ -193,6 +203,13 @@ GI8_DEVICE uint64_t l2_policy_evict_first()
 {
     uint64_t p;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+
+GI8_DEVICE uint64_t l2_policy_evict_normal()
+{
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
     return p;
 }
 

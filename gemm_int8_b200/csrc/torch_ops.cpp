@@ -232,6 +232,150 @@ at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tenso
     return out;
 }
 
+// ------------------------------------------------------------------------------------------------ experts
+void check_vector(const char* name, const char* what, const at::Tensor& t, at::ScalarType dtype, at::IntArrayRef shape, const at::Device& device)
+{
+    TORCH_CHECK(t.device() == device, name, ": ", what, " must be on ", device, ", got ", t.device());
+    TORCH_CHECK(t.scalar_type() == dtype, name, ": ", what, " must be ", dtype, ", got ", t.scalar_type());
+    TORCH_CHECK(t.sizes() == shape, name, ": ", what, " must have shape ", shape, ", got ", t.sizes());
+}
+
+int float_type(const char* name, const char* what, const at::Tensor& t)
+{
+    TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16, name, ": ", what, " must be float32 or bfloat16, got ", t.scalar_type());
+    return t.scalar_type() == at::kFloat ? 0 : 1;
+}
+
+// Contiguous, with a base that vectors of `bytes` can be read from.
+at::Tensor aligned(const at::Tensor& t, uintptr_t bytes = 16)
+{
+    const at::Tensor c = t.contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % bytes ? c.clone() : c;
+}
+
+std::tuple<at::Tensor, at::Tensor> route_experts(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t top_k, bool sigmoid, int64_t groups,
+                                                 int64_t top_groups, bool group_top2, bool renormalize, double scale)
+{
+    const char* name = "route_experts";
+    TORCH_CHECK(logits.is_cuda(), name, ": logits must be a CUDA tensor");
+    TORCH_CHECK(logits.dim() == 2, name, ": logits must be 2-D [tokens, experts]");
+    const int dtype = float_type(name, "logits", logits);
+    TORCH_CHECK(top_k >= 1 && top_k <= logits.size(1), name, ": top_k=", top_k, " of ", logits.size(1), " experts");
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const at::Tensor l = logits.contiguous();
+    at::Tensor b;
+    if (bias.has_value()) {
+        check_vector(name, "bias", *bias, at::kFloat, {l.size(1)}, l.device());
+        b = bias->contiguous();
+    }
+    at::Tensor weights = new_tensor({l.size(0), top_k}, at::kFloat, l), experts = new_tensor({l.size(0), top_k}, at::kInt, l);
+    check(gi8_route_experts(l.data_ptr(), dtype, b.defined() ? f32(b) : nullptr, static_cast<float*>(weights.data_ptr()), static_cast<int32_t*>(experts.data_ptr()),
+                            l.size(0), l.size(1), top_k, sigmoid, groups, top_groups, group_top2, renormalize, static_cast<float>(scale), stream_of(l)));
+    return {weights, experts};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> group_by_expert(const at::Tensor& experts, int64_t num_experts, int64_t first_expert)
+{
+    const char* name = "group_by_expert";
+    TORCH_CHECK(experts.is_cuda() && experts.scalar_type() == at::kInt && experts.dim() == 2, name, ": experts must be a 2-D int32 CUDA tensor [tokens, top_k]");
+    TORCH_CHECK(num_experts >= 1, name, ": num_experts=", num_experts);
+    const c10::cuda::CUDAGuard guard(experts.device());
+    const at::Tensor e = experts.contiguous();
+    at::Tensor offsets = new_tensor({num_experts + 1}, at::kInt, e), slots = new_tensor({e.numel()}, at::kInt, e), places = new_tensor(e.sizes(), at::kInt, e);
+    check(gi8_group_by_expert(static_cast<const int32_t*>(e.data_ptr()), e.numel(), num_experts, first_expert, static_cast<int32_t*>(offsets.data_ptr()),
+                              static_cast<int32_t*>(slots.data_ptr()), static_cast<int32_t*>(places.data_ptr()), stream_of(e)));
+    return {offsets, slots, places};
+}
+
+at::Tensor int8_matmul_experts(const at::Tensor& x, const at::Tensor& w, const at::Tensor& x_scale, const at::Tensor& w_scale, const at::Tensor& offsets,
+                               const std::optional<at::Tensor>& slots, int64_t top_k, bool swiglu)
+{
+    const char* name = "int8_matmul_experts";
+    TORCH_CHECK(x.is_cuda(), name, ": x must be a CUDA tensor");
+    TORCH_CHECK(w.device() == x.device(), name, ": the weight must be on ", x.device(), ", got ", w.device());
+    TORCH_CHECK(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, name, ": x and the weight must be int8");
+    TORCH_CHECK(x.dim() == 2 && w.dim() == 3, name, ": x must be 2-D [rows, K] and the weight 3-D [experts, N, K]");
+    TORCH_CHECK(x.size(1) == w.size(2), name, ": x has ", x.size(1), " features, the weight ", w.size(2));
+    TORCH_CHECK(x.is_contiguous() && w.is_contiguous(), name, ": x and the weight must be contiguous");
+    TORCH_CHECK(!swiglu || w.size(1) % 2 == 0, name, ": gate and up rows must be the two halves of the weight, got ", w.size(1), " rows");
+    TORCH_CHECK(top_k >= 1, name, ": top_k=", top_k);
+    const int64_t E = w.size(0), N = swiglu ? w.size(1) / 2 : w.size(1), K = x.size(1);
+    const at::Tensor sx = row_scale(name, "x_scale", x_scale, x.size(0), x.device());
+    check_scale(name, "w_scale", w_scale, {E, w.size(1)}, x.device());
+    check_vector(name, "offsets", offsets, at::kInt, {E + 1}, x.device());
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor sw = w_scale.contiguous(), off = offsets.contiguous();
+    at::Tensor sl;
+    int64_t rows = x.size(0);
+    if (slots.has_value()) {
+        check_vector(name, "slots", *slots, at::kInt, {slots->numel()}, x.device());
+        sl = slots->contiguous();
+        rows = sl.numel();
+    }
+    at::Tensor out = new_tensor({rows, N}, at::kBFloat16, x);
+    // (an empty list of pairs has no data, and is not the absence of one)
+    if (rows == 0) return out;
+    check(gi8_matmul_experts(i8(x), i8(w), f32(sx), f32(sw), static_cast<const int32_t*>(off.data_ptr()),
+                             sl.defined() ? static_cast<const int32_t*>(sl.data_ptr()) : nullptr, top_k, out.data_ptr(), rows, x.size(0), E, N, K, swiglu, stream_of(x)));
+    return out;
+}
+
+at::Tensor combine_experts(const at::Tensor& y, const at::Tensor& weights, const at::Tensor& places, const std::optional<at::Tensor>& add)
+{
+    const char* name = "combine_experts";
+    TORCH_CHECK(y.is_cuda() && y.scalar_type() == at::kBFloat16 && y.dim() == 2, name, ": y must be a 2-D bfloat16 CUDA tensor [rows, N]");
+    TORCH_CHECK(weights.dim() == 2, name, ": weights must be 2-D [tokens, top_k]");
+    check_vector(name, "weights", weights, at::kFloat, weights.sizes(), y.device());
+    check_vector(name, "places", places, at::kInt, weights.sizes(), y.device());
+    const int64_t T = weights.size(0), N = y.size(1);
+    const c10::cuda::CUDAGuard guard(y.device());
+    const at::Tensor yc = y.contiguous(), wc = weights.contiguous(), pc = places.contiguous();
+    at::Tensor ac;
+    if (add.has_value()) {
+        check_vector(name, "add", *add, at::kBFloat16, {T, N}, y.device());
+        ac = add->contiguous();
+    }
+    at::Tensor out = new_tensor({T, N}, at::kBFloat16, y);
+    check(gi8_combine_experts(yc.data_ptr(), f32(wc), static_cast<const int32_t*>(pc.data_ptr()), ac.defined() ? ac.data_ptr() : nullptr, out.data_ptr(), T,
+                              weights.size(1), yc.size(0), N, stream_of(y)));
+    return out;
+}
+
+at::Tensor int8_experts(const at::Tensor& x, const at::Tensor& logits, const std::optional<at::Tensor>& bias, const at::Tensor& gate_up,
+                        const at::Tensor& gate_up_scale, const at::Tensor& down, const at::Tensor& down_scale, int64_t top_k, bool sigmoid, int64_t groups,
+                        int64_t top_groups, bool group_top2, bool renormalize, double scale, int64_t first_expert, const std::optional<at::Tensor>& add)
+{
+    const char* name = "int8_experts";
+    check_activations(name, x);
+    TORCH_CHECK(logits.device() == x.device() && logits.dim() == 2 && logits.size(0) == x.size(0), name, ": logits must have shape [", x.size(0), ", experts] on ", x.device());
+    const int logits_dtype = float_type(name, "logits", logits);
+    TORCH_CHECK(gate_up.device() == x.device() && gate_up.scalar_type() == at::kChar && gate_up.dim() == 3 && gate_up.is_contiguous() && gate_up.size(1) % 2 == 0 &&
+                    gate_up.size(2) == x.size(1),
+                name, ": gate_up must be a contiguous int8 tensor [experts, 2 inner, ", x.size(1), "] on ", x.device());
+    const int64_t T = x.size(0), H = x.size(1), I = gate_up.size(1) / 2, E = gate_up.size(0);
+    check_vector(name, "down", down, at::kChar, {E, H, I}, x.device());
+    TORCH_CHECK(down.is_contiguous(), name, ": down must be contiguous");
+    check_scale(name, "gate_up_scale", gate_up_scale, {E, 2 * I}, x.device());
+    check_scale(name, "down_scale", down_scale, {E, H}, x.device());
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = aligned(x), lc = logits.contiguous(), gs = gate_up_scale.contiguous(), ds = down_scale.contiguous();
+    at::Tensor b, ac;
+    if (bias.has_value()) {
+        check_vector(name, "bias", *bias, at::kFloat, {logits.size(1)}, x.device());
+        b = bias->contiguous();
+    }
+    if (add.has_value()) {
+        check_vector(name, "add", *add, at::kBFloat16, {T, H}, x.device());
+        ac = add->contiguous();
+    }
+    at::Tensor out = new_tensor({T, H}, at::kBFloat16, x);
+    at::Tensor scratch = new_tensor({gi8_experts_scratch_bytes(T, H, I, E, top_k)}, at::kByte, x);
+    check(gi8_experts(xc.data_ptr(), xc.scalar_type() == at::kFloat ? 0 : 1, lc.data_ptr(), logits_dtype, b.defined() ? f32(b) : nullptr, i8(gate_up), f32(gs), i8(down), f32(ds),
+                      ac.defined() ? ac.data_ptr() : nullptr, out.data_ptr(), scratch.data_ptr(), scratch.numel(), T, H, I, logits.size(1), E, first_expert, top_k,
+                      sigmoid, groups, top_groups, group_top2, renormalize, static_cast<float>(scale), stream_of(x)));
+    return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(gemm_int8_CUDA, CUDA, m)
@@ -245,4 +389,9 @@ TORCH_LIBRARY_IMPL(gemm_int8_CUDA, CUDA, m)
     m.impl("quantize_token", &quantize_token);
     m.impl("hadamard_quantize_token_block", &hadamard_quantize_token_block);
     m.impl("int8_linear", &int8_linear);
+    m.impl("route_experts", &route_experts);
+    m.impl("group_by_expert", &group_by_expert);
+    m.impl("int8_matmul_experts", &int8_matmul_experts);
+    m.impl("combine_experts", &combine_experts);
+    m.impl("int8_experts", &int8_experts);
 }

@@ -212,6 +212,69 @@ int gi8_linear(const void* x, int x_dtype, const int8_t* w, const float* w_scale
                int64_t had_block, int8_t* xq, float* xs, void* out_bf16, int64_t M, int64_t N, int64_t K, void* stream);
 
 /*
+ * The operators of a mixture-of-experts layer (no reference counterpart).  All of them read what the one in front left on the device:
+ * nothing is read back by the host, and a captured graph of them replays with other tokens.
+ *
+ * gi8_route_experts: the top_k experts of T tokens out of E, logits [T,E] fp32 (logits_dtype 0) or bf16 (1), row-major, contiguous.
+ *   score  s = softmax(logits) or, with sigmoid, 1 / (1 + exp(-logits));  choice c = s + bias (fp32 [E]), without a bias the logits
+ *   themselves, of which s is an increasing function
+ *   groups  the experts form `groups` runs of E / groups; a group's value is its largest choice or, with group_top2, the sum of its
+ *           two largest (without a bias, of the scores); only the best top_groups groups keep their experts
+ *   chosen  the top_k largest choices in descending order, the lower index first among equals.  Decided as in exact arithmetic: where fp32
+ *           cannot tell two choices apart the token is decided in fp64.  A choice of -inf or NaN is never chosen; where fewer than top_k
+ *           are left, the places hold expert -1 and weight 0
+ *   weights [T,top_k] fp32 = s of the chosen (renormalize: / their sum) * scale;  experts [T,top_k] int32
+ *   E <= 1024, top_k <= 32, groups <= 32.
+ */
+int gi8_route_experts(const void* logits, int logits_dtype, const float* bias, float* weights, int32_t* experts, int64_t T, int64_t E,
+                      int64_t top_k, int sigmoid, int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale,
+                      void* stream);
+
+/*
+ * The S = T * top_k (token, choice) pairs of a routed batch in the order of their experts, of which this caller holds first .. first + E - 1:
+ *   offsets int32 [E+1]  rows [offsets[e], offsets[e+1]) belong to expert first + e
+ *   slots   int32 [S]    the pair (token * top_k + choice) of each row, ascending within an expert; -1 behind offsets[E]
+ *   places  int32 [S]    the row of each pair; -1 where its expert is not held here
+ * E <= 1024, S <= 2^28.
+ */
+int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t first, int32_t* offsets, int32_t* slots, int32_t* places, void* stream);
+
+/*
+ * out[p,n] = bf16( fp32(sum_k x[src(p),k] * w[e,n,k]) * (sx[src(p)] * sw[e,n]) ) for offsets[e] <= p < offsets[e+1]: gi8_matmul_scaled with a
+ * weight of its own for every group of rows.  Rows [offsets[E], rows) are set to zero.
+ *   x    int8 [tokens,K];  src(p) = p, or with slots the token slots[p] / top_k
+ *   w    int8 [E,N,K], sw fp32 [E,N];  with swiglu [E,2N,K] and [E,2N] (N gate rows, then N up rows), and
+ *        out[p,n] = bf16( g / (1 + exp(-g)) * u ) of the two fp32 products g and u
+ *   out  bf16 [rows,N], any alignment of its rows
+ * offsets must ascend within [0, rows] and slots hold pairs of `tokens` tokens; others give wrong rows, never an access out of bounds.
+ * K % 16 == 0, x and w 16-byte aligned, E <= 1024.
+ */
+int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
+                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* stream);
+
+/*
+ * out[t,n] = bf16( add[t,n] + sum_j weights[t,j] * y[places[t,j],n] ), one fp32 fused multiply-add per choice in ascending j; places below
+ * zero (or at or above `rows`) are left out, add (bf16 [T,N]) may be NULL.  y bf16 [rows,N], out bf16 [T,N]; top_k <= 32.
+ */
+int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
+                        int64_t rows, int64_t N, void* stream);
+
+/*
+ * The whole layer: route, group, quantise the tokens per row, gate and up product with SwiGLU, quantise its rows, down product, weighted sum
+ * (onto add [T,H] bf16, or NULL) into out bf16 [T,H]; the results of these steps, one after the other, bit for bit.
+ *   x        [T,H] fp32 (x_dtype 0) or bf16 (1), 16-byte aligned;  logits [T,E_router]
+ *   gate_up  int8 [E,2I,H], gate_up_scale fp32 [E,2I];  down int8 [E,H,I], down_scale fp32 [E,H]: experts first .. first + E - 1 of the router's,
+ *            the sum runs over those of a token's choices that are among them
+ *   scratch  gi8_experts_scratch_bytes(T, H, I, E, top_k) bytes, 256-byte aligned, of any contents.  Two calls that may overlap need two.
+ * H and I are multiples of 16; T * top_k <= 2^28.  Whatever a step refuses is refused before the first launch.
+ */
+int64_t gi8_experts_scratch_bytes(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k);
+int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,
+                const float* gate_up_scale, const int8_t* down, const float* down_scale, const void* add, void* out, void* scratch,
+                int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
+                int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream);
+
+/*
  * Forces a kernel variant for the calling process (tuning and tests); NULL or "" restores the fitted
  * per-shape dispatch that replaces the reference's shape table (csrc/kernels/gemm.cu:136-161).
  * Names: "dense_bn256", "dense_bn128", "dense_bn64" (tile width of the dense and of the blockwise kernel), "smallm"
