@@ -4,6 +4,7 @@
 
 #include "k_combine.cuh"
 #include "k_experts_gemm.cuh"
+#include "k_gather.cuh"
 #include "k_group.cuh"
 #include "k_route.cuh"
 
@@ -58,33 +59,65 @@ int launch_route_for(RouteParams p, cudaStream_t s)
     return fail(GI8_ERR_UNSUPPORTED_SHAPE, "too many experts");
 }
 
-template <int BT, int STAGES, bool SWIGLU>
-int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, const ExpertsParams& p, cudaStream_t s)
+// Gate and up rows of int8 weights [E, 2, N, K] in alternating runs of 16 (N a multiple of 16): dimensions K, row of a run, half, run, expert.
+// A box of 128 bytes x 16 x 2 x 4 x 1 is the weight tile of 64 channels.  Encoded for each launch (a layer's two are a microsecond).
+int make_gate_up_map(CUtensorMap* map, const int8_t* w, int64_t E, int64_t N, int64_t K)
 {
-    constexpr size_t smem = static_cast<size_t>(STAGES) * (kBM + BT) * kBK + 1024;
-    auto kernel = experts_gemm_kernel<BT, STAGES, SWIGLU>;
-    if (int rc = experts_smem(slot, kernel, smem)) return rc;
-    CUtensorMap mw, mx;
-    const int64_t rows_w = static_cast<int64_t>(p.E) * p.N * (SWIGLU ? 2 : 1);
-    if (int rc = make_operand_map(&mw, w, rows_w, p.K, SWIGLU ? 16 : kBM)) return rc;
-    if (int rc = make_operand_map(&mx, x, p.tokens, p.K, p.slots ? 1 : 32)) return rc;
-    const int channels = SWIGLU ? kBM / 2 : kBM;
-    const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
-    const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
-    const int grid = static_cast<int>(std::min<int64_t>(tiles, st->sm_count));
-    return launch(kernel, dim3(grid), kExpertsThreads, smem, s, dim3(1), knobs().pdl, mw, mx, p);
+    cuuint64_t dims[5] = {(cuuint64_t)K, 16, 2, (cuuint64_t)(N / 16), (cuuint64_t)E};
+    cuuint64_t strides[4] = {(cuuint64_t)K, (cuuint64_t)(N * K), (cuuint64_t)(16 * K), (cuuint64_t)(2 * N * K)};
+    cuuint32_t box[5] = {kBK, 16, 2, 4, 1};
+    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<int8_t*>(w), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(GI8_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
+    return GI8_OK;
 }
 
-template <bool SWIGLU>
-int dispatch_experts(DeviceState* st, const int8_t* x, const int8_t* w, const ExpertsParams& p, cudaStream_t s)
+template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
+int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, ExpertsParams p, cudaStream_t s)
 {
-    const int64_t most = p.slots ? p.tokens : p.rows;                     // rows of one expert, if no token names it twice
-    const int64_t want = std::min(most, (3 * p.rows / 2 + p.E - 1) / p.E);  // half as many again as there are on average
+    constexpr int kRowsX = PAIR ? BT / 2 : BT;
+    constexpr size_t smem = static_cast<size_t>(STAGES) * (kBM + kRowsX) * kBK + 1024;
+    auto kernel = experts_gemm_kernel<BT, STAGES, SWIGLU, PAIR>;
+    if (int rc = experts_smem(slot, kernel, smem)) return rc;
+    CUtensorMap mw;
+    TokenMaps mx;
+    const int64_t rows_w = static_cast<int64_t>(p.E) * p.N * (SWIGLU ? 2 : 1);
+    p.interleave = SWIGLU && p.N % 16 == 0;
+    if (p.interleave) {
+        if (int rc = make_gate_up_map(&mw, w, p.E, p.N, p.K)) return rc;
+    } else if (int rc = make_operand_map(&mw, w, rows_w, p.K, SWIGLU ? 16 : kBM)) {
+        return rc;
+    }
+    for (int i = 0; i < 4; ++i)
+        if (int rc = make_operand_map(&mx.m[i], x, p.rows_x, p.K, p.slots && !p.in_order ? 1 : (i + 1) * kRowsX / 4)) return rc;
+    const int channels = (SWIGLU ? kBM / 2 : kBM) * (PAIR ? 2 : 1);
+    const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
+    const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
+    const int grid = static_cast<int>(std::min<int64_t>(tiles, st->sm_count / (PAIR ? 2 : 1))) * (PAIR ? 2 : 1);
+    return launch(kernel, dim3(grid), kExpertsThreads, smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
+}
+
+// Rows of a token tile.
+int experts_tile(int64_t rows, int64_t tokens, int64_t E, bool gathered)
+{
+    const int64_t most = gathered ? tokens : rows;                  // rows of one expert, if no token names it twice
+    const int64_t want = std::min(most, (3 * rows / 2 + E - 1) / E);  // half as many again as there are on average
+    return want <= 64 ? 64 : want <= 128 ? 128 : 256;
+}
+
+// Gathered rows are put in order by a pass of their own in front of the product, except those of small tiles.
+bool experts_gather_first(int64_t rows, int64_t tokens, int64_t E) { return experts_tile(rows, tokens, E, true) > 64; }
+
+template <bool SWIGLU>
+int dispatch_experts(DeviceState* st, const int8_t* x, const int8_t* w, const ExpertsParams& p, bool gathered, cudaStream_t s)
+{
     constexpr int slot = SWIGLU ? 4 : 0;
-    if (want <= 32) return launch_experts<32, 10, SWIGLU>(st, slot, x, w, p, s);
-    if (want <= 64) return launch_experts<64, 8, SWIGLU>(st, slot + 1, x, w, p, s);
-    if (want <= 128) return launch_experts<128, 6, SWIGLU>(st, slot + 2, x, w, p, s);
-    return launch_experts<256, 4, SWIGLU>(st, slot + 3, x, w, p, s);
+    switch (experts_tile(p.rows, p.tokens, p.E, gathered)) {
+        case 64: return launch_experts<64, 8, SWIGLU>(st, slot + 1, x, w, p, s);
+        case 128: return launch_experts<128, 6, SWIGLU>(st, slot + 2, x, w, p, s);
+        default: return launch_experts<256, 6, SWIGLU, true>(st, slot + 3, x, w, p, s);
+    }
 }
 
 bool misaligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
@@ -149,8 +182,15 @@ int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t fi
     return launch(group_by_expert_kernel<W>, dim3(ctas), W * 32, smem, s, dim3(ctas), knobs().pdl, p, ctas);
 }
 
+int64_t gi8_matmul_experts_workspace_bytes(int64_t rows, int64_t tokens, int64_t E, int64_t K)
+{
+    if (rows <= 0 || tokens <= 0 || E <= 0 || K <= 0 || rows > INT32_MAX || K > kMaxK) return 0;
+    return experts_gather_first(rows, tokens, E) ? rows * K : 0;
+}
+
 int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
-                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* stream)
+                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* workspace,
+                       int64_t workspace_bytes, void* stream)
 {
     if (E < 1 || E > kExpertsMaxExperts) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts: 1 to %d are supported", (long long)E, kExpertsMaxExperts);
     if (rows < 0 || tokens < 0 || N < 0) return fail(GI8_ERR_INVALID_ARGUMENT, "negative dimension");
@@ -170,13 +210,26 @@ int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const 
     if (int rc = check_scale_pointers(sx, sw)) return rc;
     if (!offsets) return fail(GI8_ERR_INVALID_ARGUMENT, "null offsets");
     if (misaligned(offsets, 4) || misaligned(slots, 4)) return fail(GI8_ERR_MISALIGNED, "offsets and slots must be 4-byte aligned");
+    const int64_t needed = slots ? gi8_matmul_experts_workspace_bytes(rows, tokens, E, K) : 0;
+    if (needed > 0 && (!workspace || workspace_bytes < needed))
+        return fail(GI8_ERR_WORKSPACE, "the gathered product of this shape needs %lld bytes of workspace, got %lld", (long long)needed, (long long)workspace_bytes);
+    if (needed > 0 && misaligned(workspace, 16)) return fail(GI8_ERR_MISALIGNED, "workspace must be 16-byte aligned");
     if (int rc = get_device_state(&st)) return rc;
     ExpertsParams p{};
     p.out = static_cast<uint16_t*>(out), p.sx = sx, p.sw = sw, p.offsets = offsets, p.slots = slots, p.status = st->status;
     p.rows = rows, p.tokens = (int)tokens, p.E = (int)E, p.N = (int)N, p.K = (int)K, p.top_k = (int)top_k;
     p.vec_zero = !misaligned(out, 16) && N % 8 == 0;
     p.weight_policy_first = rows <= 32 * E;
-    return swiglu ? dispatch_experts<true>(st, x, w, p, s) : dispatch_experts<false>(st, x, w, p, s);
+    const bool gathered = slots != nullptr;
+    if (gathered && experts_gather_first(rows, tokens, E)) {
+        if (int rc = launch(gather_rows_kernel, dim3((unsigned)std::min<int64_t>((rows + 7) / 8, st->sm_count * 8)), kGatherThreads, 0, s, dim3(1), knobs().pdl,
+                            reinterpret_cast<const uint4*>(x), slots, offsets + E, static_cast<uint4*>(workspace), rows, (int)tokens, (int)top_k, (int)(K / 16)))
+            return rc;
+        x = static_cast<const int8_t*>(workspace);
+        p.in_order = 1;
+    }
+    p.rows_x = (int)(p.in_order ? rows : tokens);
+    return swiglu ? dispatch_experts<true>(st, x, w, p, gathered, s) : dispatch_experts<false>(st, x, w, p, gathered, s);
 }
 
 int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
@@ -211,7 +264,7 @@ int gi8_combine_experts(const void* y, const float* weights, const int32_t* plac
 namespace {
 
 struct ExpertsScratch {
-    int64_t weights, experts, offsets, slots, places, x_q, x_scale, h, h_q, h_scale, y, bytes;
+    int64_t weights, experts, offsets, slots, places, x_q, x_scale, rows, h, h_q, h_scale, y, bytes;
 };
 
 ExpertsScratch experts_scratch(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k)
@@ -225,6 +278,7 @@ ExpertsScratch experts_scratch(int64_t T, int64_t H, int64_t I, int64_t E, int64
     };
     s.weights = take(4 * S), s.experts = take(4 * S), s.offsets = take(4 * (E + 1)), s.slots = take(4 * S), s.places = take(4 * S);
     s.x_q = take(T * H), s.x_scale = take(4 * T);
+    s.rows = take(gi8_matmul_experts_workspace_bytes(S, T, E, H));
     s.h = take(2 * S * I), s.h_q = take(S * I), s.h_scale = take(4 * S);
     s.y = take(2 * S * H);
     return s;
@@ -274,9 +328,9 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
         return rc;
     if (int rc = gi8_group_by_expert(i32(m.experts), S, E, first, i32(m.offsets), i32(m.slots), i32(m.places), stream)) return rc;
     if (int rc = gi8_quantize_token(x, x_dtype, i8(m.x_q), f32(m.x_scale), T, H, stream)) return rc;
-    if (int rc = gi8_matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, stream)) return rc;
+    if (int rc = gi8_matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, b + m.rows, m.h - m.rows, stream)) return rc;
     if (int rc = gi8_quantize_token(b + m.h, 1, i8(m.h_q), f32(m.h_scale), S, I, stream)) return rc;
-    if (int rc = gi8_matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, stream)) return rc;
+    if (int rc = gi8_matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, nullptr, 0, stream)) return rc;
     return gi8_combine_experts(b + m.y, f32(m.weights), i32(m.places), add, out, T, top_k, S, H, stream);
 }
 

@@ -10,8 +10,8 @@
 // is what makes ragged groups and single tokens cheap.  An expert's rows are cut into equal tiles of at most BT.
 //
 // Structure (one persistent CTA per SM, 192 threads), as in the dense kernel:
-//   warp 0      TMA producer: weight tiles (128 rows x 128 bytes) and token rows, the latter in boxes of 32 rows or, gathered, four
-//               rows per instruction wherever they lie; all lanes issue
+//   warp 0      TMA producer: weight tiles (128 rows x 128 bytes) and token rows, either with one instruction; gathered rows four
+//               per instruction wherever they lie
 //   warp 1      MMA issuer, kind::i8, two accumulators in tensor memory
 //   warps 2..5  epilogue: a lane holds one output channel and walks over the tile's tokens
 // SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes
@@ -33,19 +33,30 @@ struct ExpertsParams {
     const int32_t* slots;    // [rows], or null: row p reads x[p]
     uint32_t* status;
     int64_t rows;            // S
-    int tokens;              // rows of x
+    int tokens;              // what slots name
+    int rows_x;              // (host) rows of x
+    int in_order;            // x has been gathered: rows of x are those of out, scales go by slots
     int E, N, K;             // N: columns of out; Nw = N or 2 N rows of weight per expert
     int top_k;
     int vec_zero;            // rows behind the last group can be cleared in 16-byte pieces
+    int interleave;          // SWIGLU: the weight's map is over runs of 16 rows and loads a whole tile (N a multiple of 16)
     int weight_policy_first; // weights are met once or twice: keep them from displacing the rest of L2
 };
 
-// g / (1 + exp(-g)), by the exponential that does not overflow: far below zero the result fades out through the subnormals.
+// g / (1 + exp(-g)), by the exponential that does not overflow: far below zero the result fades out through the subnormals.  The quotient
+// is within two units in the last place (the divisor lies in [1, 2]); the correctly rounded one branches, and its sixteen per lane and
+// 32 tokens then run one after the other.
 GI8_DEVICE float silu(float g)
 {
     const float t = expf(-fabsf(g));
-    return g * ((g < 0.0f ? t : 1.0f) / (1.0f + t));
+    return g * __fdividef(g < 0.0f ? t : 1.0f, 1.0f + t);
 }
+
+// Tensor maps of the token rows, with boxes of a quarter, half, three quarters and all of a token tile: a tile's rows are loaded by one
+// instruction whatever their number.  Gathered rows use the first, whose box is one row.
+struct TokenMaps {
+    CUtensorMap m[4];
+};
 
 // One tile of the list.
 struct ExpertTile {
@@ -88,7 +99,7 @@ GI8_DEVICE void build_expert_list(ExpertList<BT>& list, const int32_t* offsets, 
 
 // Tile `item` of the list, if there is one: experts in order, within an expert weight tile by weight tile with the token tiles inside,
 // so that CTAs that run at the same time share weights.  Whole warp; `chunk` is the 32 experts where the last search ended.
-template <int BT>
+template <int BT, int ALIGN>
 GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_tiles, int64_t item, int& chunk, ExpertTile& t)
 {
     const int lane = threadIdx.x & 31;
@@ -103,7 +114,7 @@ GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_t
             const int r = static_cast<int>(item - static_cast<int64_t>(before) * weight_tiles);
             t.weight_tile = r / tiles;
             const int n = list.start[t.expert + 1] - list.start[t.expert];
-            const int per = ((n + tiles - 1) / tiles + 15) & ~15;  // <= BT, and the last tile keeps at least a row
+            const int per = ((n + tiles - 1) / tiles + ALIGN - 1) & ~(ALIGN - 1);  // <= BT, and the last tile keeps at least a row
             const int first = (r - t.weight_tile * tiles) * per;
             t.row0 = list.start[t.expert] + first;
             t.rows = min(per, n - first);
@@ -113,13 +124,29 @@ GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_t
     return false;
 }
 
-template <int BT, int STAGES, bool SWIGLU>
-__global__ void __launch_bounds__(kExpertsThreads, 1)
-experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const ExpertsParams p)
+// Tile loads whose bytes are counted on the barrier at cluster address `bar` (the leader's) or on one of this CTA.
+template <bool PAIR>
+GI8_DEVICE void load_tile_2d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t c0, int32_t c1, uint64_t policy)
 {
-    static_assert(BT == 32 || BT == 64 || BT == 128 || BT == 256, "token rows come in boxes of 32, at most 256 columns of an MMA");
+    if constexpr (PAIR) tma_load_2d_pair_hint(dst, map, bar, c0, c1, policy);
+    else tma_load_2d_hint_addr(dst, map, bar, c0, c1, policy);
+}
+template <bool PAIR>
+GI8_DEVICE void load_tile_5d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t c0, int32_t c1, int32_t c2, int32_t c3, int32_t c4, uint64_t policy)
+{
+    if constexpr (PAIR) tma_load_5d_pair_hint(dst, map, bar, c0, c1, c2, c3, c4, policy);
+    else tma_load_5d_hint(dst, map, bar, c0, c1, c2, c3, c4, policy);
+}
+
+template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
+__global__ void __launch_bounds__(kExpertsThreads, 1)
+experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const ExpertsParams p)
+{
+    static_assert(BT == 64 || BT == 128 || BT == 256, "quarters of a tile are columns of an MMA, of which there are at most 256");
     constexpr uint32_t kBytesW = kBM * kBK;
-    constexpr uint32_t kStageBytes = kBytesW + BT * kBK;
+    constexpr int kRowsX = PAIR ? BT / 2 : BT;  // token rows that this CTA loads
+    constexpr int kAlign = PAIR ? 32 : 16;      // what the columns of an MMA are a multiple of
+    constexpr uint32_t kStageBytes = kBytesW + kRowsX * kBK;
     constexpr uint32_t kTmemCols = 2 * BT;
     constexpr int kChannels = SWIGLU ? kBM / 2 : kBM;  // output channels of a weight tile
 
@@ -133,12 +160,17 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile uint32_t abort_flag;
     __shared__ __align__(16) float token_scale[2][BT];
+    __shared__ __align__(16) int32_t gather_rows[BT];
     __shared__ ExpertList<BT> list;
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int num_kb = (p.K + kBK - 1) / kBK;
-    const int weight_tiles = (p.N + kChannels - 1) / kChannels;
+    // PAIR: the two CTAs of a cluster take neighbouring weight tiles of one pair of them; the pair is the scheduling unit.
+    const int weight_tiles = (p.N + kChannels * (PAIR ? 2 : 1) - 1) / (kChannels * (PAIR ? 2 : 1));
+    const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
+    const int64_t first_item = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+    const int64_t item_step = PAIR ? gridDim.x >> 1 : gridDim.x;
     const int rows_w = SWIGLU ? 2 * p.N : p.N;  // of one expert
 
     if (threadIdx.x == 0) {
@@ -149,18 +181,25 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bar_acc_full[b], 1);
-            mbar_init(&bar_acc_empty[b], 4);
+            mbar_init(&bar_acc_empty[b], PAIR ? 8 : 4);
         }
         fence_barrier_init();
         prefetch_tensormap(&map_w);
-        prefetch_tensormap(&map_x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) prefetch_tensormap(&map_x.m[i]);
     }
     if (warp == 1) {
-        tmem_alloc(&tmem_base_slot, kTmemCols);
-        tmem_relinquish_alloc_permit();
+        if constexpr (PAIR) {
+            tmem_alloc_pair(&tmem_base_slot, kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(&tmem_base_slot, kTmemCols);
+            tmem_relinquish_alloc_permit();
+        }
     }
     tcgen05_fence_before_sync();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers exist before anything signals them remotely
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = tmem_base_slot;
     pdl_wait();
@@ -174,24 +213,22 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         bool ok = true;
         int chunk = 0;
         ExpertTile t;
-        const uint64_t pol_w = p.weight_policy_first ? l2_policy_evict_first() : l2_policy_evict_normal();
-        for (int64_t item = blockIdx.x; ok && find_expert_tile(list, p.E, weight_tiles, item, chunk, t); item += gridDim.x) {
-            const int cols = (t.rows + 15) & ~15;
-            // This lane's part of the token rows: four consecutive places of the tile per gather, 32 per box.
-            constexpr int kGathers = (BT + 127) / 128;
-            int32_t src[kGathers][4];
-            if (p.slots) {
-#pragma unroll
-                for (int g = 0; g < kGathers; ++g)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int r = (g * 32 + lane) * 4 + i;  // rows that pad the tile read token 0, and are not stored
-                        const int slot = r < t.rows ? __ldg(p.slots + t.row0 + r) : 0;
-                        src[g][i] = min(max(slot, 0) / p.top_k, p.tokens - 1);
-                    }
+        const uint64_t pol_x = l2_policy_evict_normal();
+        const uint64_t pol_w = p.weight_policy_first ? l2_policy_evict_first() : pol_x;
+        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, chunk, t); item += item_step) {
+            const int cols = ((t.rows + kAlign - 1) & ~(kAlign - 1)) / (PAIR ? 2 : 1);  // of this CTA
+            if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank), t.row0 += static_cast<int>(rank) * cols;
+            if (!PAIR && p.slots && !p.in_order) {
+                __syncwarp();
+                for (int r = lane; r < cols; r += 32) {  // rows that pad the tile read token 0, and are not stored
+                    const int slot = r < t.rows ? __ldg(p.slots + t.row0 + r) : 0;
+                    gather_rows[r] = min(max(slot, 0) / p.top_k, p.tokens - 1);
+                }
+                __syncwarp();
             }
-            const uint32_t bytes = kBytesW + (p.slots ? cols : (cols + 31) & ~31) * kBK;
-            const int w_row = t.expert * rows_w + t.weight_tile * kChannels;
+            const int box = (cols - 1) / (kRowsX / 4);  // the smallest one that holds the tile
+            const uint32_t bytes = kBytesW + (!PAIR && p.slots && !p.in_order ? cols : (box + 1) * (kRowsX / 4)) * kBK;
+            const int w_row = t.weight_tile * kChannels;
             for (int kb = 0; kb < num_kb; ++kb) {
                 if (!warp_agrees(wait_or_abort(&bar_empty[s], ph ^ 1, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_PRODUCER)) {
                     ok = false;
@@ -200,42 +237,49 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 uint8_t* sw_tile = smem + s * kStageBytes;
                 uint8_t* sx_tile = sw_tile + kBytesW;
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(&bar_full[s], bytes);
-                    if constexpr (!SWIGLU) tma_load_2d_hint(sw_tile, &map_w, &bar_full[s], kb * kBK, w_row, pol_w);
-                }
-                __syncwarp();
-                if constexpr (SWIGLU) {
-                    // runs of 16 rows: gate, up, gate, up, ...
-                    if (lane < 8) tma_load_2d_hint(sw_tile + lane * 16 * kBK, &map_w, &bar_full[s], kb * kBK, w_row + (lane >> 1) * 16 + (lane & 1) * p.N, pol_w);
-                }
-                if (p.slots) {
+                    // PAIR: the leader arms its barrier for the bytes of both CTAs, the peer only sends bytes
+                    const uint32_t full = PAIR ? map_to_cta(smem_u32(&bar_full[s]), 0) : smem_u32(&bar_full[s]);
+                    if (rank == 0) mbar_arrive_expect_tx(&bar_full[s], PAIR ? 2 * bytes : bytes);
+                    if constexpr (!SWIGLU) {
+                        load_tile_2d<PAIR>(sw_tile, &map_w, full, kb * kBK, t.expert * rows_w + w_row, pol_w);
+                    } else if (p.interleave) {
+                        load_tile_5d<PAIR>(sw_tile, &map_w, full, kb * kBK, 0, 0, w_row / 16, t.expert, pol_w);
+                    } else {
 #pragma unroll
-                    for (int g = 0; g < kGathers; ++g)
-                        if ((g * 32 + lane) * 4 < cols)
-                            tma_gather4(sx_tile + (g * 32 + lane) * 4 * kBK, &map_x, &bar_full[s], kb * kBK, src[g][0], src[g][1], src[g][2], src[g][3]);
-                } else {
-                    if (lane * 32 < cols) tma_load_2d(sx_tile + lane * 32 * kBK, &map_x, &bar_full[s], kb * kBK, t.row0 + lane * 32);
+                        for (int i = 0; i < 8; ++i)
+                            load_tile_2d<PAIR>(sw_tile + i * 16 * kBK, &map_w, full, kb * kBK, t.expert * rows_w + w_row + (i >> 1) * 16 + (i & 1) * p.N, pol_w);
+                    }
+                    if (!PAIR && p.slots && !p.in_order) {
+#pragma unroll 4
+                        for (int r = 0; r < cols; r += 4) {
+                            const int4 q = *reinterpret_cast<const int4*>(&gather_rows[r]);
+                            tma_gather4(sx_tile + r * kBK, &map_x.m[0], &bar_full[s], kb * kBK, q.x, q.y, q.z, q.w);
+                        }
+                    } else {
+                        load_tile_2d<PAIR>(sx_tile, &map_x.m[box], full, kb * kBK, t.row0, pol_x);
+                    }
                 }
                 __syncwarp();
                 if (armed < STAGES) ++armed;
                 if (++s == STAGES) s = 0, ph ^= 1;
             }
         }
-        drain_stages<STAGES>(bar_full, bar_empty, s, ph, armed, p.status, &abort_flag);
+        // (PAIR: the leader's bar_full complete only when both CTAs' bytes have landed; the peer's own are never used)
+        drain_stages<STAGES>(PAIR && rank != 0 ? nullptr : bar_full, bar_empty, s, ph, armed, p.status, &abort_flag);
     } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issuer
+        // ------------------------------------------------------------------ MMA issuer (of the leader)
         uint32_t s = 0, ph = 0;
         uint32_t local_tile = 0;
-        bool ok = true;
+        bool ok = rank == 0;
         int chunk = 0;
         ExpertTile t;
         const uint32_t w_0 = smem_desc_lo(smem_u32(smem));
-        for (int64_t item = blockIdx.x; ok && find_expert_tile(list, p.E, weight_tiles, item, chunk, t); item += gridDim.x, ++local_tile) {
+        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, chunk, t); item += item_step, ++local_tile) {
             const uint32_t buf = local_tile & 1;
             const uint32_t acc_ph = (local_tile >> 1) & 1;
             if (!warp_agrees(wait_or_abort(&bar_acc_empty[buf], acc_ph ^ 1, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_MMA)) break;
             tcgen05_fence_after_sync();
-            const uint32_t idesc = make_idesc_i8(kBM, 0, false) | (static_cast<uint32_t>((t.rows + 15) & ~15) >> 3) << 17;
+            const uint32_t idesc = make_idesc_i8(PAIR ? 2 * kBM : kBM, 0, false) | (static_cast<uint32_t>((t.rows + kAlign - 1) & ~(kAlign - 1)) >> 3) << 17;
             const uint32_t tmem_d = tmem_base + buf * BT;
             for (int kb = 0; kb < num_kb; ++kb) {
                 if (!warp_agrees(wait_or_abort(&bar_full[s], ph, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_MMA)) {
@@ -246,13 +290,28 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 const uint32_t dw = w_0 + s * (kStageBytes / 16), dx = dw + kBytesW / 16;
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < kBK / kUmmaK; ++k) umma_i8(tmem_d, smem_desc_k128_of(dw + 2 * k), smem_desc_k128_of(dx + 2 * k), idesc, (kb | k) != 0);
-                    umma_commit(&bar_empty[s]);
+                    for (int k = 0; k < kBK / kUmmaK; ++k) {
+                        if constexpr (PAIR) umma_i8_pair(tmem_d, smem_desc_k128_of(dw + 2 * k), smem_desc_k128_of(dx + 2 * k), idesc, (kb | k) != 0);
+                        else umma_i8(tmem_d, smem_desc_k128_of(dw + 2 * k), smem_desc_k128_of(dx + 2 * k), idesc, (kb | k) != 0);
+                    }
+                    if constexpr (PAIR) {
+                        umma_commit_pair(map_to_cta(smem_u32(&bar_empty[s]), 0));
+                        umma_commit_pair(map_to_cta(smem_u32(&bar_empty[s]), 1));
+                    } else {
+                        umma_commit(&bar_empty[s]);
+                    }
                 }
                 __syncwarp();
                 if (++s == STAGES) s = 0, ph ^= 1;
             }
-            if (ok && elect_one()) umma_commit(&bar_acc_full[buf]);
+            if (ok && elect_one()) {
+                if constexpr (PAIR) {
+                    umma_commit_pair(map_to_cta(smem_u32(&bar_acc_full[buf]), 0));
+                    umma_commit_pair(map_to_cta(smem_u32(&bar_acc_full[buf]), 1));
+                } else {
+                    umma_commit(&bar_acc_full[buf]);
+                }
+            }
             __syncwarp();
         }
     } else {
@@ -273,9 +332,10 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         bool ok = true;
         int chunk = 0;
         ExpertTile t;
-        for (int64_t item = blockIdx.x; find_expert_tile(list, p.E, weight_tiles, item, chunk, t); item += gridDim.x, ++local_tile) {
+        for (int64_t item = first_item; find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, chunk, t); item += item_step, ++local_tile) {
             const uint32_t buf = local_tile & 1;
             const uint32_t acc_ph = (local_tile >> 1) & 1;
+            if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank);
             // The scales are fetched while the tile is computed.  (A warp that fills this buffer again has passed the barrier of the tile
             // in between, behind which nobody reads it any more.)
             for (int r = et; r < BT; r += 128) {
@@ -337,16 +397,21 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             }
             tcgen05_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bar_acc_empty[buf]);
+            if (lane == 0) {
+                if constexpr (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_acc_empty[buf]), 0));
+                else mbar_arrive(&bar_acc_empty[buf]);
+            }
         }
     }
 
     tcgen05_fence_before_sync();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync_all();  // neither CTA leaves while the other may still read or signal it
     if (warp == 1) {
         __syncwarp();
         tcgen05_fence_after_sync();
-        tmem_dealloc(tmem_base, kTmemCols);
+        if constexpr (PAIR) tmem_dealloc_pair(tmem_base, kTmemCols);
+        else tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 

@@ -164,6 +164,27 @@ GI8_DEVICE void tma_load_2d_hint(void* smem_dst, const CUtensorMap* map, uint64_
         : "memory");
 }
 
+// (the barrier by its shared-memory address)
+GI8_DEVICE void tma_load_2d_hint_addr(void* smem_dst, const CUtensorMap* map, uint32_t bar_addr, int32_t c0, int32_t c1, uint64_t cache_policy)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4}], [%2], %5;"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_addr), "r"(c0), "r"(c1), "l"(cache_policy)
+        : "memory");
+}
+
+GI8_DEVICE void tma_load_5d_hint(void* smem_dst, const CUtensorMap* map, uint32_t bar_addr, int32_t c0, int32_t c1, int32_t c2, int32_t c3,
+                                 int32_t c4, uint64_t cache_policy)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_addr), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
+        "l"(cache_policy)
+        : "memory");
+}
+
 // Four rows of a matrix, wherever they lie, into 4 x 128 consecutive bytes of shared memory (swizzled as a tile at that address would
 // be).  The tensor map's box is one row high; c0 as above.
 GI8_DEVICE void tma_gather4(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t r0, int32_t r1, int32_t r2, int32_t r3)
@@ -477,6 +498,27 @@ GI8_DEVICE void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, uint32_
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
         " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar_cluster_addr), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+GI8_DEVICE void tma_load_2d_pair_hint(void* smem_dst, const CUtensorMap* map, uint32_t leader_bar_cluster_addr, int32_t c0, int32_t c1,
+                                      uint64_t cache_policy)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint"
+        " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar_cluster_addr), "r"(c0), "r"(c1), "l"(cache_policy)
+        : "memory");
+}
+
+GI8_DEVICE void tma_load_5d_pair_hint(void* smem_dst, const CUtensorMap* map, uint32_t leader_bar_cluster_addr, int32_t c0, int32_t c1, int32_t c2, int32_t c3,
+                                 int32_t c4, uint64_t cache_policy)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(leader_bar_cluster_addr), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
+        "l"(cache_policy)
         : "memory");
 }
 
