@@ -73,6 +73,17 @@ int make_gate_up_map(CUtensorMap* map, const int8_t* w, int64_t E, int64_t N, in
     return GI8_OK;
 }
 
+template <int WARPS, int LOADS>
+int launch_group(GroupParams p, int ctas, int slot, cudaStream_t s)
+{
+    auto kernel = group_by_expert_kernel<WARPS, LOADS>;
+    auto smem = [](int64_t E) { return static_cast<size_t>((WARPS + 3) * E + WARPS * 32 * LOADS) * 4; };
+    static_assert((WARPS + 3) * kGroupMaxExperts * 4 + WARPS * 32 * LOADS * 4 <= 227 * 1024 - 1024, "fits shared memory at the most experts");
+    if (int rc = experts_smem(slot, kernel, smem(kGroupMaxExperts))) return rc;
+    p.per_warp = static_cast<int>((p.S + static_cast<int64_t>(ctas) * WARPS * 32 - 1) / (ctas * WARPS * 32)) * 32;
+    return launch(kernel, dim3(ctas), WARPS * 32, smem(p.E), s, dim3(ctas), knobs().pdl, p, ctas);
+}
+
 template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
 int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, ExpertsParams p, cudaStream_t s)
 {
@@ -95,7 +106,7 @@ int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, 
     const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
     const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
     const int grid = static_cast<int>(std::min<int64_t>(tiles, st->sm_count / (PAIR ? 2 : 1))) * (PAIR ? 2 : 1);
-    return launch(kernel, dim3(grid), kExpertsThreads, smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
+    return launch(kernel, dim3(grid), experts_threads(SWIGLU), smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
 }
 
 // Rows of a token tile.
@@ -168,18 +179,10 @@ int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t fi
     p.experts = experts, p.offsets = offsets, p.slots = slots, p.places = places;
     p.S = (int)S, p.E = (int)E, p.first = (int)first;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (S <= 2048) {
-        constexpr int W = 8;
-        p.per_warp = (int)((S + W * 32 - 1) / (W * 32)) * 32;
-        const size_t smem = static_cast<size_t>(W + 1) * E * 4;
-        return launch(group_by_expert_kernel<W>, dim3(1), W * 32, smem, s, dim3(1), knobs().pdl, p, 1);
-    }
-    constexpr int W = 32;
-    const int ctas = S <= 4096 ? 2 : S <= 8192 ? 4 : 8;
-    p.per_warp = (int)((S + ctas * W * 32 - 1) / (ctas * W * 32)) * 32;
-    const size_t smem = static_cast<size_t>(W + 1) * E * 4;
-    if (int rc = experts_smem(8, group_by_expert_kernel<W>, static_cast<size_t>(W + 1) * kGroupMaxExperts * 4)) return rc;
-    return launch(group_by_expert_kernel<W>, dim3(ctas), W * 32, smem, s, dim3(ctas), knobs().pdl, p, ctas);
+    // Up to 2048 pairs in one CTA of eight warps, up to 131072 in runs that registers hold, more in longer runs.
+    if (S <= 2048) return launch_group<8, 8>(p, 1, 8, s);
+    if (S <= 8 * 32 * 32 * 16) return launch_group<32, 16>(p, S <= 16384 ? 1 : S <= 32768 ? 2 : S <= 65536 ? 4 : 8, 9, s);
+    return launch_group<32, 0>(p, 8, 10, s);
 }
 
 int64_t gi8_matmul_experts_workspace_bytes(int64_t rows, int64_t tokens, int64_t E, int64_t K)

@@ -9,11 +9,11 @@
 // whose extent is an operand of the instruction: a tile of r rows costs roundup(r, 16) columns instead of a multiple of 128, which
 // is what makes ragged groups and single tokens cheap.  An expert's rows are cut into equal tiles of at most BT.
 //
-// Structure (one persistent CTA per SM, 192 threads), as in the dense kernel:
+// Structure (one persistent CTA per SM, 192 threads, 320 with SWIGLU), as in the dense kernel:
 //   warp 0      TMA producer: weight tiles (128 rows x 128 bytes) and token rows, either with one instruction; gathered rows four
 //               per instruction wherever they lie
 //   warp 1      MMA issuer, kind::i8, two accumulators in tensor memory
-//   warps 2..5  epilogue: a lane holds one output channel and walks over the tile's tokens
+//   the others  epilogue: a lane holds one output channel and walks over the tile's tokens
 // SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes
 // apart in one warp, which exchanges half of the tokens by shuffles and computes 16 results per lane.
 #pragma once
@@ -22,7 +22,10 @@
 
 namespace gi8 {
 
-constexpr int kExpertsThreads = 192;
+// Epilogue warps: eight where a result costs an exponential and a quotient, four else, as eight disturb the MMAs under which they run
+// (16384 rows, E = 8, K = 4096: SwiGLU 2 x 14336 channels with four / eight 1516 / 1270 us, product of 14336 channels 633 / 694).
+constexpr int experts_epilogue_warps(bool swiglu) { return swiglu ? 8 : 4; }
+constexpr int experts_threads(bool swiglu) { return 64 + 32 * experts_epilogue_warps(swiglu); }
 constexpr int kExpertsMaxExperts = 1024;
 
 struct ExpertsParams {
@@ -139,7 +142,7 @@ GI8_DEVICE void load_tile_5d(void* dst, const CUtensorMap* map, uint32_t bar, in
 }
 
 template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
-__global__ void __launch_bounds__(kExpertsThreads, 1)
+__global__ void __launch_bounds__(experts_threads(SWIGLU), 1)
 experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const ExpertsParams p)
 {
     static_assert(BT == 64 || BT == 128 || BT == 256, "quarters of a tile are columns of an MMA, of which there are at most 256");
@@ -148,6 +151,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     constexpr int kAlign = PAIR ? 32 : 16;      // what the columns of an MMA are a multiple of
     constexpr uint32_t kStageBytes = kBytesW + kRowsX * kBK;
     constexpr uint32_t kTmemCols = 2 * BT;
+    constexpr int kEpilogueThreads = SWIGLU ? 256 : 128;
     constexpr int kChannels = SWIGLU ? kBM / 2 : kBM;  // output channels of a weight tile
 
     extern __shared__ uint8_t smem_raw[];
@@ -181,7 +185,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bar_acc_full[b], 1);
-            mbar_init(&bar_acc_empty[b], PAIR ? 8 : 4);
+            mbar_init(&bar_acc_empty[b], (PAIR ? 2 : 1) * kEpilogueThreads / 32);
         }
         fence_barrier_init();
         prefetch_tensormap(&map_w);
@@ -321,7 +325,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         {
             // rows that belong to no expert
             const int64_t first = static_cast<int64_t>(list.start[p.E]) * p.N, end = p.rows * p.N;
-            const int64_t step = static_cast<int64_t>(gridDim.x) * 128, at = static_cast<int64_t>(blockIdx.x) * 128 + et;
+            const int64_t step = static_cast<int64_t>(gridDim.x) * kEpilogueThreads, at = static_cast<int64_t>(blockIdx.x) * kEpilogueThreads + et;
             if (p.vec_zero) {
                 for (int64_t i = first / 8 + at; i < end / 8; i += step) reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
             } else {
@@ -338,7 +342,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank);
             // The scales are fetched while the tile is computed.  (A warp that fills this buffer again has passed the barrier of the tile
             // in between, behind which nobody reads it any more.)
-            for (int r = et; r < BT; r += 128) {
+            for (int r = et; r < BT; r += kEpilogueThreads) {
                 float v = 0.0f;
                 if (r < t.rows) {
                     int src = t.row0 + r;
@@ -351,9 +355,9 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             const bool channel_ok = channel < p.N;
             float channel_scale = 0.0f;
             if (channel_ok) channel_scale = __ldg(p.sw + static_cast<int64_t>(t.expert) * rows_w + channel + (SWIGLU && lane >= 16 ? p.N : 0));
-            asm volatile("bar.sync 1, 128;" ::: "memory");  // the four epilogue warps
+            asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");  // the epilogue warps
             // After a failed wait the warp goes on through the list without touching anything: the named barrier above has no time limit and
-            // needs all four warps once per tile.
+            // needs every warp once per tile.
             if (!ok || !warp_agrees(wait_or_abort(&bar_acc_full[buf], acc_ph, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_EPILOGUE)) {
                 ok = false;
                 continue;
@@ -361,7 +365,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             tcgen05_fence_after_sync();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BT;
 #pragma unroll 1
-            for (int c = 0; c < t.rows; c += 32) {
+            for (int c = (et / 128) * 32; c < t.rows; c += kEpilogueThreads / 4) {  // 32 tokens; with eight warps every other 32
                 uint32_t v[32];
                 __syncwarp();
                 tmem_ld_32x32b_x32(taddr + c, v);

@@ -86,11 +86,15 @@ GI8_DEVICE void route_two(F c, F& first, F& second)
     else if (c > second) second = c;
 }
 
-// The bound on the difference of two fp32 choices' errors.  |error of s| <= 2.5e-7 (expf 2 ulp, s (1 - s) <= 1/4, one rounding each for
-// the sum and the quotient), for softmax also V + 5 roundings of the denominator's sum; the bias is added with one rounding more.
-// Twice that for the two of them, and twice again to be safe.
+// The bound on the difference of two fp32 choices' errors, in units of 2^-24.  A score's error: 4 (2 ulp) of the exponential where the score
+// moves by at most a quarter of it, 1 for the sum, 4 (2 ulp) for the quotient, 1 for its argument's rounding: 7; softmax: up to V + 5 roundings
+// of the denominator's sum and 4 of each exponential instead of the sum's 1: V + 16; the sum with the bias: one rounding of at most |c| + its
+// error.  Twice that for the two of them, and half as much again to be safe.
 template <int V>
-GI8_DEVICE float route_margin(float c, bool softmax) { return 1.3e-6f + 2.5e-7f * fabsf(c) + (softmax ? 2.5e-7f * (V + 5) : 0.0f); }
+GI8_DEVICE float route_margin(float c, bool softmax) { return (3.0f * 5.9604645e-8f) * (fabsf(c) + (softmax ? V + 16.0f : 8.0f)); }
+
+GI8_DEVICE float route_quotient(float a, float b) { return __fdividef(a, b); }  // 2 ulp for b below 2^126, 0 up to infinity
+GI8_DEVICE double route_quotient(double a, double b) { return a / b; }
 
 // Selects one token's experts; the id of place j ends up in lane j.  Returns whether a decision was closer than fp32 can tell
 // (F = float only).  l: this lane's logits (-inf behind E).  scratch: E values of this warp.
@@ -119,7 +123,7 @@ GI8_DEVICE bool route_select(const RouteParams& p, const float (&l)[V], F* scrat
     }
     auto score = [&](float v) -> F {
         if (!(v > -INFINITY)) return F(0);
-        return softmax ? route_exp(static_cast<F>(v) - m) / z : F(1) / (F(1) + route_exp(-static_cast<F>(v)));
+        return softmax ? route_quotient(route_exp(static_cast<F>(v) - m), z) : route_quotient(F(1), F(1) + route_exp(-static_cast<F>(v)));
     };
 
     F c[V];
@@ -141,7 +145,7 @@ GI8_DEVICE bool route_select(const RouteParams& p, const float (&l)[V], F* scrat
         bool holds = true;
         if (!scratch) {  // whole lanes, a power of two of them
             const int span = size / V;
-            group_here = lane / span;
+            group_here = lane >> (__ffs(span) - 1);
             holds = group_here < p.groups;
             for (int o = 1; o < span; o <<= 1) {
                 const F f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
@@ -174,25 +178,29 @@ GI8_DEVICE bool route_select(const RouteParams& p, const float (&l)[V], F* scrat
             kept |= 1u << g;
             if (group_here == g) key = 0;
         }
+        if (!scratch) {  // a lane's experts are of one group
+            const bool out = holds && !((kept >> group_here) & 1u);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int g = (e0 + i) / size;
-            if (g < p.groups && !((kept >> g) & 1u)) c[i] = -INFINITY;
+            for (int i = 0; i < V; ++i) c[i] = out ? F(-INFINITY) : c[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const int g = (e0 + i) / size;
+                if (g < p.groups && !((kept >> g) & 1u)) c[i] = -INFINITY;
+            }
         }
     }
 
     Key key[V];
-    Key best = 0;
-    int at = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        key[i] = route_key(c[i]);
-        if (key[i] > best) best = key[i], at = i;
-    }
+    for (int i = 0; i < V; ++i) key[i] = route_key(c[i]);
     my_expert = -1;
     F last = 0;
     const int rounds = p.top_k + (p.bias ? 1 : 0);  // one more to see how far the first one left out is
     for (int j = 0; j < rounds; ++j) {
+        Key best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = max(best, key[i]);
         const Key top = warp_max_key(best);
         if (top == 0) break;
         if (p.bias) {
@@ -201,19 +209,19 @@ GI8_DEVICE bool route_select(const RouteParams& p, const float (&l)[V], F* scrat
             last = here;
         }
         if (j == p.top_k) break;
+        // the first lane that has it, and its first
         const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-        const int e = __shfl_sync(0xffffffffu, e0 + at, src);
-        if (lane == j) my_expert = e;
-        if (lane == src) {
+        int at = 0;
+        bool looking = lane == src;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (i == at) key[i] = 0;
-            best = 0;
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (key[i] > best) best = key[i], at = i;
+        for (int i = 0; i < V; ++i) {
+            const bool hit = looking && key[i] == top;
+            key[i] = hit ? Key(0) : key[i];
+            at = hit ? i : at;
+            looking = looking && !hit;
         }
-        __syncwarp();
+        const int e = __shfl_sync(0xffffffffu, e0 + at, src);
+        my_expert = lane == j ? e : my_expert;
     }
     return close;
 }

@@ -11,6 +11,9 @@ import torch
 from . import quant
 
 _NS = "gemm_int8_CUDA"
+_ops = torch.ops.gemm_int8_CUDA
+# (the overloads themselves: a call that looks for them first takes half a microsecond longer)
+_route, _group, _matmul, _combine, _layer = (op.default for op in (_ops.route_experts, _ops.group_by_expert, _ops.int8_matmul_experts, _ops.combine_experts, _ops.int8_experts))
 _SCORINGS = ("softmax", "sigmoid")
 _GROUP_SCORES = ("max", "top2")
 
@@ -37,7 +40,7 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     score.  E <= 1024, top_k <= 32, groups <= 32.
     """
     k, sigmoid, g, tg, top2, renorm, sc = _router_args(top_k, scoring, groups, top_groups, group_score, renormalize, scale)
-    return torch.ops.gemm_int8_CUDA.route_experts(logits, bias, k, sigmoid, g, tg, top2, renorm, sc)
+    return _route(logits, bias, k, sigmoid, g, tg, top2, renorm, sc)
 
 
 def group_by_expert(experts: torch.Tensor, num_experts: int, first_expert: int = 0):
@@ -47,7 +50,7 @@ def group_by_expert(experts: torch.Tensor, num_experts: int, first_expert: int =
     pair, token * top_k + choice, of each row (-1 behind the last one), places the row of each pair (-1 for an expert that is not one of
     the num_experts here: expert -1, or one of another rank's).
     """
-    return torch.ops.gemm_int8_CUDA.group_by_expert(experts, num_experts, first_expert)
+    return _group(experts, num_experts, first_expert)
 
 
 def matmul_experts(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
@@ -58,14 +61,14 @@ def matmul_experts(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.Tensor, 
     slots, the token slots[p] // top_k: rows are then read where the tokens lie, without a copy.  Rows behind offsets[-1] are zero.
     x_q int8 [rows or tokens, K], w_q int8 [E, N, K], x_scale fp32 [rows or tokens], w_scale fp32 [E, N]; K a multiple of 16.
     """
-    return torch.ops.gemm_int8_CUDA.int8_matmul_experts(x_q, w_q, x_scale, w_scale, offsets, slots, top_k, False)
+    return _matmul(x_q, w_q, x_scale, w_scale, offsets, slots, top_k, False)
 
 
 def matmul_experts_swiglu(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
                           slots: torch.Tensor | None = None, top_k: int = 1) -> torch.Tensor:
     """`matmul_experts` for a weight [E, 2 N, K] of N gate rows and then N up rows -> bf16 [rows, N]: ``silu(gate) * up`` of the two products in
     fp32, rounded once."""
-    return torch.ops.gemm_int8_CUDA.int8_matmul_experts(x_q, w_q, x_scale, w_scale, offsets, slots, top_k, True)
+    return _matmul(x_q, w_q, x_scale, w_scale, offsets, slots, top_k, True)
 
 
 def combine_experts(y: torch.Tensor, weights: torch.Tensor, places: torch.Tensor, add: torch.Tensor | None = None) -> torch.Tensor:
@@ -73,7 +76,7 @@ def combine_experts(y: torch.Tensor, weights: torch.Tensor, places: torch.Tensor
 
     y bf16 [rows, N], weights fp32 [T, top_k], places int32 [T, top_k] (negative: left out), add bf16 [T, N] or None; top_k <= 32.
     """
-    return torch.ops.gemm_int8_CUDA.combine_experts(y, weights, places, add)
+    return _combine(y, weights, places, add)
 
 
 # --------------------------------------------------------------------------------------------------
@@ -163,6 +166,6 @@ class Int8Experts(torch.nn.Module):
             logits = logits.to(torch.float32)
         if add is not None:
             add = add.reshape(x2.shape).to(torch.bfloat16)
-        out = torch.ops.gemm_int8_CUDA.int8_experts(x2, logits, self.bias, self.gate_up_q, self.gate_up_scale, self.down_q, self.down_scale, *self._router,
+        out = _layer(x2, logits, self.bias, self.gate_up_q, self.gate_up_scale, self.down_q, self.down_scale, *self._router,
                                                     self.first_expert, add)
         return out if x.dim() == 2 else out.reshape(x.shape)
