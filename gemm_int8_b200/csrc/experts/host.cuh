@@ -25,6 +25,8 @@ int experts_smem(int slot, Kernel kernel, size_t bytes)
     return GI8_OK;
 }
 
+bool misaligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
 template <typename T, int V>
 int launch_route(const RouteParams& p, cudaStream_t s)
 {
@@ -42,11 +44,14 @@ template <typename T>
 int launch_route_for(RouteParams p, cudaStream_t s)
 {
     const int per_lane = (p.E + 31) / 32;
-    auto vec = [&](int v) { return p.E % v == 0 && reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && (v * static_cast<int>(sizeof(T))) % 16 == 0; };
-#define GI8_ROUTE(V_)                                   \
-    if (per_lane <= V_) {                               \
-        p.vec = vec(V_);                                \
-        return launch_route<T, V_>(p, s);               \
+    auto vec = [&](const void* base, int v, int size) { return p.E % v == 0 && !misaligned(base, 16) && v * size % 16 == 0; };
+    for (p.half_k = 1; 2 * p.half_k < p.top_k;) p.half_k *= 2;
+    if (p.top_k == 1) p.half_k = 0;
+#define GI8_ROUTE(V_)                                              \
+    if (per_lane <= V_) {                                          \
+        p.vec = vec(p.logits, V_, static_cast<int>(sizeof(T)));    \
+        p.vec_bias = vec(p.bias, V_, 4);                           \
+        return launch_route<T, V_>(p, s);                          \
     }
     GI8_ROUTE(1)
     GI8_ROUTE(2)
@@ -130,8 +135,6 @@ int dispatch_experts(DeviceState* st, const int8_t* x, const int8_t* w, const Ex
         default: return launch_experts<256, 6, SWIGLU, true>(st, slot + 3, x, w, p, s);
     }
 }
-
-bool misaligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
 }  // namespace
 

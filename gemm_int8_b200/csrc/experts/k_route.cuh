@@ -8,11 +8,14 @@
 //           and where fewer are left the places hold expert -1 and weight 0
 //   weight  w_j = s_chosen(j) (/ their sum) * scale
 //
-// Exactness: which of two experts is chosen must not depend on how a score was rounded to fp32.  The scores are computed in fp32
-// together with a bound on their error; a token at which two neighbours in the order (or the last group kept and the first one
-// dropped) lie closer than that is decided again in fp64 by the same warp.
+// Exactness: which of two experts is chosen must not depend on how a score was rounded to fp32.  A token is first decided by fp32
+// scores, with a bound on their error; where two neighbours in the order (or the last group kept and the first one dropped) lie closer
+// than that, the same warp decides it again in fp64.
 //
-// One warp per token; a lane holds V consecutive experts, so that the groups of the usual models are runs of whole lanes.
+// One warp per token; a lane holds V consecutive experts, so that the groups of the usual models are runs of whole lanes.  The choices become
+// unsigned keys whose lowest bits are the place within the lane, so that a round of the selection is one maximum over the lane's
+// keys, one over the warp, and a comparison per key that removes the winner.  Bound by instruction issue for large batches (16384
+// tokens of 256 experts, bias, groups: ROUTE_US us, of which the bytes take 3; with keys and indices apart 38, 1735 instructions a token).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -35,17 +38,19 @@ struct RouteParams {
     int groups, top_groups;
     int sigmoid, group_top2, renormalize;
     float scale;
-    int vec;             // rows start on whole vectors of a lane's V experts
+    int vec, vec_bias;   // rows (the bias) can be read in 16-byte pieces of a lane's V experts
+    int half_k;          // half of the power of two that holds top_k
 };
 
-// Order-preserving maps of choices to unsigned keys; 0 for what cannot be chosen.
+// Order-preserving map of choices to unsigned keys.  What cannot be chosen is -inf, whose key is kRouteNone.
+constexpr uint32_t kRouteNone = 0x007fffffu;
 GI8_DEVICE uint32_t route_key(float c)
 {
-    if (!(c > -INFINITY)) return 0u;
     const uint32_t u = __float_as_uint(c + 0.0f);  // -0 becomes +0
-    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+    return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
 }
-GI8_DEVICE uint64_t route_key(double c)
+GI8_DEVICE float route_unkey(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
+GI8_DEVICE uint64_t route_key(double c)  // 0: cannot be chosen
 {
     if (!(c > -INFINITY)) return 0ull;
     const uint64_t u = static_cast<uint64_t>(__double_as_longlong(c + 0.0));
@@ -58,172 +63,212 @@ GI8_DEVICE uint64_t warp_max_key(uint64_t k)
     const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
     return (static_cast<uint64_t>(hi) << 32) | lo;
 }
-GI8_DEVICE float route_unkey(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
-GI8_DEVICE double route_unkey(uint64_t k)
-{
-    return __longlong_as_double(static_cast<long long>(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
-}
-
-GI8_DEVICE float route_exp(float x) { return expf(x); }
-GI8_DEVICE double route_exp(double x) { return exp(x); }
-
-template <typename F>
-struct RouteKeyOf;
-template <>
-struct RouteKeyOf<float> {
-    using type = uint32_t;
-};
-template <>
-struct RouteKeyOf<double> {
-    using type = uint64_t;
-};
 
 // A group's two largest choices so far (second = -inf: only one).
 template <typename F>
 GI8_DEVICE void route_two(F c, F& first, F& second)
 {
-    if (c > first) second = first, first = c;
-    else if (c > second) second = c;
+    second = max(second, min(first, c));
+    first = max(first, c);
 }
 
-// The bound on the difference of two fp32 choices' errors, in units of 2^-24.  A score's error: 4 (2 ulp) of the exponential where the score
-// moves by at most a quarter of it, 1 for the sum, 4 (2 ulp) for the quotient, 1 for its argument's rounding: 7; softmax: up to V + 5 roundings
-// of the denominator's sum and 4 of each exponential instead of the sum's 1: V + 16; the sum with the bias: one rounding of at most |c| + its
-// error.  Twice that for the two of them, and half as much again to be safe.
-template <int V>
-GI8_DEVICE float route_margin(float c, bool softmax) { return (3.0f * 5.9604645e-8f) * (fabsf(c) + (softmax ? V + 16.0f : 8.0f)); }
-
-GI8_DEVICE float route_quotient(float a, float b) { return __fdividef(a, b); }  // 2 ulp for b below 2^126, 0 up to infinity
-GI8_DEVICE double route_quotient(double a, double b) { return a / b; }
-
-// Selects one token's experts; the id of place j ends up in lane j.  Returns whether a decision was closer than fp32 can tell
-// (F = float only).  l: this lane's logits (-inf behind E).  scratch: E values of this warp.
+// The largest and second largest of a group's choices, in every lane of the group (whole lanes, a power of two of them) or, through shared
+// memory, in lane g for group g.  first, second: of this lane's choices.  Returns the group whose values the lane holds, or -1.
 template <typename F, int V>
-GI8_DEVICE bool route_select(const RouteParams& p, const float (&l)[V], F* scratch, int& my_expert, float& row_max, float& denominator)
+GI8_DEVICE int route_group_best(const RouteParams& p, const F (&of_group)[V], F* scratch, F& first, F& second)
 {
-    using Key = typename RouteKeyOf<F>::type;
     const int lane = threadIdx.x & 31;
-    const int e0 = lane * V;
-    const bool softmax = !p.sigmoid;
-    const bool need_scores = p.bias != nullptr || (p.groups > 1 && p.group_top2);
-    bool close = false;
-
-    F m = -INFINITY, z = 0;
-    if (softmax && (need_scores || !p.renormalize)) {
-        float mm = -INFINITY;
+    const int size = p.E / p.groups;
+    first = second = -INFINITY;
+    if (!scratch) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) mm = fmaxf(mm, l[i]);
-        const uint32_t mk = __reduce_max_sync(0xffffffffu, route_key(mm));
-        m = mk ? static_cast<F>(route_unkey(mk)) : F(0);
-#pragma unroll
-        for (int i = 0; i < V; ++i) z += l[i] > -INFINITY ? route_exp(static_cast<F>(l[i]) - m) : F(0);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-        row_max = static_cast<float>(m), denominator = static_cast<float>(z);
+        for (int i = 0; i < V; ++i) route_two(of_group[i], first, second);
+        const int span = size / V;
+        for (int o = 1; o < span; o <<= 1) {
+            const F f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
+            second = max(max(second, s2), min(first, f2));
+            first = max(first, f2);
+        }
+        const int g = lane >> (__ffs(span) - 1);
+        return g < p.groups ? g : -1;
     }
-    auto score = [&](float v) -> F {
-        if (!(v > -INFINITY)) return F(0);
-        return softmax ? route_quotient(route_exp(static_cast<F>(v) - m), z) : route_quotient(F(1), F(1) + route_exp(-static_cast<F>(v)));
-    };
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (lane * V + i < p.E) scratch[lane * V + i] = of_group[i];
+    __syncwarp();
+    if (lane < p.groups)
+        for (int i = 0; i < size; ++i) route_two(scratch[lane * size + i], first, second);
+    return lane < p.groups ? lane : -1;
+}
 
-    F c[V];
-    F first = -INFINITY, second = -INFINITY;  // of this lane's choices, as far as groups need them
+// Takes the experts of the groups that are not kept out of the choice.  group_here: what route_group_best returned.
+template <typename F, int V>
+GI8_DEVICE void route_drop_groups(const RouteParams& p, uint32_t kept, int group_here, bool by_lane, F (&c)[V])
+{
+    if (by_lane) {
+        const bool out = group_here >= 0 && !((kept >> group_here) & 1u);
+#pragma unroll
+        for (int i = 0; i < V; ++i) c[i] = out ? F(-INFINITY) : c[i];
+    } else {
+        const int size = p.E / p.groups, e0 = (threadIdx.x & 31) * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int g = (e0 + i) / size;
+            if (g < p.groups && !((kept >> g) & 1u)) c[i] = -INFINITY;
+        }
+    }
+}
+
+// A bound on the difference of two fp32 scores' errors, in units of 2^-24, where the choice is by scores.  Sigmoid: the exponential's (2 + 1.173
+// |l|) ulp move the score by at most 1/4, and by less far out: 1.6; the sum 1 (times a quarter), the quotient 4 (2 ulp): below 7.  Softmax: 5
+// for the score's own exponential and 4 for the quotient, the denominator's sum V + 5 and its exponentials 4: below V + 20.  The bias is
+// added with one rounding, of at most |c|.  Twice that for the two of them, and half as much again to be safe.
+template <int V>
+GI8_DEVICE float route_margin(float c, bool softmax) { return (3.0f * 5.9604645e-8f) * (fabsf(c) + (softmax ? V + 21.0f : 8.0f)); }
+
+// The softmax's largest logit and denominator (0 and 0 for a row without logits), in fp32 or fp64.
+template <typename F, int V>
+GI8_DEVICE void route_denominator(const float (&l)[V], F& m, F& z)
+{
+    float mm = l[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) mm = fmaxf(mm, l[i]);
+    mm = route_unkey(warp_max_key(route_key(mm)));
+    m = mm > -INFINITY ? static_cast<F>(mm) : F(0);
+    z = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) z += exp(static_cast<F>(l[i]) - m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+}
+
+// One token by fp32 keys; the expert of place j ends up in lane j, -1 for none.  Returns whether two choices were too close for that.
+// l: this lane's logits (-inf behind E and for NaN).  exact: the keys' lost bits are zeros in all logits, and the choice is by logits.
+template <int V>
+GI8_DEVICE bool route_fast(const RouteParams& p, const float (&l)[V], const float (&bias)[V], bool exact, float* scratch, float row_max, float denominator, int& my_expert)
+{
+    constexpr uint32_t kPlace = V <= 1 ? 0u : V <= 2 ? 1u : V <= 4 ? 3u : V <= 8 ? 7u : V <= 16 ? 15u : 31u;
+    const int lane = threadIdx.x & 31;
+    const bool softmax = !p.sigmoid;
+    const bool scores_of_groups = p.groups > 1 && p.group_top2;
+    const bool by_scores = p.bias != nullptr;
+    bool close = false;
+    float c[V];
+    auto score = [&](float v) { return softmax ? __fdividef(expf(v - row_max), denominator) : __fdividef(1.0f, 1.0f + __expf(-v)); };
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const bool masked = !(l[i] > -INFINITY);
-        const F s = need_scores && !masked ? score(l[i]) : F(0);
-        const F choice = p.bias ? s + static_cast<F>(e0 + i < p.E ? __ldg(p.bias + e0 + i) : 0.0f) : static_cast<F>(l[i]);
-        c[i] = masked || !(choice > -INFINITY) ? F(-INFINITY) : choice;
-        const F of_group = masked ? F(-INFINITY) : (p.group_top2 && !p.bias) ? s : c[i];
-        if (p.groups > 1) route_two(of_group, first, second);
-        if (p.groups > 1 && scratch && e0 + i < p.E) scratch[e0 + i] = of_group;
+        c[i] = l[i];
+        if (by_scores) c[i] = l[i] > -INFINITY ? fmaxf(score(l[i]) + bias[i], -INFINITY) : -INFINITY;
     }
-
     if (p.groups > 1) {
-        const int size = p.E / p.groups;
-        int group_here;  // the group whose value this lane holds
-        bool holds = true;
-        if (!scratch) {  // whole lanes, a power of two of them
-            const int span = size / V;
-            group_here = lane >> (__ffs(span) - 1);
-            holds = group_here < p.groups;
-            for (int o = 1; o < span; o <<= 1) {
-                const F f2 = __shfl_xor_sync(0xffffffffu, first, o), s2 = __shfl_xor_sync(0xffffffffu, second, o);
-                route_two(f2, first, second);
-                route_two(s2, first, second);
-            }
-        } else {
-            __syncwarp();
-            group_here = lane;
-            holds = lane < p.groups;
-            first = second = -INFINITY;
-            if (holds)
-                for (int i = 0; i < size; ++i) route_two(scratch[lane * size + i], first, second);
-            __syncwarp();
-        }
-        const F value = p.group_top2 && second > -INFINITY ? first + second : first;
-        Key key = holds ? route_key(value) : Key(0);
-        uint32_t kept = 0;
-        F last = 0;
+        float of_group[V], first, second;
+#pragma unroll
+        for (int i = 0; i < V; ++i) of_group[i] = scores_of_groups && !by_scores && l[i] > -INFINITY ? score(l[i]) : c[i];
+        const int group_here = route_group_best(p, of_group, scratch, first, second);
+        const float value = p.group_top2 && second > -INFINITY ? first + second : first;
+        uint32_t key = group_here >= 0 ? route_key(value) : 0u;
+        uint32_t kept = 0, last = 0;
         for (int n = 0; n <= p.top_groups; ++n) {
-            const Key best = warp_max_key(key);
-            if (best == 0) break;
-            const int src = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
-            const int g = __shfl_sync(0xffffffffu, group_here, src);
+            const uint32_t best = warp_max_key(key);
+            if (best <= kRouteNone) break;
             if (n == p.top_groups) {  // the best one that stays out
-                if (need_scores && last - route_unkey(best) <= 2 * route_margin<V>(static_cast<float>(last), softmax)) close = true;
+                if ((by_scores || scores_of_groups) && route_unkey(last) - route_unkey(best) <= 2.0f * route_margin<V>(route_unkey(last), softmax)) close = true;
                 break;
             }
-            last = route_unkey(best);
+            last = best;
+            const int g = __shfl_sync(0xffffffffu, group_here, __ffs(__ballot_sync(0xffffffffu, key == best)) - 1);
             kept |= 1u << g;
             if (group_here == g) key = 0;
         }
-        if (!scratch) {  // a lane's experts are of one group
-            const bool out = holds && !((kept >> group_here) & 1u);
-#pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = out ? F(-INFINITY) : c[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const int g = (e0 + i) / size;
-                if (g < p.groups && !((kept >> g) & 1u)) c[i] = -INFINITY;
-            }
-        }
+        route_drop_groups(p, kept, group_here, !scratch, c);
     }
+    uint32_t key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = (route_key(c[i]) & ~kPlace) | (kPlace - i);
+    uint32_t mine = 0;
+    my_expert = -1;
+    for (int j = 0; j <= p.top_k; ++j) {  // one more to see how far the first one left out is
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = max(best, key[i]);
+        const uint32_t top = warp_max_key(best);
+        if (top <= kRouteNone) break;
+        // the first lane that has this value, and the first place there
+        const int src = __ffs(__ballot_sync(0xffffffffu, (best | kPlace) == (top | kPlace))) - 1;
+        const uint32_t taken = __shfl_sync(0xffffffffu, best, src);
+        mine = lane == j ? taken : mine;
+        my_expert = lane == j ? src * V + static_cast<int>(kPlace - (taken & kPlace)) : my_expert;
+        const uint32_t gone = lane == src ? taken : 0u;
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = key[i] == gone ? 0u : key[i];
+    }
+    if (lane >= p.top_k) my_expert = -1;
+    if (!exact) {
+        // neighbours in the order; what keys drop below a value is at most their lowest bits' worth of it
+        const uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1);
+        if (lane < 31 && next > kRouteNone) {
+            const float a = route_unkey(mine & ~kPlace), b = route_unkey(next & ~kPlace);
+            const float lost = (kPlace + 1) * 1.1920929e-7f * fmaxf(fabsf(a), fabsf(b));
+            close = close || (by_scores ? a - b <= route_margin<V>(a, softmax) + lost : a - b <= lost);
+        }
+        if (p.top_k == 32) close = true;  // (the first one left out has no lane)
+    }
+    return __any_sync(0xffffffffu, close);
+}
 
-    Key key[V];
+// The same in fp64.
+template <int V>
+GI8_DEVICE void route_exact(const RouteParams& p, const float (&l)[V], double* scratch, int& my_expert)
+{
+    const int lane = threadIdx.x & 31;
+    const int e0 = lane * V;
+    const bool softmax = !p.sigmoid;
+    const bool scores_of_groups = p.groups > 1 && p.group_top2 && !p.bias;
+    double m = 0.0, z = 1.0;
+    if (softmax && (p.bias || scores_of_groups)) route_denominator(l, m, z);
+    auto score = [&](float v) { return softmax ? exp(static_cast<double>(v) - m) / z : 1.0 / (1.0 + exp(-static_cast<double>(v))); };
+    double c[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const bool masked = !(l[i] > -INFINITY);
+        const double choice = masked ? -INFINITY : p.bias ? score(l[i]) + static_cast<double>(e0 + i < p.E ? __ldg(p.bias + e0 + i) : 0.0f) : static_cast<double>(l[i]);
+        c[i] = choice > -INFINITY ? choice : -INFINITY;
+    }
+    if (p.groups > 1) {
+        double of_group[V], first, second;
+#pragma unroll
+        for (int i = 0; i < V; ++i) of_group[i] = scores_of_groups && l[i] > -INFINITY ? score(l[i]) : c[i];
+        const int group_here = route_group_best(p, of_group, scratch, first, second);
+        uint64_t key = group_here >= 0 ? route_key(p.group_top2 && second > -INFINITY ? first + second : first) : 0ull;
+        uint32_t kept = 0;
+        for (int n = 0; n < p.top_groups; ++n) {
+            const uint64_t best = warp_max_key(key);
+            if (best == 0) break;
+            const int g = __shfl_sync(0xffffffffu, group_here, __ffs(__ballot_sync(0xffffffffu, key == best)) - 1);
+            kept |= 1u << g;
+            if (group_here == g) key = 0;
+        }
+        route_drop_groups(p, kept, group_here, !scratch, c);
+    }
+    uint64_t key[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i] = route_key(c[i]);
     my_expert = -1;
-    F last = 0;
-    const int rounds = p.top_k + (p.bias ? 1 : 0);  // one more to see how far the first one left out is
-    for (int j = 0; j < rounds; ++j) {
-        Key best = key[0];
-#pragma unroll
-        for (int i = 1; i < V; ++i) best = max(best, key[i]);
-        const Key top = warp_max_key(best);
-        if (top == 0) break;
-        if (p.bias) {
-            const F here = route_unkey(top);
-            if (j > 0 && last - here <= route_margin<V>(static_cast<float>(last), softmax)) close = true;
-            last = here;
-        }
-        if (j == p.top_k) break;
-        // the first lane that has it, and its first
-        const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+    for (int j = 0; j < p.top_k; ++j) {
+        uint64_t best = 0;
         int at = 0;
-        bool looking = lane == src;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const bool hit = looking && key[i] == top;
-            key[i] = hit ? Key(0) : key[i];
-            at = hit ? i : at;
-            looking = looking && !hit;
-        }
+        for (int i = 0; i < V; ++i)
+            if (key[i] > best) best = key[i], at = i;
+        const uint64_t top = warp_max_key(best);
+        if (top == 0) break;
+        const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
         const int e = __shfl_sync(0xffffffffu, e0 + at, src);
         my_expert = lane == j ? e : my_expert;
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = lane == src && i == at ? 0ull : key[i];
     }
-    return close;
 }
 
 GI8_DEVICE float route_load(const float* p) { return __ldg(p); }
@@ -273,25 +318,25 @@ route_experts_kernel(const RouteParams p, int use_scratch)
     const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
     if (t >= p.T) return;
     const T* row = static_cast<const T*>(p.logits) + t * p.E;
-    float l[V];
+    float l[V], bias[V];
     route_load_lane<T, V>(row, lane * V, p.E, p.vec, l);
+    if (p.bias) route_load_lane<float, V>(p.bias, lane * V, p.E, p.vec_bias, bias);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-        if (!(l[i] > -INFINITY)) l[i] = -INFINITY;  // NaN is never chosen
+    for (int i = 0; i < V; ++i) l[i] = fmaxf(l[i], -INFINITY);  // NaN is never chosen
 
     int expert;
     float row_max = 0.0f, denominator = 1.0f;
+    if (!p.sigmoid && (p.bias || !p.renormalize || (p.groups > 1 && p.group_top2))) route_denominator(l, row_max, denominator);
     double* mine = use_scratch ? route_scratch + static_cast<int64_t>(warp) * p.E : nullptr;
-    if (route_select<float, V>(p, l, reinterpret_cast<float*>(mine), expert, row_max, denominator))
-        route_select<double, V>(p, l, mine, expert, row_max, denominator);
+    if (route_fast<V>(p, l, bias, sizeof(T) == 2 && !p.bias && !(p.groups > 1 && p.group_top2), reinterpret_cast<float*>(mine), row_max, denominator, expert))
+        route_exact<V>(p, l, mine, expert);
 
     // Weights, lane j those of place j.  Their ratios do not depend on the softmax's denominator, nor on the sigmoid's where it is
     // all but exp(l): renormalised weights are taken relative to the largest logit chosen, so that they never are 0 / 0.
-    const bool chosen = lane < p.top_k && expert >= 0;
+    const bool chosen = expert >= 0;
     const float v = chosen ? route_load(row + expert) : -INFINITY;
     float top = v;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = p.half_k; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float w = 0.0f;
     if (chosen) {
         if (!p.sigmoid) w = p.renormalize ? expf(v - top) : expf(v - row_max) / denominator;
@@ -300,8 +345,7 @@ route_experts_kernel(const RouteParams p, int use_scratch)
     }
     if (p.renormalize) {
         float sum = w;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        for (int o = p.half_k; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (chosen) w /= sum;
     }
     if (lane < p.top_k) {
