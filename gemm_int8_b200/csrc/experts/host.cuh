@@ -28,7 +28,7 @@ int experts_smem(int slot, Kernel kernel, size_t bytes)
 bool misaligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
 template <typename T, int V>
-int launch_route(const RouteParams& p, cudaStream_t s)
+int launch_route(const RouteParams& p, int sms, cudaStream_t s)
 {
     // Groups that are not whole runs of a power of two of lanes have their values looked up through shared memory.
     int use_scratch = 0;
@@ -36,12 +36,14 @@ int launch_route(const RouteParams& p, cudaStream_t s)
         const int size = p.E / p.groups, span = size / V;
         use_scratch = size % V != 0 || (span & (span - 1)) != 0;
     }
-    const size_t smem = use_scratch ? static_cast<size_t>(kRouteWarps) * p.E * sizeof(double) : 0;
-    return launch(route_experts_kernel<T, V>, dim3((p.T + kRouteWarps - 1) / kRouteWarps), kRouteWarps * 32, smem, s, dim3(1), knobs().pdl, p, use_scratch);
+    const size_t smem = static_cast<size_t>(kRouteWarps) * p.E * sizeof(double);
+    // As many CTAs as are resident: a warp takes token after token, the next one's logits on their way.
+    const int64_t ctas = std::min<int64_t>((static_cast<int64_t>(p.T) + kRouteWarps - 1) / kRouteWarps, static_cast<int64_t>(sms) * (V <= 8 ? 8 : 3));
+    return launch(route_experts_kernel<T, V>, dim3((unsigned)ctas), kRouteWarps * 32, smem, s, dim3(1), knobs().pdl, p, use_scratch);
 }
 
 template <typename T>
-int launch_route_for(RouteParams p, cudaStream_t s)
+int launch_route_for(RouteParams p, int sms, cudaStream_t s)
 {
     const int per_lane = (p.E + 31) / 32;
     auto vec = [&](const void* base, int v, int size) { return p.E % v == 0 && !misaligned(base, 16) && v * size % 16 == 0; };
@@ -51,7 +53,7 @@ int launch_route_for(RouteParams p, cudaStream_t s)
     if (per_lane <= V_) {                                          \
         p.vec = vec(p.logits, V_, static_cast<int>(sizeof(T)));    \
         p.vec_bias = vec(p.bias, V_, 4);                           \
-        return launch_route<T, V_>(p, s);                          \
+        return launch_route<T, V_>(p, sms, s);                        \
     }
     GI8_ROUTE(1)
     GI8_ROUTE(2)
@@ -165,7 +167,7 @@ int gi8_route_experts(const void* logits, int logits_dtype, const float* bias, f
     p.groups = top_groups == groups ? 1 : (int)groups, p.top_groups = (int)top_groups;  // where all groups are kept there are none
     p.group_top2 = group_top2 != 0, p.renormalize = renormalize != 0, p.scale = scale;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return logits_dtype == 0 ? launch_route_for<float>(p, s) : launch_route_for<__nv_bfloat16>(p, s);
+    return logits_dtype == 0 ? launch_route_for<float>(p, st->sm_count, s) : launch_route_for<__nv_bfloat16>(p, st->sm_count, s);
 }
 
 int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t first, int32_t* offsets, int32_t* slots, int32_t* places, void* stream)

@@ -9,12 +9,15 @@
 //   weight  w_j = s_chosen(j) (/ their sum) * scale
 //
 // Exactness: which of two experts is chosen must not depend on how a score was rounded to fp32.  A token is first decided by fp32
-// scores, with a bound on their error; where two neighbours in the order (or the last group kept and the first one dropped) lie closer
-// than that, the same warp decides it again in fp64.
+// scores, with a bound on their error.  Where two neighbours in the order lie closer than that, the selection goes on to the last one that may
+// still belong to it, and the candidates are put in order by their choices in fp64, a lane each; where the last group kept and the
+// first one dropped lie that close, the groups' values are taken again in fp64.  One token in a thousand or so comes there, and
+// the warp that it holds up may be the launch's last: what counts is how long it takes (all of a token's scores in fp64 and the whole
+// selection again took 13 us, and the launch of 16384 tokens 39).
 //
 // One warp per token; a lane holds V consecutive experts, so that the groups of the usual models are runs of whole lanes.  The choices become
-// unsigned keys whose lowest bits are the place within the lane, so that a round of the selection is one maximum over the lane's
-// keys, one over the warp, and a comparison per key that removes the winner.  Bound by instruction issue for large batches (16384
+// unsigned keys whose lowest bits are the place within the lane, so that a round of the selection is one maximum over the lanes'
+// sorted keys' first, one over the warp, and a shift of the winner's lane.  Bound by instruction issue for large batches (16384
 // tokens of 256 experts, bias, groups: ROUTE_US us, of which the bytes take 3; with keys and indices apart 38, 1735 instructions a token).
 #pragma once
 
@@ -121,7 +124,7 @@ GI8_DEVICE void route_drop_groups(const RouteParams& p, uint32_t kept, int group
 }
 
 // A bound on the difference of two fp32 scores' errors, in units of 2^-24, where the choice is by scores.  Sigmoid: the exponential's (2 + 1.173
-// |l|) ulp move the score by at most 1/4, and by less far out: 1.6; the sum 1 (times a quarter), the quotient 4 (2 ulp): below 7.  Softmax: 5
+// |l|) ulp move the score by at most 1/4, and by less far out: 1.6; the sum 1 (times a quarter), the reciprocal 2 (1 ulp): below 7.  Softmax: 5
 // for the score's own exponential and 4 for the quotient, the denominator's sum V + 5 and its exponentials 4: below V + 20.  The bias is
 // added with one rounding, of at most |c|.  Twice that for the two of them, and half as much again to be safe.
 template <int V>
@@ -143,132 +146,29 @@ GI8_DEVICE void route_denominator(const float (&l)[V], F& m, F& z)
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
 }
 
-// One token by fp32 keys; the expert of place j ends up in lane j, -1 for none.  Returns whether two choices were too close for that.
-// l: this lane's logits (-inf behind E and for NaN).  exact: the keys' lost bits are zeros in all logits, and the choice is by logits.
+// Descending order within a lane: Batcher's merge exchange sort, unrolled.
 template <int V>
-GI8_DEVICE bool route_fast(const RouteParams& p, const float (&l)[V], const float (&bias)[V], bool exact, float* scratch, float row_max, float denominator, int& my_expert)
+GI8_DEVICE void route_sort(uint32_t (&key)[V])
 {
-    constexpr uint32_t kPlace = V <= 1 ? 0u : V <= 2 ? 1u : V <= 4 ? 3u : V <= 8 ? 7u : V <= 16 ? 15u : 31u;
-    const int lane = threadIdx.x & 31;
-    const bool softmax = !p.sigmoid;
-    const bool scores_of_groups = p.groups > 1 && p.group_top2;
-    const bool by_scores = p.bias != nullptr;
-    bool close = false;
-    float c[V];
-    auto score = [&](float v) { return softmax ? __fdividef(expf(v - row_max), denominator) : __fdividef(1.0f, 1.0f + __expf(-v)); };
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        c[i] = l[i];
-        if (by_scores) c[i] = l[i] > -INFINITY ? fmaxf(score(l[i]) + bias[i], -INFINITY) : -INFINITY;
-    }
-    if (p.groups > 1) {
-        float of_group[V], first, second;
+    for (int p = 1; p < V; p *= 2)
 #pragma unroll
-        for (int i = 0; i < V; ++i) of_group[i] = scores_of_groups && !by_scores && l[i] > -INFINITY ? score(l[i]) : c[i];
-        const int group_here = route_group_best(p, of_group, scratch, first, second);
-        const float value = p.group_top2 && second > -INFINITY ? first + second : first;
-        uint32_t key = group_here >= 0 ? route_key(value) : 0u;
-        uint32_t kept = 0, last = 0;
-        for (int n = 0; n <= p.top_groups; ++n) {
-            const uint32_t best = warp_max_key(key);
-            if (best <= kRouteNone) break;
-            if (n == p.top_groups) {  // the best one that stays out
-                if ((by_scores || scores_of_groups) && route_unkey(last) - route_unkey(best) <= 2.0f * route_margin<V>(route_unkey(last), softmax)) close = true;
-                break;
-            }
-            last = best;
-            const int g = __shfl_sync(0xffffffffu, group_here, __ffs(__ballot_sync(0xffffffffu, key == best)) - 1);
-            kept |= 1u << g;
-            if (group_here == g) key = 0;
-        }
-        route_drop_groups(p, kept, group_here, !scratch, c);
-    }
-    uint32_t key[V];
+        for (int k = p; k >= 1; k /= 2)
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = (route_key(c[i]) & ~kPlace) | (kPlace - i);
-    uint32_t mine = 0;
-    my_expert = -1;
-    for (int j = 0; j <= p.top_k; ++j) {  // one more to see how far the first one left out is
-        uint32_t best = key[0];
+            for (int j = k % p; j + k < V; j += 2 * k)
 #pragma unroll
-        for (int i = 1; i < V; ++i) best = max(best, key[i]);
-        const uint32_t top = warp_max_key(best);
-        if (top <= kRouteNone) break;
-        // the first lane that has this value, and the first place there
-        const int src = __ffs(__ballot_sync(0xffffffffu, (best | kPlace) == (top | kPlace))) - 1;
-        const uint32_t taken = __shfl_sync(0xffffffffu, best, src);
-        mine = lane == j ? taken : mine;
-        my_expert = lane == j ? src * V + static_cast<int>(kPlace - (taken & kPlace)) : my_expert;
-        const uint32_t gone = lane == src ? taken : 0u;
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = key[i] == gone ? 0u : key[i];
-    }
-    if (lane >= p.top_k) my_expert = -1;
-    if (!exact) {
-        // neighbours in the order; what keys drop below a value is at most their lowest bits' worth of it
-        const uint32_t next = __shfl_down_sync(0xffffffffu, mine, 1);
-        if (lane < 31 && next > kRouteNone) {
-            const float a = route_unkey(mine & ~kPlace), b = route_unkey(next & ~kPlace);
-            const float lost = (kPlace + 1) * 1.1920929e-7f * fmaxf(fabsf(a), fabsf(b));
-            close = close || (by_scores ? a - b <= route_margin<V>(a, softmax) + lost : a - b <= lost);
-        }
-        if (p.top_k == 32) close = true;  // (the first one left out has no lane)
-    }
-    return __any_sync(0xffffffffu, close);
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const uint32_t hi = max(key[i + j], key[i + j + k]), lo = min(key[i + j], key[i + j + k]);
+                        key[i + j] = hi, key[i + j + k] = lo;
+                    }
 }
 
-// The same in fp64.
-template <int V>
-GI8_DEVICE void route_exact(const RouteParams& p, const float (&l)[V], double* scratch, int& my_expert)
+GI8_DEVICE float approx_reciprocal(float x)  // 1 ulp
 {
-    const int lane = threadIdx.x & 31;
-    const int e0 = lane * V;
-    const bool softmax = !p.sigmoid;
-    const bool scores_of_groups = p.groups > 1 && p.group_top2 && !p.bias;
-    double m = 0.0, z = 1.0;
-    if (softmax && (p.bias || scores_of_groups)) route_denominator(l, m, z);
-    auto score = [&](float v) { return softmax ? exp(static_cast<double>(v) - m) / z : 1.0 / (1.0 + exp(-static_cast<double>(v))); };
-    double c[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const bool masked = !(l[i] > -INFINITY);
-        const double choice = masked ? -INFINITY : p.bias ? score(l[i]) + static_cast<double>(e0 + i < p.E ? __ldg(p.bias + e0 + i) : 0.0f) : static_cast<double>(l[i]);
-        c[i] = choice > -INFINITY ? choice : -INFINITY;
-    }
-    if (p.groups > 1) {
-        double of_group[V], first, second;
-#pragma unroll
-        for (int i = 0; i < V; ++i) of_group[i] = scores_of_groups && l[i] > -INFINITY ? score(l[i]) : c[i];
-        const int group_here = route_group_best(p, of_group, scratch, first, second);
-        uint64_t key = group_here >= 0 ? route_key(p.group_top2 && second > -INFINITY ? first + second : first) : 0ull;
-        uint32_t kept = 0;
-        for (int n = 0; n < p.top_groups; ++n) {
-            const uint64_t best = warp_max_key(key);
-            if (best == 0) break;
-            const int g = __shfl_sync(0xffffffffu, group_here, __ffs(__ballot_sync(0xffffffffu, key == best)) - 1);
-            kept |= 1u << g;
-            if (group_here == g) key = 0;
-        }
-        route_drop_groups(p, kept, group_here, !scratch, c);
-    }
-    uint64_t key[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = route_key(c[i]);
-    my_expert = -1;
-    for (int j = 0; j < p.top_k; ++j) {
-        uint64_t best = 0;
-        int at = 0;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (key[i] > best) best = key[i], at = i;
-        const uint64_t top = warp_max_key(best);
-        if (top == 0) break;
-        const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
-        const int e = __shfl_sync(0xffffffffu, e0 + at, src);
-        my_expert = lane == j ? e : my_expert;
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = lane == src && i == at ? 0ull : key[i];
-    }
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 GI8_DEVICE float route_load(const float* p) { return __ldg(p); }
@@ -307,50 +207,295 @@ GI8_DEVICE void route_load_lane(const T* row, int e0, int E, bool vec, float (&l
     for (int i = 0; i < V; ++i) l[i] = e0 + i < E ? route_load(row + e0 + i) : -INFINITY;
 }
 
+// The groups that are kept, in fp64 (groups of whole lanes).
+template <int V>
+GI8_DEVICE uint32_t route_groups_exact(const RouteParams& p, const float (&l)[V], const float (&bias)[V])
+{
+    const bool softmax = !p.sigmoid, scores = p.bias || p.group_top2;
+    double m = 0.0, z = 1.0;
+    if (softmax && scores) route_denominator(l, m, z);
+    double of_group[V], first, second;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        double v = static_cast<double>(l[i]);
+        if (scores) {
+            const double x = exp(softmax ? v - m : -v);
+            v = softmax ? x / z : 1.0 / (1.0 + x);
+        }
+        if (p.bias) v += static_cast<double>(bias[i]);
+        of_group[i] = l[i] > -INFINITY && v > -INFINITY ? v : -INFINITY;
+    }
+    const int group_here = route_group_best(p, of_group, static_cast<double*>(nullptr), first, second);
+    uint64_t key = group_here >= 0 ? route_key(p.group_top2 && second > -INFINITY ? first + second : first) : 0ull;
+    uint32_t kept = 0;
+    for (int n = 0; n < p.top_groups; ++n) {
+        const uint64_t best = warp_max_key(key);
+        if (best == 0) break;
+        const int g = __shfl_sync(0xffffffffu, group_here, __ffs(__ballot_sync(0xffffffffu, key == best)) - 1);
+        kept |= 1u << g;
+        if (group_here == g) key = 0;
+    }
+    return kept;
+}
+
+// The candidates e of lanes 0 .. n - 1, put in descending order of their choices in fp64, the lower index first among equals.
 template <typename T, int V>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+GI8_DEVICE int route_order_exact(const RouteParams& p, const float (&l)[V], const T* row, int e, int n)
+{
+    const int lane = threadIdx.x & 31;
+    const bool softmax = !p.sigmoid;
+    double m = 0.0, z = 1.0;
+    if (softmax && p.bias) route_denominator(l, m, z);
+    double c = lane < n ? static_cast<double>(route_load(row + e)) : 0.0;
+    if (p.bias && lane < n) {
+        const double x = exp(softmax ? c - m : -c);
+        c = (softmax ? x / z : 1.0 / (1.0 + x)) + static_cast<double>(__ldg(p.bias + e));
+    }
+    int rank = 0;
+    for (int i = 0; i < n; ++i) {
+        const double ci = __shfl_sync(0xffffffffu, c, i);
+        const int ei = __shfl_sync(0xffffffffu, e, i);
+        rank += ci > c || (ci == c && ei < e);
+    }
+    int mine = -1;
+    for (int i = 0; i < n; ++i) {
+        const int r = __shfl_sync(0xffffffffu, rank, i), ei = __shfl_sync(0xffffffffu, e, i);
+        mine = r == lane ? ei : mine;
+    }
+    return mine;
+}
+
+// One token by fp32 keys; the expert of place j ends up in lane j, -1 for none.
+// l: this lane's logits (-inf behind E and for NaN).  exact: the keys' lost bits are zeros in all logits, and the choice is by logits.
+// Returns true where the candidates are more than there are lanes, or the groups' values too close and not to be had from lanes.
+template <typename T, int V>
+GI8_DEVICE bool route_fast(const RouteParams& p, const T* row, const float (&l)[V], const float (&bias)[V], bool exact, float* scratch, float row_max, float denominator, int& my_expert)
+{
+    constexpr uint32_t kPlace = V <= 1 ? 0u : V <= 2 ? 1u : V <= 4 ? 3u : V <= 8 ? 7u : V <= 16 ? 15u : 31u;
+    const int lane = threadIdx.x & 31;
+    const bool softmax = !p.sigmoid;
+    const bool scores_of_groups = p.groups > 1 && p.group_top2;
+    const bool by_scores = p.bias != nullptr;
+    bool close = false;
+    float c[V];
+    auto score = [&](float v) { return softmax ? __fdividef(expf(v - row_max), denominator) : approx_reciprocal(1.0f + __expf(-v)); };
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        c[i] = l[i];
+        if (by_scores) c[i] = l[i] > -INFINITY ? fmaxf(score(l[i]) + bias[i], -INFINITY) : -INFINITY;
+    }
+    if (p.groups > 1) {
+        float of_group[V], first, second;
+#pragma unroll
+        for (int i = 0; i < V; ++i) of_group[i] = scores_of_groups && !by_scores && l[i] > -INFINITY ? score(l[i]) : c[i];
+        const int group_here = route_group_best(p, of_group, scratch, first, second);
+        const float value = p.group_top2 && second > -INFINITY ? first + second : first;
+        uint32_t key = group_here >= 0 ? route_key(value) : 0u;
+        uint32_t kept = 0, last = 0;
+        for (int n = 0; n <= p.top_groups; ++n) {
+            const uint32_t best = warp_max_key(key);
+            if (best <= kRouteNone) break;
+            if (n == p.top_groups) {  // the best one that stays out
+                close = (by_scores || scores_of_groups) && route_unkey(last) - route_unkey(best) <= 2.0f * route_margin<V>(route_unkey(last), softmax);
+                break;
+            }
+            last = best;
+            const int g = __shfl_sync(0xffffffffu, group_here, __ffs(__ballot_sync(0xffffffffu, key == best)) - 1);
+            kept |= 1u << g;
+            if (group_here == g) key = 0;
+        }
+        if (close) {  // (the same in all lanes)
+            if (scratch) return true;
+            kept = route_groups_exact(p, l, bias);
+            close = false;
+        }
+        route_drop_groups(p, kept, group_here, !scratch, c);
+    }
+    uint32_t key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = (route_key(c[i]) & ~kPlace) | (kPlace - i);
+    route_sort(key);
+    uint32_t mine = 0;
+    int found = 0;
+    my_expert = -1;
+    // Takes the largest key that is left; false: nobody can be chosen any more.
+    auto take = [&]() {
+        const uint32_t top = warp_max_key(key[0]);
+        if (top <= kRouteNone) return false;
+        // the first lane that has this value, and the first place there
+        const int src = __ffs(__ballot_sync(0xffffffffu, (key[0] | kPlace) == (top | kPlace))) - 1;
+        const uint32_t taken = __shfl_sync(0xffffffffu, key[0], src);
+        mine = lane == found ? taken : mine;
+        my_expert = lane == found ? src * V + static_cast<int>(kPlace - (taken & kPlace)) : my_expert;
+        const bool next = lane == src;
+#pragma unroll
+        for (int i = 0; i + 1 < V; ++i) key[i] = next ? key[i + 1] : key[i];
+        key[V - 1] = next ? 0u : key[V - 1];
+        ++found;
+        return true;
+    };
+    for (int j = 0; j < p.top_k; ++j)
+        if (!take()) break;
+    if (!exact) {
+        // Neighbours in the order, the first one left out among them; what keys drop below a value is at most their lowest bits' worth of it.
+        auto bound = [&](float a, float b) {
+            const float lost = (kPlace + 1) * 1.1920929e-7f * fmaxf(fabsf(a), fabsf(b));
+            return by_scores ? route_margin<V>(a, softmax) + lost : lost;
+        };
+        const uint32_t left = warp_max_key(key[0]);
+        uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
+        if (lane == found - 1) after = left;
+        if (lane < found && after > kRouteNone) {
+            const float a = route_unkey(mine & ~kPlace), b = route_unkey(after & ~kPlace);
+            close = a - b <= bound(a, b);
+        }
+        if (__any_sync(0xffffffffu, close)) {
+            const float last = route_unkey(__shfl_sync(0xffffffffu, mine, found - 1) & ~kPlace);
+            while (true) {
+                const uint32_t top = warp_max_key(key[0]);
+                if (top <= kRouteNone) break;
+                const float b = route_unkey(top & ~kPlace);
+                if (last - b > bound(last, b)) break;
+                if (found == 32) return true;
+                take();
+            }
+            my_expert = route_order_exact(p, l, row, my_expert, found);
+        }
+    }
+    if (lane >= p.top_k) my_expert = -1;
+    return false;
+}
+
+// The same in fp64 from the start, for what is left: through shared memory (E values of the warp) and in loops, so that it costs the
+// others neither registers nor room for instructions.
+template <typename T, int V>
+GI8_DEVICE int route_exact(const RouteParams& p, const T* row, double* c)
+{
+    const int lane = threadIdx.x & 31;
+    const bool softmax = !p.sigmoid;
+    const bool scores_of_groups = p.groups > 1 && p.group_top2 && !p.bias;
+    double m = -INFINITY, z = 0.0;
+    if (softmax) {
+#pragma unroll 1
+        for (int e = lane; e < p.E; e += 32) m = fmax(m, static_cast<double>(route_load(row + e)));
+#pragma unroll 1
+        for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!(m > -INFINITY)) m = 0.0;
+#pragma unroll 1
+        for (int e = lane; e < p.E; e += 32) {
+            const float l = route_load(row + e);
+            if (l > -INFINITY) z += exp(static_cast<double>(l) - m);
+        }
+#pragma unroll 1
+        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    }
+    // Choices, or first the scores that the groups' values are sums of.
+    auto fill = [&](bool scores, bool bias) {
+        __syncwarp();
+#pragma unroll 1
+        for (int e = lane; e < p.E; e += 32) {
+            const double l = static_cast<double>(route_load(row + e));
+            double v = l;
+            if (scores) {
+                const double x = exp(softmax ? l - m : -l);
+                v = (softmax ? x : 1.0) / (softmax ? z : 1.0 + x);
+            }
+            if (bias) v += static_cast<double>(__ldg(p.bias + e));
+            c[e] = l > -INFINITY && v > -INFINITY ? v : -INFINITY;
+        }
+        __syncwarp();
+    };
+    const bool by_scores = p.bias != nullptr;
+    uint32_t kept = 0xffffffffu;
+    const int size = p.E / p.groups;
+    if (p.groups > 1) {
+        fill(by_scores || scores_of_groups, by_scores);
+        double first = -INFINITY, second = -INFINITY;
+        if (lane < p.groups)
+#pragma unroll 1
+            for (int i = 0; i < size; ++i) route_two(c[lane * size + i], first, second);
+        uint64_t key = route_key(p.group_top2 && second > -INFINITY ? first + second : first);
+        kept = 0;
+#pragma unroll 1
+        for (int n = 0; n < p.top_groups; ++n) {
+            const uint64_t best = warp_max_key(key);
+            if (best == 0) break;
+            const int g = __ffs(__ballot_sync(0xffffffffu, key == best)) - 1;
+            kept |= 1u << g;
+            if (lane == g) key = 0;
+        }
+    }
+    if (p.groups == 1 || (scores_of_groups && !by_scores)) fill(by_scores, by_scores);
+    int my_expert = -1;
+#pragma unroll 1
+    for (int j = 0; j < p.top_k; ++j) {
+        uint64_t best = 0;
+        int at = 0;
+#pragma unroll 1
+        for (int e = lane * V; e < min((lane + 1) * V, p.E); ++e) {
+            const uint64_t key = (kept >> (e / size)) & 1u ? route_key(c[e]) : 0ull;
+            if (key > best) best = key, at = e;
+        }
+        const uint64_t top = warp_max_key(best);
+        if (top == 0) break;
+        const int src = __ffs(__ballot_sync(0xffffffffu, best == top)) - 1;
+        const int e = __shfl_sync(0xffffffffu, at, src);
+        my_expert = lane == j ? e : my_expert;
+        if (lane == src) c[e] = -INFINITY;
+        __syncwarp();
+    }
+    return my_expert;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRouteWarps * 32, V <= 8 ? 7 : 3)
 route_experts_kernel(const RouteParams p, int use_scratch)
 {
-    extern __shared__ double route_scratch[];  // use_scratch: E values per warp
+    extern __shared__ double route_scratch[];  // E values per warp
     pdl_wait();
     if (threadIdx.x == 0) pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRouteWarps;
+    int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
     if (t >= p.T) return;
-    const T* row = static_cast<const T*>(p.logits) + t * p.E;
+    double* exact_c = route_scratch + warp * p.E;
+    float* scratch = use_scratch ? reinterpret_cast<float*>(exact_c) : nullptr;
+    const bool need_denominator = !p.sigmoid && (p.bias || !p.renormalize || (p.groups > 1 && p.group_top2));
+    const bool exact = sizeof(T) == 2 && !p.bias && !(p.groups > 1 && p.group_top2);
     float l[V], bias[V];
-    route_load_lane<T, V>(row, lane * V, p.E, p.vec, l);
     if (p.bias) route_load_lane<float, V>(p.bias, lane * V, p.E, p.vec_bias, bias);
+    for (; t < p.T; t += step) {
+        const T* row = static_cast<const T*>(p.logits) + t * p.E;
+        route_load_lane<T, V>(row, lane * V, p.E, p.vec, l);
 #pragma unroll
-    for (int i = 0; i < V; ++i) l[i] = fmaxf(l[i], -INFINITY);  // NaN is never chosen
+        for (int i = 0; i < V; ++i) l[i] = fmaxf(l[i], -INFINITY);  // NaN is never chosen
 
-    int expert;
-    float row_max = 0.0f, denominator = 1.0f;
-    if (!p.sigmoid && (p.bias || !p.renormalize || (p.groups > 1 && p.group_top2))) route_denominator(l, row_max, denominator);
-    double* mine = use_scratch ? route_scratch + static_cast<int64_t>(warp) * p.E : nullptr;
-    if (route_fast<V>(p, l, bias, sizeof(T) == 2 && !p.bias && !(p.groups > 1 && p.group_top2), reinterpret_cast<float*>(mine), row_max, denominator, expert))
-        route_exact<V>(p, l, mine, expert);
+        int expert;
+        float row_max = 0.0f, denominator = 1.0f;
+        if (need_denominator) route_denominator(l, row_max, denominator);
+        if (route_fast<T, V>(p, row, l, bias, exact, scratch, row_max, denominator, expert)) expert = route_exact<T, V>(p, row, exact_c);
 
-    // Weights, lane j those of place j.  Their ratios do not depend on the softmax's denominator, nor on the sigmoid's where it is
-    // all but exp(l): renormalised weights are taken relative to the largest logit chosen, so that they never are 0 / 0.
-    const bool chosen = expert >= 0;
-    const float v = chosen ? route_load(row + expert) : -INFINITY;
-    float top = v;
-    for (int o = p.half_k; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float w = 0.0f;
-    if (chosen) {
-        if (!p.sigmoid) w = p.renormalize ? expf(v - top) : expf(v - row_max) / denominator;
-        else if (p.renormalize && top < -80.0f) w = expf(v - top);
-        else w = 1.0f / (1.0f + expf(-v));
-    }
-    if (p.renormalize) {
-        float sum = w;
-        for (int o = p.half_k; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (chosen) w /= sum;
-    }
-    if (lane < p.top_k) {
-        p.weights[t * p.top_k + lane] = w * p.scale;
-        p.experts[t * p.top_k + lane] = expert;
+        // Weights, lane j those of place j.  Their ratios do not depend on the softmax's denominator, nor on the sigmoid's where it is
+        // all but exp(l): renormalised weights are taken relative to the largest logit chosen, so that they never are 0 / 0.
+        const bool chosen = expert >= 0;
+        const float v = chosen ? route_load(row + expert) : -INFINITY;
+        float top = v;
+        for (int o = p.half_k; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float w = 0.0f;
+        if (chosen) {
+            if (!p.sigmoid) w = p.renormalize ? expf(v - top) : __fdividef(expf(v - row_max), denominator);
+            else if (p.renormalize && top < -80.0f) w = expf(v - top);
+            else w = __fdividef(1.0f, 1.0f + expf(-v));
+        }
+        if (p.renormalize) {
+            float sum = w;
+            for (int o = p.half_k; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (chosen) w = __fdividef(w, sum);
+        }
+        if (lane < p.top_k) {
+            p.weights[t * p.top_k + lane] = w * p.scale;
+            p.experts[t * p.top_k + lane] = expert;
+        }
     }
 }
 
