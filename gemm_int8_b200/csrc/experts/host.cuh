@@ -80,16 +80,20 @@ int make_gate_up_map(CUtensorMap* map, const int8_t* w, int64_t E, int64_t N, in
     return GI8_OK;
 }
 
-template <int WARPS, int LOADS>
+template <int WARPS, int LOADS, GroupStep STEP>
 int launch_group(GroupParams p, int ctas, int slot, cudaStream_t s)
 {
-    auto kernel = group_by_expert_kernel<WARPS, LOADS>;
+    auto kernel = group_by_expert_kernel<WARPS, LOADS, STEP>;
     auto smem = [](int64_t E) { return static_cast<size_t>((WARPS + 3) * E + WARPS * 32 * LOADS) * 4; };
     static_assert((WARPS + 3) * kGroupMaxExperts * 4 + WARPS * 32 * LOADS * 4 <= 227 * 1024 - 1024, "fits shared memory at the most experts");
     if (int rc = experts_smem(slot, kernel, smem(kGroupMaxExperts))) return rc;
     p.per_warp = static_cast<int>((p.S + static_cast<int64_t>(ctas) * WARPS * 32 - 1) / (ctas * WARPS * 32)) * 32;
-    return launch(kernel, dim3(ctas), WARPS * 32, smem(p.E), s, dim3(ctas), knobs().pdl, p, ctas);
+    return launch(kernel, dim3(ctas), WARPS * 32, smem(p.E), s, dim3(1), knobs().pdl, p);
 }
+
+// CTAs of a grouping: 1 up to 8192 pairs; of 2048 pairs up to 262144, of 16384 above.
+constexpr int64_t kGroupMaxPairs = int64_t(1) << 24;
+int group_ctas(int64_t S) { return S <= 8192 ? 1 : static_cast<int>(S <= 262144 ? (S + 2047) / 2048 : (S + 16383) / 16384); }
 
 template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
 int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, ExpertsParams p, cudaStream_t s)
@@ -170,24 +174,43 @@ int gi8_route_experts(const void* logits, int logits_dtype, const float* bias, f
     return logits_dtype == 0 ? launch_route_for<float>(p, st->sm_count, s) : launch_route_for<__nv_bfloat16>(p, st->sm_count, s);
 }
 
-int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t first, int32_t* offsets, int32_t* slots, int32_t* places, void* stream)
+int64_t gi8_group_by_expert_workspace_bytes(int64_t S, int64_t E)
 {
-    if (S < 0 || S > (int64_t(1) << 28)) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "S=%lld must be in [0, 2^28]", (long long)S);
+    if (S <= 0 || S > kGroupMaxPairs || E <= 0 || E > kGroupMaxExperts) return 0;
+    const int ctas = group_ctas(S);
+    return ctas > 1 ? 4 * E * ctas : 0;
+}
+
+int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t first, int32_t* offsets, int32_t* slots, int32_t* places, void* workspace,
+                        int64_t workspace_bytes, void* stream)
+{
+    if (S < 0 || S > kGroupMaxPairs) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "S=%lld must be in [0, 2^24]", (long long)S);
     if (E < 1 || E > kGroupMaxExperts) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts: 1 to %d are supported", (long long)E, kGroupMaxExperts);
     if (first < 0 || first > INT32_MAX - E) return fail(GI8_ERR_INVALID_ARGUMENT, "first expert %lld out of range", (long long)first);
     if (!offsets || (S > 0 && (!experts || !slots || !places))) return fail(GI8_ERR_INVALID_ARGUMENT, "null pointer");
     if (misaligned(experts, 4) || misaligned(offsets, 4) || misaligned(slots, 4) || misaligned(places, 4))
         return fail(GI8_ERR_MISALIGNED, "a pointer is not 4-byte aligned");
+    const int64_t needed = gi8_group_by_expert_workspace_bytes(S, E);
+    if (needed > 0 && (!workspace || workspace_bytes < needed))
+        return fail(GI8_ERR_WORKSPACE, "grouping %lld pairs needs %lld bytes of workspace, got %lld", (long long)S, (long long)needed, (long long)workspace_bytes);
+    if (misaligned(workspace, 4)) return fail(GI8_ERR_MISALIGNED, "workspace must be 4-byte aligned");
     DeviceState* st;
     if (int rc = get_device_state(&st)) return rc;
     GroupParams p{};
     p.experts = experts, p.offsets = offsets, p.slots = slots, p.places = places;
     p.S = (int)S, p.E = (int)E, p.first = (int)first;
+    while ((E >> p.bits) != 0) ++p.bits;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // Up to 2048 pairs in one CTA of eight warps, up to 131072 in runs that registers hold, more in longer runs.
-    if (S <= 2048) return launch_group<8, 8>(p, 1, 8, s);
-    if (S <= 8 * 32 * 32 * 16) return launch_group<32, 16>(p, S <= 16384 ? 1 : S <= 32768 ? 2 : S <= 65536 ? 4 : 8, 9, s);
-    return launch_group<32, 0>(p, 8, 10, s);
+    p.counts = static_cast<int32_t*>(workspace);
+    const int ctas = group_ctas(S);
+    if (S <= 2048) return launch_group<8, 8, GROUP_ALL>(p, 1, 8, s);
+    if (S <= 8192) return launch_group<32, 8, GROUP_ALL>(p, 1, 9, s);
+    if (S <= 262144) {
+        if (int rc = launch_group<16, 4, GROUP_COUNT>(p, ctas, 10, s)) return rc;
+        return launch_group<16, 4, GROUP_PLACE>(p, ctas, 11, s);
+    }
+    if (int rc = launch_group<32, 16, GROUP_COUNT>(p, ctas, 12, s)) return rc;
+    return launch_group<32, 16, GROUP_PLACE>(p, ctas, 13, s);
 }
 
 int64_t gi8_matmul_experts_workspace_bytes(int64_t rows, int64_t tokens, int64_t E, int64_t K)
@@ -272,7 +295,7 @@ int gi8_combine_experts(const void* y, const float* weights, const int32_t* plac
 namespace {
 
 struct ExpertsScratch {
-    int64_t weights, experts, offsets, slots, places, x_q, x_scale, rows, h, h_q, h_scale, y, bytes;
+    int64_t weights, experts, offsets, slots, places, counts, x_q, x_scale, rows, h, h_q, h_scale, y, bytes;
 };
 
 ExpertsScratch experts_scratch(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k)
@@ -285,6 +308,7 @@ ExpertsScratch experts_scratch(int64_t T, int64_t H, int64_t I, int64_t E, int64
         return at;
     };
     s.weights = take(4 * S), s.experts = take(4 * S), s.offsets = take(4 * (E + 1)), s.slots = take(4 * S), s.places = take(4 * S);
+    s.counts = take(gi8_group_by_expert_workspace_bytes(S, E));
     s.x_q = take(T * H), s.x_scale = take(4 * T);
     s.rows = take(gi8_matmul_experts_workspace_bytes(S, T, E, H));
     s.h = take(2 * S * I), s.h_q = take(S * I), s.h_scale = take(4 * S);
@@ -312,7 +336,7 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
     if (int rc = gi8_route_experts(logits, logits_dtype, bias, nullptr, nullptr, 0, E_router, top_k, sigmoid, groups, top_groups, group_top2, renormalize,
                                    scale, stream))
         return rc;
-    if (T < 0 || T > INT32_MAX || T * top_k > (int64_t(1) << 28)) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "T=%lld with top_k=%lld is out of range", (long long)T, (long long)top_k);
+    if (T < 0 || T > INT32_MAX || T * top_k > kGroupMaxPairs) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "T=%lld with top_k=%lld is out of range", (long long)T, (long long)top_k);
     if (E < 1 || first < 0 || first + E > E_router)
         return fail(GI8_ERR_INVALID_ARGUMENT, "experts %lld .. %lld of a router over %lld", (long long)first, (long long)(first + E - 1), (long long)E_router);
     if (H < 1 || I < 1 || H % 16 || I % 16) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "hidden size %lld and inner size %lld must be positive multiples of 16", (long long)H, (long long)I);
@@ -334,7 +358,7 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
     if (int rc = gi8_route_experts(logits, logits_dtype, bias, f32(m.weights), i32(m.experts), T, E_router, top_k, sigmoid, groups, top_groups, group_top2, renormalize,
                                    scale, stream))
         return rc;
-    if (int rc = gi8_group_by_expert(i32(m.experts), S, E, first, i32(m.offsets), i32(m.slots), i32(m.places), stream)) return rc;
+    if (int rc = gi8_group_by_expert(i32(m.experts), S, E, first, i32(m.offsets), i32(m.slots), i32(m.places), b + m.counts, m.x_q - m.counts, stream)) return rc;
     if (int rc = gi8_quantize_token(x, x_dtype, i8(m.x_q), f32(m.x_scale), T, H, stream)) return rc;
     if (int rc = gi8_matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, b + m.rows, m.h - m.rows, stream)) return rc;
     if (int rc = gi8_quantize_token(b + m.h, 1, i8(m.h_q), f32(m.h_scale), S, I, stream)) return rc;

@@ -235,9 +235,11 @@ int gi8_route_experts(const void* logits, int logits_dtype, const float* bias, f
  *   offsets int32 [E+1]  rows [offsets[e], offsets[e+1]) belong to expert first + e
  *   slots   int32 [S]    the pair (token * top_k + choice) of each row, ascending within an expert; -1 behind offsets[E]
  *   places  int32 [S]    the row of each pair; -1 where its expert is not held here
- * E <= 1024, S <= 2^28.
+ * E <= 1024, S <= 2^24.  workspace: gi8_group_by_expert_workspace_bytes bytes (0 up to 8192 pairs, NULL then), 4-byte aligned, of any contents.
  */
-int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t first, int32_t* offsets, int32_t* slots, int32_t* places, void* stream);
+int64_t gi8_group_by_expert_workspace_bytes(int64_t S, int64_t E);
+int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t first, int32_t* offsets, int32_t* slots, int32_t* places, void* workspace,
+                        int64_t workspace_bytes, void* stream);
 
 /*
  * out[p,n] = bf16( fp32(sum_k x[src(p),k] * w[e,n,k]) * (sx[src(p)] * sw[e,n]) ) for offsets[e] <= p < offsets[e+1]: gi8_matmul_scaled with a
@@ -270,7 +272,7 @@ int gi8_combine_experts(const void* y, const float* weights, const int32_t* plac
  *   gate_up  int8 [E,2I,H], gate_up_scale fp32 [E,2I];  down int8 [E,H,I], down_scale fp32 [E,H]: experts first .. first + E - 1 of the router's,
  *            the sum runs over those of a token's choices that are among them
  *   scratch  gi8_experts_scratch_bytes(T, H, I, E, top_k) bytes, 256-byte aligned, of any contents.  Two calls that may overlap need two.
- * H and I are multiples of 16; T * top_k <= 2^28.  Whatever a step refuses is refused before the first launch.
+ * H and I are multiples of 16; T * top_k <= 2^24.  Whatever a step refuses is refused before the first launch.
  */
 int64_t gi8_experts_scratch_bytes(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k);
 int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,

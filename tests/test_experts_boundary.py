@@ -29,7 +29,7 @@ def call():
             return C.gi8_route_experts(a(arg("logits", base)), arg("dtype", 0), a(arg("bias", None)), a(arg("weights", base)), a(arg("experts", base)), arg("T", 4), arg("E", 16),
                                        arg("k", 2), 0, arg("groups", 1), arg("top_groups", 1), 0, 1, 1.0, None)
         if name == "group":
-            return C.gi8_group_by_expert(a(arg("experts", base)), arg("S", 8), arg("E", 4), arg("first", 0), a(arg("offsets", base)), a(arg("slots", base)), a(arg("places", base)), None)
+            return C.gi8_group_by_expert(a(arg("experts", base)), arg("S", 8), arg("E", 4), arg("first", 0), a(arg("offsets", base)), a(arg("slots", base)), a(arg("places", base)), a(arg("ws", None)), arg("ws_bytes", 0), None)
         if name == "product":
             return C.gi8_matmul_experts(a(arg("x", base)), a(arg("w", base)), a(arg("sx", base)), a(arg("sw", base)), a(arg("offsets", base)), a(arg("slots", None)), arg("k", 1),
                                         a(arg("out", base)), arg("rows", 8), arg("tokens", 8), arg("E", 2), arg("N", 16), arg("K", 32), arg("swiglu", 0), a(arg("ws", None)), arg("ws_bytes", 0), None)
@@ -56,9 +56,12 @@ def test_router_refuses(call):
 
 
 def test_grouping_refuses(call):
-    assert call("group", E=0) == 2 and call("group", E=1025) == 2 and call("group", S=-1) == 2 and call("group", S=(1 << 28) + 1) == 2
+    assert call("group", E=0) == 2 and call("group", E=1025) == 2 and call("group", S=-1) == 2 and call("group", S=(1 << 24) + 1) == 2
     assert call("group", first=-1) == 1 and call("group", first=2 ** 31 - 2) == 1
     assert call("group", offsets=None) == 1 and call("group", slots=None) == 1 and call("group", places=call.base + 2) == 3
+    need = call.C.gi8_group_by_expert_workspace_bytes(8193, 4)
+    assert need > 0 and call.C.gi8_group_by_expert_workspace_bytes(8192, 4) == 0
+    assert call("group", S=8193) == 6 and call("group", S=8193, ws=call.base, ws_bytes=need - 1) == 6 and call("group", S=8193, ws=call.base + 2, ws_bytes=need) == 3
 
 
 def test_product_refuses(call):

@@ -53,4 +53,6 @@ def test_one_expert_takes_all_and_none_takes_any(T):
 def test_large_and_strided():
     gen = torch.Generator().manual_seed(9)
     _check(torch.randint(0, 512, (70001, 9), dtype=torch.int32, generator=gen), 512)
+    _check(torch.randint(-1, 1024, (20001, 8), dtype=torch.int32, generator=gen), 1024)
+    _check(torch.randint(0, 3, (30000, 8), dtype=torch.int32, generator=gen), 3)
     _check(torch.randint(0, 16, (300, 16), dtype=torch.int32, generator=gen)[:, 3:9], 16)
