@@ -116,7 +116,8 @@ int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, 
     const int channels = (SWIGLU ? kBM / 2 : kBM) * (PAIR ? 2 : 1);
     const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
     const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
-    const int grid = static_cast<int>(std::min<int64_t>(tiles, st->sm_count / (PAIR ? 2 : 1))) * (PAIR ? 2 : 1);
+    const int64_t slots = BT <= 64 ? 2 * st->sm_count : PAIR ? st->sm_count / 2 : st->sm_count;
+    const int grid = static_cast<int>(std::min<int64_t>(tiles, slots)) * (PAIR ? 2 : 1);
     return launch(kernel, dim3(grid), experts_threads(SWIGLU), smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
 }
 
@@ -125,7 +126,7 @@ int experts_tile(int64_t rows, int64_t tokens, int64_t E, bool gathered)
 {
     const int64_t most = gathered ? tokens : rows;                  // rows of one expert, if no token names it twice
     const int64_t want = std::min(most, (3 * rows / 2 + E - 1) / E);  // half as many again as there are on average
-    return want <= 64 ? 64 : want <= 128 ? 128 : 256;
+    return want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 256;
 }
 
 // Gathered rows are put in order by a pass of their own in front of the product, except those of small tiles.
@@ -136,7 +137,8 @@ int dispatch_experts(DeviceState* st, const int8_t* x, const int8_t* w, const Ex
 {
     constexpr int slot = SWIGLU ? 4 : 0;
     switch (experts_tile(p.rows, p.tokens, p.E, gathered)) {
-        case 64: return launch_experts<64, 8, SWIGLU>(st, slot + 1, x, w, p, s);
+        case 32: return launch_experts<32, 5, SWIGLU>(st, slot, x, w, p, s);
+        case 64: return launch_experts<64, 4, SWIGLU>(st, slot + 1, x, w, p, s);
         case 128: return launch_experts<128, 6, SWIGLU>(st, slot + 2, x, w, p, s);
         default: return launch_experts<256, 6, SWIGLU, true>(st, slot + 3, x, w, p, s);
     }
@@ -219,9 +221,10 @@ int64_t gi8_matmul_experts_workspace_bytes(int64_t rows, int64_t tokens, int64_t
     return experts_gather_first(rows, tokens, E) ? rows * K : 0;
 }
 
-int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
-                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* workspace,
-                       int64_t workspace_bytes, void* stream)
+// early: the launch in front writes neither w nor offsets, and what does had ended when it let this one start (the quantiser of a layer).
+static int matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
+                          int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* workspace,
+                          int64_t workspace_bytes, void* stream, bool early)
 {
     if (E < 1 || E > kExpertsMaxExperts) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts: 1 to %d are supported", (long long)E, kExpertsMaxExperts);
     if (rows < 0 || tokens < 0 || N < 0) return fail(GI8_ERR_INVALID_ARGUMENT, "negative dimension");
@@ -260,7 +263,15 @@ int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const 
         p.in_order = 1;
     }
     p.rows_x = (int)(p.in_order ? rows : tokens);
+    p.early = early && !p.in_order && knobs().pdl;
     return swiglu ? dispatch_experts<true>(st, x, w, p, gathered, s) : dispatch_experts<false>(st, x, w, p, gathered, s);
+}
+
+int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
+                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* workspace,
+                       int64_t workspace_bytes, void* stream)
+{
+    return matmul_experts(x, w, sx, sw, offsets, slots, top_k, out, rows, tokens, E, N, K, swiglu, workspace, workspace_bytes, stream, false);
 }
 
 int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
@@ -360,9 +371,9 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
         return rc;
     if (int rc = gi8_group_by_expert(i32(m.experts), S, E, first, i32(m.offsets), i32(m.slots), i32(m.places), b + m.counts, m.x_q - m.counts, stream)) return rc;
     if (int rc = gi8_quantize_token(x, x_dtype, i8(m.x_q), f32(m.x_scale), T, H, stream)) return rc;
-    if (int rc = gi8_matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, b + m.rows, m.h - m.rows, stream)) return rc;
+    if (int rc = matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, b + m.rows, m.h - m.rows, stream, true)) return rc;
     if (int rc = gi8_quantize_token(b + m.h, 1, i8(m.h_q), f32(m.h_scale), S, I, stream)) return rc;
-    if (int rc = gi8_matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, nullptr, 0, stream)) return rc;
+    if (int rc = matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, nullptr, 0, stream, true)) return rc;
     return gi8_combine_experts(b + m.y, f32(m.weights), i32(m.places), add, out, T, top_k, S, H, stream);
 }
 

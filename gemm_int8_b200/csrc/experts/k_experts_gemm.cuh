@@ -43,6 +43,7 @@ struct ExpertsParams {
     int top_k;
     int vec_zero;            // rows behind the last group can be cleared in 16-byte pieces
     int interleave;          // SWIGLU: the weight's map is over runs of 16 rows and loads a whole tile (N a multiple of 16)
+    int early;               // the kernel in front writes neither weights nor offsets: the first weights are requested while it runs
     int weight_policy_first; // weights are met once or twice: keep them from displacing the rest of L2
 };
 
@@ -72,6 +73,7 @@ template <int BT>
 struct ExpertList {
     int32_t start[kExpertsMaxExperts + 1];
     int32_t tiles_end[kExpertsMaxExperts];
+    int32_t chunk_tiles[kExpertsMaxExperts / 32];
 };
 
 // Whole CTA.  Offsets that are no ascending sequence within [0, rows] give wrong rows, never an access out of bounds.
@@ -81,50 +83,55 @@ GI8_DEVICE void build_expert_list(ExpertList<BT>& list, const int32_t* offsets, 
     for (int e = threadIdx.x; e <= E; e += blockDim.x)
         list.start[e] = static_cast<int32_t>(min(max(static_cast<int64_t>(__ldg(offsets + e)), static_cast<int64_t>(0)), rows));
     __syncthreads();
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        int carry = 0;
-        for (int base = 0; base < E; base += 32) {
-            const int e = base + lane;
-            int n = e < E ? max(0, list.start[e + 1] - list.start[e]) : 0;
-            n = (n + BT - 1) / BT;
+    // sums within chunks of 32 experts, a warp each, then what lies in front of a chunk
+    const int lane = threadIdx.x & 31, warps = blockDim.x / 32, chunks = (E + 31) / 32;
+    for (int c = threadIdx.x >> 5; c < chunks; c += warps) {
+        const int e = c * 32 + lane;
+        int n = e < E ? max(0, list.start[e + 1] - list.start[e]) : 0;
+        n = (n + BT - 1) / BT;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, n, o);
-                if (lane >= o) n += v;
-            }
-            if (e < E) list.tiles_end[e] = carry + n;
-            carry += __shfl_sync(0xffffffffu, n, 31);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, n, o);
+            if (lane >= o) n += v;
         }
+        if (e < E) list.tiles_end[e] = n;
+        if (lane == 31) list.chunk_tiles[c] = n;
+    }
+    __syncthreads();
+    if (chunks == 1) return;
+    for (int c = threadIdx.x >> 5; c < chunks; c += warps) {
+        const int before = __reduce_add_sync(0xffffffffu, lane < c ? list.chunk_tiles[lane] : 0);
+        if (c * 32 + lane < E) list.tiles_end[c * 32 + lane] += before;
     }
     __syncthreads();
 }
 
 // Tile `item` of the list, if there is one: experts in order, within an expert weight tile by weight tile with the token tiles inside,
-// so that CTAs that run at the same time share weights.  Whole warp; `chunk` is the 32 experts where the last search ended.
+// so that CTAs that run at the same time share weights.  Whole warp: the chunk of 32 experts that it lies in, then the expert.
 template <int BT, int ALIGN>
-GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_tiles, int64_t item, int& chunk, ExpertTile& t)
+GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_tiles, int64_t item, ExpertTile& t)
 {
     const int lane = threadIdx.x & 31;
-    for (; chunk < E; chunk += 32) {
-        const int e = chunk + lane;
-        const bool past = e < E && static_cast<int64_t>(list.tiles_end[e]) * weight_tiles > item;
-        const uint32_t hit = __ballot_sync(0xffffffffu, past);
-        if (hit) {
-            t.expert = chunk + __ffs(hit) - 1;
-            const int before = t.expert ? list.tiles_end[t.expert - 1] : 0;
-            const int tiles = list.tiles_end[t.expert] - before;
-            const int r = static_cast<int>(item - static_cast<int64_t>(before) * weight_tiles);
-            t.weight_tile = r / tiles;
-            const int n = list.start[t.expert + 1] - list.start[t.expert];
-            const int per = ((n + tiles - 1) / tiles + ALIGN - 1) & ~(ALIGN - 1);  // <= BT, and the last tile keeps at least a row
-            const int first = (r - t.weight_tile * tiles) * per;
-            t.row0 = list.start[t.expert] + first;
-            t.rows = min(per, n - first);
-            return true;
-        }
+    auto past = [&](int e) { return e < E && static_cast<int64_t>(list.tiles_end[e]) * weight_tiles > item; };
+    int chunk = 0;
+    if (E > 32) {
+        const uint32_t hit = __ballot_sync(0xffffffffu, lane * 32 < E && past(min(lane * 32 + 31, E - 1)));
+        if (!hit) return false;
+        chunk = __ffs(hit) - 1;
     }
-    return false;
+    const uint32_t hit = __ballot_sync(0xffffffffu, past(chunk * 32 + lane));
+    if (!hit) return false;
+    t.expert = chunk * 32 + __ffs(hit) - 1;
+    const int before = t.expert ? list.tiles_end[t.expert - 1] : 0;
+    const int tiles = list.tiles_end[t.expert] - before;
+    const int r = static_cast<int>(item - static_cast<int64_t>(before) * weight_tiles);
+    t.weight_tile = r / tiles;
+    const int n = list.start[t.expert + 1] - list.start[t.expert];
+    const int per = ((n + tiles - 1) / tiles + ALIGN - 1) & ~(ALIGN - 1);  // <= BT, and the last tile keeps at least a row
+    const int first = (r - t.weight_tile * tiles) * per;
+    t.row0 = list.start[t.expert] + first;
+    t.rows = min(per, n - first);
+    return true;
 }
 
 // Tile loads whose bytes are counted on the barrier at cluster address `bar` (the leader's) or on one of this CTA.
@@ -142,10 +149,10 @@ GI8_DEVICE void load_tile_5d(void* dst, const CUtensorMap* map, uint32_t bar, in
 }
 
 template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
-__global__ void __launch_bounds__(experts_threads(SWIGLU), 1)
+__global__ void __launch_bounds__(experts_threads(SWIGLU), BT <= 64 ? 2 : 1)
 experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const ExpertsParams p)
 {
-    static_assert(BT == 64 || BT == 128 || BT == 256, "quarters of a tile are columns of an MMA, of which there are at most 256");
+    static_assert(BT == 32 || BT == 64 || BT == 128 || BT == 256, "at most 256 columns of an MMA, boxes of a quarter of the rows");
     constexpr uint32_t kBytesW = kBM * kBK;
     constexpr int kRowsX = PAIR ? BT / 2 : BT;  // token rows that this CTA loads
     constexpr int kAlign = PAIR ? 32 : 16;      // what the columns of an MMA are a multiple of
@@ -206,8 +213,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if constexpr (PAIR) cluster_sync_all();  // both CTAs' barriers exist before anything signals them remotely
     tcgen05_fence_after_sync();
     const uint32_t tmem_base = tmem_base_slot;
-    pdl_wait();
-    if (threadIdx.x == 0) pdl_launch_dependents();
+    if (!p.early) pdl_wait();
     build_expert_list(list, p.offsets, p.E, p.rows);
 
     if (warp == 0) {
@@ -215,14 +221,42 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         uint32_t s = 0, ph = 0;
         uint32_t armed = 0;
         bool ok = true;
-        int chunk = 0;
         ExpertTile t;
         const uint64_t pol_x = l2_policy_evict_normal();
         const uint64_t pol_w = p.weight_policy_first ? l2_policy_evict_first() : pol_x;
-        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, chunk, t); item += item_step) {
+        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step) {
             const int cols = ((t.rows + kAlign - 1) & ~(kAlign - 1)) / (PAIR ? 2 : 1);  // of this CTA
             if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank), t.row0 += static_cast<int>(rank) * cols;
-            if (!PAIR && p.slots && !p.in_order) {
+            const bool gather = !PAIR && p.slots && !p.in_order;
+            const int box = (cols - 1) / (kRowsX / 4);  // the smallest one that holds the tile
+            const uint32_t bytes = kBytesW + (gather ? cols : (box + 1) * (kRowsX / 4)) * kBK;
+            const int w_row = t.weight_tile * kChannels;
+            // (one lane) PAIR: the leader arms its barrier for the bytes of both CTAs, the peer only sends bytes
+            auto load_weights = [&](int stage, int kb) {
+                const uint32_t full = PAIR ? map_to_cta(smem_u32(&bar_full[stage]), 0) : smem_u32(&bar_full[stage]);
+                uint8_t* dst = smem + stage * kStageBytes;
+                if (rank == 0) mbar_arrive_expect_tx(&bar_full[stage], PAIR ? 2 * bytes : bytes);
+                if constexpr (!SWIGLU) {
+                    load_tile_2d<PAIR>(dst, &map_w, full, kb * kBK, t.expert * rows_w + w_row, pol_w);
+                } else if (p.interleave) {
+                    load_tile_5d<PAIR>(dst, &map_w, full, kb * kBK, 0, 0, w_row / 16, t.expert, pol_w);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        load_tile_2d<PAIR>(dst + i * 16 * kBK, &map_w, full, kb * kBK, t.expert * rows_w + w_row + (i >> 1) * 16 + (i & 1) * p.N, pol_w);
+                }
+            };
+            // The weights of the first tile's first K blocks need nothing but its place in the list.
+            int ahead = 0;
+            if (item == first_item) {
+                ahead = min(num_kb, STAGES);
+                if (elect_one())
+                    for (int kb = 0; kb < ahead; ++kb) load_weights(kb, kb);
+                __syncwarp();
+                if (p.early) pdl_wait();
+                if (lane == 0) pdl_launch_dependents();
+            }
+            if (gather) {
                 __syncwarp();
                 for (int r = lane; r < cols; r += 32) {  // rows that pad the tile read token 0, and are not stored
                     const int slot = r < t.rows ? __ldg(p.slots + t.row0 + r) : 0;
@@ -230,38 +264,35 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 }
                 __syncwarp();
             }
-            const int box = (cols - 1) / (kRowsX / 4);  // the smallest one that holds the tile
-            const uint32_t bytes = kBytesW + (!PAIR && p.slots && !p.in_order ? cols : (box + 1) * (kRowsX / 4)) * kBK;
-            const int w_row = t.weight_tile * kChannels;
-            for (int kb = 0; kb < num_kb; ++kb) {
+            auto load_tokens = [&](int stage, int kb) {  // (one lane)
+                const uint32_t full = PAIR ? map_to_cta(smem_u32(&bar_full[stage]), 0) : smem_u32(&bar_full[stage]);
+                uint8_t* dst = smem + stage * kStageBytes + kBytesW;
+                if (gather) {
+#pragma unroll 4
+                    for (int r = 0; r < cols; r += 4) {
+                        const int4 q = *reinterpret_cast<const int4*>(&gather_rows[r]);
+                        tma_gather4(dst + r * kBK, &map_x.m[0], &bar_full[stage], kb * kBK, q.x, q.y, q.z, q.w);
+                    }
+                } else {
+                    load_tile_2d<PAIR>(dst, &map_x.m[box], full, kb * kBK, t.row0, pol_x);
+                }
+            };
+            if (ahead > 0) {
+                if (elect_one())
+                    for (int kb = 0; kb < ahead; ++kb) load_tokens(kb, kb);
+                __syncwarp();
+                armed = ahead;
+                if (ahead == STAGES) s = 0, ph ^= 1;
+                else s = ahead;
+            }
+            for (int kb = ahead; kb < num_kb; ++kb) {
                 if (!warp_agrees(wait_or_abort(&bar_empty[s], ph ^ 1, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_PRODUCER)) {
                     ok = false;
                     break;
                 }
-                uint8_t* sw_tile = smem + s * kStageBytes;
-                uint8_t* sx_tile = sw_tile + kBytesW;
                 if (elect_one()) {
-                    // PAIR: the leader arms its barrier for the bytes of both CTAs, the peer only sends bytes
-                    const uint32_t full = PAIR ? map_to_cta(smem_u32(&bar_full[s]), 0) : smem_u32(&bar_full[s]);
-                    if (rank == 0) mbar_arrive_expect_tx(&bar_full[s], PAIR ? 2 * bytes : bytes);
-                    if constexpr (!SWIGLU) {
-                        load_tile_2d<PAIR>(sw_tile, &map_w, full, kb * kBK, t.expert * rows_w + w_row, pol_w);
-                    } else if (p.interleave) {
-                        load_tile_5d<PAIR>(sw_tile, &map_w, full, kb * kBK, 0, 0, w_row / 16, t.expert, pol_w);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            load_tile_2d<PAIR>(sw_tile + i * 16 * kBK, &map_w, full, kb * kBK, t.expert * rows_w + w_row + (i >> 1) * 16 + (i & 1) * p.N, pol_w);
-                    }
-                    if (!PAIR && p.slots && !p.in_order) {
-#pragma unroll 4
-                        for (int r = 0; r < cols; r += 4) {
-                            const int4 q = *reinterpret_cast<const int4*>(&gather_rows[r]);
-                            tma_gather4(sx_tile + r * kBK, &map_x.m[0], &bar_full[s], kb * kBK, q.x, q.y, q.z, q.w);
-                        }
-                    } else {
-                        load_tile_2d<PAIR>(sx_tile, &map_x.m[box], full, kb * kBK, t.row0, pol_x);
-                    }
+                    load_weights(s, kb);
+                    load_tokens(s, kb);
                 }
                 __syncwarp();
                 if (armed < STAGES) ++armed;
@@ -275,10 +306,9 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         uint32_t s = 0, ph = 0;
         uint32_t local_tile = 0;
         bool ok = rank == 0;
-        int chunk = 0;
         ExpertTile t;
         const uint32_t w_0 = smem_desc_lo(smem_u32(smem));
-        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, chunk, t); item += item_step, ++local_tile) {
+        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step, ++local_tile) {
             const uint32_t buf = local_tile & 1;
             const uint32_t acc_ph = (local_tile >> 1) & 1;
             if (!warp_agrees(wait_or_abort(&bar_acc_empty[buf], acc_ph ^ 1, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_MMA)) break;
@@ -322,6 +352,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         // ------------------------------------------------------------------ epilogue warps
         const int quarter = warp & 3;  // TMEM lanes [32 * quarter, 32 * quarter + 32)
         const int et = static_cast<int>(threadIdx.x) - 64;
+        if (p.early) pdl_wait();
         {
             // rows that belong to no expert
             const int64_t first = static_cast<int64_t>(list.start[p.E]) * p.N, end = p.rows * p.N;
@@ -334,9 +365,8 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         }
         uint32_t local_tile = 0;
         bool ok = true;
-        int chunk = 0;
         ExpertTile t;
-        for (int64_t item = first_item; find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, chunk, t); item += item_step, ++local_tile) {
+        for (int64_t item = first_item; find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step, ++local_tile) {
             const uint32_t buf = local_tile & 1;
             const uint32_t acc_ph = (local_tile >> 1) & 1;
             if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank);
