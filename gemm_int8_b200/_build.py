@@ -15,7 +15,7 @@ LIB_NAME = "libgemm_int8_b200.so"
 LIB_PATH = os.path.join(_PKG, LIB_NAME)
 SOURCES = [os.path.join(_PKG, "csrc", "api.cu")]
 HEADERS = [os.path.join(_PKG, "csrc", f) for f in ("ptx.cuh", "k_dense.cuh", "k_dense_splitk.cuh", "k_blockwise.cuh", "k_blockwise_smallm.cuh", "k_smallm.cuh", "k_quant.cuh")]
-HEADERS += [os.path.join(_PKG, "csrc", "experts", f) for f in ("host.cuh", "k_route.cuh", "k_group.cuh", "k_gather.cuh", "k_experts_gemm.cuh", "k_combine.cuh")]
+HEADERS += [os.path.join(_PKG, "csrc", "experts", f) for f in ("host.cuh", "k_route.cuh", "k_group.cuh", "k_experts_gemm.cuh", "k_combine.cuh")]
 HEADERS.append(os.path.join(os.path.dirname(_PKG), "include", "gemm_int8_b200.h"))
 
 OPS_NAME = "libgemm_int8_b200_torch.so"

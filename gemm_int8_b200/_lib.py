@@ -51,8 +51,7 @@ SYMBOLS = {
     "gi8_route_experts": (_i, [_p, _i, _p, _p, _p, _i64, _i64, _i64, _i, _i64, _i64, _i, _i, _f, _p]),
     "gi8_group_by_expert_workspace_bytes": (_i64, [_i64, _i64]),
     "gi8_group_by_expert": (_i, [_p, _i64, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
-    "gi8_matmul_experts_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
-    "gi8_matmul_experts": (_i, [_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _p, _i64, _p]),
+    "gi8_matmul_experts": (_i, [_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i, _p]),
     "gi8_combine_experts": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
     "gi8_experts_scratch_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "gi8_experts": (_i, [_p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i64, _i64, _i, _i, _f, _p]),

@@ -4,7 +4,6 @@
 
 #include "k_combine.cuh"
 #include "k_experts_gemm.cuh"
-#include "k_gather.cuh"
 #include "k_group.cuh"
 #include "k_route.cuh"
 
@@ -95,12 +94,12 @@ int launch_group(GroupParams p, int ctas, int slot, cudaStream_t s)
 constexpr int64_t kGroupMaxPairs = int64_t(1) << 24;
 int group_ctas(int64_t S) { return S <= 8192 ? 1 : static_cast<int>(S <= 262144 ? (S + 2047) / 2048 : (S + 16383) / 16384); }
 
-template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
-int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, ExpertsParams p, cudaStream_t s)
+template <int BT, int STAGES, bool SWIGLU, bool PAIR, bool GATHER>
+int launch_experts(DeviceState* st, int slot, const int8_t* w, ExpertsParams p, cudaStream_t s)
 {
     constexpr int kRowsX = PAIR ? BT / 2 : BT;
     constexpr size_t smem = static_cast<size_t>(STAGES) * (kBM + kRowsX) * kBK + 1024;
-    auto kernel = experts_gemm_kernel<BT, STAGES, SWIGLU, PAIR>;
+    auto kernel = experts_gemm_kernel<BT, STAGES, SWIGLU, PAIR, GATHER>;
     if (int rc = experts_smem(slot, kernel, smem)) return rc;
     CUtensorMap mw;
     TokenMaps mx;
@@ -111,36 +110,35 @@ int launch_experts(DeviceState* st, int slot, const int8_t* x, const int8_t* w, 
     } else if (int rc = make_operand_map(&mw, w, rows_w, p.K, SWIGLU ? 16 : kBM)) {
         return rc;
     }
-    for (int i = 0; i < 4; ++i)
-        if (int rc = make_operand_map(&mx.m[i], x, p.rows_x, p.K, p.slots && !p.in_order ? 1 : (i + 1) * kRowsX / 4)) return rc;
+    for (int i = 0; i < 4; ++i) {
+        if (GATHER) mx.m[i] = mw;  // (unused by the kernel)
+        else if (int rc = make_operand_map(&mx.m[i], p.x, p.tokens, p.K, (i + 1) * kRowsX / 4)) return rc;
+    }
     const int channels = (SWIGLU ? kBM / 2 : kBM) * (PAIR ? 2 : 1);
     const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
     const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
     const int64_t slots = BT <= 64 ? 2 * st->sm_count : PAIR ? st->sm_count / 2 : st->sm_count;
     const int grid = static_cast<int>(std::min<int64_t>(tiles, slots)) * (PAIR ? 2 : 1);
-    return launch(kernel, dim3(grid), experts_threads(SWIGLU), smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
+    return launch(kernel, dim3(grid), experts_threads(SWIGLU, GATHER), smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
 }
 
-// Rows of a token tile.
-int experts_tile(int64_t rows, int64_t tokens, int64_t E, bool gathered)
+// Rows of a token tile: half as many again as an expert has on average, or all that it can have if no token names it twice.
+int experts_tile(const ExpertsParams& p)
 {
-    const int64_t most = gathered ? tokens : rows;                  // rows of one expert, if no token names it twice
-    const int64_t want = std::min(most, (3 * rows / 2 + E - 1) / E);  // half as many again as there are on average
+    const int64_t most = p.slots ? p.tokens : p.rows;
+    const int64_t want = std::min(most, (3 * p.rows / 2 + p.E - 1) / p.E);
     return want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 256;
 }
 
-// Gathered rows are put in order by a pass of their own in front of the product, except those of small tiles.
-bool experts_gather_first(int64_t rows, int64_t tokens, int64_t E) { return experts_tile(rows, tokens, E, true) > 64; }
-
-template <bool SWIGLU>
-int dispatch_experts(DeviceState* st, const int8_t* x, const int8_t* w, const ExpertsParams& p, bool gathered, cudaStream_t s)
+template <bool SWIGLU, bool GATHER>
+int dispatch_experts(DeviceState* st, const int8_t* w, const ExpertsParams& p, cudaStream_t s)
 {
-    constexpr int slot = SWIGLU ? 4 : 0;
-    switch (experts_tile(p.rows, p.tokens, p.E, gathered)) {
-        case 32: return launch_experts<32, 5, SWIGLU>(st, slot, x, w, p, s);
-        case 64: return launch_experts<64, 4, SWIGLU>(st, slot + 1, x, w, p, s);
-        case 128: return launch_experts<128, 6, SWIGLU>(st, slot + 2, x, w, p, s);
-        default: return launch_experts<256, 6, SWIGLU, true>(st, slot + 3, x, w, p, s);
+    constexpr int slot = (SWIGLU ? 4 : 0) + (GATHER ? 16 : 0);
+    switch (experts_tile(p)) {
+        case 32: return launch_experts<32, 5, SWIGLU, false, GATHER>(st, slot, w, p, s);
+        case 64: return launch_experts<64, 4, SWIGLU, false, GATHER>(st, slot + 1, w, p, s);
+        case 128: return launch_experts<128, 6, SWIGLU, false, GATHER>(st, slot + 2, w, p, s);
+        default: return launch_experts<256, 6, SWIGLU, true, GATHER>(st, slot + 3, w, p, s);
     }
 }
 
@@ -215,16 +213,10 @@ int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t fi
     return launch_group<32, 16, GROUP_PLACE>(p, ctas, 13, s);
 }
 
-int64_t gi8_matmul_experts_workspace_bytes(int64_t rows, int64_t tokens, int64_t E, int64_t K)
-{
-    if (rows <= 0 || tokens <= 0 || E <= 0 || K <= 0 || rows > INT32_MAX || K > kMaxK) return 0;
-    return experts_gather_first(rows, tokens, E) ? rows * K : 0;
-}
-
 // early: the launch in front writes neither w nor offsets, and what does had ended when it let this one start (the quantiser of a layer).
 static int matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
-                          int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* workspace,
-                          int64_t workspace_bytes, void* stream, bool early)
+                          int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* stream,
+                          bool early)
 {
     if (E < 1 || E > kExpertsMaxExperts) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts: 1 to %d are supported", (long long)E, kExpertsMaxExperts);
     if (rows < 0 || tokens < 0 || N < 0) return fail(GI8_ERR_INVALID_ARGUMENT, "negative dimension");
@@ -244,34 +236,21 @@ static int matmul_experts(const int8_t* x, const int8_t* w, const float* sx, con
     if (int rc = check_scale_pointers(sx, sw)) return rc;
     if (!offsets) return fail(GI8_ERR_INVALID_ARGUMENT, "null offsets");
     if (misaligned(offsets, 4) || misaligned(slots, 4)) return fail(GI8_ERR_MISALIGNED, "offsets and slots must be 4-byte aligned");
-    const int64_t needed = slots ? gi8_matmul_experts_workspace_bytes(rows, tokens, E, K) : 0;
-    if (needed > 0 && (!workspace || workspace_bytes < needed))
-        return fail(GI8_ERR_WORKSPACE, "the gathered product of this shape needs %lld bytes of workspace, got %lld", (long long)needed, (long long)workspace_bytes);
-    if (needed > 0 && misaligned(workspace, 16)) return fail(GI8_ERR_MISALIGNED, "workspace must be 16-byte aligned");
     if (int rc = get_device_state(&st)) return rc;
     ExpertsParams p{};
-    p.out = static_cast<uint16_t*>(out), p.sx = sx, p.sw = sw, p.offsets = offsets, p.slots = slots, p.status = st->status;
+    p.x = x, p.out = static_cast<uint16_t*>(out), p.sx = sx, p.sw = sw, p.offsets = offsets, p.slots = slots, p.status = st->status;
     p.rows = rows, p.tokens = (int)tokens, p.E = (int)E, p.N = (int)N, p.K = (int)K, p.top_k = (int)top_k;
     p.vec_zero = !misaligned(out, 16) && N % 8 == 0;
     p.weight_policy_first = rows <= 32 * E;
-    const bool gathered = slots != nullptr;
-    if (gathered && experts_gather_first(rows, tokens, E)) {
-        if (int rc = launch(gather_rows_kernel, dim3((unsigned)std::min<int64_t>((rows + 7) / 8, st->sm_count * 8)), kGatherThreads, 0, s, dim3(1), knobs().pdl,
-                            reinterpret_cast<const uint4*>(x), slots, offsets + E, static_cast<uint4*>(workspace), rows, (int)tokens, (int)top_k, (int)(K / 16)))
-            return rc;
-        x = static_cast<const int8_t*>(workspace);
-        p.in_order = 1;
-    }
-    p.rows_x = (int)(p.in_order ? rows : tokens);
-    p.early = early && !p.in_order && knobs().pdl;
-    return swiglu ? dispatch_experts<true>(st, x, w, p, gathered, s) : dispatch_experts<false>(st, x, w, p, gathered, s);
+    p.early = early && knobs().pdl;
+    if (slots) return swiglu ? dispatch_experts<true, true>(st, w, p, s) : dispatch_experts<false, true>(st, w, p, s);
+    return swiglu ? dispatch_experts<true, false>(st, w, p, s) : dispatch_experts<false, false>(st, w, p, s);
 }
 
 int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
-                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* workspace,
-                       int64_t workspace_bytes, void* stream)
+                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* stream)
 {
-    return matmul_experts(x, w, sx, sw, offsets, slots, top_k, out, rows, tokens, E, N, K, swiglu, workspace, workspace_bytes, stream, false);
+    return matmul_experts(x, w, sx, sw, offsets, slots, top_k, out, rows, tokens, E, N, K, swiglu, stream, false);
 }
 
 int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
@@ -306,7 +285,7 @@ int gi8_combine_experts(const void* y, const float* weights, const int32_t* plac
 namespace {
 
 struct ExpertsScratch {
-    int64_t weights, experts, offsets, slots, places, counts, x_q, x_scale, rows, h, h_q, h_scale, y, bytes;
+    int64_t weights, experts, offsets, slots, places, counts, x_q, x_scale, h, h_q, h_scale, y, bytes;
 };
 
 ExpertsScratch experts_scratch(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k)
@@ -321,7 +300,6 @@ ExpertsScratch experts_scratch(int64_t T, int64_t H, int64_t I, int64_t E, int64
     s.weights = take(4 * S), s.experts = take(4 * S), s.offsets = take(4 * (E + 1)), s.slots = take(4 * S), s.places = take(4 * S);
     s.counts = take(gi8_group_by_expert_workspace_bytes(S, E));
     s.x_q = take(T * H), s.x_scale = take(4 * T);
-    s.rows = take(gi8_matmul_experts_workspace_bytes(S, T, E, H));
     s.h = take(2 * S * I), s.h_q = take(S * I), s.h_scale = take(4 * S);
     s.y = take(2 * S * H);
     return s;
@@ -371,9 +349,9 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
         return rc;
     if (int rc = gi8_group_by_expert(i32(m.experts), S, E, first, i32(m.offsets), i32(m.slots), i32(m.places), b + m.counts, m.x_q - m.counts, stream)) return rc;
     if (int rc = gi8_quantize_token(x, x_dtype, i8(m.x_q), f32(m.x_scale), T, H, stream)) return rc;
-    if (int rc = matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, b + m.rows, m.h - m.rows, stream, true)) return rc;
+    if (int rc = matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, stream, true)) return rc;
     if (int rc = gi8_quantize_token(b + m.h, 1, i8(m.h_q), f32(m.h_scale), S, I, stream)) return rc;
-    if (int rc = matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, nullptr, 0, stream, true)) return rc;
+    if (int rc = matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, stream, true)) return rc;
     return gi8_combine_experts(b + m.y, f32(m.weights), i32(m.places), add, out, T, top_k, S, H, stream);
 }
 

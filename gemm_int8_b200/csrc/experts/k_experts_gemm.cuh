@@ -10,10 +10,13 @@
 // is what makes ragged groups and single tokens cheap.  An expert's rows are cut into equal tiles of at most BT.
 //
 // Structure (one persistent CTA per SM, 192 threads, 320 with SWIGLU), as in the dense kernel:
-//   warp 0      TMA producer: weight tiles (128 rows x 128 bytes) and token rows, either with one instruction; gathered rows four
-//               per instruction wherever they lie
+//   warp 0      TMA producer: weight tiles (128 rows x 128 bytes) and token rows, either with one instruction
 //   warp 1      MMA issuer, kind::i8, two accumulators in tensor memory
-//   the others  epilogue: a lane holds one output channel and walks over the tile's tokens
+//   next 4, 8   epilogue: a lane holds one output channel and walks over the tile's tokens
+//   last 4      (GATHER) token rows from wherever they lie, by 16-byte asynchronous copies into the places where TMA's 128-byte swizzle would
+//               put them: eight lanes a row, a whole line per row.  (TMA's own gather, four rows an instruction, delivers a row in 14
+//               cycles: 32768 rows gathered for 4096 x 4096 that way took 2010 us, put in order by a pass in front 475, rows that lie in
+//               order 446.)
 // SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes
 // apart in one warp, which exchanges half of the tokens by shuffles and computes 16 results per lane.
 #pragma once
@@ -25,10 +28,12 @@ namespace gi8 {
 // Epilogue warps: eight where a result costs an exponential and a quotient, four else, as eight disturb the MMAs under which they run
 // (16384 rows, E = 8, K = 4096: SwiGLU 2 x 14336 channels with four / eight 1516 / 1270 us, product of 14336 channels 633 / 694).
 constexpr int experts_epilogue_warps(bool swiglu) { return swiglu ? 8 : 4; }
-constexpr int experts_threads(bool swiglu) { return 64 + 32 * experts_epilogue_warps(swiglu); }
+constexpr int kExpertsLoaderWarps = 4;
+constexpr int experts_threads(bool swiglu, bool gather) { return 64 + 32 * (experts_epilogue_warps(swiglu) + (gather ? kExpertsLoaderWarps : 0)); }
 constexpr int kExpertsMaxExperts = 1024;
 
 struct ExpertsParams {
+    const int8_t* x;         // int8 [tokens, K]
     uint16_t* out;           // bf16 [rows, N]
     const float* sx;         // [rows of x]
     const float* sw;         // [E, Nw]
@@ -36,9 +41,7 @@ struct ExpertsParams {
     const int32_t* slots;    // [rows], or null: row p reads x[p]
     uint32_t* status;
     int64_t rows;            // S
-    int tokens;              // what slots name
-    int rows_x;              // (host) rows of x
-    int in_order;            // x has been gathered: rows of x are those of out, scales go by slots
+    int tokens;              // rows of x
     int E, N, K;             // N: columns of out; Nw = N or 2 N rows of weight per expert
     int top_k;
     int vec_zero;            // rows behind the last group can be cleared in 16-byte pieces
@@ -57,7 +60,7 @@ GI8_DEVICE float silu(float g)
 }
 
 // Tensor maps of the token rows, with boxes of a quarter, half, three quarters and all of a token tile: a tile's rows are loaded by one
-// instruction whatever their number.  Gathered rows use the first, whose box is one row.
+// instruction whatever their number.
 struct TokenMaps {
     CUtensorMap m[4];
 };
@@ -148,8 +151,10 @@ GI8_DEVICE void load_tile_5d(void* dst, const CUtensorMap* map, uint32_t bar, in
     else tma_load_5d_hint(dst, map, bar, c0, c1, c2, c3, c4, policy);
 }
 
-template <int BT, int STAGES, bool SWIGLU, bool PAIR = false>
-__global__ void __launch_bounds__(experts_threads(SWIGLU), BT <= 64 ? 2 : 1)
+// PAIR: two CTAs on neighbouring SMs share a tile of 2 x 128 weight rows, as in the dense kernel; each loads half of the token rows.
+// GATHER: row p of the result reads token slots[p] / top_k.
+template <int BT, int STAGES, bool SWIGLU, bool PAIR, bool GATHER>
+__global__ void __launch_bounds__(experts_threads(SWIGLU, GATHER), BT <= 64 ? 2 : 1)
 experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const ExpertsParams p)
 {
     static_assert(BT == 32 || BT == 64 || BT == 128 || BT == 256, "at most 256 columns of an MMA, boxes of a quarter of the rows");
@@ -171,7 +176,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     __shared__ uint32_t tmem_base_slot;
     __shared__ volatile uint32_t abort_flag;
     __shared__ __align__(16) float token_scale[2][BT];
-    __shared__ __align__(16) int32_t gather_rows[BT];
+    __shared__ __align__(8) uint64_t bar_loaded[STAGES];  // PAIR and GATHER: the peer's copies have landed
     __shared__ ExpertList<BT> list;
 
     const int warp = threadIdx.x >> 5;
@@ -187,8 +192,10 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) {
-            mbar_init(&bar_full[s], 1);
+            // the producer's own arrival, the loader warps', and the one that speaks for the peer's loader warps
+            mbar_init(&bar_full[s], 1 + (GATHER ? kExpertsLoaderWarps : 0) + (GATHER && PAIR ? 1 : 0));
             mbar_init(&bar_empty[s], 1);
+            if constexpr (GATHER && PAIR) mbar_init(&bar_loaded[s], kExpertsLoaderWarps);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bar_acc_full[b], 1);
@@ -196,8 +203,10 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         }
         fence_barrier_init();
         prefetch_tensormap(&map_w);
+        if constexpr (!GATHER) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) prefetch_tensormap(&map_x.m[i]);
+            for (int i = 0; i < 4; ++i) prefetch_tensormap(&map_x.m[i]);
+        }
     }
     if (warp == 1) {
         if constexpr (PAIR) {
@@ -227,9 +236,8 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step) {
             const int cols = ((t.rows + kAlign - 1) & ~(kAlign - 1)) / (PAIR ? 2 : 1);  // of this CTA
             if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank), t.row0 += static_cast<int>(rank) * cols;
-            const bool gather = !PAIR && p.slots && !p.in_order;
             const int box = (cols - 1) / (kRowsX / 4);  // the smallest one that holds the tile
-            const uint32_t bytes = kBytesW + (gather ? cols : (box + 1) * (kRowsX / 4)) * kBK;
+            const uint32_t bytes = kBytesW + (GATHER ? 0 : (box + 1) * (kRowsX / 4) * kBK);
             const int w_row = t.weight_tile * kChannels;
             // (one lane) PAIR: the leader arms its barrier for the bytes of both CTAs, the peer only sends bytes
             auto load_weights = [&](int stage, int kb) {
@@ -256,25 +264,10 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 if (p.early) pdl_wait();
                 if (lane == 0) pdl_launch_dependents();
             }
-            if (gather) {
-                __syncwarp();
-                for (int r = lane; r < cols; r += 32) {  // rows that pad the tile read token 0, and are not stored
-                    const int slot = r < t.rows ? __ldg(p.slots + t.row0 + r) : 0;
-                    gather_rows[r] = min(max(slot, 0) / p.top_k, p.tokens - 1);
-                }
-                __syncwarp();
-            }
             auto load_tokens = [&](int stage, int kb) {  // (one lane)
-                const uint32_t full = PAIR ? map_to_cta(smem_u32(&bar_full[stage]), 0) : smem_u32(&bar_full[stage]);
-                uint8_t* dst = smem + stage * kStageBytes + kBytesW;
-                if (gather) {
-#pragma unroll 4
-                    for (int r = 0; r < cols; r += 4) {
-                        const int4 q = *reinterpret_cast<const int4*>(&gather_rows[r]);
-                        tma_gather4(dst + r * kBK, &map_x.m[0], &bar_full[stage], kb * kBK, q.x, q.y, q.z, q.w);
-                    }
-                } else {
-                    load_tile_2d<PAIR>(dst, &map_x.m[box], full, kb * kBK, t.row0, pol_x);
+                if constexpr (!GATHER) {
+                    const uint32_t full = PAIR ? map_to_cta(smem_u32(&bar_full[stage]), 0) : smem_u32(&bar_full[stage]);
+                    load_tile_2d<PAIR>(smem + stage * kStageBytes + kBytesW, &map_x.m[box], full, kb * kBK, t.row0, pol_x);
                 }
             };
             if (ahead > 0) {
@@ -303,6 +296,28 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         drain_stages<STAGES>(PAIR && rank != 0 ? nullptr : bar_full, bar_empty, s, ph, armed, p.status, &abort_flag);
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer (of the leader)
+        if constexpr (PAIR && GATHER) {
+            // In the peer this warp passes on that the loader warps' copies have landed, with one arrival per stage in the leader's shared
+            // memory.  What reads the copies is the peer's own tensor core, through its own shared memory: the loader warps have waited for
+            // them and made them visible there before this warp sees their barrier complete, and nothing of them has to become visible in
+            // the leader, whose instruction only starts that read.  So the arrival has the default semantics of the hand-backs between the
+            // CTAs; a release at cluster scope takes longer than the MMAs of a K block (32768 rows, SwiGLU 4096 x 4096: 1290 us for 485).
+            if (rank != 0) {
+                uint32_t fs = 0, fph = 0;
+                bool going = true;
+                ExpertTile f;
+                for (int64_t item = first_item; going && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, f); item += item_step)
+                    for (int kb = 0; kb < num_kb; ++kb) {
+                        if (!warp_agrees(wait_or_abort(&bar_loaded[fs], fph, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_MMA)) {
+                            going = false;
+                            break;
+                        }
+                        if (elect_one()) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_full[fs]), 0));
+                        __syncwarp();
+                        if (++fs == STAGES) fs = 0, fph ^= 1;
+                    }
+            }
+        }
         uint32_t s = 0, ph = 0;
         uint32_t local_tile = 0;
         bool ok = rank == 0;
@@ -348,6 +363,62 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             }
             __syncwarp();
         }
+    } else if (GATHER && warp >= 2 + kEpilogueThreads / 32) {
+        // ------------------------------------------------------------------ loader warps
+        if constexpr (GATHER) {
+            if (p.early) pdl_wait();
+            // Stages whose copies are on their way while the next one's are issued.  What is not yet signalled is missing from the ring: two
+            // (777 tokens, 2501 x 2832: with one, two, three, five 27.0, 25.4, 25.5, 36.8 us), three where tiles are small and wait for memory.
+            constexpr int kLag = BT == 32 ? 3 : 2;
+            static_assert(kLag + 2 <= STAGES, "a stage is signalled before its place in the ring comes round again");
+            const int chunk = lane & 7;                // 16 bytes of a row's 128
+            const int sub = (warp - 2 - kEpilogueThreads / 32) * 4 + (lane >> 3);  // of 16 rows
+            const uint32_t place = smem_u32(smem) + kBytesW + sub * kBK + ((chunk ^ (sub & 7)) << 4);
+            uint32_t s = 0, ph = 0, done = 0;
+            int under_way = 0;
+            bool ok = true;
+            // The oldest stage under way has landed (the caller has waited for it).
+            auto landed = [&]() {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(PAIR && rank != 0 ? &bar_loaded[done] : &bar_full[done]);
+                if (++done == STAGES) done = 0;
+                --under_way;
+            };
+            ExpertTile t;
+            for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step) {
+                const int cols = ((t.rows + kAlign - 1) & ~(kAlign - 1)) / (PAIR ? 2 : 1);  // of this CTA
+                const int before = static_cast<int>(rank) * cols;
+                const int8_t* src[kRowsX / 16];
+#pragma unroll
+                for (int j = 0; j < kRowsX / 16; ++j) {
+                    const int r = before + j * 16 + sub;  // rows that pad the tile read token 0, and are not stored
+                    const int slot = j * 16 < cols && r < t.rows ? __ldg(p.slots + t.row0 + r) : 0;
+                    src[j] = p.x + static_cast<int64_t>(min(max(slot, 0) / p.top_k, p.tokens - 1)) * p.K;
+                }
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    if (!warp_agrees(wait_or_abort(&bar_empty[s], ph ^ 1, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_PRODUCER)) {
+                        ok = false;
+                        break;
+                    }
+                    const int k = kb * kBK + chunk * 16;
+                    const uint32_t bytes = k < p.K ? 16u : 0u;  // zeros behind K
+                    const uint32_t dst = place + s * kStageBytes;
+#pragma unroll
+                    for (int j = 0; j < kRowsX / 16; ++j)
+                        if (j * 16 < cols) cp_async_16(dst + j * 16 * kBK, src[j] + (bytes ? k : 0), bytes);
+                    cp_async_commit();
+                    ++under_way;
+                    if (under_way > kLag) {
+                        cp_async_wait<kLag>();
+                        landed();
+                    }
+                    if (++s == STAGES) s = 0, ph ^= 1;
+                }
+            }
+            cp_async_wait<0>();
+            while (under_way > 0) landed();
+        }
     } else {
         // ------------------------------------------------------------------ epilogue warps
         const int quarter = warp & 3;  // TMEM lanes [32 * quarter, 32 * quarter + 32)
@@ -376,7 +447,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 float v = 0.0f;
                 if (r < t.rows) {
                     int src = t.row0 + r;
-                    if (p.slots) src = min(max(__ldg(p.slots + src), 0) / p.top_k, p.tokens - 1);
+                    if constexpr (GATHER) src = min(max(__ldg(p.slots + src), 0) / p.top_k, p.tokens - 1);
                     v = __ldg(p.sx + src);
                 }
                 token_scale[buf][r] = v;

@@ -185,14 +185,17 @@ GI8_DEVICE void tma_load_5d_hint(void* smem_dst, const CUtensorMap* map, uint32_
         : "memory");
 }
 
-// Four rows of a matrix, wherever they lie, into 4 x 128 consecutive bytes of shared memory (swizzled as a tile at that address would
-// be).  The tensor map's box is one row high; c0 as above.
-GI8_DEVICE void tma_gather4(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t c0, int32_t r0, int32_t r1, int32_t r2, int32_t r3)
+// global -> shared copies of 16 bytes each by the threads themselves (src_bytes 0: zeros); waits until at most N of this thread's groups
+// are incomplete.
+GI8_DEVICE void cp_async_16(uint32_t smem_dst, const void* src, uint32_t src_bytes)
 {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3)
-        : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(src_bytes) : "memory");
+}
+GI8_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+GI8_DEVICE void cp_async_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // shared -> global tile store (bulk async-group completion).  Never issued at a negative coordinate.

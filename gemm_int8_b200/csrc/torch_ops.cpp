@@ -320,12 +320,8 @@ at::Tensor int8_matmul_experts(const at::Tensor& x, const at::Tensor& w, const a
     at::Tensor out = new_tensor({rows, N}, at::kBFloat16, x);
     // (an empty list of pairs has no data, and is not the absence of one)
     if (rows == 0) return out;
-    at::Tensor ws;
-    const int64_t bytes = sl.defined() ? gi8_matmul_experts_workspace_bytes(rows, x.size(0), E, K) : 0;
-    if (bytes > 0) ws = new_tensor({bytes}, at::kByte, x);
     check(gi8_matmul_experts(i8(x), i8(w), f32(sx), f32(sw), static_cast<const int32_t*>(off.data_ptr()),
-                             sl.defined() ? static_cast<const int32_t*>(sl.data_ptr()) : nullptr, top_k, out.data_ptr(), rows, x.size(0), E, N, K, swiglu,
-                             bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(x)));
+                             sl.defined() ? static_cast<const int32_t*>(sl.data_ptr()) : nullptr, top_k, out.data_ptr(), rows, x.size(0), E, N, K, swiglu, stream_of(x)));
     return out;
 }
 

@@ -250,13 +250,9 @@ int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t fi
  *   out  bf16 [rows,N], any alignment of its rows
  * offsets must ascend within [0, rows] and slots hold pairs of `tokens` tokens; others give wrong rows, never an access out of bounds.
  * K % 16 == 0, x and w 16-byte aligned, E <= 1024.
- * workspace  with slots: gi8_matmul_experts_workspace_bytes bytes (0 where few rows go to an expert), 16-byte aligned, of any contents:
- *            the tokens' rows in the order of the result.  Without slots NULL and 0.
  */
-int64_t gi8_matmul_experts_workspace_bytes(int64_t rows, int64_t tokens, int64_t E, int64_t K);
 int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
-                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* workspace,
-                       int64_t workspace_bytes, void* stream);
+                       int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* stream);
 
 /*
  * out[t,n] = bf16( add[t,n] + sum_j weights[t,j] * y[places[t,j],n] ), one fp32 fused multiply-add per choice in ascending j; places below
