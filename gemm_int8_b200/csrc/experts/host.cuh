@@ -114,6 +114,8 @@ int launch_experts(DeviceState* st, int slot, const int8_t* w, ExpertsParams p, 
         if (GATHER) mx.m[i] = mw;  // (unused by the kernel)
         else if (int rc = make_operand_map(&mx.m[i], p.x, p.tokens, p.K, (i + 1) * kRowsX / 4)) return rc;
     }
+    // A band's rows take about 16 MB, as in the dense kernel (one expert, 32768 rows, 4096 x 4096, for a second on end, without bands and with: 547 and 430 us).
+    p.band = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(4, (int64_t(16) << 20) / (static_cast<int64_t>(BT) * p.K))));
     const int channels = (SWIGLU ? kBM / 2 : kBM) * (PAIR ? 2 : 1);
     const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
     const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);

@@ -44,6 +44,7 @@ struct ExpertsParams {
     int tokens;              // rows of x
     int E, N, K;             // N: columns of out; Nw = N or 2 N rows of weight per expert
     int top_k;
+    int band;                // token tiles of a band
     int vec_zero;            // rows behind the last group can be cleared in 16-byte pieces
     int interleave;          // SWIGLU: the weight's map is over runs of 16 rows and loads a whole tile (N a multiple of 16)
     int early;               // the kernel in front writes neither weights nor offsets: the first weights are requested while it runs
@@ -109,10 +110,11 @@ GI8_DEVICE void build_expert_list(ExpertList<BT>& list, const int32_t* offsets, 
     __syncthreads();
 }
 
-// Tile `item` of the list, if there is one: experts in order, within an expert weight tile by weight tile with the token tiles inside,
-// so that CTAs that run at the same time share weights.  Whole warp: the chunk of 32 experts that it lies in, then the expert.
+// Tile `item` of the list, if there is one: experts in order, within an expert bands of `band` token tiles, whose rows stay in L2 while the
+// band goes through the weights, within a band weight tile by weight tile with the token tiles inside, so that CTAs that run at the same
+// time share weights.  Whole warp: the chunk of 32 experts that the tile lies in, then the expert.
 template <int BT, int ALIGN>
-GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_tiles, int64_t item, ExpertTile& t)
+GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_tiles, int band, int64_t item, ExpertTile& t)
 {
     const int lane = threadIdx.x & 31;
     auto past = [&](int e) { return e < E && static_cast<int64_t>(list.tiles_end[e]) * weight_tiles > item; };
@@ -128,10 +130,12 @@ GI8_DEVICE bool find_expert_tile(const ExpertList<BT>& list, int E, int weight_t
     const int before = t.expert ? list.tiles_end[t.expert - 1] : 0;
     const int tiles = list.tiles_end[t.expert] - before;
     const int r = static_cast<int>(item - static_cast<int64_t>(before) * weight_tiles);
-    t.weight_tile = r / tiles;
+    const int band0 = r / (band * weight_tiles) * band;  // first token tile of its band
+    const int in_band = r - band0 * weight_tiles, wide = min(band, tiles - band0);
+    t.weight_tile = in_band / wide;
     const int n = list.start[t.expert + 1] - list.start[t.expert];
     const int per = ((n + tiles - 1) / tiles + ALIGN - 1) & ~(ALIGN - 1);  // <= BT, and the last tile keeps at least a row
-    const int first = (r - t.weight_tile * tiles) * per;
+    const int first = (band0 + in_band - t.weight_tile * wide) * per;
     t.row0 = list.start[t.expert] + first;
     t.rows = min(per, n - first);
     return true;
@@ -233,7 +237,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         ExpertTile t;
         const uint64_t pol_x = l2_policy_evict_normal();
         const uint64_t pol_w = p.weight_policy_first ? l2_policy_evict_first() : pol_x;
-        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step) {
+        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, p.band, item, t); item += item_step) {
             const int cols = ((t.rows + kAlign - 1) & ~(kAlign - 1)) / (PAIR ? 2 : 1);  // of this CTA
             if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank), t.row0 += static_cast<int>(rank) * cols;
             const int box = (cols - 1) / (kRowsX / 4);  // the smallest one that holds the tile
@@ -306,7 +310,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 uint32_t fs = 0, fph = 0;
                 bool going = true;
                 ExpertTile f;
-                for (int64_t item = first_item; going && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, f); item += item_step)
+                for (int64_t item = first_item; going && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, p.band, item, f); item += item_step)
                     for (int kb = 0; kb < num_kb; ++kb) {
                         if (!warp_agrees(wait_or_abort(&bar_loaded[fs], fph, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_MMA)) {
                             going = false;
@@ -323,7 +327,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         bool ok = rank == 0;
         ExpertTile t;
         const uint32_t w_0 = smem_desc_lo(smem_u32(smem));
-        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step, ++local_tile) {
+        for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, p.band, item, t); item += item_step, ++local_tile) {
             const uint32_t buf = local_tile & 1;
             const uint32_t acc_ph = (local_tile >> 1) & 1;
             if (!warp_agrees(wait_or_abort(&bar_acc_empty[buf], acc_ph ^ 1, &abort_flag), p.status, &abort_flag, ERR_TIMEOUT_MMA)) break;
@@ -386,7 +390,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 --under_way;
             };
             ExpertTile t;
-            for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step) {
+            for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, p.band, item, t); item += item_step) {
                 const int cols = ((t.rows + kAlign - 1) & ~(kAlign - 1)) / (PAIR ? 2 : 1);  // of this CTA
                 const int before = static_cast<int>(rank) * cols;
                 const int8_t* src[kRowsX / 16];
@@ -437,7 +441,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         uint32_t local_tile = 0;
         bool ok = true;
         ExpertTile t;
-        for (int64_t item = first_item; find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, item, t); item += item_step, ++local_tile) {
+        for (int64_t item = first_item; find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, p.band, item, t); item += item_step, ++local_tile) {
             const uint32_t buf = local_tile & 1;
             const uint32_t acc_ph = (local_tile >> 1) & 1;
             if constexpr (PAIR) t.weight_tile = 2 * t.weight_tile + static_cast<int>(rank);
