@@ -27,7 +27,7 @@ int experts_smem(int slot, Kernel kernel, size_t bytes)
 bool misaligned(const void* p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
 template <typename T, int V>
-int launch_route(const RouteParams& p, int sms, cudaStream_t s)
+int launch_route(RouteParams p, int sms, cudaStream_t s)
 {
     // Groups that are not whole runs of a power of two of lanes have their values looked up through shared memory.
     int use_scratch = 0;
@@ -37,7 +37,10 @@ int launch_route(const RouteParams& p, int sms, cudaStream_t s)
     }
     const size_t smem = static_cast<size_t>(kRouteWarps) * p.E * sizeof(double);
     // As many CTAs as are resident: a warp takes token after token, the next one's logits on their way.
-    const int64_t ctas = std::min<int64_t>((static_cast<int64_t>(p.T) + kRouteWarps - 1) / kRouteWarps, static_cast<int64_t>(sms) * (V <= 8 ? 8 : 3));
+    const int64_t resident = static_cast<int64_t>(sms) * (V <= 8 ? 8 : 3);
+    p.batch = static_cast<int>(std::min<int64_t>(32 / (p.half_k > 0 ? 2 * p.half_k : 1), std::max<int64_t>(1, p.T / (resident * kRouteWarps))));
+    const int64_t per_cta = static_cast<int64_t>(kRouteWarps) * p.batch;
+    const int64_t ctas = std::min<int64_t>((p.T + per_cta - 1) / per_cta, resident);
     return launch(route_experts_kernel<T, V>, dim3((unsigned)ctas), kRouteWarps * 32, smem, s, dim3(1), knobs().pdl, p, use_scratch);
 }
 
@@ -119,28 +122,40 @@ int launch_experts(DeviceState* st, int slot, const int8_t* w, ExpertsParams p, 
     const int channels = (SWIGLU ? kBM / 2 : kBM) * (PAIR ? 2 : 1);
     const int64_t token_tiles = std::min<int64_t>(p.rows, p.E + p.rows / BT);  // at most
     const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
-    const int64_t slots = BT <= 64 ? 2 * st->sm_count : PAIR ? st->sm_count / 2 : st->sm_count;
+    const int64_t slots = BT == 64 ? 2 * st->sm_count : PAIR ? st->sm_count / 2 : st->sm_count;
     const int grid = static_cast<int>(std::min<int64_t>(tiles, slots)) * (PAIR ? 2 : 1);
     return launch(kernel, dim3(grid), experts_threads(SWIGLU, GATHER), smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
 }
 
-// Rows of a token tile: half as many again as an expert has on average, or all that it can have if no token names it twice.
-int experts_tile(const ExpertsParams& p)
+// The form of a product, by the rows that an expert can be expected to have (half as many again as on average, or all that it can have
+// if no token names it twice):
+//   up to 64   one-CTA tiles of 64 tokens, two CTAs per SM, so that the next launch's CTAs can sit down beside this one's; where the tiles
+//              leave SMs without one for long, tiles of 32 tokens with ten stages, more bytes in flight for the few
+//   more       two-CTA tiles of 256 tokens
+// us (graph replays), tiles of 64 / 256 tokens, at so many rows per expert on average: E = 64, k = 8, product 4096 x 1408: 32 59.6 / 57.8,
+// 64 68.4 / 66.1, 128 97.9 / 76.3; SwiGLU 1408 x 4096: 32 113.6 / 119.4, 64 132 / 139, 128 183 / 157; E = 8, k = 2, product 4096 x 14336: 32
+// 74.8 / 78.9, 64 96.3 / 81.7.  (One-CTA tiles of 128 tokens were level with or behind the better of the two everywhere.)  One token to two
+// experts, product 4096 x 14336, 64 tiles: 40.0, ten stages 32.0 (one to six, 2048 x 1408, 96 short tiles: 8.3 and 9.7).
+enum ExpertsForm { EXPERTS_FEW, EXPERTS_64, EXPERTS_256 };
+
+ExpertsForm experts_form(const ExpertsParams& p, bool swiglu, int sms)
 {
     const int64_t most = p.slots ? p.tokens : p.rows;
     const int64_t want = std::min(most, (3 * p.rows / 2 + p.E - 1) / p.E);
-    return want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 256;
+    if (want > 64) return EXPERTS_256;
+    const int channels = swiglu ? kBM / 2 : kBM;
+    const int64_t tiles = std::min<int64_t>(p.rows, p.E + p.rows / 32) * ((p.N + channels - 1) / channels);
+    return want <= 32 && tiles <= sms && p.K >= 48 * kBK ? EXPERTS_FEW : EXPERTS_64;
 }
 
 template <bool SWIGLU, bool GATHER>
 int dispatch_experts(DeviceState* st, const int8_t* w, const ExpertsParams& p, cudaStream_t s)
 {
     constexpr int slot = (SWIGLU ? 4 : 0) + (GATHER ? 16 : 0);
-    switch (experts_tile(p)) {
-        case 32: return launch_experts<32, 5, SWIGLU, false, GATHER>(st, slot, w, p, s);
-        case 64: return launch_experts<64, 4, SWIGLU, false, GATHER>(st, slot + 1, w, p, s);
-        case 128: return launch_experts<128, 6, SWIGLU, false, GATHER>(st, slot + 2, w, p, s);
-        default: return launch_experts<256, 6, SWIGLU, true, GATHER>(st, slot + 3, w, p, s);
+    switch (experts_form(p, SWIGLU, st->sm_count)) {
+        case EXPERTS_FEW: return launch_experts<32, 10, SWIGLU, false, GATHER>(st, slot, w, p, s);
+        case EXPERTS_64: return launch_experts<64, 4, SWIGLU, false, GATHER>(st, slot + 1, w, p, s);
+        default: return launch_experts<256, 6, SWIGLU, true, GATHER>(st, slot + 2, w, p, s);
     }
 }
 

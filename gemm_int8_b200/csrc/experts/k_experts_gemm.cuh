@@ -158,10 +158,10 @@ GI8_DEVICE void load_tile_5d(void* dst, const CUtensorMap* map, uint32_t bar, in
 // PAIR: two CTAs on neighbouring SMs share a tile of 2 x 128 weight rows, as in the dense kernel; each loads half of the token rows.
 // GATHER: row p of the result reads token slots[p] / top_k.
 template <int BT, int STAGES, bool SWIGLU, bool PAIR, bool GATHER>
-__global__ void __launch_bounds__(experts_threads(SWIGLU, GATHER), BT <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(experts_threads(SWIGLU, GATHER), BT == 64 ? 2 : 1)
 experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const ExpertsParams p)
 {
-    static_assert(BT == 32 || BT == 64 || BT == 128 || BT == 256, "at most 256 columns of an MMA, boxes of a quarter of the rows");
+    static_assert(BT == 32 || BT == 64 || BT == 256, "at most 256 columns of an MMA, boxes of a quarter of the rows");
     constexpr uint32_t kBytesW = kBM * kBK;
     constexpr int kRowsX = PAIR ? BT / 2 : BT;  // token rows that this CTA loads
     constexpr int kAlign = PAIR ? 32 : 16;      // what the columns of an MMA are a multiple of

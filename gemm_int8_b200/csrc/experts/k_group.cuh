@@ -8,8 +8,8 @@
 // warps' rows are summed up per expert, and a pair's row is its rank plus what lies in front of its warp.  A CTA's pairs are put in order in
 // shared memory before they leave, as runs of an expert instead of one 32-byte sector for each.  No atomics: the result does not depend
 // on timing.  Up to 8192 pairs one CTA does it all; more are counted by one launch and placed by a second one, which adds up the counts of the
-// CTAs in front of its own.  Bound by latencies and launches: 131072 pairs of 256 experts GROUP_US us, of which the two launches are
-// half (in one launch of a cluster of eight CTAs, which exchange their counts through distributed shared memory, 20.9: eight SMs are too few).
+// CTAs in front of its own.  Bound by latencies and launches: 131072 pairs of 256 experts 8.2 us, of which two empty launches take
+// 3.6 (in one launch of a cluster of eight CTAs, which exchange their counts through distributed shared memory, 20.9: eight SMs are too few).
 #pragma once
 
 #include "../ptx.cuh"

@@ -8,17 +8,19 @@
 //           and where fewer are left the places hold expert -1 and weight 0
 //   weight  w_j = s_chosen(j) (/ their sum) * scale
 //
-// Exactness: which of two experts is chosen must not depend on how a score was rounded to fp32.  A token is first decided by fp32
-// scores, with a bound on their error.  Where two neighbours in the order lie closer than that, the selection goes on to the last one that may
-// still belong to it, and the candidates are put in order by their choices in fp64, a lane each; where the last group kept and the
-// first one dropped lie that close, the groups' values are taken again in fp64.  One token in a thousand or so comes there, and
-// the warp that it holds up may be the launch's last: what counts is how long it takes (all of a token's scores in fp64 and the whole
-// selection again took 13 us, and the launch of 16384 tokens 39).
+// Exactness: which of two experts is chosen must not depend on how a score was rounded to fp32.  A token is decided by fp32 scores, with a
+// bound on their error.  Where two neighbours in the order, or the last group kept and the first one dropped, lie closer than that, the
+// token is marked and decided again behind the loop over the warp's tokens: the groups' values in fp64, and the candidates, which are
+// those chosen and what lies as close behind them, put in order by their choices in fp64, a lane each.  One token in a thousand or so
+// comes there, and the warp that it holds up may be the launch's last: what counts is how long it takes (all of a token's scores in fp64 and the
+// whole selection again took 13 us, and the launch of 16384 tokens 39), and that it costs the other tokens no registers.
 //
 // One warp per token; a lane holds V consecutive experts, so that the groups of the usual models are runs of whole lanes.  The choices become
-// unsigned keys whose lowest bits are the place within the lane, so that a round of the selection is one maximum over the lanes'
-// sorted keys' first, one over the warp, and a shift of the winner's lane.  Bound by instruction issue for large batches (16384
-// tokens of 256 experts, bias, groups: ROUTE_US us, of which the bytes take 3; with keys and indices apart 38, 1735 instructions a token).
+// unsigned keys whose lowest bits are the place within the lane, sorted in every lane, so that a round of the selection is one maximum over
+// the lanes' first keys and a shift of the winner's lane.  Up to four tokens' weights (eight experts each) are made together, a lane each.
+// Bound by instruction issue and latencies: 16384 tokens of 256 experts, bias, groups 28.2 us (1005 instructions a token, issued in 55 % of
+// the cycles; 1735 and 38 us with whole choices and indices apart), of which the bytes take 2.7; the selection alone, one expert without bias and
+// groups, 14.5; 16 tokens 4.1, of which an empty launch takes 1.8.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -42,7 +44,8 @@ struct RouteParams {
     int sigmoid, group_top2, renormalize;
     float scale;
     int vec, vec_bias;   // rows (the bias) can be read in 16-byte pieces of a lane's V experts
-    int half_k;          // half of the power of two that holds top_k
+    int half_k;          // half of the power of two that holds top_k (0: one)
+    int batch;           // tokens that a warp decides before it makes their weights together, at most 32 / that power of two
 };
 
 // Order-preserving map of choices to unsigned keys.  What cannot be chosen is -inf, whose key is kRouteNone.
@@ -266,10 +269,10 @@ GI8_DEVICE int route_order_exact(const RouteParams& p, const float (&l)[V], cons
 }
 
 // One token by fp32 keys; the expert of place j ends up in lane j, -1 for none.
-// l: this lane's logits (-inf behind E and for NaN).  exact: the keys' lost bits are zeros in all logits, and the choice is by logits.
+// l: this lane's logits (-inf behind E and for NaN).
 // Returns true where the candidates are more than there are lanes, or the groups' values too close and not to be had from lanes.
 template <typename T, int V>
-GI8_DEVICE bool route_fast(const RouteParams& p, const T* row, const float (&l)[V], const float (&bias)[V], bool exact, float* scratch, float row_max, float denominator, int& my_expert)
+GI8_DEVICE bool route_fast(const RouteParams& p, const T* row, const float (&l)[V], const float (&bias)[V], float* scratch, float row_max, float denominator, int& my_expert)
 {
     constexpr uint32_t kPlace = V <= 1 ? 0u : V <= 2 ? 1u : V <= 4 ? 3u : V <= 8 ? 7u : V <= 16 ? 15u : 31u;
     const int lane = threadIdx.x & 31;
@@ -336,7 +339,7 @@ GI8_DEVICE bool route_fast(const RouteParams& p, const T* row, const float (&l)[
     };
     for (int j = 0; j < p.top_k; ++j)
         if (!take()) break;
-    if (!exact) {
+    {
         // Neighbours in the order, the first one left out among them; what keys drop below a value is at most their lowest bits' worth of it.
         auto bound = [&](float a, float b) {
             const float lost = (kPlace + 1) * 1.1920929e-7f * fmaxf(fabsf(a), fabsf(b));
@@ -447,43 +450,54 @@ GI8_DEVICE int route_exact(const RouteParams& p, const T* row, double* c)
     return my_expert;
 }
 
+// A token by the careful way, from its logits on.
 template <typename T, int V>
-__global__ void __launch_bounds__(kRouteWarps * 32, V <= 8 ? 7 : 3)
-route_experts_kernel(const RouteParams p, int use_scratch)
+GI8_DEVICE int route_carefully(const RouteParams& p, const T* row, double* scratch, int use_scratch, float& m, float& z)
+{
+    const int lane = threadIdx.x & 31;
+    float l[V], bias[V];
+    route_load_lane<T, V>(row, lane * V, p.E, p.vec, l);
+    if (p.bias) route_load_lane<float, V>(p.bias, lane * V, p.E, p.vec_bias, bias);
+#pragma unroll
+    for (int i = 0; i < V; ++i) l[i] = fmaxf(l[i], -INFINITY);
+    m = 0.0f, z = 1.0f;
+    if (!p.sigmoid && (p.bias || !p.renormalize || (p.groups > 1 && p.group_top2))) route_denominator(l, m, z);
+    int expert;
+    if (route_fast<T, V>(p, row, l, bias, use_scratch ? reinterpret_cast<float*>(scratch) : nullptr, m, z, expert)) expert = route_exact<T, V>(p, row, scratch);
+    return expert;
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kRouteWarps * 32, V <= 8 ? 8 : 3)
+route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
 {
     extern __shared__ double route_scratch[];  // E values per warp
     pdl_wait();
     if (threadIdx.x == 0) pdl_launch_dependents();
+    constexpr uint32_t kPlace = V <= 1 ? 0u : V <= 2 ? 1u : V <= 4 ? 3u : V <= 8 ? 7u : V <= 16 ? 15u : 31u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kRouteWarps;
-    int64_t t = static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp;
-    if (t >= p.T) return;
     double* exact_c = route_scratch + warp * p.E;
     float* scratch = use_scratch ? reinterpret_cast<float*>(exact_c) : nullptr;
-    const bool need_denominator = !p.sigmoid && (p.bias || !p.renormalize || (p.groups > 1 && p.group_top2));
-    const bool exact = sizeof(T) == 2 && !p.bias && !(p.groups > 1 && p.group_top2);
-    float l[V], bias[V];
-    if (p.bias) route_load_lane<float, V>(p.bias, lane * V, p.E, p.vec_bias, bias);
-    for (; t < p.T; t += step) {
-        const T* row = static_cast<const T*>(p.logits) + t * p.E;
-        route_load_lane<T, V>(row, lane * V, p.E, p.vec, l);
-#pragma unroll
-        for (int i = 0; i < V; ++i) l[i] = fmaxf(l[i], -INFINITY);  // NaN is never chosen
+    const bool softmax = !p.sigmoid, by_scores = p.bias != nullptr;
+    const bool scores_of_groups = p.groups > 1 && p.group_top2 && !by_scores;
+    const bool need_denominator = softmax && (by_scores || scores_of_groups || !p.renormalize);
+    // Equal keys mean equal logits where the bits that keys lose are zeros in all of them.
+    const bool exact = sizeof(T) == 2 && !by_scores;
+    const int wide = p.half_k > 0 ? 2 * p.half_k : 1;  // lanes of a token's places
+    const int my_slot = lane / wide, my_place = lane - my_slot * wide;
+    float bias[V];
+    if (by_scores) route_load_lane<float, V>(p.bias, lane * V, p.E, p.vec_bias, bias);
 
-        int expert;
-        float row_max = 0.0f, denominator = 1.0f;
-        if (need_denominator) route_denominator(l, row_max, denominator);
-        if (route_fast<T, V>(p, row, l, bias, exact, scratch, row_max, denominator, expert)) expert = route_exact<T, V>(p, row, exact_c);
-
-        // Weights, lane j those of place j.  Their ratios do not depend on the softmax's denominator, nor on the sigmoid's where it is
-        // all but exp(l): renormalised weights are taken relative to the largest logit chosen, so that they never are 0 / 0.
-        const bool chosen = expert >= 0;
-        const float v = chosen ? route_load(row + expert) : -INFINITY;
+    // Weights, by the lanes of a token's places.  Their ratios do not depend on the softmax's denominator, nor on the sigmoid's where it is all
+    // but exp(l): renormalised weights are taken relative to the largest logit chosen, so that they never are 0 / 0.
+    auto finish = [&](int64_t t, bool token, int expert, float row_max, float denominator) {
+        const bool chosen = token && my_place < p.top_k && expert >= 0;
+        const float v = chosen ? route_load(static_cast<const T*>(p.logits) + t * p.E + expert) : -INFINITY;
         float top = v;
         for (int o = p.half_k; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         float w = 0.0f;
         if (chosen) {
-            if (!p.sigmoid) w = p.renormalize ? expf(v - top) : __fdividef(expf(v - row_max), denominator);
+            if (softmax) w = p.renormalize ? expf(v - top) : __fdividef(expf(v - row_max), denominator);
             else if (p.renormalize && top < -80.0f) w = expf(v - top);
             else w = __fdividef(1.0f, 1.0f + expf(-v));
         }
@@ -492,9 +506,111 @@ route_experts_kernel(const RouteParams p, int use_scratch)
             for (int o = p.half_k; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (chosen) w = __fdividef(w, sum);
         }
-        if (lane < p.top_k) {
-            p.weights[t * p.top_k + lane] = w * p.scale;
-            p.experts[t * p.top_k + lane] = expert;
+        if (token && my_place < p.top_k) {
+            p.weights[t * p.top_k + my_place] = w * p.scale;
+            p.experts[t * p.top_k + my_place] = expert;
+        }
+    };
+
+    constexpr int kUnsure = -2;
+    bool any_unsure = false;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRouteWarps * p.batch;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp) * p.batch; t0 < p.T; t0 += step) {
+        const int count = static_cast<int>(min(static_cast<int64_t>(p.batch), p.T - t0));
+        uint32_t mine = 0, left = 0;  // of the token of my_slot: the key of my_place, and that of the first expert left out
+        int expert = -1;
+        float row_max = 0.0f, denominator = 1.0f;
+        bool unsure = false;
+        for (int q = 0; q < count; ++q) {
+            float c[V];
+            route_load_lane<T, V>(static_cast<const T*>(p.logits) + (t0 + q) * p.E, lane * V, p.E, p.vec, c);
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = fmaxf(c[i], -INFINITY);  // NaN is never chosen
+            float m = 0.0f, z = 1.0f;
+            if (need_denominator) {
+                route_denominator(c, m, z);
+                if (my_slot == q) row_max = m, denominator = z;
+            }
+            auto score = [&](float v) { return softmax ? __fdividef(expf(v - m), z) : approx_reciprocal(1.0f + __expf(-v)); };
+            float of_group[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                if (scores_of_groups) of_group[i] = c[i] > -INFINITY ? score(c[i]) : -INFINITY;
+                if (by_scores) c[i] = c[i] > -INFINITY ? fmaxf(score(c[i]) + bias[i], -INFINITY) : -INFINITY;
+                if (!scores_of_groups) of_group[i] = c[i];
+            }
+            if (p.groups > 1) {
+                float first, second;
+                const int g = route_group_best(p, of_group, scratch, first, second);
+                const float value = p.group_top2 && second > -INFINITY ? first + second : first;
+                // The place of this lane's group in their order; the lowest value kept and the highest one dropped.
+                const int span = scratch ? 1 : p.E / p.groups / V;
+                int rank = 0;
+                for (int o = 0; o < p.groups; ++o) {
+                    const float other = __shfl_sync(0xffffffffu, value, o * span);
+                    rank += other > value || (other == value && o < g);
+                }
+                const bool live = g >= 0 && value > -INFINITY, kept = live && rank < p.top_groups;
+                if (by_scores || scores_of_groups) {
+                    const uint32_t low = __reduce_min_sync(0xffffffffu, kept ? route_key(value) : 0xffffffffu);
+                    const uint32_t high = __reduce_max_sync(0xffffffffu, live && !kept ? route_key(value) : 0u);
+                    if (high != 0 && my_slot == q) unsure = route_unkey(low) - route_unkey(high) <= 2.0f * route_margin<V>(route_unkey(low), softmax);
+                }
+                if (!scratch) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) c[i] = kept ? c[i] : -INFINITY;
+                } else {
+                    route_drop_groups(p, __ballot_sync(0xffffffffu, kept), g, false, c);
+                }
+            }
+            uint32_t key[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) key[i] = (route_key(c[i]) & ~kPlace) | (kPlace - i);
+            route_sort(key);
+            const int at = q * wide;
+            for (int j = 0; j < p.top_k; ++j) {
+                const uint32_t top = warp_max_key(key[0]);
+                if (top <= kRouteNone) break;
+                // the first lane that has this value, and the first place there
+                const int src = __ffs(__ballot_sync(0xffffffffu, (key[0] | kPlace) == (top | kPlace))) - 1;
+                const uint32_t taken = __shfl_sync(0xffffffffu, key[0], src);
+                if (lane == at + j) mine = taken, expert = src * V + static_cast<int>(kPlace - (taken & kPlace));
+                const bool next = lane == src;
+#pragma unroll
+                for (int i = 0; i + 1 < V; ++i) key[i] = next ? key[i + 1] : key[i];
+                key[V - 1] = next ? 0u : key[V - 1];
+            }
+            if (!exact) {
+                const uint32_t rest = warp_max_key(key[0]);
+                if (my_slot == q) left = rest;
+            }
+        }
+        if (!exact) {
+            // Neighbours in the order, the first one left out among them; what keys drop below a value is at most their lowest bits' worth of it.
+            uint32_t after = __shfl_down_sync(0xffffffffu, mine, 1);
+            if (my_place + 1 >= p.top_k) after = left;
+            if (my_place < p.top_k && mine > kRouteNone && after > kRouteNone) {
+                const float a = route_unkey(mine & ~kPlace), b = route_unkey(after & ~kPlace);
+                const float lost = (kPlace + 1) * 1.1920929e-7f * fmaxf(fabsf(a), fabsf(b));
+                unsure = unsure || a - b <= (by_scores ? route_margin<V>(a, softmax) + lost : lost);
+            }
+        }
+        // What fp32 cannot tell is marked, and decided behind the loop.
+        const uint32_t again = __ballot_sync(0xffffffffu, unsure);
+        if (again >> (my_slot * wide) & (wide == 32 ? 0xffffffffu : (1u << wide) - 1u)) expert = kUnsure;
+        any_unsure = any_unsure || again != 0;
+        finish(t0 + my_slot, my_slot < count, expert, row_max, denominator);
+    }
+    if (!any_unsure) return;
+    __syncwarp();
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp) * p.batch; t0 < p.T; t0 += step) {
+        const int count = static_cast<int>(min(static_cast<int64_t>(p.batch), p.T - t0));
+        const int32_t mark = lane < count ? *reinterpret_cast<const volatile int32_t*>(p.experts + (t0 + lane) * p.top_k) : 0;
+        for (uint32_t again = __ballot_sync(0xffffffffu, mark == kUnsure); again; again &= again - 1) {
+            const int64_t t = t0 + __ffs(again) - 1;
+            float m, z;
+            const int expert = route_carefully<T, V>(p, static_cast<const T*>(p.logits) + t * p.E, exact_c, use_scratch, m, z);
+            finish(t, my_slot == 0, expert, m, z);
         }
     }
 }
