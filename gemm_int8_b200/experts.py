@@ -14,16 +14,14 @@ _NS = "gemm_int8_CUDA"
 _ops = torch.ops.gemm_int8_CUDA
 # (the overloads themselves: a call that looks for them first takes half a microsecond longer)
 _route, _group, _matmul, _combine, _layer = (op.default for op in (_ops.route_experts, _ops.group_by_expert, _ops.int8_matmul_experts, _ops.combine_experts, _ops.int8_experts))
-_SCORINGS = ("softmax", "sigmoid")
-_GROUP_SCORES = ("max", "top2")
+_SIGMOID = {"softmax": False, "sigmoid": True}
+_TOP2 = {"max": False, "top2": True}
 
 
-def _router_args(top_k: int, scoring: str, groups: int, top_groups: int | None, group_score: str, renormalize: bool, scale: float):
-    if scoring not in _SCORINGS:
-        raise ValueError("scoring must be 'softmax' or 'sigmoid'")
-    if group_score not in _GROUP_SCORES:
-        raise ValueError("group_score must be 'max' or 'top2'")
-    return top_k, scoring == "sigmoid", groups, groups if top_groups is None else top_groups, group_score == "top2", renormalize, float(scale)
+def _refuse(scoring, group_score):
+    if scoring not in _SIGMOID:
+        raise ValueError("scoring must be 'softmax' or 'sigmoid'") from None
+    raise ValueError("group_score must be 'max' or 'top2'") from None
 
 
 def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1,
@@ -39,8 +37,11 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     expert -1 and weight 0, which the operators below skip.  Near ties are decided as in exact arithmetic, not by how fp32 rounds a
     score.  E <= 1024, top_k <= 32, groups <= 32.
     """
-    k, sigmoid, g, tg, top2, renorm, sc = _router_args(top_k, scoring, groups, top_groups, group_score, renormalize, scale)
-    return _route(logits, bias, k, sigmoid, g, tg, top2, renorm, sc)
+    try:
+        sigmoid, top2 = _SIGMOID[scoring], _TOP2[group_score]
+    except (KeyError, TypeError):
+        _refuse(scoring, group_score)
+    return _route(logits, bias, top_k, sigmoid, groups, groups if top_groups is None else top_groups, top2, renormalize, scale)
 
 
 def group_by_expert(experts: torch.Tensor, num_experts: int, first_expert: int = 0):
@@ -142,7 +143,9 @@ class Int8Experts(torch.nn.Module):
                  scoring: str = "softmax", bias: torch.Tensor | None = None, groups: int = 1, top_groups: int | None = None,
                  group_score: str = "max", renormalize: bool = True, scale: float = 1.0, first_expert: int = 0):
         super().__init__()
-        self._router = _router_args(top_k, scoring, groups, top_groups, group_score, renormalize, scale)
+        if scoring not in _SIGMOID or group_score not in _TOP2:
+            _refuse(scoring, group_score)
+        self._router = (top_k, _SIGMOID[scoring], groups, groups if top_groups is None else top_groups, _TOP2[group_score], renormalize, float(scale))
         self.top_k = top_k
         self.first_expert = first_expert
         self.register_buffer("gate_up_q", gate_up_q.contiguous())
