@@ -164,7 +164,7 @@ int get_device_state(DeviceState** out)
 struct MapKey {
     const void* base;
     uint64_t d0, d1, stride_bytes;
-    uint32_t box0, box1, kind;  // kind: 0 = int8 operand, 1 = bf16 output, 2 = fp32 output
+    uint32_t box0, box1, kind;  // kind: 0 = int8 operand, 1 = bf16 output, 2 = fp32 output, 3 = gate and up rows (d0 K, d1 N, stride_bytes experts)
     bool operator==(const MapKey& o) const
     {
         return base == o.base && d0 == o.d0 && d1 == o.d1 && stride_bytes == o.stride_bytes && box0 == o.box0 &&
@@ -196,7 +196,15 @@ int cached_map(CUtensorMap* out, const MapKey& key)
     cuuint32_t box[2] = {key.box0, key.box1};
     cuuint32_t estr[2] = {1, 1};
     CUresult r;
-    if (key.kind == 0)
+    if (key.kind == 3) {
+        const cuuint64_t K = key.d0, N = key.d1, E = key.stride_bytes;
+        cuuint64_t dims5[5] = {K, 16, 2, N / 16, E};
+        cuuint64_t strides5[4] = {K, N * K, 16 * K, 2 * N * K};
+        cuuint32_t box5[5] = {static_cast<cuuint32_t>(kBK), 16, 2, 4, 1};
+        cuuint32_t estr5[5] = {1, 1, 1, 1, 1};
+        r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(key.base), dims5, strides5, box5, estr5, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    } else if (key.kind == 0)
         r = g_encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(key.base), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

@@ -69,17 +69,10 @@ int launch_route_for(RouteParams p, int sms, cudaStream_t s)
 }
 
 // Gate and up rows of int8 weights [E, 2, N, K] in alternating runs of 16 (N a multiple of 16): dimensions K, row of a run, half, run, expert.
-// A box of 128 bytes x 16 x 2 x 4 x 1 is the weight tile of 64 channels.  Encoded for each launch (a layer's two are a microsecond).
+// A box of 128 bytes x 16 x 2 x 4 x 1 is the weight tile of 64 channels.
 int make_gate_up_map(CUtensorMap* map, const int8_t* w, int64_t E, int64_t N, int64_t K)
 {
-    cuuint64_t dims[5] = {(cuuint64_t)K, 16, 2, (cuuint64_t)(N / 16), (cuuint64_t)E};
-    cuuint64_t strides[4] = {(cuuint64_t)K, (cuuint64_t)(N * K), (cuuint64_t)(16 * K), (cuuint64_t)(2 * N * K)};
-    cuuint32_t box[5] = {kBK, 16, 2, 4, 1};
-    cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-    const CUresult r = g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<int8_t*>(w), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(GI8_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", static_cast<int>(r));
-    return GI8_OK;
+    return cached_map(map, MapKey{w, static_cast<uint64_t>(K), static_cast<uint64_t>(N), static_cast<uint64_t>(E), 0u, 0u, 3u});
 }
 
 template <int WARPS, int LOADS, GroupStep STEP>

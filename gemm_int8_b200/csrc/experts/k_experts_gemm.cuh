@@ -428,16 +428,17 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         const int quarter = warp & 3;  // TMEM lanes [32 * quarter, 32 * quarter + 32)
         const int et = static_cast<int>(threadIdx.x) - 64;
         if (p.early) pdl_wait();
-        {
-            // rows that belong to no expert
-            const int64_t first = static_cast<int64_t>(list.start[p.E]) * p.N, end = p.rows * p.N;
+        // rows that belong to no expert: in front of the first and behind the last
+        auto clear = [&](int64_t first, int64_t end) {
             const int64_t step = static_cast<int64_t>(gridDim.x) * kEpilogueThreads, at = static_cast<int64_t>(blockIdx.x) * kEpilogueThreads + et;
             if (p.vec_zero) {
                 for (int64_t i = first / 8 + at; i < end / 8; i += step) reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
             } else {
                 for (int64_t i = first + at; i < end; i += step) p.out[i] = 0;
             }
-        }
+        };
+        clear(0, static_cast<int64_t>(list.start[0]) * p.N);
+        clear(static_cast<int64_t>(max(list.start[p.E], list.start[0])) * p.N, p.rows * p.N);
         uint32_t local_tile = 0;
         bool ok = true;
         ExpertTile t;

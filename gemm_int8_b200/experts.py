@@ -59,7 +59,7 @@ def matmul_experts(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.Tensor, 
     """`matmul_scaled` with a weight of its own for every group of rows -> bf16 [rows, N].
 
     ``out[p, n] = bf16( fp32(x_q[s] . w_q[e, n]) * (x_scale[s] * w_scale[e, n]) )`` for offsets[e] <= p < offsets[e + 1], where s is p or, with
-    slots, the token slots[p] // top_k: rows are then read where the tokens lie, without a copy.  Rows behind offsets[-1] are zero.
+    slots, the token slots[p] // top_k: rows are then read where the tokens lie, without a copy.  Rows in front of offsets[0] and from offsets[-1] on are zero.
     x_q int8 [rows or tokens, K], w_q int8 [E, N, K], x_scale fp32 [rows or tokens], w_scale fp32 [E, N]; K a multiple of 16.
     """
     return _matmul(x_q, w_q, x_scale, w_scale, offsets, slots, top_k, False)

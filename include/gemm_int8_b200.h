@@ -243,7 +243,7 @@ int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t fi
 
 /*
  * out[p,n] = bf16( fp32(sum_k x[src(p),k] * w[e,n,k]) * (sx[src(p)] * sw[e,n]) ) for offsets[e] <= p < offsets[e+1]: gi8_matmul_scaled with a
- * weight of its own for every group of rows.  Rows [offsets[E], rows) are set to zero.
+ * weight of its own for every group of rows.  Rows in front of offsets[0] and from offsets[E] on are set to zero.
  *   x    int8 [tokens,K];  src(p) = p, or with slots the token slots[p] / top_k
  *   w    int8 [E,N,K], sw fp32 [E,N];  with swiglu [E,2N,K] and [E,2N] (N gate rows, then N up rows), and
  *        out[p,n] = bf16( g / (1 + exp(-g)) * u ) of the two fp32 products g and u

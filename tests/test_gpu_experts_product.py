@@ -86,6 +86,30 @@ def test_large_groups_over_many_tiles():
         _check_swiglu(_problem(counts, 1400, 384, seed=rows))
 
 
+@pytest.mark.parametrize("counts", [[1, 1], [0, 3, 0, 17, 1], [32], [40, 1]], ids=lambda c: "-".join(map(str, c)))
+@pytest.mark.parametrize("K", [6144, 6160])
+def test_few_long_tiles(counts, K):
+    """Fewer weight tiles than SMs and a long K: the form with a deep ring (and, with more rows, the ordinary one)."""
+    _check_product(_problem(counts, 200, K, seed=K))
+    _check_product(_problem(counts, 200, K, seed=K, gather=(3, 2), tail=2))
+    _check_swiglu(_problem(counts, 160, K, seed=K))
+    _check_swiglu(_problem(counts, 160, K, seed=K, gather=(3, 2), tail=2))
+
+
+def test_rows_of_nobody_are_zero():
+    """Rows in front of the first expert's and behind the last one's, over memory that held something else."""
+    import gemm_int8_b200 as g
+
+    for N in (128, 130):
+        x_q, w_q, x_scale, w_scale, offsets, _, _ = _problem([5, 40], N, 64, seed=N, tail=30)
+        offsets = offsets + 11
+        junk = torch.full((75, N), 9.0, dtype=torch.bfloat16, device="cuda")  # (the allocator hands this memory to the result)
+        del junk
+        out = g.matmul_experts(*_cuda(x_q, w_q, x_scale, w_scale, offsets)).cpu()
+        _, single = R.product(x_q, w_q, x_scale, w_scale, offsets)
+        assert torch.equal(out, single.to(torch.bfloat16)) and (out[:11] == 0).all() and (out[56:] == 0).all() and (out[11:56] != 0).any()
+
+
 def test_extreme_operands():
     """The largest sums there are, scales of zero, infinity and NaN in a row of their own."""
     import gemm_int8_b200 as g
