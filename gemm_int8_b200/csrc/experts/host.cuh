@@ -94,7 +94,7 @@ template <int BT, int STAGES, bool SWIGLU, bool PAIR, bool GATHER>
 int launch_experts(DeviceState* st, int slot, const int8_t* w, ExpertsParams p, cudaStream_t s)
 {
     constexpr int kRowsX = PAIR ? BT / 2 : BT;
-    constexpr size_t smem = static_cast<size_t>(STAGES) * (kBM + kRowsX) * kBK + 1024;
+    constexpr size_t smem = static_cast<size_t>(STAGES) * (kBM + kRowsX) * kBK + experts_turn_bytes(SWIGLU, PAIR) + 1024;
     auto kernel = experts_gemm_kernel<BT, STAGES, SWIGLU, PAIR, GATHER>;
     if (int rc = experts_smem(slot, kernel, smem)) return rc;
     CUtensorMap mw;
@@ -117,7 +117,7 @@ int launch_experts(DeviceState* st, int slot, const int8_t* w, ExpertsParams p, 
     const int64_t tiles = token_tiles * ((p.N + channels - 1) / channels);
     const int64_t slots = BT == 64 ? 2 * st->sm_count : PAIR ? st->sm_count / 2 : st->sm_count;
     const int grid = static_cast<int>(std::min<int64_t>(tiles, slots)) * (PAIR ? 2 : 1);
-    return launch(kernel, dim3(grid), experts_threads(SWIGLU, GATHER), smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
+    return launch(kernel, dim3(grid), experts_threads(GATHER), smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mw, mx, p);
 }
 
 // The form of a product, by the rows that an expert can be expected to have (half as many again as on average, or all that it can have
@@ -250,7 +250,7 @@ static int matmul_experts(const int8_t* x, const int8_t* w, const float* sx, con
     ExpertsParams p{};
     p.x = x, p.out = static_cast<uint16_t*>(out), p.sx = sx, p.sw = sw, p.offsets = offsets, p.slots = slots, p.status = st->status;
     p.rows = rows, p.tokens = (int)tokens, p.E = (int)E, p.N = (int)N, p.K = (int)K, p.top_k = (int)top_k;
-    p.vec_zero = !misaligned(out, 16) && N % 8 == 0;
+    p.vec = !misaligned(out, 16) && N % 8 == 0;
     p.weight_policy_first = rows <= 32 * E;
     p.early = early && knobs().pdl;
     if (slots) return swiglu ? dispatch_experts<true, true>(st, w, p, s) : dispatch_experts<false, true>(st, w, p, s);

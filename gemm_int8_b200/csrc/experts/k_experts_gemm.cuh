@@ -9,28 +9,32 @@
 // whose extent is an operand of the instruction: a tile of r rows costs roundup(r, 16) columns instead of a multiple of 128, which
 // is what makes ragged groups and single tokens cheap.  An expert's rows are cut into equal tiles of at most BT.
 //
-// Structure (one persistent CTA per SM, 192 threads, 320 with SWIGLU), as in the dense kernel:
+// Structure (one persistent CTA per SM, 192 threads, 320 with GATHER), as in the dense kernel:
 //   warp 0      TMA producer: weight tiles (128 rows x 128 bytes) and token rows, either with one instruction
 //   warp 1      MMA issuer, kind::i8, two accumulators in tensor memory
-//   next 4, 8   epilogue: a lane holds one output channel and walks over the tile's tokens
+//   next 4      epilogue: accumulators come as pairs of tokens of a channel, are scaled in packed arithmetic, and turned by stmatrix into runs of
+//               channels of a token, which leave 16 bytes a lane.  (With a channel per lane and 2-byte stores, three times the
+//               instructions, 32768 x 4096 x 2048 took 241 us for 235, SwiGLU 4096 x 4096 491 for 472.)
 //   last 4      (GATHER) token rows from wherever they lie, by 16-byte asynchronous copies into the places where TMA's 128-byte swizzle would
 //               put them: eight lanes a row, a whole line per row.  (TMA's own gather, four rows an instruction, delivers a row in 14
 //               cycles: 32768 rows gathered for 4096 x 4096 that way took 2010 us, put in order by a pass in front 475, rows that lie in
 //               order 446.)
-// SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes
-// apart in one warp, which exchanges half of the tokens by shuffles and computes 16 results per lane.
+// SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes of tensor
+// memory apart and come to the same thread.
 #pragma once
 
 #include "../k_dense.cuh"
+#include "../k_quant.cuh"
 
 namespace gi8 {
 
-// Epilogue warps: eight where a result costs an exponential and a quotient, four else, as eight disturb the MMAs under which they run
-// (16384 rows, E = 8, K = 4096: SwiGLU 2 x 14336 channels with four / eight 1516 / 1270 us, product of 14336 channels 633 / 694).
-constexpr int experts_epilogue_warps(bool swiglu) { return swiglu ? 8 : 4; }
+constexpr int kExpertsEpilogueThreads = 128;  // (eight warps instead of four: level with SwiGLU's exponentials, slower without)
 constexpr int kExpertsLoaderWarps = 4;
-constexpr int experts_threads(bool swiglu, bool gather) { return 64 + 32 * (experts_epilogue_warps(swiglu) + (gather ? kExpertsLoaderWarps : 0)); }
+constexpr int experts_threads(bool gather) { return 64 + kExpertsEpilogueThreads + (gather ? 32 * kExpertsLoaderWarps : 0); }
 constexpr int kExpertsMaxExperts = 1024;
+// Tokens at a time, and shared memory behind the stages: per epilogue warp 32 channels (SwiGLU: 16) of so many tokens, bf16.
+__host__ __device__ constexpr int experts_chunk(bool pair) { return pair ? 32 : 16; }
+__host__ __device__ constexpr int experts_turn_bytes(bool swiglu, bool pair) { return experts_chunk(pair) * (swiglu ? 32 * 4 : 64 * 4); }
 
 struct ExpertsParams {
     const int8_t* x;         // int8 [tokens, K]
@@ -45,19 +49,26 @@ struct ExpertsParams {
     int E, N, K;             // N: columns of out; Nw = N or 2 N rows of weight per expert
     int top_k;
     int band;                // token tiles of a band
-    int vec_zero;            // rows behind the last group can be cleared in 16-byte pieces
+    int vec;                 // rows of out are whole 16-byte pieces
     int interleave;          // SWIGLU: the weight's map is over runs of 16 rows and loads a whole tile (N a multiple of 16)
     int early;               // the kernel in front writes neither weights nor offsets: the first weights are requested while it runs
     int weight_policy_first; // weights are met once or twice: keep them from displacing the rest of L2
 };
 
-// g / (1 + exp(-g)), by the exponential that does not overflow: far below zero the result fades out through the subnormals.  The quotient
-// is within two units in the last place (the divisor lies in [1, 2]); the correctly rounded one branches, and its sixteen per lane and
-// 32 tokens then run one after the other.
+// g / (1 + exp(-g)), by the exponential that does not overflow: far below zero the result fades out through the subnormals.  The fast
+// exponential is off by 2 + 1.173 |g| units in the last place, the reciprocal by one (its argument lies in [1, 2]): next to nothing to a
+// result that is rounded to 8 bits.
 GI8_DEVICE float silu(float g)
 {
-    const float t = expf(-fabsf(g));
-    return g * __fdividef(g < 0.0f ? t : 1.0f, 1.0f + t);
+    const float t = __expf(-fabsf(g));
+    return g * ((g < 0.0f ? t : 1.0f) * approx_reciprocal(1.0f + t));
+}
+
+GI8_DEVICE uint4 ld_shared_v4(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
 }
 
 // Tensor maps of the token rows, with boxes of a quarter, half, three quarters and all of a token tile: a tile's rows are loaded by one
@@ -158,7 +169,7 @@ GI8_DEVICE void load_tile_5d(void* dst, const CUtensorMap* map, uint32_t bar, in
 // PAIR: two CTAs on neighbouring SMs share a tile of 2 x 128 weight rows, as in the dense kernel; each loads half of the token rows.
 // GATHER: row p of the result reads token slots[p] / top_k.
 template <int BT, int STAGES, bool SWIGLU, bool PAIR, bool GATHER>
-__global__ void __launch_bounds__(experts_threads(SWIGLU, GATHER), BT == 64 ? 2 : 1)
+__global__ void __launch_bounds__(experts_threads(GATHER), BT == 64 ? 2 : 1)
 experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps map_x, const ExpertsParams p)
 {
     static_assert(BT == 32 || BT == 64 || BT == 256, "at most 256 columns of an MMA, boxes of a quarter of the rows");
@@ -167,8 +178,10 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     constexpr int kAlign = PAIR ? 32 : 16;      // what the columns of an MMA are a multiple of
     constexpr uint32_t kStageBytes = kBytesW + kRowsX * kBK;
     constexpr uint32_t kTmemCols = 2 * BT;
-    constexpr int kEpilogueThreads = SWIGLU ? 256 : 128;
+    constexpr int kEpilogueThreads = kExpertsEpilogueThreads;
     constexpr int kChannels = SWIGLU ? kBM / 2 : kBM;  // output channels of a weight tile
+    constexpr int kChunk = experts_chunk(PAIR);        // tokens that an epilogue warp turns at a time
+    constexpr uint32_t kTurnBytes = experts_turn_bytes(SWIGLU, PAIR) / (kEpilogueThreads / 32);  // of a warp
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -427,11 +440,12 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         // ------------------------------------------------------------------ epilogue warps
         const int quarter = warp & 3;  // TMEM lanes [32 * quarter, 32 * quarter + 32)
         const int et = static_cast<int>(threadIdx.x) - 64;
+        const uint32_t turn = smem_u32(smem) + STAGES * kStageBytes + (et >> 5) * kTurnBytes;
         if (p.early) pdl_wait();
         // rows that belong to no expert: in front of the first and behind the last
         auto clear = [&](int64_t first, int64_t end) {
             const int64_t step = static_cast<int64_t>(gridDim.x) * kEpilogueThreads, at = static_cast<int64_t>(blockIdx.x) * kEpilogueThreads + et;
-            if (p.vec_zero) {
+            if (p.vec) {
                 for (int64_t i = first / 8 + at; i < end / 8; i += step) reinterpret_cast<uint4*>(p.out)[i] = make_uint4(0, 0, 0, 0);
             } else {
                 for (int64_t i = first + at; i < end; i += step) p.out[i] = 0;
@@ -457,10 +471,15 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                 }
                 token_scale[buf][r] = v;
             }
-            const int channel = t.weight_tile * kChannels + (SWIGLU ? quarter * 16 + (lane & 15) : quarter * 32 + lane);
-            const bool channel_ok = channel < p.N;
-            float channel_scale = 0.0f;
-            if (channel_ok) channel_scale = __ldg(p.sw + static_cast<int64_t>(t.expert) * rows_w + channel + (SWIGLU && lane >= 16 ? p.N : 0));
+            // This thread's channels: lane / 4 + 0, 8 (SWIGLU: gate and up of them), 16, 24 of the warp's run.
+            const int channel0 = t.weight_tile * kChannels + quarter * (kChannels / 4);
+            uint64_t channel_scale[4];
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int ch = channel0 + (lane >> 2) + (SWIGLU ? (m & 1) * 8 : m * 8);
+                const float v = ch < p.N ? __ldg(p.sw + static_cast<int64_t>(t.expert) * rows_w + ch + (SWIGLU && m >= 2 ? p.N : 0)) : 0.0f;
+                channel_scale[m] = f32x2(v, v);
+            }
             asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");  // the epilogue warps
             // After a failed wait the warp goes on through the list without touching anything: the named barrier above has no time limit and
             // needs every warp once per tile.
@@ -471,37 +490,74 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             tcgen05_fence_after_sync();
             const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * BT;
 #pragma unroll 1
-            for (int c = (et / 128) * 32; c < t.rows; c += kEpilogueThreads / 4) {  // 32 tokens; with eight warps every other 32
-                uint32_t v[32];
-                __syncwarp();
-                tmem_ld_32x32b_x32(taddr + c, v);
+            for (int c = 0; c < t.rows; c += kChunk) {
+                uint32_t v[2][kChunk / 2];  // lanes 0 .. 15 and 16 .. 31 of the warp's quarter
+                __syncwarp();  // (the last chunk has left the turning buffer)
+                tmem_ld_16x256b(taddr + c, v[0]);
+                tmem_ld_16x256b(taddr + (16u << 16) + c, v[1]);
                 tmem_ld_wait();
-                float f[32];
+                uint32_t w[kChunk / 8][SWIGLU ? 2 : 4];  // pairs of tokens, per run of eight channels
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 s4 = *reinterpret_cast<const float4*>(&token_scale[buf][c + j]);
-                    f[j] = __int2float_rn(static_cast<int32_t>(v[j])) * (s4.x * channel_scale);
-                    f[j + 1] = __int2float_rn(static_cast<int32_t>(v[j + 1])) * (s4.y * channel_scale);
-                    f[j + 2] = __int2float_rn(static_cast<int32_t>(v[j + 2])) * (s4.z * channel_scale);
-                    f[j + 3] = __int2float_rn(static_cast<int32_t>(v[j + 3])) * (s4.w * channel_scale);
+                for (int i = 0; i < kChunk / 8; ++i) {
+                    const uint64_t token_pair = *reinterpret_cast<const uint64_t*>(&token_scale[buf][c + 8 * i + 2 * (lane & 3)]);
+                    uint64_t f[4];
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) {
+                        const uint32_t a = v[m >> 1][4 * i + 2 * (m & 1)], b = v[m >> 1][4 * i + 2 * (m & 1) + 1];
+                        f[m] = mul2(f32x2(__int2float_rn(static_cast<int32_t>(a)), __int2float_rn(static_cast<int32_t>(b))), mul2(token_pair, channel_scale[m]));
+                    }
+#pragma unroll
+                    for (int m = 0; m < (SWIGLU ? 2 : 4); ++m) {
+                        float x, y;
+                        f32x2_split(f[m], x, y);
+                        if constexpr (SWIGLU) {
+                            float ux, uy;
+                            f32x2_split(f[m + 2], ux, uy);
+                            x = silu(x) * ux, y = silu(y) * uy;
+                        }
+                        w[i][m] = pack_bf16x2(x, y);
+                    }
                 }
+                // Rows of the turning buffer are tokens, of 64 (32) bytes, whose 16-byte pieces are permuted so that neither side meets bank conflicts.
                 if constexpr (SWIGLU) {
-                    const bool up_lane = lane >= 16;
-                    const int first = c + (up_lane ? 16 : 0);  // this lane's sixteen tokens
-                    uint16_t* dst = p.out + static_cast<int64_t>(t.row0 + first) * p.N + channel;
+                    const uint32_t at = turn + (lane & 7) * 32 + (lane >> 4) * 256 + ((((lane >> 3) & 1) ^ ((lane >> 2) & 1)) << 4);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float other = __shfl_xor_sync(0xffffffffu, up_lane ? f[j] : f[16 + j], 16);
-                        const float gate = up_lane ? other : f[j], up = up_lane ? f[16 + j] : other;
-                        if (channel_ok && first + j < t.rows) *dst = to_bf16_bits(silu(gate) * up);
-                        dst += p.N;
+                    for (int i = 0; i < kChunk / 8; i += 2) stmatrix_x4_trans(at + i * 256, w[i][0], w[i][1], w[i + 1][0], w[i + 1][1]);
+                } else {
+                    const uint32_t at = turn + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
+#pragma unroll
+                    for (int i = 0; i < kChunk / 8; ++i) stmatrix_x4_trans(at + i * 512, w[i][0], w[i][1], w[i][2], w[i][3]);
+                }
+                __syncwarp();
+                constexpr int kPieces = SWIGLU ? 2 : 4;  // of 16 bytes in a token's run
+                auto piece_at = [&](int token, int piece) {
+                    return turn + token * (16 * kPieces) + ((piece ^ (SWIGLU ? (token >> 2) & 1 : (token >> 1) & 3)) << 4);
+                };
+                if (p.vec) {
+                    const int piece = lane & (kPieces - 1), ch = channel0 + piece * 8;
+                    uint16_t* dst = p.out + static_cast<int64_t>(t.row0 + c + lane / kPieces) * p.N + ch;
+#pragma unroll
+                    for (int i = 0; i < kChunk * kPieces / 32; ++i) {
+                        const int token = i * (32 / kPieces) + lane / kPieces;
+                        const uint4 u = ld_shared_v4(piece_at(token, piece));
+                        if (c + token < t.rows && ch < p.N) *reinterpret_cast<uint4*>(dst) = u;
+                        dst += static_cast<int64_t>(32 / kPieces) * p.N;
                     }
                 } else {
-                    uint16_t* dst = p.out + static_cast<int64_t>(t.row0 + c) * p.N + channel;
+                    // 2 bytes a lane: a token's run (SWIGLU: those of two) at a time, eight of them read before the first is written
+                    const int ch = lane & (8 * kPieces - 1);
+                    constexpr int kStep = 4 / kPieces;
+                    const bool ch_ok = channel0 + ch < p.N;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (channel_ok && c + j < t.rows) *dst = to_bf16_bits(f[j]);
-                        dst += p.N;
+                    for (int first = 0; first < kChunk; first += 8 * kStep) {
+                        const int token0 = first + lane / (8 * kPieces);
+                        uint16_t u[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) u[i] = ld_shared_u16(piece_at(token0 + i * kStep, ch >> 3) + (ch & 7) * 2);
+                        uint16_t* dst = p.out + static_cast<int64_t>(t.row0 + c + token0) * p.N + channel0 + ch;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i, dst += static_cast<int64_t>(kStep) * p.N)
+                            if (ch_ok && c + token0 + i * kStep < t.rows) *dst = u[i];
                     }
                 }
             }

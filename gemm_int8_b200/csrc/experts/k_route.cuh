@@ -167,13 +167,6 @@ GI8_DEVICE void route_sort(uint32_t (&key)[V])
                     }
 }
 
-GI8_DEVICE float approx_reciprocal(float x)  // 1 ulp
-{
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 GI8_DEVICE float route_load(const float* p) { return __ldg(p); }
 GI8_DEVICE float route_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 

@@ -386,6 +386,33 @@ GI8_DEVICE void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8])
                  : "memory");
 }
 
+// Shape 16x256b: sixteen lanes (the first or the second half of the warp's quarter, by the lane field of taddr).  Of every eight columns
+// thread t holds columns 2 (t % 4) and 2 (t % 4) + 1 of lane t / 4 (registers 0, 1) and of lane t / 4 + 8 (registers 2, 3).
+GI8_DEVICE void tmem_ld_16x256b(uint32_t taddr, uint32_t (&r)[8])
+{
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+GI8_DEVICE void tmem_ld_16x256b(uint32_t taddr, uint32_t (&r)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+// Four 8 x 8 matrices of 16-bit elements, transposed on the way: thread t holds elements 2 (t % 4) and 2 (t % 4) + 1 of row t / 4 of
+// each; thread 8 m + j gives the address of the 16 bytes that receive column j of matrix m.
+GI8_DEVICE void stmatrix_x4_trans(uint32_t smem_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 GI8_DEVICE void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------------------------
@@ -399,6 +426,13 @@ GI8_DEVICE uint32_t pack_bf16x2(float lo, float hi)
     return r;
 }
 
+
+GI8_DEVICE float approx_reciprocal(float x)  // 1 ulp
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
 
 // A pair of fp32 values in one 64-bit register (element 0 in the low half), as the packed instructions take them.
 GI8_DEVICE uint64_t f32x2(float lo, float hi)
