@@ -9,6 +9,7 @@ Mirrors gemm_int8/__init__.py of the reference:
 
 and adds the W8A8 entry points the reference lacks: ``matmul_scaled`` (per-token x per-channel scales)
 and ``matmul_blockwise`` (per-token-per-128-K activation scales, per-128x128 weight scales).
+``experts`` holds the operators of a mixture-of-experts layer on such products, and the layer.
 
 The schemas and fake kernels of the torch ops are defined here; their CUDA implementations are a thin C++ layer
 (csrc/torch_ops.cpp) over the C ABI of ``libgemm_int8_b200.so`` (raw device pointers and the current CUDA stream).  Importing this package without the compiled

@@ -2,7 +2,7 @@
 torch operators over it, with g++ against the installed torch.
 
 Replaces the reference's CMake/ninja build of gemm_int8_CUDA.so (CMakeLists.txt, build.sh): one
-translation unit, one nvcc command, a few seconds.
+translation unit, one nvcc command, about a minute.
 """
 from __future__ import annotations
 
