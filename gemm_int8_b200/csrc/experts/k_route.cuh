@@ -18,9 +18,9 @@
 // One warp per token; a lane holds V consecutive experts, so that the groups of the usual models are runs of whole lanes.  The choices become
 // unsigned keys whose lowest bits are the place within the lane, sorted in every lane, so that a round of the selection is one maximum over
 // the lanes' first keys and a shift of the winner's lane.  Up to four tokens' weights (eight experts each) are made together, a lane each.
-// Bound by instruction issue and latencies: 16384 tokens of 256 experts, bias, groups 28.2 us (1005 instructions a token, issued in 55 % of
-// the cycles; 1735 and 38 us with whole choices and indices apart), of which the bytes take 2.7; the selection alone, one expert without bias and
-// groups, 14.5; 16 tokens 4.1, of which an empty launch takes 1.8.
+// Bound by instruction issue and latencies: 16384 tokens of 256 experts, bias, groups 26.8 us (about 1000 instructions a token, issued in 60 % of
+// the cycles; 1735 and 38 us with whole choices and indices apart), of which the bytes take 2.7; the selection alone, without bias and groups,
+// 14.5; 16 tokens 4.1, of which an empty launch takes 1.8.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -511,7 +511,7 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
     for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kRouteWarps + warp) * p.batch; t0 < p.T; t0 += step) {
         const int count = static_cast<int>(min(static_cast<int64_t>(p.batch), p.T - t0));
         uint32_t mine = 0, left = 0;  // of the token of my_slot: the key of my_place, and that of the first expert left out
-        int expert = -1;
+        int owner = 0;  // the lane that it comes from
         float row_max = 0.0f, denominator = 1.0f;
         bool unsure = false;
         for (int q = 0; q < count; ++q) {
@@ -525,16 +525,26 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
                 if (my_slot == q) row_max = m, denominator = z;
             }
             auto score = [&](float v) { return softmax ? __fdividef(expf(v - m), z) : approx_reciprocal(1.0f + __expf(-v)); };
-            float of_group[V];
+            if (by_scores) {
+                if (softmax) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (scores_of_groups) of_group[i] = c[i] > -INFINITY ? score(c[i]) : -INFINITY;
-                if (by_scores) c[i] = c[i] > -INFINITY ? fmaxf(score(c[i]) + bias[i], -INFINITY) : -INFINITY;
-                if (!scores_of_groups) of_group[i] = c[i];
+                    for (int i = 0; i < V; ++i) c[i] = c[i] > -INFINITY ? fmaxf(__fdividef(expf(c[i] - m), z) + bias[i], -INFINITY) : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) c[i] = c[i] > -INFINITY ? fmaxf(approx_reciprocal(1.0f + __expf(-c[i])) + bias[i], -INFINITY) : -INFINITY;
+                }
             }
             if (p.groups > 1) {
                 float first, second;
-                const int g = route_group_best(p, of_group, scratch, first, second);
+                int g;
+                if (scores_of_groups) {
+                    float of_group[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) of_group[i] = c[i] > -INFINITY ? score(c[i]) : -INFINITY;
+                    g = route_group_best(p, of_group, scratch, first, second);
+                } else {
+                    g = route_group_best(p, c, scratch, first, second);
+                }
                 const float value = p.group_top2 && second > -INFINITY ? first + second : first;
                 // The place of this lane's group in their order; the lowest value kept and the highest one dropped.
                 const int span = scratch ? 1 : p.E / p.groups / V;
@@ -567,7 +577,7 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
                 // the first lane that has this value, and the first place there
                 const int src = __ffs(__ballot_sync(0xffffffffu, (key[0] | kPlace) == (top | kPlace))) - 1;
                 const uint32_t taken = __shfl_sync(0xffffffffu, key[0], src);
-                if (lane == at + j) mine = taken, expert = src * V + static_cast<int>(kPlace - (taken & kPlace));
+                if (lane == at + j) mine = taken, owner = src;
                 const bool next = lane == src;
 #pragma unroll
                 for (int i = 0; i + 1 < V; ++i) key[i] = next ? key[i + 1] : key[i];
@@ -588,6 +598,7 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
                 unsure = unsure || a - b <= (by_scores ? route_margin<V>(a, softmax) + lost : lost);
             }
         }
+        int expert = mine > kRouteNone ? owner * V + static_cast<int>(kPlace - (mine & kPlace)) : -1;
         // What fp32 cannot tell is marked, and decided behind the loop.
         const uint32_t again = __ballot_sync(0xffffffffu, unsure);
         if (again >> (my_slot * wide) & (wide == 32 ? 0xffffffffu : (1u << wide) - 1u)) expert = kUnsure;

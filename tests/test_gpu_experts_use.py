@@ -140,3 +140,36 @@ def test_results_beyond_32_bits():
     places = torch.tensor([[139989, 5], [139000, -1]], dtype=torch.int32, device="cuda")
     s = g.combine_experts(out, torch.ones(2, 2, device="cuda"), places)
     assert torch.equal(s[1], out[139000]) and torch.equal(s[0], (out[139989].float() + out[5].float()).bfloat16())
+
+
+def test_ordinary_launches_give_the_same(monkeypatch):
+    """GEMM_INT8_PDL=0: every launch waits for the one in front as a whole, and no weight is requested early."""
+    import gemm_int8_b200 as g
+
+    states = [_state(*a, seed) for seed, a in enumerate(((1, 8, 2, 128, 64), (40, 16, 4, 256, 128), (700, 4, 2, 256, 192)))]
+    want = [layer(x, l) for layer, x, l in states]
+    try:
+        monkeypatch.setenv("GEMM_INT8_PDL", "0")
+        g.reload_env()
+        assert all(torch.equal(layer(x, l), w) for (layer, x, l), w in zip(states, want))
+    finally:
+        monkeypatch.delenv("GEMM_INT8_PDL")
+        g.reload_env()
+    assert all(torch.equal(layer(x, l), w) for (layer, x, l), w in zip(states, want))
+
+
+def test_each_pass_of_a_layer_waits_for_its_weights():
+    """The layer requests its first weights early: weights that change between two calls are those of the call."""
+    import gemm_int8_b200 as g
+
+    layer, x, logits = _state(24, 8, 2, 512, 256, 9)
+    other, _, _ = _state(24, 8, 2, 512, 256, 10)
+    want = [layer(x, logits), other(x, logits)]
+    versions = [tuple(getattr(m, n).clone() for n in ("gate_up_q", "gate_up_scale", "down_q", "down_scale")) for m in (layer, other)]
+    got = []
+    for i in range(20):
+        for n, v in zip(("gate_up_q", "gate_up_scale", "down_q", "down_scale"), versions[i % 2]):
+            getattr(layer, n).copy_(v)
+        got.append(layer(x, logits))
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(got))
+    assert g.device_status() == 0
