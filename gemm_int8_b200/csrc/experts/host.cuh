@@ -36,7 +36,7 @@ int launch_route(RouteParams p, int sms, cudaStream_t s)
         use_scratch = size % V != 0 || (span & (span - 1)) != 0;
     }
     const size_t smem = static_cast<size_t>(kRouteWarps) * p.E * sizeof(double);
-    // As many CTAs as are resident: a warp takes token after token, the next one's logits on their way.
+    // As many CTAs as are resident: a warp takes batch after batch of its tokens.
     const int64_t resident = static_cast<int64_t>(sms) * (V <= 8 ? 8 : 3);
     p.batch = static_cast<int>(std::min<int64_t>(32 / (p.half_k > 0 ? 2 * p.half_k : 1), std::max<int64_t>(1, p.T / (resident * kRouteWarps))));
     const int64_t per_cta = static_cast<int64_t>(kRouteWarps) * p.batch;
@@ -55,7 +55,7 @@ int launch_route_for(RouteParams p, int sms, cudaStream_t s)
     if (per_lane <= V_) {                                          \
         p.vec = vec(p.logits, V_, static_cast<int>(sizeof(T)));    \
         p.vec_bias = vec(p.bias, V_, 4);                           \
-        return launch_route<T, V_>(p, sms, s);                        \
+        return launch_route<T, V_>(p, sms, s);                     \
     }
     GI8_ROUTE(1)
     GI8_ROUTE(2)

@@ -2,7 +2,7 @@
 //   out[p, n] = bf16( fp32(sum_k X[src(p), k] * W[e, n, k]) * (sx[src(p)] * sw[e, n]) )    for offsets[e] <= p < offsets[e + 1]
 // and, with SWIGLU, for a weight of 2 N rows (N gate rows, then N up rows) per expert:
 //   out[p, n] = bf16( g / (1 + exp(-g)) * u ),  g, u = the fp32 values of channels n and N + n
-// src(p) is p, or the token slots[p] / top_k.  Rows behind offsets[E] are written as zeros.  How many rows an expert has is known on the
+// src(p) is p, or the token slots[p] / top_k.  Rows of no expert are written as zeros.  How many rows an expert has is known on the
 // device alone, so every CTA works the list of tiles out of the offsets by itself.
 //
 // Operands are swapped: the 128 rows of a WEIGHT tile fill the M = 128 side of tcgen05.mma and the expert's rows are the N side,
