@@ -16,7 +16,9 @@
 //               channels of a token, which leave 16 bytes a lane.  (With a channel per lane and 2-byte stores, three times the
 //               instructions, 32768 x 4096 x 2048 took 241 us for 235, SwiGLU 4096 x 4096 491 for 472.)
 //   last 4      (GATHER) token rows from wherever they lie, by 16-byte asynchronous copies into the places where TMA's 128-byte swizzle would
-//               put them: eight lanes a row, a whole line per row.  (TMA's own gather, four rows an instruction, delivers a row in 14
+//               put them: eight lanes a row, a whole line per row; their arrivals follow the copies by themselves, and the issuer makes them
+//               visible to the tensor core behind its wait.  (With loader warps that wait for their copies, two stages behind those they
+//               issue, SwiGLU of 4096 tokens to 8 of 64 experts, 4096 x 4096, took 458 us for 428.  TMA's own gather, four rows an instruction, delivers a row in 14
 //               cycles: 32768 rows gathered for 4096 x 4096 that way took 2010 us, put in order by a pass in front 475, rows that lie in
 //               order 446.)
 // SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes of tensor
@@ -194,6 +196,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     __shared__ volatile uint32_t abort_flag;
     __shared__ __align__(16) float token_scale[2][BT];
     __shared__ __align__(8) uint64_t bar_loaded[STAGES];  // PAIR and GATHER: the peer's copies have landed
+    __shared__ __align__(8) uint64_t bar_drained;         // GATHER: all copies of this CTA have
     __shared__ ExpertList<BT> list;
 
     const int warp = threadIdx.x >> 5;
@@ -209,11 +212,12 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < STAGES; ++s) {
-            // the producer's own arrival, the loader warps', and the one that speaks for the peer's loader warps
-            mbar_init(&bar_full[s], 1 + (GATHER ? kExpertsLoaderWarps : 0) + (GATHER && PAIR ? 1 : 0));
+            // the producer's own arrival, the loader threads', and the one that speaks for the peer's loader threads
+            mbar_init(&bar_full[s], 1 + (GATHER ? 32 * kExpertsLoaderWarps : 0) + (GATHER && PAIR ? 1 : 0));
             mbar_init(&bar_empty[s], 1);
-            if constexpr (GATHER && PAIR) mbar_init(&bar_loaded[s], kExpertsLoaderWarps);
+            if constexpr (GATHER && PAIR) mbar_init(&bar_loaded[s], 32 * kExpertsLoaderWarps);
         }
+        if constexpr (GATHER) mbar_init(&bar_drained, 32 * kExpertsLoaderWarps);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&bar_acc_full[b], 1);
             mbar_init(&bar_acc_empty[b], (PAIR ? 2 : 1) * kEpilogueThreads / 32);
@@ -315,9 +319,9 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         // ------------------------------------------------------------------ MMA issuer (of the leader)
         if constexpr (PAIR && GATHER) {
             // In the peer this warp passes on that the loader warps' copies have landed, with one arrival per stage in the leader's shared
-            // memory.  What reads the copies is the peer's own tensor core, through its own shared memory: the loader warps have waited for
-            // them and made them visible there before this warp sees their barrier complete, and nothing of them has to become visible in
-            // the leader, whose instruction only starts that read.  So the arrival has the default semantics of the hand-backs between the
+            // memory.  What reads the copies is the peer's own tensor core, through its own shared memory: they have landed when this warp sees
+            // their barrier complete, it makes them visible to the async proxy there, and nothing of them has to become visible in the
+            // leader, whose instruction only starts that read.  So the arrival has the default semantics of the hand-backs between the
             // CTAs; a release at cluster scope takes longer than the MMAs of a K block (32768 rows, SwiGLU 4096 x 4096: 1290 us for 485).
             if (rank != 0) {
                 uint32_t fs = 0, fph = 0;
@@ -329,6 +333,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                             going = false;
                             break;
                         }
+                        fence_proxy_async_smem();
                         if (elect_one()) mbar_arrive_cluster(map_to_cta(smem_u32(&bar_full[fs]), 0));
                         __syncwarp();
                         if (++fs == STAGES) fs = 0, fph ^= 1;
@@ -352,6 +357,7 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
                     ok = false;
                     break;
                 }
+                if constexpr (GATHER) fence_proxy_async_smem();  // the loader threads' copies, made by the generic proxy
                 tcgen05_fence_after_sync();
                 const uint32_t dw = w_0 + s * (kStageBytes / 16), dx = dw + kBytesW / 16;
                 if (elect_one()) {
@@ -384,24 +390,11 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
         // ------------------------------------------------------------------ loader warps
         if constexpr (GATHER) {
             if (p.early) pdl_wait();
-            // Stages whose copies are on their way while the next one's are issued.  What is not yet signalled is missing from the ring: two
-            // (777 tokens, 2501 x 2832: with one, two, three, five 27.0, 25.4, 25.5, 36.8 us), three where tiles are small and wait for memory.
-            constexpr int kLag = BT == 32 ? 3 : 2;
-            static_assert(kLag + 2 <= STAGES, "a stage is signalled before its place in the ring comes round again");
             const int chunk = lane & 7;                // 16 bytes of a row's 128
             const int sub = (warp - 2 - kEpilogueThreads / 32) * 4 + (lane >> 3);  // of 16 rows
             const uint32_t place = smem_u32(smem) + kBytesW + sub * kBK + ((chunk ^ (sub & 7)) << 4);
-            uint32_t s = 0, ph = 0, done = 0;
-            int under_way = 0;
+            uint32_t s = 0, ph = 0;
             bool ok = true;
-            // The oldest stage under way has landed (the caller has waited for it).
-            auto landed = [&]() {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(PAIR && rank != 0 ? &bar_loaded[done] : &bar_full[done]);
-                if (++done == STAGES) done = 0;
-                --under_way;
-            };
             ExpertTile t;
             for (int64_t item = first_item; ok && find_expert_tile<BT, kAlign>(list, p.E, weight_tiles, p.band, item, t); item += item_step) {
                 const int cols = ((t.rows + kAlign - 1) & ~(kAlign - 1)) / (PAIR ? 2 : 1);  // of this CTA
@@ -424,17 +417,16 @@ experts_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
 #pragma unroll
                     for (int j = 0; j < kRowsX / 16; ++j)
                         if (j * 16 < cols) cp_async_16(dst + j * 16 * kBK, src[j] + (bytes ? k : 0), bytes);
-                    cp_async_commit();
-                    ++under_way;
-                    if (under_way > kLag) {
-                        cp_async_wait<kLag>();
-                        landed();
-                    }
+                    // every thread's arrival follows its copies when they have landed; whoever waits for it makes them visible to the async proxy
+                    cp_async_arrive(PAIR && rank != 0 ? &bar_loaded[s] : &bar_full[s]);
                     if (++s == STAGES) s = 0, ph ^= 1;
                 }
             }
-            cp_async_wait<0>();
-            while (under_way > 0) landed();
+            // No copy and no arrival is on its way any more when the CTA exits (those on the stages have been waited for by the roles behind
+            // them, unless a wait has failed).
+            cp_async_arrive(&bar_drained);
+            cp_async_wait_all();
+            mbar_wait(&bar_drained, 0);
         }
     } else {
         // ------------------------------------------------------------------ epilogue warps

@@ -185,18 +185,17 @@ GI8_DEVICE void tma_load_5d_hint(void* smem_dst, const CUtensorMap* map, uint32_
         : "memory");
 }
 
-// global -> shared copies of 16 bytes each by the threads themselves (src_bytes 0: zeros); waits until at most N of this thread's groups
-// are incomplete.
+// global -> shared copies of 16 bytes each by the threads themselves (src_bytes 0: zeros); an arrival of this thread on `bar` (which counts it)
+// once all its copies so far have landed; a wait until all of them have.
 GI8_DEVICE void cp_async_16(uint32_t smem_dst, const void* src, uint32_t src_bytes)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_dst), "l"(src), "r"(src_bytes) : "memory");
 }
-GI8_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-GI8_DEVICE void cp_async_wait()
+GI8_DEVICE void cp_async_arrive(uint64_t* bar)
 {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+GI8_DEVICE void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // shared -> global tile store (bulk async-group completion).  Never issued at a negative coordinate.
 GI8_DEVICE void tma_store_2d(const CUtensorMap* map, const void* smem_src, int32_t c0, int32_t c1)
