@@ -15,12 +15,12 @@
 //   next 4      epilogue: accumulators come as pairs of tokens of a channel, are scaled in packed arithmetic, and turned by stmatrix into runs of
 //               channels of a token, which leave 16 bytes a lane.  (With a channel per lane and 2-byte stores, three times the
 //               instructions, 32768 x 4096 x 2048 took 241 us for 235, SwiGLU 4096 x 4096 491 for 472.)
-//   last 4      (GATHER) token rows from wherever they lie, by 16-byte asynchronous copies into the places where TMA's 128-byte swizzle would
-//               put them: eight lanes a row, a whole line per row; their arrivals follow the copies by themselves, and the issuer makes them
-//               visible to the tensor core behind its wait.  (With loader warps that wait for their copies, two stages behind those they
-//               issue, SwiGLU of 4096 tokens to 8 of 64 experts, 4096 x 4096, took 458 us for 428.  TMA's own gather, four rows an instruction, delivers a row in 14
-//               cycles: 32768 rows gathered for 4096 x 4096 that way took 2010 us, put in order by a pass in front 475, rows that lie in
-//               order 446.)
+//   last 4      (GATHER) token rows from wherever they lie, by 16-byte asynchronous copies into the places where TMA's 128-byte swizzle
+//               would put them: eight lanes a row, a whole line per row; their arrivals follow the copies by themselves, and the issuer
+//               makes them visible to the tensor core behind its wait.  SwiGLU of 4096 tokens to 8 of 64 experts, 4096 x 4096, took
+//               458 us for 428 with loader warps that wait for their copies, two stages behind those they issue.  TMA's own gather,
+//               four rows an instruction, delivers a row in 14 cycles: 32768 rows gathered for 4096 x 4096 that way took 2010 us, put
+//               in order by a pass in front 475, rows that lie in order 446.
 // SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes of tensor
 // memory apart and come to the same thread.
 #pragma once
