@@ -133,6 +133,22 @@ GI8_DEVICE void route_drop_groups(const RouteParams& p, uint32_t kept, int group
 template <int V>
 GI8_DEVICE float route_margin(float c, bool softmax) { return (3.0f * 5.9604645e-8f) * (fabsf(c) + (softmax ? V + 21.0f : 8.0f)); }
 
+// A bound on the error of a group's fp32 value (three times what a choice is off by, for each of those that it is made of; the sum's own rounding
+// is at most theirs).  It goes by the choices' magnitudes and not by the value's: choices of opposite signs cancel, their errors do not.
+template <int V>
+GI8_DEVICE float route_group_slack(const RouteParams& p, float first, float second, bool softmax)
+{
+    return route_margin<V>(fabsf(first) + (p.group_top2 && second > -INFINITY ? fabsf(second) : 0.0f), softmax);
+}
+
+// Whole warp: may a group that is dropped be ahead of one that is kept?  value, slack: of the lane's group, where it is live (has a choice).
+GI8_DEVICE bool route_groups_close(float value, float slack, bool live, bool kept)
+{
+    const uint32_t low = __reduce_min_sync(0xffffffffu, kept ? route_key(value - slack) : 0xffffffffu);
+    const uint32_t high = __reduce_max_sync(0xffffffffu, live && !kept ? route_key(value + slack) : 0u);
+    return high != 0 && high >= low;
+}
+
 // The softmax's largest logit and denominator (0 and 0 for a row without logits), in fp32 or fp64.
 template <typename F, int V>
 GI8_DEVICE void route_denominator(const float (&l)[V], F& m, F& z)
@@ -287,18 +303,17 @@ GI8_DEVICE bool route_fast(const RouteParams& p, const T* row, const float (&l)[
         const int group_here = route_group_best(p, of_group, scratch, first, second);
         const float value = p.group_top2 && second > -INFINITY ? first + second : first;
         uint32_t key = group_here >= 0 ? route_key(value) : 0u;
-        uint32_t kept = 0, last = 0;
-        for (int n = 0; n <= p.top_groups; ++n) {
+        uint32_t kept = 0;
+        for (int n = 0; n < p.top_groups; ++n) {
             const uint32_t best = warp_max_key(key);
             if (best <= kRouteNone) break;
-            if (n == p.top_groups) {  // the best one that stays out
-                close = (by_scores || scores_of_groups) && route_unkey(last) - route_unkey(best) <= 2.0f * route_margin<V>(route_unkey(last), softmax);
-                break;
-            }
-            last = best;
             const int g = __shfl_sync(0xffffffffu, group_here, __ffs(__ballot_sync(0xffffffffu, key == best)) - 1);
             kept |= 1u << g;
             if (group_here == g) key = 0;
+        }
+        if (by_scores || scores_of_groups) {
+            const bool live = group_here >= 0 && value > -INFINITY;
+            close = route_groups_close(value, route_group_slack<V>(p, first, second, softmax), live, live && ((kept >> group_here) & 1u));
         }
         if (close) {  // (the same in all lanes)
             if (scratch) return true;
@@ -555,9 +570,8 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
                 }
                 const bool live = g >= 0 && value > -INFINITY, kept = live && rank < p.top_groups;
                 if (by_scores || scores_of_groups) {
-                    const uint32_t low = __reduce_min_sync(0xffffffffu, kept ? route_key(value) : 0xffffffffu);
-                    const uint32_t high = __reduce_max_sync(0xffffffffu, live && !kept ? route_key(value) : 0u);
-                    if (high != 0 && my_slot == q) unsure = route_unkey(low) - route_unkey(high) <= 2.0f * route_margin<V>(route_unkey(low), softmax);
+                    const bool close = route_groups_close(value, route_group_slack<V>(p, first, second, softmax), live, kept);
+                    if (my_slot == q) unsure = close;
                 }
                 if (!scratch) {
 #pragma unroll
