@@ -133,12 +133,19 @@ GI8_DEVICE void route_drop_groups(const RouteParams& p, uint32_t kept, int group
 template <int V>
 GI8_DEVICE float route_margin(float c, bool softmax) { return (3.0f * 5.9604645e-8f) * (fabsf(c) + (softmax ? V + 21.0f : 8.0f)); }
 
-// A bound on the error of a group's fp32 value (three times what a choice is off by, for each of those that it is made of; the sum's own rounding
-// is at most theirs).  It goes by the choices' magnitudes and not by the value's: choices of opposite signs cancel, their errors do not.
+// A group's fp32 value.  A sum of two largest choices is halved, as all of them are: two finite choices can be beyond fp32 together.
+GI8_DEVICE float route_group_value(const RouteParams& p, float first, float second)
+{
+    return !p.group_top2 ? first : second > -INFINITY ? 0.5f * first + 0.5f * second : 0.5f * first;
+}
+
+// A bound on its error (three times what a choice is off by, for each of those that it is made of; the sum's own rounding is at most theirs).
+// It goes by the choices' magnitudes and not by the value's: choices of opposite signs cancel, their errors do not.
 template <int V>
 GI8_DEVICE float route_group_slack(const RouteParams& p, float first, float second, bool softmax)
 {
-    return route_margin<V>(fabsf(first) + (p.group_top2 && second > -INFINITY ? fabsf(second) : 0.0f), softmax);
+    if (!p.group_top2) return route_margin<V>(first, softmax);
+    return 0.5f * route_margin<V>(fabsf(first) + (second > -INFINITY ? fabsf(second) : 0.0f), softmax);  // (infinite: fp64 decides)
 }
 
 // Whole warp: may a group that is dropped be ahead of one that is kept?  value, slack: of the lane's group, where it is live (has a choice).
@@ -301,7 +308,7 @@ GI8_DEVICE bool route_fast(const RouteParams& p, const T* row, const float (&l)[
 #pragma unroll
         for (int i = 0; i < V; ++i) of_group[i] = scores_of_groups && !by_scores && l[i] > -INFINITY ? score(l[i]) : c[i];
         const int group_here = route_group_best(p, of_group, scratch, first, second);
-        const float value = p.group_top2 && second > -INFINITY ? first + second : first;
+        const float value = route_group_value(p, first, second);
         uint32_t key = group_here >= 0 ? route_key(value) : 0u;
         uint32_t kept = 0;
         for (int n = 0; n < p.top_groups; ++n) {
@@ -560,7 +567,7 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
                 } else {
                     g = route_group_best(p, c, scratch, first, second);
                 }
-                const float value = p.group_top2 && second > -INFINITY ? first + second : first;
+                const float value = route_group_value(p, first, second);
                 // The place of this lane's group in their order; the lowest value kept and the highest one dropped.
                 const int span = scratch ? 1 : p.E / p.groups / V;
                 int rank = 0;

@@ -25,3 +25,21 @@ def test_sums_that_cancel(E, groups, top_groups, B, scoring):
     logits = logits.reshape(1, E) + spread * torch.randn(150, E, generator=gen)
     k = min(6, top_groups * size)
     _check(logits, k, scoring=scoring, bias=bias.reshape(E), groups=groups, top_groups=top_groups, group_score="top2")
+
+
+@pytest.mark.parametrize("E,groups", [(64, 8), (32, 8), (60, 5), (72, 4)])
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_masks_and_favours_of_the_largest_magnitude(E, groups, group_score, scoring):
+    """A bias of fp32's lowest value masks all but one group: finite choices, whose groups are kept (the lower index first) and whose experts are chosen
+    where nothing better is left, although the sum of two of them is beyond fp32.  The same for biases of the largest value."""
+    gen = torch.Generator().manual_seed(E)
+    size, top = E // groups, torch.finfo(torch.float32).max
+    logits = torch.randn(20, E, generator=gen)
+    bias = torch.full((groups, size), -top)
+    bias[2] = torch.randn(size, generator=gen) * 0.1
+    for top_groups in (1, 2, groups - 1):
+        _check(logits, min(32, size * top_groups), scoring=scoring, bias=bias.reshape(E), groups=groups, top_groups=top_groups, group_score=group_score)
+    bias = torch.randn(groups, size, generator=gen)
+    bias[:, 0], bias[:, 1] = top, top * torch.linspace(0.1, 0.9, groups)
+    _check(logits, min(2 * size, 8), scoring=scoring, bias=bias.reshape(E), groups=groups, top_groups=2, group_score=group_score)
