@@ -4,6 +4,7 @@
 //   choice c_e = s_e + bias_e;  without a bias l_e itself (s_e increases with it, and l_e needs no rounding)
 //   groups: E / G consecutive experts each; a group's value is its largest choice, or the sum of its two largest (of s_e without a
 //           bias); the top_groups best groups keep their experts
+//           (l_e = +inf counts as the largest finite value: a softmax shares its weight among the infinite ones)
 //   chosen: the top_k largest c_e among them, in that order, the lower index first among equals; c_e = -inf or NaN is never chosen,
 //           and where fewer are left the places hold expert -1 and weight 0
 //   weight  w_j = s_chosen(j) (/ their sum) * scale
@@ -193,6 +194,9 @@ GI8_DEVICE void route_sort(uint32_t (&key)[V])
 GI8_DEVICE float route_load(const float* p) { return __ldg(p); }
 GI8_DEVICE float route_load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
 
+// A logit as it counts: NaN as -inf, +inf as the largest finite value (a softmax of it is finite then).
+GI8_DEVICE float route_logit(float l) { return fminf(fmaxf(l, -INFINITY), 3.402823466e38f); }
+
 template <typename T, int V>
 GI8_DEVICE void route_load_lane(const T* row, int e0, int E, bool vec, float (&l)[V])
 {
@@ -265,7 +269,7 @@ GI8_DEVICE int route_order_exact(const RouteParams& p, const float (&l)[V], cons
     const bool softmax = !p.sigmoid;
     double m = 0.0, z = 1.0;
     if (softmax && p.bias) route_denominator(l, m, z);
-    double c = lane < n ? static_cast<double>(route_load(row + e)) : 0.0;
+    double c = lane < n ? static_cast<double>(route_logit(route_load(row + e))) : 0.0;
     if (p.bias && lane < n) {
         const double x = exp(softmax ? c - m : -c);
         c = (softmax ? x / z : 1.0 / (1.0 + x)) + static_cast<double>(__ldg(p.bias + e));
@@ -395,13 +399,13 @@ GI8_DEVICE int route_exact(const RouteParams& p, const T* row, double* c)
     double m = -INFINITY, z = 0.0;
     if (softmax) {
 #pragma unroll 1
-        for (int e = lane; e < p.E; e += 32) m = fmax(m, static_cast<double>(route_load(row + e)));
+        for (int e = lane; e < p.E; e += 32) m = fmax(m, static_cast<double>(route_logit(route_load(row + e))));
 #pragma unroll 1
         for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (!(m > -INFINITY)) m = 0.0;
 #pragma unroll 1
         for (int e = lane; e < p.E; e += 32) {
-            const float l = route_load(row + e);
+            const float l = route_logit(route_load(row + e));
             if (l > -INFINITY) z += exp(static_cast<double>(l) - m);
         }
 #pragma unroll 1
@@ -412,7 +416,7 @@ GI8_DEVICE int route_exact(const RouteParams& p, const T* row, double* c)
         __syncwarp();
 #pragma unroll 1
         for (int e = lane; e < p.E; e += 32) {
-            const double l = static_cast<double>(route_load(row + e));
+            const double l = static_cast<double>(route_logit(route_load(row + e)));
             double v = l;
             if (scores) {
                 const double x = exp(softmax ? l - m : -l);
@@ -474,7 +478,7 @@ GI8_DEVICE int route_carefully(const RouteParams& p, const T* row, double* scrat
     route_load_lane<T, V>(row, lane * V, p.E, p.vec, l);
     if (p.bias) route_load_lane<float, V>(p.bias, lane * V, p.E, p.vec_bias, bias);
 #pragma unroll
-    for (int i = 0; i < V; ++i) l[i] = fmaxf(l[i], -INFINITY);
+    for (int i = 0; i < V; ++i) l[i] = route_logit(l[i]);
     m = 0.0f, z = 1.0f;
     if (!p.sigmoid && (p.bias || !p.renormalize || (p.groups > 1 && p.group_top2))) route_denominator(l, m, z);
     int expert;
@@ -507,7 +511,7 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
     // but exp(l): renormalised weights are taken relative to the largest logit chosen, so that they never are 0 / 0.
     auto finish = [&](int64_t t, bool token, int expert, float row_max, float denominator) {
         const bool chosen = token && my_place < p.top_k && expert >= 0;
-        const float v = chosen ? route_load(static_cast<const T*>(p.logits) + t * p.E + expert) : -INFINITY;
+        const float v = chosen ? route_logit(route_load(static_cast<const T*>(p.logits) + t * p.E + expert)) : -INFINITY;
         float top = v;
         for (int o = p.half_k; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         float w = 0.0f;
@@ -540,7 +544,7 @@ route_experts_kernel(const __grid_constant__ RouteParams p, int use_scratch)
             float c[V];
             route_load_lane<T, V>(static_cast<const T*>(p.logits) + (t0 + q) * p.E, lane * V, p.E, p.vec, c);
 #pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = fmaxf(c[i], -INFINITY);  // NaN is never chosen
+            for (int i = 0; i < V; ++i) c[i] = route_logit(c[i]);
             float m = 0.0f, z = 1.0f;
             if (need_denominator) {
                 route_denominator(c, m, z);
