@@ -55,22 +55,31 @@ def group_by_expert(experts: torch.Tensor, num_experts: int, first_expert: int =
     return _group(experts, num_experts, first_expert)
 
 
+def _pairs(slots, top_k):
+    if top_k is None:
+        if slots is not None:
+            raise ValueError("slots are pairs of a token and a choice: top_k must be given with them")
+        return 1
+    return top_k
+
+
 def matmul_experts(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
-                   slots: torch.Tensor | None = None, top_k: int = 1) -> torch.Tensor:
+                   slots: torch.Tensor | None = None, top_k: int | None = None) -> torch.Tensor:
     """`matmul_scaled` with a weight of its own for every group of rows -> bf16 [rows, N].
 
     ``out[p, n] = bf16( fp32(x_q[s] . w_q[e, n]) * (x_scale[s] * w_scale[e, n]) )`` for offsets[e] <= p < offsets[e + 1], where s is p or, with
     slots, the token slots[p] // top_k: rows are then read where the tokens lie, without a copy.  Rows in front of offsets[0] and from offsets[-1] on are zero.
-    x_q int8 [rows or tokens, K], w_q int8 [E, N, K], x_scale fp32 [rows or tokens], w_scale fp32 [E, N]; K a multiple of 16.
+    x_q int8 [rows or tokens, K], w_q int8 [E, N, K], x_scale fp32 [rows or tokens], w_scale fp32 [E, N]; K a multiple of 16.  top_k, the
+    pairs of a token, has to be given with slots and means nothing without.
     """
-    return _matmul(x_q, w_q, x_scale, w_scale, offsets, slots, top_k, False)
+    return _matmul(x_q, w_q, x_scale, w_scale, offsets, slots, _pairs(slots, top_k), False)
 
 
 def matmul_experts_swiglu(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor,
-                          slots: torch.Tensor | None = None, top_k: int = 1) -> torch.Tensor:
+                          slots: torch.Tensor | None = None, top_k: int | None = None) -> torch.Tensor:
     """`matmul_experts` for a weight [E, 2 N, K] of N gate rows and then N up rows -> bf16 [rows, N]: ``silu(gate) * up`` of the two products in
     fp32, rounded once."""
-    return _matmul(x_q, w_q, x_scale, w_scale, offsets, slots, top_k, True)
+    return _matmul(x_q, w_q, x_scale, w_scale, offsets, slots, _pairs(slots, top_k), True)
 
 
 def combine_experts(y: torch.Tensor, weights: torch.Tensor, places: torch.Tensor, add: torch.Tensor | None = None) -> torch.Tensor:
