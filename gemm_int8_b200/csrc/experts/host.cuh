@@ -321,7 +321,8 @@ extern "C" {
 
 int64_t gi8_experts_scratch_bytes(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k)
 {
-    if (T < 0 || H < 0 || I < 0 || E < 0 || top_k < 0 || top_k > kRouteMaxTopK || T > INT32_MAX || H > INT32_MAX || I > INT32_MAX || E > INT32_MAX) return 0;
+    // (what gi8_experts refuses needs none; within its limits nothing here passes 2^44)
+    if (T < 0 || H < 1 || I < 1 || E < 1 || top_k < 1 || top_k > kRouteMaxTopK || T > kGroupMaxPairs / top_k || H >= kMaxK || I >= kMaxK || E > kExpertsMaxExperts) return 0;
     return experts_scratch(T, H, I, E, top_k).bytes;
 }
 

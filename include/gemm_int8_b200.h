@@ -269,7 +269,8 @@ int gi8_combine_experts(const void* y, const float* weights, const int32_t* plac
  *   gate_up  int8 [E,2I,H], gate_up_scale fp32 [E,2I];  down int8 [E,H,I], down_scale fp32 [E,H]: experts first .. first + E - 1 of the router's,
  *            the sum runs over those of a token's choices that are among them
  *   scratch  gi8_experts_scratch_bytes(T, H, I, E, top_k) bytes, 256-byte aligned, of any contents.  Two calls that may overlap need two.
- * H and I are multiples of 16; T * top_k <= 2^24.  Whatever a step refuses is refused before the first launch.
+ * H and I are multiples of 16 below 131072; T * top_k <= 2^24.  Whatever a step refuses is refused before the first launch, and
+ * gi8_experts_scratch_bytes is 0 for sizes that are.
  */
 int64_t gi8_experts_scratch_bytes(int64_t T, int64_t H, int64_t I, int64_t E, int64_t top_k);
 int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_experts_boundary import call  # noqa: F401  (the fixture)
+
 
 def test_slots_need_the_number_of_choices():
     """Without it every row would read another token than its own."""
@@ -17,3 +19,16 @@ def test_slots_need_the_number_of_choices():
                 f(x, w, sx, sw, offsets, slots)
             assert f(x, w, sx, sw, offsets, slots, 2).shape[0] == 10 and f(x, w, sx, sw, offsets, slots, top_k=2).shape[0] == 10
             assert f(x, w, sx, sw, offsets).shape[0] == 5 and f(x, w, sx, sw, offsets, None, 2).shape[0] == 5
+
+
+def test_scratch_of_sizes_that_the_layer_refuses(call):
+    """0 for whatever the layer refuses by its sizes: 2 T top_k I of the largest arguments is beyond 64 bits."""
+    f = call.C.gi8_experts_scratch_bytes
+    big = 2 ** 31 - 1
+    assert f(big, big, big, 8, 32) == 0
+    for T, H, I, E, k in ((big, 64, 32, 8, 2), (2 ** 23 + 1, 64, 32, 8, 2), (4, 131072, 32, 8, 2), (4, 64, 131072, 8, 2), (4, 64, 32, 1025, 2), (4, 64, 32, 8, 33), (4, 64, 32, 0, 2),
+                          (4, 0, 32, 8, 2), (4, 64, 0, 8, 2), (4, 64, 32, 8, 0), (2 ** 62, 64, 32, 8, 2)):
+        assert f(T, H, I, E, k) == 0, (T, H, I, E, k)
+    largest = f(2 ** 19, 131056, 131056, 1024, 32)
+    pairs = 2 ** 24
+    assert 2 ** 19 * 131056 + pairs * (3 * 131056 + 2 * 131056) < largest < 2 ** 44
