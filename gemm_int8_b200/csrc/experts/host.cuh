@@ -337,8 +337,8 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
                                    scale, stream))
         return rc;
     if (T < 0 || T > INT32_MAX || T * top_k > kGroupMaxPairs) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "T=%lld with top_k=%lld is out of range", (long long)T, (long long)top_k);
-    if (E < 1 || first < 0 || first + E > E_router)
-        return fail(GI8_ERR_INVALID_ARGUMENT, "experts %lld .. %lld of a router over %lld", (long long)first, (long long)(first + E - 1), (long long)E_router);
+    if (E < 1 || E > E_router || first < 0 || first > E_router - E)
+        return fail(GI8_ERR_INVALID_ARGUMENT, "%lld experts from %lld on of a router over %lld", (long long)E, (long long)first, (long long)E_router);
     if (H < 1 || I < 1 || H % 16 || I % 16) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "hidden size %lld and inner size %lld must be positive multiples of 16", (long long)H, (long long)I);
     if (H >= kMaxK || I >= kMaxK) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "hidden and inner size must be below %lld", (long long)kMaxK);
     if (E * 2 * I > INT32_MAX - 256 || E * H > INT32_MAX - 256) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "experts times channels must be below 2^31 - 256");

@@ -32,3 +32,13 @@ def test_scratch_of_sizes_that_the_layer_refuses(call):
     largest = f(2 ** 19, 131056, 131056, 1024, 32)
     pairs = 2 ** 24
     assert 2 ** 19 * 131056 + pairs * (3 * 131056 + 2 * 131056) < largest < 2 ** 44
+
+
+def test_first_expert_of_any_size(call):
+    """first + E may not wrap around on its way to the comparison with the router's experts."""
+    for first in (2 ** 63 - 1, 2 ** 63 - 4, 2 ** 62, 2 ** 31, 1):
+        assert call("layer", first=first) == 1, first  # GI8_ERR_INVALID_ARGUMENT
+    assert call("layer", first=2 ** 63 - 1, E=1) == 1 and call("layer", first=1, T=0) == 1
+    assert call("layer", E=2 ** 62) == 1 and call("layer", E=2 ** 62, first=2 ** 62) == 1
+    for first in (2 ** 63 - 1, 2 ** 31):
+        assert call("group", first=first) == 1, first
