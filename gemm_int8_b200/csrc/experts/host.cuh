@@ -233,6 +233,9 @@ static int matmul_experts(const int8_t* x, const int8_t* w, const float* sx, con
     if (top_k < 1 || top_k > INT32_MAX) return fail(GI8_ERR_INVALID_ARGUMENT, "top_k=%lld must be positive", (long long)top_k);
     if (!slots && tokens < rows) return fail(GI8_ERR_INVALID_ARGUMENT, "%lld rows of x for %lld rows of the result", (long long)tokens, (long long)rows);
     if (tokens > INT32_MAX - 256 || rows > INT32_MAX - 256) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "rows must be below 2^31 - 256");
+    // Offsets that do not ascend may give every expert all rows.  The kernel counts token tiles in 32 bits, of 64 rows at least where there are many.
+    if (E * ((rows + 63) / 64) > INT32_MAX)
+        return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts times %lld rows must be below 2^37", (long long)E, (long long)rows);
     if (N > (int64_t(1) << 30) || E * N * (swiglu ? 2 : 1) > INT32_MAX - 256)
         return fail(GI8_ERR_UNSUPPORTED_SHAPE, "%lld experts of %lld channels: together below 2^31 - 256", (long long)E, (long long)N);
     if (int rc = check_common(x, w, out, rows, N, K, 2)) return rc;

@@ -250,7 +250,7 @@ int gi8_group_by_expert(const int32_t* experts, int64_t S, int64_t E, int64_t fi
  *        out[p,n] = bf16( g / (1 + exp(-g)) * u ) of the two fp32 products g and u
  *   out  bf16 [rows,N], any alignment of its rows
  * offsets must ascend within [0, rows] and slots hold pairs of `tokens` tokens; others give wrong rows, never an access out of bounds.
- * K % 16 == 0, x and w 16-byte aligned, E <= 1024.
+ * K % 16 == 0, x and w 16-byte aligned, E <= 1024, E * rows < 2^37.
  */
 int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const float* sw, const int32_t* offsets, const int32_t* slots,
                        int64_t top_k, void* out, int64_t rows, int64_t tokens, int64_t E, int64_t N, int64_t K, int swiglu, void* stream);

@@ -42,3 +42,10 @@ def test_first_expert_of_any_size(call):
     assert call("layer", E=2 ** 62) == 1 and call("layer", E=2 ** 62, first=2 ** 62) == 1
     for first in (2 ** 63 - 1, 2 ** 31):
         assert call("group", first=first) == 1, first
+
+
+def test_more_tiles_than_are_counted(call):
+    """Offsets that do not ascend may give every expert all rows: the products count the tiles of all of them in 32 bits."""
+    assert call("product", E=1024, rows=2 ** 28, tokens=2 ** 28) == 2
+    assert call("product", E=1024, rows=2 ** 27, tokens=2 ** 27) == 2 and call("product", E=1024, rows=2 ** 27, tokens=4, slots=call.base, k=2) == 2
+    assert call("product", E=100, rows=2 ** 31 - 300, tokens=2 ** 31 - 300) == 2
