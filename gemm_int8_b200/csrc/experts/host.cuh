@@ -266,19 +266,19 @@ int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const 
     return matmul_experts(x, w, sx, sw, offsets, slots, top_k, out, rows, tokens, E, N, K, swiglu, stream, false);
 }
 
-int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
-                        int64_t rows, int64_t N, void* stream)
+static int combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, bool add_f32, void* out, int64_t T, int64_t top_k,
+                           int64_t rows, int64_t N, void* stream)
 {
     if (T < 0 || T > INT32_MAX || rows < 0 || rows > INT32_MAX || N < 0 || N > INT32_MAX - 4096) return fail(GI8_ERR_INVALID_ARGUMENT, "a dimension is out of range");
     if (top_k < 1 || top_k > kCombineMaxTopK) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "top_k=%lld must be in [1, %d]", (long long)top_k, kCombineMaxTopK);
     if (T == 0 || N == 0) return GI8_OK;
     if ((!y && rows > 0) || !weights || !places || !out) return fail(GI8_ERR_INVALID_ARGUMENT, "null pointer");
-    if (misaligned(y, 2) || misaligned(add, 2) || misaligned(out, 2) || misaligned(weights, 4) || misaligned(places, 4))
+    if (misaligned(y, 2) || misaligned(add, add_f32 ? 4 : 2) || misaligned(out, 2) || misaligned(weights, 4) || misaligned(places, 4))
         return fail(GI8_ERR_MISALIGNED, "a pointer is not aligned to its elements");
     DeviceState* st;
     if (int rc = get_device_state(&st)) return rc;
     CombineParams p{};
-    p.y = static_cast<const uint16_t*>(y), p.weights = weights, p.places = places, p.add = static_cast<const uint16_t*>(add), p.out = static_cast<uint16_t*>(out);
+    p.y = static_cast<const uint16_t*>(y), p.weights = weights, p.places = places, p.add = add, p.out = static_cast<uint16_t*>(out);
     p.rows = rows, p.T = (int)T, p.N = (int)N, p.top_k = (int)top_k;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool vec = N % 8 == 0 && !misaligned(y, 16) && !misaligned(add, 16) && !misaligned(out, 16);
@@ -286,8 +286,21 @@ int gi8_combine_experts(const void* y, const float* weights, const int32_t* plac
     const int64_t blocks_y = (N + per_block - 1) / per_block;
     if (blocks_y > 65535) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "N=%lld is too large", (long long)N);
     const dim3 grid((unsigned)T, (unsigned)blocks_y);
-    if (vec) return launch(combine_experts_kernel<8>, grid, kCombineThreads, 0, s, dim3(1), knobs().pdl, p);
-    return launch(combine_experts_kernel<1>, grid, kCombineThreads, 0, s, dim3(1), knobs().pdl, p);
+    auto kernel = add_f32 ? (vec ? combine_experts_kernel<8, true> : combine_experts_kernel<1, true>)
+                          : (vec ? combine_experts_kernel<8, false> : combine_experts_kernel<1, false>);
+    return launch(kernel, grid, kCombineThreads, 0, s, dim3(1), knobs().pdl, p);
+}
+
+int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
+                        int64_t rows, int64_t N, void* stream)
+{
+    return combine_experts(y, weights, places, add, false, out, T, top_k, rows, N, stream);
+}
+
+int gi8_combine_experts_add_f32(const void* y, const float* weights, const int32_t* places, const float* add, void* out, int64_t T, int64_t top_k,
+                                int64_t rows, int64_t N, void* stream)
+{
+    return combine_experts(y, weights, places, add, true, out, T, top_k, rows, N, stream);
 }
 
 }  // extern "C"
@@ -329,10 +342,10 @@ int64_t gi8_experts_scratch_bytes(int64_t T, int64_t H, int64_t I, int64_t E, in
     return experts_scratch(T, H, I, E, top_k).bytes;
 }
 
-int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,
-                const float* gate_up_scale, const int8_t* down, const float* down_scale, const void* add, void* out, void* scratch,
-                int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
-                int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream)
+static int experts_layer(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,
+                         const float* gate_up_scale, const int8_t* down, const float* down_scale, const void* add, bool add_f32, void* out, void* scratch,
+                         int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
+                         int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream)
 {
     // What any step refuses is refused before the first launch: an empty batch goes through the checks of the router, and the limits of
     // the others are looked at here.
@@ -349,7 +362,7 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
     if (T == 0) return GI8_OK;
     if (!x || !logits || !gate_up || !gate_up_scale || !down || !down_scale || !out || !scratch) return fail(GI8_ERR_INVALID_ARGUMENT, "null pointer");
     if (misaligned(x, 16) || misaligned(gate_up, 16) || misaligned(down, 16) || misaligned(scratch, 256) || misaligned(gate_up_scale, 4) || misaligned(down_scale, 4) ||
-        misaligned(logits, logits_dtype == 0 ? 4 : 2) || misaligned(bias, 4) || misaligned(add, 2) || misaligned(out, 2))
+        misaligned(logits, logits_dtype == 0 ? 4 : 2) || misaligned(bias, 4) || misaligned(add, add_f32 ? 4 : 2) || misaligned(out, 2))
         return fail(GI8_ERR_MISALIGNED, "x and weights must be 16-byte aligned, scratch 256-byte aligned, the rest to its elements");
     const ExpertsScratch m = experts_scratch(T, H, I, E, top_k);
     if (scratch_bytes < m.bytes) return fail(GI8_ERR_WORKSPACE, "the layer needs %lld bytes of scratch, got %lld", (long long)m.bytes, (long long)scratch_bytes);
@@ -366,7 +379,25 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
     if (int rc = matmul_experts(i8(m.x_q), gate_up, f32(m.x_scale), gate_up_scale, i32(m.offsets), i32(m.slots), top_k, b + m.h, S, T, E, I, H, 1, stream, true)) return rc;
     if (int rc = gi8_quantize_token(b + m.h, 1, i8(m.h_q), f32(m.h_scale), S, I, stream)) return rc;
     if (int rc = matmul_experts(i8(m.h_q), down, f32(m.h_scale), down_scale, i32(m.offsets), nullptr, 1, b + m.y, S, S, E, H, I, 0, stream, true)) return rc;
-    return gi8_combine_experts(b + m.y, f32(m.weights), i32(m.places), add, out, T, top_k, S, H, stream);
+    return combine_experts(b + m.y, f32(m.weights), i32(m.places), add, add_f32, out, T, top_k, S, H, stream);
+}
+
+int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,
+                const float* gate_up_scale, const int8_t* down, const float* down_scale, const void* add, void* out, void* scratch,
+                int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
+                int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream)
+{
+    return experts_layer(x, x_dtype, logits, logits_dtype, bias, gate_up, gate_up_scale, down, down_scale, add, false, out, scratch, scratch_bytes, T, H, I, E_router, E, first,
+                         top_k, sigmoid, groups, top_groups, group_top2, renormalize, scale, stream);
+}
+
+int gi8_experts_add_f32(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,
+                        const float* gate_up_scale, const int8_t* down, const float* down_scale, const float* add, void* out, void* scratch,
+                        int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
+                        int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream)
+{
+    return experts_layer(x, x_dtype, logits, logits_dtype, bias, gate_up, gate_up_scale, down, down_scale, add, true, out, scratch, scratch_bytes, T, H, I, E_router, E, first,
+                         top_k, sigmoid, groups, top_groups, group_top2, renormalize, scale, stream);
 }
 
 }  // extern "C"

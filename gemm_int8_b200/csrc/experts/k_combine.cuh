@@ -13,14 +13,14 @@ struct CombineParams {
     const uint16_t* y;      // bf16 [rows, N]
     const float* weights;   // [T, k]
     const int32_t* places;  // [T, k]
-    const uint16_t* add;    // bf16 [T, N] or null
+    const void* add;        // fp32 or bf16 [T, N], or null
     uint16_t* out;          // bf16 [T, N]
     int64_t rows;
     int T, N, top_k;
 };
 
-// VEC columns per thread: 8 (16-byte accesses) or 1.
-template <int VEC>
+// VEC columns per thread: 8 (16-byte accesses) or 1.  ADD_F32: `add` is fp32 and starts the sum as it is.
+template <int VEC, bool ADD_F32>
 __global__ void __launch_bounds__(kCombineThreads)
 combine_experts_kernel(const CombineParams p)
 {
@@ -49,10 +49,21 @@ combine_experts_kernel(const CombineParams p)
         }
     };
     if (live && p.add) {
-        uint32_t w[(VEC + 1) / 2];
-        load(p.add + t * p.N + col, w);
+        const int64_t at = t * p.N + col;
+        if constexpr (ADD_F32) {
+            const float* add = static_cast<const float*>(p.add) + at;
+            if constexpr (VEC == 8) {
+                const float4 lo = __ldg(reinterpret_cast<const float4*>(add)), hi = __ldg(reinterpret_cast<const float4*>(add) + 1);
+                acc[0] = lo.x, acc[1] = lo.y, acc[2] = lo.z, acc[3] = lo.w, acc[4] = hi.x, acc[5] = hi.y, acc[6] = hi.z, acc[7] = hi.w;
+            } else {
+                acc[0] = __ldg(add);
+            }
+        } else {
+            uint32_t w[(VEC + 1) / 2];
+            load(static_cast<const uint16_t*>(p.add) + at, w);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) acc[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16));
+            for (int i = 0; i < VEC; ++i) acc[i] = __uint_as_float((i & 1) ? (w[i / 2] & 0xffff0000u) : (w[i / 2] << 16));
+        }
     }
     constexpr int kAhead = 4;  // rows requested together
     for (int j0 = 0; j0 < p.top_k; j0 += kAhead) {

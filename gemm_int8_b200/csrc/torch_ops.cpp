@@ -255,6 +255,15 @@ at::Tensor aligned(const at::Tensor& t, uintptr_t bytes = 16)
     return reinterpret_cast<uintptr_t>(c.data_ptr()) % bytes ? c.clone() : c;
 }
 
+// What a sum starts from: fp32 or bf16, contiguous; undefined without one.
+at::Tensor check_add(const char* name, const std::optional<at::Tensor>& add, at::IntArrayRef shape, const at::Device& device)
+{
+    if (!add.has_value()) return {};
+    float_type(name, "add", *add);
+    check_vector(name, "add", *add, add->scalar_type(), shape, device);
+    return add->contiguous();
+}
+
 std::tuple<at::Tensor, at::Tensor> route_experts(const at::Tensor& logits, const std::optional<at::Tensor>& bias, int64_t top_k, bool sigmoid, int64_t groups,
                                                  int64_t top_groups, bool group_top2, bool renormalize, double scale)
 {
@@ -335,14 +344,13 @@ at::Tensor combine_experts(const at::Tensor& y, const at::Tensor& weights, const
     const int64_t T = weights.size(0), N = y.size(1);
     const c10::cuda::CUDAGuard guard(y.device());
     const at::Tensor yc = y.contiguous(), wc = weights.contiguous(), pc = places.contiguous();
-    at::Tensor ac;
-    if (add.has_value()) {
-        check_vector(name, "add", *add, at::kBFloat16, {T, N}, y.device());
-        ac = add->contiguous();
-    }
+    const at::Tensor ac = check_add(name, add, {T, N}, y.device());
     at::Tensor out = new_tensor({T, N}, at::kBFloat16, y);
-    check(gi8_combine_experts(yc.data_ptr(), f32(wc), static_cast<const int32_t*>(pc.data_ptr()), ac.defined() ? ac.data_ptr() : nullptr, out.data_ptr(), T,
-                              weights.size(1), yc.size(0), N, stream_of(y)));
+    const int32_t* places_p = static_cast<const int32_t*>(pc.data_ptr());
+    if (ac.defined() && ac.scalar_type() == at::kFloat)
+        check(gi8_combine_experts_add_f32(yc.data_ptr(), f32(wc), places_p, f32(ac), out.data_ptr(), T, weights.size(1), yc.size(0), N, stream_of(y)));
+    else
+        check(gi8_combine_experts(yc.data_ptr(), f32(wc), places_p, ac.defined() ? ac.data_ptr() : nullptr, out.data_ptr(), T, weights.size(1), yc.size(0), N, stream_of(y)));
     return out;
 }
 
@@ -364,20 +372,21 @@ at::Tensor int8_experts(const at::Tensor& x, const at::Tensor& logits, const std
     check_scale(name, "down_scale", down_scale, {E, H}, x.device());
     const c10::cuda::CUDAGuard guard(x.device());
     const at::Tensor xc = aligned(x), lc = logits.contiguous(), gs = gate_up_scale.contiguous(), ds = down_scale.contiguous();
-    at::Tensor b, ac;
+    at::Tensor b;
     if (bias.has_value()) {
         check_vector(name, "bias", *bias, at::kFloat, {logits.size(1)}, x.device());
         b = bias->contiguous();
     }
-    if (add.has_value()) {
-        check_vector(name, "add", *add, at::kBFloat16, {T, H}, x.device());
-        ac = add->contiguous();
-    }
+    const at::Tensor ac = check_add(name, add, {T, H}, x.device());
     at::Tensor out = new_tensor({T, H}, at::kBFloat16, x);
     at::Tensor scratch = new_tensor({gi8_experts_scratch_bytes(T, H, I, E, top_k)}, at::kByte, x);
-    check(gi8_experts(xc.data_ptr(), xc.scalar_type() == at::kFloat ? 0 : 1, lc.data_ptr(), logits_dtype, b.defined() ? f32(b) : nullptr, i8(gate_up), f32(gs), i8(down), f32(ds),
-                      ac.defined() ? ac.data_ptr() : nullptr, out.data_ptr(), scratch.data_ptr(), scratch.numel(), T, H, I, logits.size(1), E, first_expert, top_k,
-                      sigmoid, groups, top_groups, group_top2, renormalize, static_cast<float>(scale), stream_of(x)));
+    auto run = [&](auto entry, auto* add_p) {
+        check(entry(xc.data_ptr(), xc.scalar_type() == at::kFloat ? 0 : 1, lc.data_ptr(), logits_dtype, b.defined() ? f32(b) : nullptr, i8(gate_up), f32(gs), i8(down), f32(ds),
+                    add_p, out.data_ptr(), scratch.data_ptr(), scratch.numel(), T, H, I, logits.size(1), E, first_expert, top_k, sigmoid, groups, top_groups, group_top2,
+                    renormalize, static_cast<float>(scale), stream_of(x)));
+    };
+    if (ac.defined() && ac.scalar_type() == at::kFloat) run(gi8_experts_add_f32, f32(ac));
+    else run(gi8_experts, ac.defined() ? ac.data_ptr() : nullptr);
     return out;
 }
 

@@ -85,7 +85,7 @@ def matmul_experts_swiglu(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.T
 def combine_experts(y: torch.Tensor, weights: torch.Tensor, places: torch.Tensor, add: torch.Tensor | None = None) -> torch.Tensor:
     """Weighted sum of every token's rows: ``out[t] = bf16( add[t] + sum_j weights[t, j] * y[places[t, j]] )`` in fp32, ascending j.
 
-    y bf16 [rows, N], weights fp32 [T, top_k], places int32 [T, top_k] (negative: left out), add bf16 [T, N] or None; top_k <= 32.
+    y bf16 [rows, N], weights fp32 [T, top_k], places int32 [T, top_k] (negative: left out), add fp32 or bf16 [T, N] or None; top_k <= 32.
     """
     return _combine(y, weights, places, add)
 
@@ -170,7 +170,10 @@ class Int8Experts(torch.nn.Module):
         return cls(*_quantize_experts(gate_up), *_quantize_experts(down), top_k, **router)
 
     def forward(self, x: torch.Tensor, logits: torch.Tensor, add: torch.Tensor | None = None) -> torch.Tensor:
-        """x [..., hidden], logits [..., experts of the router], add (the residual stream, a shared expert's result) [..., hidden] -> bf16 [..., hidden]."""
+        """x [..., hidden], logits [..., experts of the router], add (the residual stream, a shared expert's result) [..., hidden] -> bf16 [..., hidden].
+
+        x, logits and add are taken as they are in fp32 and bf16.  Of other types, x goes to bf16, as in `Int8Linear`, logits and add to fp32.
+        """
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         if x2.dtype not in (torch.float32, torch.bfloat16):
             x2 = x2.to(torch.bfloat16)
@@ -178,7 +181,9 @@ class Int8Experts(torch.nn.Module):
         if logits.dtype not in (torch.float32, torch.bfloat16):
             logits = logits.to(torch.float32)
         if add is not None:
-            add = add.reshape(x2.shape).to(torch.bfloat16)
+            add = add.reshape(x2.shape)
+            if add.dtype not in (torch.float32, torch.bfloat16):
+                add = add.to(torch.float32)
         out = _layer(x2, logits, self.bias, self.gate_up_q, self.gate_up_scale, self.down_q, self.down_scale, *self._router,
                                                     self.first_expert, add)
         return out if x.dim() == 2 else out.reshape(x.shape)

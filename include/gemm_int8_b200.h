@@ -257,14 +257,16 @@ int gi8_matmul_experts(const int8_t* x, const int8_t* w, const float* sx, const 
 
 /*
  * out[t,n] = bf16( add[t,n] + sum_j weights[t,j] * y[places[t,j],n] ), one fp32 fused multiply-add per choice in ascending j; places below
- * zero (or at or above `rows`) are left out, add (bf16 [T,N]) may be NULL.  y bf16 [rows,N], out bf16 [T,N]; top_k <= 32.
+ * zero (or at or above `rows`) are left out, add (bf16 [T,N]; fp32 in the second form) may be NULL.  y bf16 [rows,N], out bf16 [T,N]; top_k <= 32.
  */
 int gi8_combine_experts(const void* y, const float* weights, const int32_t* places, const void* add, void* out, int64_t T, int64_t top_k,
                         int64_t rows, int64_t N, void* stream);
+int gi8_combine_experts_add_f32(const void* y, const float* weights, const int32_t* places, const float* add, void* out, int64_t T, int64_t top_k,
+                                int64_t rows, int64_t N, void* stream);
 
 /*
  * The whole layer: route, group, quantise the tokens per row, gate and up product with SwiGLU, quantise its rows, down product, weighted sum
- * (onto add [T,H] bf16, or NULL) into out bf16 [T,H]; the results of these steps, one after the other, bit for bit.
+ * (onto add [T,H], bf16 or in the second form fp32, or NULL) into out bf16 [T,H]; the results of these steps, one after the other, bit for bit.
  *   x        [T,H] fp32 (x_dtype 0) or bf16 (1), 16-byte aligned;  logits [T,E_router]
  *   gate_up  int8 [E,2I,H], gate_up_scale fp32 [E,2I];  down int8 [E,H,I], down_scale fp32 [E,H]: experts first .. first + E - 1 of the router's,
  *            the sum runs over those of a token's choices that are among them
@@ -277,6 +279,10 @@ int gi8_experts(const void* x, int x_dtype, const void* logits, int logits_dtype
                 const float* gate_up_scale, const int8_t* down, const float* down_scale, const void* add, void* out, void* scratch,
                 int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
                 int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream);
+int gi8_experts_add_f32(const void* x, int x_dtype, const void* logits, int logits_dtype, const float* bias, const int8_t* gate_up,
+                        const float* gate_up_scale, const int8_t* down, const float* down_scale, const float* add, void* out, void* scratch,
+                        int64_t scratch_bytes, int64_t T, int64_t H, int64_t I, int64_t E_router, int64_t E, int64_t first, int64_t top_k, int sigmoid,
+                        int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream);
 
 /*
  * Forces a kernel variant for the calling process (tuning and tests); NULL or "" restores the fitted

@@ -49,3 +49,14 @@ def test_more_tiles_than_are_counted(call):
     assert call("product", E=1024, rows=2 ** 28, tokens=2 ** 28) == 2
     assert call("product", E=1024, rows=2 ** 27, tokens=2 ** 27) == 2 and call("product", E=1024, rows=2 ** 27, tokens=4, slots=call.base, k=2) == 2
     assert call("product", E=100, rows=2 ** 31 - 300, tokens=2 ** 31 - 300) == 2
+
+
+def test_fp32_forms_refuse_as_the_others_do(call, monkeypatch):
+    """The C entries whose sum starts from fp32: the checks of the bf16 ones, and alignment to four bytes."""
+    C = call.C
+    for name, f32 in (("gi8_combine_experts", C.gi8_combine_experts_add_f32), ("gi8_experts", C.gi8_experts_add_f32)):
+        monkeypatch.setattr(C, name, f32)
+    assert call("combine", k=0) == 2 and call("combine", T=-1) == 1 and call("combine", y=None) == 1 and call("combine", T=0) == 0
+    assert call("combine", add=call.base + 2) == 3 and call("combine", out=call.base + 1) == 3
+    assert call("layer", H=72) == 2 and call("layer", E=9) == 1 and call("layer", scratch=None) == 1 and call("layer", T=0) == 0
+    assert call("layer", add=call.base + 2) == 3
