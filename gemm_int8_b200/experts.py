@@ -172,11 +172,12 @@ class Int8Experts(torch.nn.Module):
     def forward(self, x: torch.Tensor, logits: torch.Tensor, add: torch.Tensor | None = None) -> torch.Tensor:
         """x [..., hidden], logits [..., experts of the router], add (the residual stream, a shared expert's result) [..., hidden] -> bf16 [..., hidden].
 
-        x, logits and add are taken as they are in fp32 and bf16.  Of other types, x goes to bf16, as in `Int8Linear`, logits and add to fp32.
+        x, logits and add are taken as they are in fp32 and bf16.  Of other types, fp16 activations go to bf16, as in `Int8Linear`, and everything
+        else to fp32.
         """
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         if x2.dtype not in (torch.float32, torch.bfloat16):
-            x2 = x2.to(torch.bfloat16)
+            x2 = x2.to(torch.bfloat16 if x2.dtype == torch.float16 else torch.float32)
         logits = logits.reshape(-1, logits.shape[-1])
         if logits.dtype not in (torch.float32, torch.bfloat16):
             logits = logits.to(torch.float32)

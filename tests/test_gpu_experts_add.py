@@ -48,3 +48,4 @@ def test_layer_onto_other_types(T):
     assert torch.equal(layer(x, logits, add.double()), want)
     assert torch.equal(layer(x, logits, add.half()), _step_by_step(layer, x, logits, add.half().float()))
     assert torch.equal(layer(x, logits, add.bfloat16()), _step_by_step(layer, x, logits, add.bfloat16()))
+    assert torch.equal(layer(x.double(), logits.double(), add), want)  # activations and logits of 64 bits go to fp32
