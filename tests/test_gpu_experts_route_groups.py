@@ -43,3 +43,48 @@ def test_masks_and_favours_of_the_largest_magnitude(E, groups, group_score, scor
     bias = torch.randn(groups, size, generator=gen)
     bias[:, 0], bias[:, 1] = top, top * torch.linspace(0.1, 0.9, groups)
     _check(logits, min(2 * size, 8), scoring=scoring, bias=bias.reshape(E), groups=groups, top_groups=2, group_score=group_score)
+
+
+@pytest.mark.parametrize("E,groups,top_groups", [(60, 5, 2), (72, 4, 2), (250, 5, 3), (256, 8, 4)])
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_ties_of_groups(E, groups, top_groups, group_score, scoring, biased):
+    """Equal groups whatever way their values are looked up, and more equal candidates than a warp has lanes."""
+    logits = torch.randint(-2, 3, (40, E), generator=torch.Generator().manual_seed(E)).float()
+    logits[0] = 0.0
+    logits[1, ::2] = -0.0
+    logits[2, :E // 2] = -float("inf")
+    bias = torch.zeros(E) if biased else None
+    for k in (1, 8, min(32, top_groups * E // groups)):
+        _check(logits, k, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_score=group_score)
+
+
+@pytest.mark.parametrize("E,groups", [(60, 5), (72, 4), (256, 8)])
+@pytest.mark.parametrize("group_score", ["max", "top2"])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_groups_that_only_fp32_sees_as_equal(E, groups, group_score, scoring, biased):
+    """The best two groups' values differ by less than fp32 resolves, in either direction: by a bias that makes them equal up to its own rounding, or
+    (without one) by logits whose scores do."""
+    gen = torch.Generator().manual_seed(E + 1)
+    n = 1 if group_score == "max" else 2
+    size = E // groups
+    for t in range(20):
+        logits = torch.randn(1, E, generator=gen)
+        if biased:
+            score = torch.softmax(logits.double(), 1) if scoring == "softmax" else torch.sigmoid(logits.double())
+            by_group = score.reshape(groups, size).sort(dim=1, descending=True)
+            value = by_group.values[:, :n].sum(1)
+            best, next_best = value.topk(2).indices.tolist()
+            bias = torch.zeros(groups, size)
+            bias[next_best, by_group.indices[next_best, 0]] = (value[best] - value[next_best]).float()
+            bias = bias.reshape(E)
+        else:
+            # the same logits in all groups, in other orders, one of them moved by an ulp or none
+            bias = None
+            row = torch.randn(size, generator=gen)
+            logits = torch.stack([row[torch.randperm(size, generator=gen)] for _ in range(groups)]).reshape(1, E)
+            i = int(torch.randint(0, E, (1,), generator=gen))
+            logits[0, i] = torch.nextafter(logits[0, i], torch.tensor(float(t % 3 - 1) * 10))
+        _check(logits, 4, scoring=scoring, bias=bias, groups=groups, top_groups=1, group_score=group_score)
