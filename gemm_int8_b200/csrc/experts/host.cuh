@@ -60,7 +60,7 @@ int launch_route_for(RouteParams p, int sms, cudaStream_t s)
     GI8_ROUTE(1)
     GI8_ROUTE(2)
     GI8_ROUTE(4)
-    GI8_ROUTE(5)
+    GI8_ROUTE(5)  // 129 to 160 experts (160 with groups, bias: 4096 tokens 8.8 us, eight to a lane 15.0; 16 tokens 3.4 and 4.2)
     GI8_ROUTE(8)
     GI8_ROUTE(16)
     GI8_ROUTE(32)
@@ -125,10 +125,15 @@ int launch_experts(DeviceState* st, int slot, const int8_t* w, ExpertsParams p, 
 //   up to 64   one-CTA tiles of 64 tokens, two CTAs per SM, so that the next launch's CTAs can sit down beside this one's; where the tiles
 //              leave SMs without one for long, tiles of 32 tokens with ten stages, more bytes in flight for the few
 //   more       two-CTA tiles of 256 tokens
-// us (graph replays), tiles of 64 / 256 tokens, at so many rows per expert on average: E = 64, k = 8, product 4096 x 1408: 32 59.6 / 57.8,
-// 64 68.4 / 66.1, 128 97.9 / 76.3; SwiGLU 1408 x 4096: 32 113.6 / 119.4, 64 132 / 139, 128 183 / 157; E = 8, k = 2, product 4096 x 14336: 32
-// 74.8 / 78.9, 64 96.3 / 81.7.  (One-CTA tiles of 128 tokens were level with or behind the better of the two everywhere.)  One token to two
-// experts, product 4096 x 14336, 64 tiles: 40.0, ten stages 32.0 (one to six, 2048 x 1408, 96 short tiles: 8.3 and 9.7).
+// us (graph replays), tiles of 64 / 256 tokens, at 32, 40, 48, 64 and 128 rows per expert on average (the rule changes over at 43):
+//   E = 64, k = 8, product 4096 x 1408, rows in order  59.4 / 57.0   63.6 / 63.2   64.6 / 63.6   67.3 / 65.4   94.4 / 74.1
+//                                       gathered       61.7 / 61.4   64.7 / 64.9   67.4 / 65.3   68.9 / 67.7   99.2 / 76.6
+//   SwiGLU 1408 x 4096, rows in order                   110 / 115     121 / 122     118 / 125     127 / 126     194 / 136
+//                       gathered                        112 / 120     120 / 123     120 / 123     128 / 126     207 / 140
+//   E = 8, k = 2, product 4096 x 14336, rows in order  73.8 / 78.7   75.9 / 81.0   97.3 / 80.8   95.5 / 82.0
+// One limit for all of them is within 6 % of the better form here.  (One-CTA tiles of 128 tokens were level with or behind the better of the
+// two everywhere.)  One token to two experts, product 4096 x 14336, 64 tiles: 40.0, ten stages 32.0 (one to six, 2048 x 1408, 96 short
+// tiles: 8.3 and 9.7).
 enum ExpertsForm { EXPERTS_FEW, EXPERTS_64, EXPERTS_256 };
 
 ExpertsForm experts_form(const ExpertsParams& p, bool swiglu, int sms)

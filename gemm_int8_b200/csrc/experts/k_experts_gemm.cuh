@@ -9,7 +9,7 @@
 // whose extent is an operand of the instruction: a tile of r rows costs roundup(r, 16) columns instead of a multiple of 128, which
 // is what makes ragged groups and single tokens cheap.  An expert's rows are cut into equal tiles of at most BT.
 //
-// Structure (one persistent CTA per SM, 192 threads, 320 with GATHER), as in the dense kernel:
+// Structure (persistent CTAs, one per SM, two of 64-token tiles; 192 threads, 320 with GATHER), as in the dense kernel:
 //   warp 0      TMA producer: weight tiles (128 rows x 128 bytes) and token rows, either with one instruction
 //   warp 1      MMA issuer, kind::i8, two accumulators in tensor memory
 //   next 4      epilogue: accumulators come as pairs of tokens of a channel, are scaled in packed arithmetic, and turned by stmatrix into runs of
@@ -18,7 +18,7 @@
 //   last 4      (GATHER) token rows from wherever they lie, by 16-byte asynchronous copies into the places where TMA's 128-byte swizzle
 //               would put them: eight lanes a row, a whole line per row; their arrivals follow the copies by themselves, and the issuer
 //               makes them visible to the tensor core behind its wait.  SwiGLU of 4096 tokens to 8 of 64 experts, 4096 x 4096, took
-//               458 us for 428 with loader warps that wait for their copies, two stages behind those they issue.  TMA's own gather,
+//               472 us for 454 with loader warps that wait for their copies, two stages behind those they issue.  TMA's own gather,
 //               four rows an instruction, delivers a row in 14 cycles: 32768 rows gathered for 4096 x 4096 that way took 2010 us, put
 //               in order by a pass in front 475, rows that lie in order 446.
 // SWIGLU: a weight tile is 64 gate rows and their 64 up rows in alternating runs of 16, so that gate and up of a channel lie 16 lanes of tensor

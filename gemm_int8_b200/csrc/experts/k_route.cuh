@@ -9,19 +9,21 @@
 //           and where fewer are left the places hold expert -1 and weight 0
 //   weight  w_j = s_chosen(j) (/ their sum) * scale
 //
-// Exactness: which of two experts is chosen must not depend on how a score was rounded to fp32.  A token is decided by fp32 scores, with a
-// bound on their error.  Where two neighbours in the order, or the last group kept and the first one dropped, lie closer than that, the
-// token is marked and decided again behind the loop over the warp's tokens: the groups' values in fp64, and the candidates, which are
-// those chosen and what lies as close behind them, put in order by their choices in fp64, a lane each.  One token in a thousand or so
-// comes there, and the warp that it holds up may be the launch's last: what counts is how long it takes (all of a token's scores in fp64 and the
-// whole selection again took 13 us, and the launch of 16384 tokens 39), and that it costs the other tokens no registers.
+// Exactness: which of two experts is chosen must not depend on how a score was rounded to fp32: what is equal in fp64 is equal, and nothing else.
+// A token is decided by fp32 scores, with a bound on their error.  Where two neighbours in the order, or a group kept and one dropped, lie closer
+// than that, the token is marked and decided again behind the loop over the warp's tokens: the groups' values in fp64, and the candidates,
+// which are those chosen and what lies as close behind them, put in order by their choices in fp64, a lane each.  Of tokens whose logits are
+// spread over all of fp32 one in a thousand or so comes there, and the warp that it holds up may be the launch's last: what counts is how long
+// it takes (all of a token's scores in fp64 and the whole selection again took 13 us, and the launch of 16384 tokens 39), and that it costs the
+// other tokens no registers.  Equal fp32 logits are marked as well: 16384 tokens whose 256 fp32 logits hold bf16 values take 30 us for 14.9 (as
+// bf16 tensors, whose keys lose nothing, 13.4).
 //
 // One warp per token; a lane holds V consecutive experts, so that the groups of the usual models are runs of whole lanes.  The choices become
 // unsigned keys whose lowest bits are the place within the lane, sorted in every lane, so that a round of the selection is one maximum over
 // the lanes' first keys and a shift of the winner's lane.  Up to four tokens' weights (eight experts each) are made together, a lane each.
-// Bound by instruction issue and latencies: 16384 tokens of 256 experts, bias, groups 26.8 us (about 1000 instructions a token, issued in 60 % of
+// Bound by instruction issue and latencies: 16384 tokens of 256 experts, bias, groups 25.7 us (890 instructions a token, issued in 60 % of
 // the cycles; 1735 and 38 us with whole choices and indices apart), of which the bytes take 2.7; the selection alone, without bias and groups,
-// 14.5; 16 tokens 4.1, of which an empty launch takes 1.8.
+// 14.9; 16 tokens 3.9, of which an empty launch takes 1.8.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -34,9 +34,9 @@ def route_experts(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bi
     ``weights = score of the chosen (/ their sum) * scale``.
 
     A logit (or bias) of -inf masks an expert, and so does NaN; a logit of +inf counts as the largest finite value of fp32, so that a softmax
-    shares its weight among the infinite ones.  Where fewer than top_k experts are left, the remaining places hold
-    expert -1 and weight 0, which the operators below skip.  Near ties are decided as in exact arithmetic, not by how fp32 rounds a
-    score.  E <= 1024, top_k <= 32, groups <= 32.
+    shares its weight among the infinite ones.  Where fewer than top_k experts are left, the remaining places hold expert -1 and weight 0,
+    which the operators below skip.  Near ties are decided by the values in 64 bits, not by how fp32 rounds a score.  E <= 1024,
+    top_k <= 32, groups <= 32.
     """
     try:
         sigmoid, top2 = _SIGMOID[scoring], _TOP2[group_score]

@@ -220,10 +220,9 @@ int gi8_linear(const void* x, int x_dtype, const int8_t* w, const float* w_scale
  *   themselves, of which s is an increasing function
  *   groups  the experts form `groups` runs of E / groups; a group's value is its largest choice or, with group_top2, the sum of its
  *           two largest (without a bias, of the scores); only the best top_groups groups keep their experts
- *   chosen  the top_k largest choices in descending order, the lower index first among equals.  Decided as in exact arithmetic: where fp32
+ *   chosen  the top_k largest choices in descending order, the lower index first among equals.  Decided by the values in 64 bits: where fp32
  *           cannot tell two choices apart the token is decided in fp64.  A choice of -inf or NaN is never chosen, a logit of +inf counts as
- *           fp32's largest finite value; where fewer than top_k
- *           are left, the places hold expert -1 and weight 0
+ *           fp32's largest finite value; where fewer than top_k are left, the places hold expert -1 and weight 0
  *   weights [T,top_k] fp32 = s of the chosen (renormalize: / their sum) * scale;  experts [T,top_k] int32
  *   E <= 1024, top_k <= 32, groups <= 32.
  */
