@@ -35,3 +35,22 @@ def test_infinite_logits(E, groups, top_groups, group_score, scoring, biased, re
     # scores of finite logits within 10 of one another or 0 beside the infinite ones: expf 2 ulp and its argument, twice, and 40 roundings
     rel = 2 * (2 ** -22 + 10 * 2 ** -24) + 40 * 2 ** -24
     assert ((w.cpu().double() - w_ref).abs() <= rel * w_ref).all()
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,top_groups,group_score", [(8, 1, 1, "max"), (64, 1, 1, "max"), (64, 8, 2, "max"), (64, 8, 2, "top2"), (60, 5, 2, "top2"), (72, 4, 1, "max")])
+def test_infinite_biases(E, groups, top_groups, group_score, scoring):
+    """A bias of +inf always chooses its expert, the lower index first; the weights do not see it."""
+    import gemm_int8_b200 as g
+
+    gen = torch.Generator().manual_seed(E)
+    logits = torch.randn(9, E, generator=gen)
+    logits[0, 3] = -math.inf
+    for favoured in ([3], [3, 5], [1, 2, 3, E - 1], list(range(0, E, 2)), list(range(E))):
+        bias = torch.randn(E, generator=gen) * 0.1
+        bias[favoured] = math.inf
+        w, e = g.route_experts(logits.cuda(), 4, scoring=scoring, bias=bias.cuda(), groups=groups, top_groups=top_groups, group_score=group_score)
+        w_ref, e_ref = R.route(logits, 4, scoring=scoring, bias=bias, groups=groups, top_groups=top_groups, group_score=group_score)
+        assert torch.equal(e.cpu(), e_ref)
+        rel = 2 * (2 ** -22 + 10 * 2 ** -24) + 40 * 2 ** -24  # (as above)
+        assert ((w.cpu().double() - w_ref).abs() <= rel * w_ref).all()
