@@ -9,7 +9,8 @@ Mirrors gemm_int8/__init__.py of the reference:
 
 and adds the W8A8 entry points the reference lacks: ``matmul_scaled`` (per-token x per-channel scales)
 and ``matmul_blockwise`` (per-token-per-128-K activation scales, per-128x128 weight scales).
-``experts`` holds the operators of a mixture-of-experts layer on such products, and the layer.
+``experts`` holds the operators of a mixture-of-experts layer on such products, and the layer; ``ffn`` the operators around the
+products of a feed-forward block (norm and SwiGLU with 8-bit results) and the block-scaled product in 8-bit floating point.
 
 The schemas and fake kernels of the torch ops are defined here; their CUDA implementations are a thin C++ layer
 (csrc/torch_ops.cpp) over the C ABI of ``libgemm_int8_b200.so`` (raw device pointers and the current CUDA stream).  Importing this package without the compiled
@@ -41,6 +42,12 @@ _libdef.define("quantize_token_block(Tensor a) -> (Tensor, Tensor)")
 _libdef.define("quantize_token(Tensor a) -> (Tensor, Tensor)")
 _libdef.define("hadamard_quantize_token_block(Tensor a, int block) -> (Tensor, Tensor)")
 _libdef.define("int8_linear(Tensor x, Tensor weight_q, Tensor weight_scale, Tensor? bias, bool blockwise, int? hadamard) -> Tensor")
+
+_libdef.define("rms_norm_quantize(Tensor x, Tensor weight, Tensor? residual, float eps, bool blockwise, bool e4m3) -> (Tensor, Tensor, Tensor)")
+_libdef.define("swiglu_quantize(Tensor gate_up, bool blockwise, bool e4m3) -> (Tensor, Tensor)")
+_libdef.define("fp8_quantize_token_block(Tensor a) -> (Tensor, Tensor)")
+_libdef.define("fp8_matmul_blockwise(Tensor A, Tensor B, Tensor A_scale, Tensor B_scale) -> Tensor")
+_libdef.define("fp8_linear(Tensor x, Tensor weight_q, Tensor weight_scale, Tensor? bias) -> Tensor")
 
 _libdef.define("route_experts(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int groups, int top_groups, bool group_top2, bool renormalize, "
                "float scale) -> (Tensor, Tensor)")
@@ -224,11 +231,16 @@ def _(a: torch.Tensor):
             torch.empty(a.shape[0], device=a.device, dtype=torch.float32))
 
 
-def quantize_per_token_block(a: torch.Tensor):
+def quantize_per_token_block(a: torch.Tensor, dtype: torch.dtype = torch.int8):
     """Fused activation quantiser for `matmul_blockwise`: a [M, K] fp32/bf16 (CUDA) -> (q int8 [M, K],
     scales fp32 [M, ceil(K/128)]), one symmetric scale per token per 128-wide K block (amax / 127, round half
-    even, clamp to +-127) -- bit-identical to `quant.quantize_per_token_block`."""
-    return torch.ops.gemm_int8_CUDA.quantize_token_block(a)
+    even, clamp to +-127) -- bit-identical to `quant.quantize_per_token_block`.
+    dtype=torch.float8_e4m3fn: the same for `matmul_blockwise_fp8` (amax / 448, rounded half to even)."""
+    if dtype == torch.int8:
+        return torch.ops.gemm_int8_CUDA.quantize_token_block(a)
+    if dtype != torch.float8_e4m3fn:
+        raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
+    return torch.ops.gemm_int8_CUDA.fp8_quantize_token_block(a)
 
 
 def hadamard_quantize_per_token_block(a: torch.Tensor, block: int | None = None):
@@ -286,10 +298,11 @@ if _os.environ.get("GEMM_INT8_KERNEL"):
     force_variant(_os.environ["GEMM_INT8_KERNEL"])
 
 
-from .linear import Int8Linear  # noqa: E402
+from .linear import Fp8Linear, Int8Linear  # noqa: E402
+from .ffn import matmul_blockwise_fp8, rms_norm_quantize, swiglu_quantize  # noqa: E402
 from .experts import Int8Experts, combine_experts, group_by_expert, matmul_experts, matmul_experts_swiglu, route_experts  # noqa: E402
 
 __all__ = ["matmul", "matmul_i32", "matmul_scaled", "matmul_blockwise", "matmul_blockwise_f32", "sum_parts_bf16",
            "quantize_per_token_block",
-           "quantize_per_token", "Int8Linear", "route_experts", "group_by_expert", "matmul_experts", "matmul_experts_swiglu", "combine_experts", "Int8Experts",
+           "quantize_per_token", "Int8Linear", "rms_norm_quantize", "swiglu_quantize", "matmul_blockwise_fp8", "Fp8Linear", "route_experts", "group_by_expert", "matmul_experts", "matmul_experts_swiglu", "combine_experts", "Int8Experts",
            "force_variant", "pick_variant", "device_status", "check_device", "reload_env"]

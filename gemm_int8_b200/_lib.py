@@ -57,6 +57,11 @@ SYMBOLS = {
     "gi8_experts_scratch_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "gi8_experts": (_i, [_p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i64, _i64, _i, _i, _f, _p]),
     "gi8_experts_add_f32": (_i, [_p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i64, _i64, _i, _i, _f, _p]),
+    "gi8_rms_norm_quantize": (_i, [_p, _i, _p, _i, _p, _i, _f, _p, _p, _i, _p, _i, _i64, _i64, _p]),
+    "gi8_swiglu_quantize": (_i, [_p, _i, _p, _i, _p, _i, _i64, _i64, _p]),
+    "gi8_fp8_quantize_token_block": (_i, [_p, _i, _p, _p, _i64, _i64, _p]),
+    "gi8_fp8_matmul_blockwise": (_i, [_p, _p, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _p]),
+    "gi8_fp8_linear": (_i, [_p, _i, _p, _p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _p]),
     "gi8_force_variant": (_i, [ctypes.c_char_p]),
     "gi8_pick_variant": (ctypes.c_char_p, [_i, _i64, _i64, _i64]),
     "gi8_device_status": (_i, [ctypes.POINTER(ctypes.c_uint32)]),

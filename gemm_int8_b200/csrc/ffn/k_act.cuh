@@ -1,0 +1,138 @@
+// Elementwise activations in 8 bits: the e4m3 quantiser, and SwiGLU behind the product of gate and up rows,
+//   v = g / (1 + exp(-g)) u   of the two halves of a row,   in fp32 from fp32 or bf16,
+// with a scale per row and 128 columns, or (SwiGLU in int8) one per row.  Bound: HBM; every element is read and written once.
+#pragma once
+
+#include "out8.cuh"
+
+namespace gi8 {
+
+struct ActParams {
+    const void* in;  // [M, K], SwiGLU: [M, 2 K]
+    uint8_t* q;      // [M, K]
+    float* s;        // [M, KB] or [M]
+    int64_t M;
+    int K, KB;
+};
+
+// (an overflowing exponential gives -0, the limit; the quick exponential and division are good to about 1e-6, next to the half step of
+// 1/254 or 2^-4 that the result is rounded by)
+GI8_DEVICE float silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+template <typename T, bool SWIGLU>
+struct ActRaw {
+    Raw8<T> a, b;
+};
+
+template <typename T>
+struct ActRaw<T, false> {
+    Raw8<T> a;
+};
+
+template <typename T, bool SWIGLU>
+GI8_DEVICE ActRaw<T, SWIGLU> act_load(const ActParams& p, int64_t row, int col, bool in)
+{
+    ActRaw<T, SWIGLU> r;
+    const T* at = static_cast<const T*>(p.in) + row * (SWIGLU ? 2 : 1) * static_cast<int64_t>(p.K) + col;
+    r.a = in ? load8(at) : zero8<T>();
+    if constexpr (SWIGLU) r.b = in ? load8(at + p.K) : zero8<T>();
+    return r;
+}
+
+template <typename T, bool SWIGLU>
+GI8_DEVICE void act_values(const ActRaw<T, SWIGLU>& r, uint64_t (&v)[4])
+{
+    unpack8<T>(r.a, v);
+    if constexpr (SWIGLU) {
+        uint64_t w[4];
+        unpack8<T>(r.b, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float g0, g1, u0, u1;
+            f32x2_split(v[i], g0, g1), f32x2_split(w[i], u0, u1);
+            v[i] = f32x2(silu_times(g0, u0), silu_times(g1, u1));
+        }
+    }
+}
+
+constexpr int kActThreads = 256;
+
+// A scale per 128 columns: sixteen lanes of eight values each.  A work item is 2 LOADS consecutive blocks of a row, for one warp.
+template <typename T, bool SWIGLU, Out8 OUT, int LOADS>
+__global__ void __launch_bounds__(kActThreads) act_quantize_block_kernel(const ActParams p)
+{
+    quant_dependency();
+    const int lane = threadIdx.x & 31;
+    const uint32_t groups = static_cast<uint32_t>((p.KB + 2 * LOADS - 1) / (2 * LOADS));
+    const uint32_t items = static_cast<uint32_t>(p.M) * groups;  // the host checks that this fits
+    const uint32_t step = gridDim.x * (kActThreads / 32);
+    for (uint32_t item = blockIdx.x * (kActThreads / 32) + (threadIdx.x >> 5); item < items; item += step) {
+        const uint32_t row = item / groups;
+        const int col0 = static_cast<int>(item - row * groups) * (2 * LOADS * 128) + lane * 8;
+        ActRaw<T, SWIGLU> raw[LOADS];
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) raw[u] = act_load<T, SWIGLU>(p, row, col0 + u * 256, col0 + u * 256 < p.K);
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int col = col0 + u * 256;
+            uint64_t v[4];
+            act_values<T, SWIGLU>(raw[u], v);
+            const QuantScale qs = make_out_scale<OUT>(lanes_max_nan<16>(amax8_nan(v)));
+            if (col < p.K) {
+                if ((lane & 15) == 0) p.s[static_cast<int64_t>(row) * p.KB + (col >> 7)] = qs.s;
+                *reinterpret_cast<uint2*>(p.q + static_cast<int64_t>(row) * p.K + col) = out8_pack8<OUT>(v, qs);
+            }
+        }
+    }
+}
+
+// SwiGLU with a scale per row: a CTA per row.  LOADS x 8 values a thread stay in registers between the maximum and the quantisation;
+// what lies beyond them is read and computed twice (it hits L2).
+template <typename T, Out8 OUT, int LOADS>
+__global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActParams p)
+{
+    quant_dependency();
+    __shared__ float slots[2][32];
+    const int span = blockDim.x * 8, warps = blockDim.x >> 5;
+    int parity = 0;
+    for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x, parity ^= 1) {
+        ActRaw<T, true> raw[LOADS];
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int col = u * span + threadIdx.x * 8;
+            raw[u] = act_load<T, true>(p, row, col, col < p.K);
+        }
+        uint64_t v[LOADS][4];
+        float m = 0.0f;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            act_values<T, true>(raw[u], v[u]);
+            m = max_nan(m, amax8_nan(v[u]));
+        }
+        for (int col = LOADS * span + threadIdx.x * 8; col < p.K; col += span) {
+            uint64_t w[4];
+            act_values<T, true>(act_load<T, true>(p, row, col, true), w);
+            m = max_nan(m, amax8_nan(w));
+        }
+        m = lanes_max_nan<32>(m);
+        // (two sets of slots in turn: one barrier per row is enough)
+        if ((threadIdx.x & 31) == 0) slots[parity][threadIdx.x >> 5] = m;
+        __syncthreads();
+        m = (threadIdx.x & 31) < warps ? slots[parity][threadIdx.x & 31] : 0.0f;
+        const QuantScale qs = make_out_scale<OUT>(lanes_max_nan<32>(m));
+        if (threadIdx.x == 0) p.s[row] = qs.s;
+        uint8_t* q = p.q + row * p.K;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int col = u * span + threadIdx.x * 8;
+            if (col < p.K) *reinterpret_cast<uint2*>(q + col) = out8_pack8<OUT>(v[u], qs);
+        }
+        for (int col = LOADS * span + threadIdx.x * 8; col < p.K; col += span) {
+            uint64_t w[4];
+            act_values<T, true>(act_load<T, true>(p, row, col, true), w);
+            *reinterpret_cast<uint2*>(q + col) = out8_pack8<OUT>(w, qs);
+        }
+    }
+}
+
+}  // namespace gi8

@@ -1,0 +1,147 @@
+// Root-mean-square norm of x (+ residual) in 8 bits, and the sum:
+//   h = x + residual (fp32),  total = h rounded to the residual's type,  r = (mean(h^2) + eps)^-1/2,  v = (h r) weight,
+//   q, s = 8-bit values and scales of v (out8.cuh), a scale per 128 columns or one per row.
+// The norm is of the sum in fp32, not of the total that is stored: one rounding less on the way to q.
+//
+// One pass: a row is read once, stays in registers (8 LOADS values a thread) while its squares, and with per-row scales its largest
+// magnitude, are summed up across its warps, and is written once.  Bound: HBM.
+#pragma once
+
+#include <type_traits>
+
+#include "out8.cuh"
+
+namespace gi8 {
+
+constexpr int kNormThreads = 512;  // of a CTA, at most
+
+struct NormParams {
+    const void* x;         // [M, H]
+    const void* residual;  // [M, H]
+    const void* weight;    // [H]
+    void* total;           // [M, H]; may be the residual or x itself: a thread writes what it alone has read
+    uint8_t* q;            // [M, H]
+    float* s;              // [M, KB] or [M]
+    int64_t M;
+    int H, KB;
+    int row_warps;         // warps of a row: all of the CTA's, or one
+    float eps, inv_h;
+};
+
+// The sum of the row's values over its warps' lanes, in a fixed order (MAX: their maximum).
+template <bool MAX>
+GI8_DEVICE float row_reduce(float v, float* slots, int row_warps)
+{
+    auto warp_all = [](float x) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const float w = __shfl_xor_sync(0xffffffffu, x, o);
+            x = MAX ? max_nan(x, w) : x + w;
+        }
+        return x;
+    };
+    v = warp_all(v);
+    if (row_warps == 1) return v;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_all(lane < row_warps ? slots[lane] : 0.0f);
+}
+
+template <typename TX, typename TR, typename TW, Out8 OUT, bool BLOCK, int LOADS>
+__global__ void __launch_bounds__(kNormThreads) rms_norm_quantize_kernel(const NormParams p)
+{
+    quant_dependency();
+    constexpr bool RESIDUAL = !std::is_same<TR, void>::value;
+    using TS = typename std::conditional<RESIDUAL, TR, TX>::type;
+    __shared__ float slots[3][32];
+    const int row_threads = p.row_warps * 32;
+    const int t = p.row_warps == 1 ? threadIdx.x & 31 : threadIdx.x;
+    const int64_t row = p.row_warps == 1 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
+    const bool live = row < p.M;
+    const int64_t base = row * p.H;
+
+    Raw8<TX> raw[LOADS];
+    [[maybe_unused]] Raw8<TS> raw_r[LOADS];
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+        const int col = (u * row_threads + t) * 8;
+        const bool in = live && col < p.H;
+        raw[u] = in ? load8(static_cast<const TX*>(p.x) + base + col) : zero8<TX>();
+        if constexpr (RESIDUAL) raw_r[u] = in ? load8(static_cast<const TS*>(p.residual) + base + col) : zero8<TS>();
+    }
+    uint64_t h[LOADS][4];
+    uint64_t sum2 = 0ull;
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+        unpack8<TX>(raw[u], h[u]);
+        if constexpr (RESIDUAL) {
+            uint64_t w[4];
+            unpack8<TS>(raw_r[u], w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[u][i] = add2(h[u][i], w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum2 = fma2(h[u][i], h[u][i], sum2);
+    }
+    if constexpr (RESIDUAL) {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+            const int col = (u * row_threads + t) * 8;
+            if (live && col < p.H) store8(static_cast<TS*>(p.total) + base + col, h[u]);
+        }
+    }
+    float lo, hi;
+    f32x2_split(sum2, lo, hi);
+    float sum = row_reduce<false>(lo + hi, slots[0], p.row_warps);
+    float eps = p.eps;
+    // Squares that fp32 cannot hold (values from about 1e17 on): once more with values 2^80 times smaller, next to which eps is nothing.
+    // (All threads that meet at the reduction's barrier hold the same sum.)
+    if (sum > 1e37f) {
+        sum2 = 0ull;
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[u][i] = mul2(h[u][i], f32x2(0x1p-80f, 0x1p-80f)), sum2 = fma2(h[u][i], h[u][i], sum2);
+        }
+        f32x2_split(sum2, lo, hi);
+        sum = row_reduce<false>(lo + hi, slots[2], p.row_warps);
+        eps = 0.0f;
+    }
+    const float r = rsqrtf(fmaf(sum, p.inv_h, eps));
+    const uint64_t r2 = f32x2(r, r);
+
+    float m[LOADS];
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+        const int col = (u * row_threads + t) * 8;
+        uint64_t w[4] = {0ull, 0ull, 0ull, 0ull};
+        if (col < p.H) unpack8<TW>(load8(static_cast<const TW*>(p.weight) + col), w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[u][i] = mul2(mul2(h[u][i], r2), w[i]);
+        m[u] = amax8_nan(h[u]);
+    }
+    QuantScale qs[LOADS];
+    if constexpr (BLOCK) {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) qs[u] = make_out_scale<OUT>(lanes_max_nan<16>(m[u]));
+    } else {
+        float top = m[0];
+#pragma unroll
+        for (int u = 1; u < LOADS; ++u) top = max_nan(top, m[u]);
+        const QuantScale all = make_out_scale<OUT>(row_reduce<true>(top, slots[1], p.row_warps));
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) qs[u] = all;
+        if (live && t == 0) p.s[row] = all.s;
+    }
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+        const int col = (u * row_threads + t) * 8;
+        if (live && col < p.H) {
+            if (BLOCK && (t & 15) == 0) p.s[row * p.KB + (col >> 7)] = qs[u].s;
+            *reinterpret_cast<uint2*>(p.q + base + col) = out8_pack8<OUT>(h[u], qs[u]);
+        }
+    }
+}
+
+}  // namespace gi8

@@ -1,0 +1,135 @@
+// What the operators around the products share: eight values a lane in, 8-bit values and their scale out.
+//   int8   s = amax / 127,  q = clamp(rint(v / s), -127, 127)
+//   e4m3   s = amax / 448,  q = v / s rounded to e4m3 (half to even)
+// with s = 1 where all values are zero.  A NaN or infinity among the values makes the scale NaN or infinite, so that every product with
+// them shows it (an int8 has no value of its own for it).
+#pragma once
+
+#include "../k_quant.cuh"
+
+namespace gi8 {
+
+enum class Out8 { kInt8, kE4m3 };
+
+// Maximum of magnitudes that propagates NaN.
+GI8_DEVICE float amax8_nan(const uint64_t (&v)[4])
+{
+    float a, b, c, d, e, f, g, h;
+    f32x2_split(v[0], a, b), f32x2_split(v[1], c, d), f32x2_split(v[2], e, f), f32x2_split(v[3], g, h);
+    return max3_abs_nan(max3_abs_nan(a, b, c), max3_abs_nan(d, e, f), max3_abs_nan(g, h, 0.0f));
+}
+
+GI8_DEVICE float max_nan(float a, float b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Over runs of LANES consecutive lanes (16: a 128-wide block of eight values a lane; 32: a warp).
+template <int LANES>
+GI8_DEVICE float lanes_max_nan(float m)
+{
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+// r: an approximate (int8) or the nearest (e4m3) reciprocal of s; NaN where the quick forms below do not hold.
+template <Out8 OUT>
+GI8_DEVICE QuantScale make_out_scale(float amax)
+{
+    QuantScale q;
+    q.s = amax == 0.0f ? 1.0f : __fdiv_rn(amax, OUT == Out8::kInt8 ? 127.0f : 448.0f);
+    if constexpr (OUT == Out8::kInt8) asm("rcp.approx.f32 %0, %1;" : "=f"(q.r) : "f"(q.s));
+    else q.r = __frcp_rn(q.s);
+    if (!(q.s > (OUT == Out8::kInt8 ? 1e-30f : 1e-20f) && q.s < 1e30f)) q.r = __int_as_float(0x7fffffff);
+    return q;
+}
+
+// Two floats -> two packed e4m3 (lo in the low byte).
+GI8_DEVICE uint32_t cvt_e4m3x2(float lo, float hi)
+{
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Four values -> four packed e4m3 of v / s, the quotient as IEEE division gives it: from the nearest reciprocal r and t = v r the exact
+// remainder v - t s corrects t (P. Markstein, IBM J. Res. Dev. 34, 1990), two multiply-adds on packed pairs; a quotient that lies
+// between two e4m3 numbers comes out exactly there.  Scales from 1e-20 on keep the remainder of every quotient that does not round to
+// zero in range.
+GI8_DEVICE uint32_t e4m3_pack4(uint64_t v0, uint64_t v1, const QuantScale& qs)
+{
+    float a, b, c, d;
+    if (qs.r == qs.r) {
+        const uint64_t r2 = f32x2(qs.r, qs.r), ns2 = f32x2(-qs.s, -qs.s);
+        const uint64_t t0 = mul2(v0, r2), t1 = mul2(v1, r2);
+        const uint64_t q0 = fma2(fma2(t0, ns2, v0), r2, t0), q1 = fma2(fma2(t1, ns2, v1), r2, t1);
+        f32x2_split(q0, a, b), f32x2_split(q1, c, d);
+    } else {
+        f32x2_split(v0, a, b), f32x2_split(v1, c, d);
+        a = __fdiv_rn(a, qs.s), b = __fdiv_rn(b, qs.s), c = __fdiv_rn(c, qs.s), d = __fdiv_rn(d, qs.s);
+    }
+    return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16);
+}
+
+// Eight values -> eight bytes.
+template <Out8 OUT>
+GI8_DEVICE uint2 out8_pack8(const uint64_t (&v)[4], const QuantScale& qs)
+{
+    if constexpr (OUT == Out8::kInt8) return make_uint2(quant_pack4(v[0], v[1], qs), quant_pack4(v[2], v[3], qs));
+    else return make_uint2(e4m3_pack4(v[0], v[1], qs), e4m3_pack4(v[2], v[3], qs));
+}
+
+// Eight consecutive values as they lie in memory (16 or 32 bytes, aligned to 16), and as fp32 pairs.
+template <typename T>
+struct Raw8 {
+    uint4 u[sizeof(T) / 2];
+};
+
+template <typename T>
+GI8_DEVICE Raw8<T> load8(const T* p)
+{
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
+    return r;
+}
+
+template <typename T>
+GI8_DEVICE Raw8<T> zero8()
+{
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.u[i] = make_uint4(0u, 0u, 0u, 0u);
+    return r;
+}
+
+template <typename T>
+GI8_DEVICE void unpack8(const Raw8<T>& r, uint64_t (&v)[4])
+{
+    if constexpr (sizeof(T) == 2) {
+        unpack16<T>(r.u[0], v);
+    } else {
+        unpack16<T>(r.u[0], reinterpret_cast<uint64_t(&)[2]>(v[0]));
+        unpack16<T>(r.u[1], reinterpret_cast<uint64_t(&)[2]>(v[2]));
+    }
+}
+
+// Eight fp32 values -> memory, rounded to T.
+template <typename T>
+GI8_DEVICE void store8(T* p, const uint64_t (&v)[4])
+{
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f32x2_split(v[i], f[2 * i], f[2 * i + 1]);
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    } else {
+        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+}
+
+}  // namespace gi8

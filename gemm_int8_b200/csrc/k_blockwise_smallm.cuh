@@ -60,13 +60,24 @@ struct BlockwiseSmallM {
     static constexpr uint32_t SMEM = STAGES * STAGE + BYTES_W + 1024;
 };
 
-template <int STAGES_>
+// OPERAND: nothing for int8, E4m3 for operands in 8-bit floating point with partials in fp32 (see k_blockwise.cuh).
+struct E4m3 {};
+template <int STAGES_, typename... OPERAND>
 __global__ void __launch_bounds__(BlockwiseSmallM<STAGES_>::THREADS)
 blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const BlockwiseSmallMParams p)
 {
     using S = BlockwiseSmallM<STAGES_>;
     constexpr int STAGES = S::STAGES, MT = S::MT;
-    constexpr uint32_t kIdesc = make_idesc_i8(128, MT, false);
+    constexpr bool E4M3 = sizeof...(OPERAND) != 0;
+    constexpr uint32_t kIdesc = E4M3 ? make_idesc_e4m3(128, MT) : make_idesc_i8(128, MT, false);
+    auto mma = [](uint32_t d, uint64_t a, uint64_t b, bool accumulate) {
+        if constexpr (E4M3) umma_f8(d, a, b, kIdesc, accumulate);
+        else umma_i8(d, a, b, kIdesc, accumulate);
+    };
+    auto promote = [](uint64_t& acc, uint32_t& v0, uint32_t& v1, uint64_t t2) {
+        if constexpr (E4M3) promote_pair_f32(acc, v0, v1, t2);
+        else promote_pair(acc, v0, v1, t2);
+    };
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -165,14 +176,14 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < kBK / kUmmaK; ++k) {
-                        umma_i8(d, smem_desc_k128_of(dw + 2 * k), smem_desc_k128_of(dx + 2 * k), kIdesc, k != 0);
-                        umma_i8(d + MT, smem_desc_k128_of(dw1 + 2 * k), smem_desc_k128_of(dx1 + 2 * k), kIdesc, k != 0);
+                        mma(d, smem_desc_k128_of(dw + 2 * k), smem_desc_k128_of(dx + 2 * k), k != 0);
+                        mma(d + MT, smem_desc_k128_of(dw1 + 2 * k), smem_desc_k128_of(dx1 + 2 * k), k != 0);
                     }
                     umma_commit(&bar_done[s]);
                 }
             } else if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kBK / kUmmaK; ++k) umma_i8(d, smem_desc_k128_of(dw + 2 * k), smem_desc_k128_of(dx + 2 * k), kIdesc, k != 0);
+                for (int k = 0; k < kBK / kUmmaK; ++k) mma(d, smem_desc_k128_of(dw + 2 * k), smem_desc_k128_of(dx + 2 * k), k != 0);
                 umma_commit(&bar_done[s]);
             }
             __syncwarp();
@@ -234,10 +245,10 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                 if (!ok) return;
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) promote_pair(acc[c], v[q][0][2 * c], v[q][0][2 * c + 1], t[0][c]);
+            for (int c = 0; c < 4; ++c) promote(acc[c], v[q][0][2 * c], v[q][0][2 * c + 1], t[0][c]);
             if (2 * i + 1 < num_kb) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) promote_pair(acc[c], v[q][1][2 * c], v[q][1][2 * c + 1], t[1][c]);
+                for (int c = 0; c < 4; ++c) promote(acc[c], v[q][1][2 * c], v[q][1][2 * c + 1], t[1][c]);
             }
         };
         for (int i = 0; i < num_st && ok; i += 2) {
@@ -251,8 +262,11 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                 if (cg * 8 + j < p.M) {
                     float lo, hi;
                     f32x2_split(acc[j / 2], lo, hi);
-                    const uint16_t r = to_bf16_bits(j & 1 ? hi : lo);
-                    p.out[static_cast<int64_t>(cg * 8 + j) * p.ldo + n] = p.bias ? add_bf16(r, b) : r;
+                    const float a = j & 1 ? hi : lo;
+                    uint16_t r;
+                    if constexpr (E4M3) r = to_bf16_bits(p.bias ? a + __uint_as_float(static_cast<uint32_t>(b) << 16) : a);
+                    else r = p.bias ? add_bf16(to_bf16_bits(a), b) : to_bf16_bits(a);
+                    p.out[static_cast<int64_t>(cg * 8 + j) * p.ldo + n] = r;
                 }
             }
         }

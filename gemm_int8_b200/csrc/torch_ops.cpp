@@ -390,6 +390,114 @@ at::Tensor int8_experts(const at::Tensor& x, const at::Tensor& logits, const std
     return out;
 }
 
+// ------------------------------------------------------------------------------------------------ around the products; e4m3
+std::tuple<at::Tensor, at::Tensor> new_out8(int64_t rows, int64_t cols, bool blockwise, bool e4m3, const at::Tensor& like)
+{
+    at::Tensor q = new_tensor({rows, cols}, e4m3 ? at::kFloat8_e4m3fn : at::kChar, like);
+    return {q, blockwise ? new_tensor({rows, blocks_of(cols)}, at::kFloat, like) : new_tensor({rows}, at::kFloat, like)};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_quantize(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& residual,
+                                                                 double eps, bool blockwise, bool e4m3)
+{
+    const char* name = "rms_norm_quantize";
+    check_activations(name, x);
+    const int64_t M = x.size(0), H = x.size(1);
+    const int weight_dtype = float_type(name, "weight", weight);
+    check_vector(name, "weight", weight, weight.scalar_type(), {H}, x.device());
+    int residual_dtype = 0;
+    if (residual.has_value()) {
+        residual_dtype = float_type(name, "residual", *residual);
+        check_vector(name, "residual", *residual, residual->scalar_type(), {M, H}, x.device());
+    }
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor xc = aligned(x), wc = aligned(weight);
+    at::Tensor rc, total;
+    if (residual.has_value()) {
+        rc = aligned(*residual);
+        total = new_tensor({M, H}, rc.scalar_type(), x);
+    } else {
+        total = new_tensor({0}, x.scalar_type(), x);
+    }
+    auto [q, s] = new_out8(M, H, blockwise, e4m3, x);
+    check(gi8_rms_norm_quantize(xc.data_ptr(), xc.scalar_type() == at::kFloat ? 0 : 1, rc.defined() ? rc.data_ptr() : nullptr, residual_dtype, wc.data_ptr(),
+                                weight_dtype, static_cast<float>(eps), total.data_ptr(), q.data_ptr(), e4m3, static_cast<float*>(s.data_ptr()), blockwise, M, H,
+                                stream_of(x)));
+    return {q, s, total};
+}
+
+std::tuple<at::Tensor, at::Tensor> swiglu_quantize(const at::Tensor& gate_up, bool blockwise, bool e4m3)
+{
+    const char* name = "swiglu_quantize";
+    check_activations(name, gate_up);
+    TORCH_CHECK(gate_up.size(1) % 2 == 0, name, ": gate and up columns must be the two halves of a row, got ", gate_up.size(1), " columns");
+    const int64_t M = gate_up.size(0), N = gate_up.size(1) / 2;
+    const c10::cuda::CUDAGuard guard(gate_up.device());
+    const at::Tensor c = aligned(gate_up);
+    auto [q, s] = new_out8(M, N, blockwise, e4m3, c);
+    check(gi8_swiglu_quantize(c.data_ptr(), c.scalar_type() == at::kFloat ? 0 : 1, q.data_ptr(), e4m3, static_cast<float*>(s.data_ptr()), blockwise, M, N, stream_of(c)));
+    return {q, s};
+}
+
+std::tuple<at::Tensor, at::Tensor> fp8_quantize_token_block(const at::Tensor& a)
+{
+    check_activations("quantize", a);
+    const c10::cuda::CUDAGuard guard(a.device());
+    const at::Tensor c = aligned(a);
+    const int64_t M = c.size(0), K = c.size(1);
+    auto [q, s] = new_out8(M, K, true, true, c);
+    check(gi8_fp8_quantize_token_block(c.data_ptr(), c.scalar_type() == at::kFloat ? 0 : 1, q.data_ptr(), static_cast<float*>(s.data_ptr()), M, K, stream_of(c)));
+    return {q, s};
+}
+
+at::Tensor fp8_matmul_blockwise(const at::Tensor& A, const at::Tensor& B, const at::Tensor& A_scale, const at::Tensor& B_scale)
+{
+    const char* name = "fp8_matmul_blockwise";
+    TORCH_CHECK(A.is_cuda() && B.is_cuda(), name, ": A and B must be CUDA tensors");
+    TORCH_CHECK(A.device() == B.device(), name, ": A and B must be on the same GPU, got ", A.device(), " and ", B.device());
+    TORCH_CHECK(A.scalar_type() == at::kFloat8_e4m3fn && B.scalar_type() == at::kFloat8_e4m3fn, name, ": A and B must be float8_e4m3fn, got ", A.scalar_type(),
+                " and ", B.scalar_type());
+    TORCH_CHECK(A.dim() == 2 && B.dim() == 2, name, ": A and B must be 2-D");
+    TORCH_CHECK(A.size(1) == B.size(1), name, ": A.shape[1] (", A.size(1), ") must equal B.shape[1] (", B.size(1), ")");
+    TORCH_CHECK(A.is_contiguous() && B.is_contiguous(), name, ": A and B must be contiguous");
+    const int64_t M = A.size(0), N = B.size(0), K = A.size(1);
+    check_scale(name, "A_scale", A_scale, {M, blocks_of(K)}, A.device());
+    check_scale(name, "B_scale", B_scale, {blocks_of(N), blocks_of(K)}, A.device());
+    const c10::cuda::CUDAGuard guard(A.device());
+    int64_t ld_sa, ld_sb;
+    const at::Tensor sa = block_scale(A_scale, ld_sa), sb = block_scale(B_scale, ld_sb);
+    at::Tensor out = new_tensor({M, N}, at::kBFloat16, A);
+    check(gi8_fp8_matmul_blockwise(A.data_ptr(), B.data_ptr(), f32(sa), ld_sa, f32(sb), ld_sb, out.data_ptr(), M, N, K, stream_of(A)));
+    return out;
+}
+
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale, const std::optional<at::Tensor>& bias)
+{
+    const char* name = "fp8_linear";
+    check_activations(name, x);
+    TORCH_CHECK(w.device() == x.device(), name, ": the weight must be on ", x.device(), ", got ", w.device());
+    TORCH_CHECK(w.scalar_type() == at::kFloat8_e4m3fn && w.dim() == 2 && w.is_contiguous(), name, ": the weight must be a contiguous 2-D float8_e4m3fn tensor");
+    TORCH_CHECK(x.size(1) == w.size(1), name, ": x has ", x.size(1), " features, the weight ", w.size(1));
+    const int64_t M = x.size(0), N = w.size(0), K = x.size(1);
+    check_scale(name, "weight_scale", w_scale, {blocks_of(N), blocks_of(K)}, x.device());
+    const c10::cuda::CUDAGuard guard(x.device());
+    int64_t ld;
+    const at::Tensor ws = block_scale(w_scale, ld);
+    at::Tensor b;
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->device() == x.device() && bias->dim() == 1 && bias->size(0) == N, name, ": bias must have shape [", N, "] on ", x.device());
+        b = bias->to(at::kBFloat16).contiguous();
+    }
+    const at::Tensor c = aligned(x);
+    at::Tensor out = new_tensor({M, N}, at::kBFloat16, x);
+    const int64_t q_bytes = (M * K + 255) / 256 * 256;
+    at::Tensor scratch = new_tensor({q_bytes + 4 * M * blocks_of(K)}, at::kByte, x);
+    uint8_t* q = static_cast<uint8_t*>(scratch.data_ptr());
+    check(gi8_fp8_linear(c.data_ptr(), c.scalar_type() == at::kFloat ? 0 : 1, w.data_ptr(), f32(ws), ld, b.defined() ? b.data_ptr() : nullptr, q,
+                         reinterpret_cast<float*>(q + q_bytes), out.data_ptr(), M, N, K, stream_of(x)));
+    return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(gemm_int8_CUDA, CUDA, m)
@@ -403,6 +511,11 @@ TORCH_LIBRARY_IMPL(gemm_int8_CUDA, CUDA, m)
     m.impl("quantize_token", &quantize_token);
     m.impl("hadamard_quantize_token_block", &hadamard_quantize_token_block);
     m.impl("int8_linear", &int8_linear);
+    m.impl("rms_norm_quantize", &rms_norm_quantize);
+    m.impl("swiglu_quantize", &swiglu_quantize);
+    m.impl("fp8_quantize_token_block", &fp8_quantize_token_block);
+    m.impl("fp8_matmul_blockwise", &fp8_matmul_blockwise);
+    m.impl("fp8_linear", &fp8_linear);
     m.impl("route_experts", &route_experts);
     m.impl("group_by_expert", &group_by_expert);
     m.impl("int8_matmul_experts", &int8_matmul_experts);

@@ -1,4 +1,4 @@
-"""W8A8 linear layer built on the INT8 GEMM entry points.
+"""W8A8 linear layers built on the INT8 GEMM entry points, and on the product in 8-bit floating point.
 
 The reference exposes only the raw matmul and leaves "arbitrary output dtype" and the layer around it to the
 caller (gemm_int8/__init__.py:31, README usage section).  `Int8Linear` is that caller: weights are quantised once
@@ -79,3 +79,51 @@ class Int8Linear(torch.nn.Module):
         if out.dtype != self.out_dtype:
             out = out.to(self.out_dtype)
         return out if x.dim() == 2 else out.reshape(*lead, weight.shape[0])
+
+
+class Fp8Linear(torch.nn.Module):
+    """y = x @ W.T (+ bias) with W and x in 8-bit floating point (float8_e4m3fn): per-128x128 weight scales, per-token-per-128-K activation scales.
+
+    The counterpart of `Int8Linear(mode="blockwise")`: activations are quantised on the fly, the product is `matmul_blockwise_fp8`, and a bias is
+    added to its fp32 sums before they are rounded to bf16 (one that broadcasts or is differentiated, to the rounded result).  weight_q
+    float8_e4m3fn [out_features, in_features], weight_scale fp32 [ceil(out/128), ceil(in/128)].  Inference only.
+    """
+
+    def __init__(self, weight_q: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16):
+        super().__init__()
+        if weight_q.dtype != torch.float8_e4m3fn:
+            raise ValueError("weight_q must be float8_e4m3fn")
+        self.out_dtype = out_dtype
+        self.register_buffer("weight_q", weight_q.contiguous())
+        self.register_buffer("weight_scale", weight_scale.contiguous())
+        self.register_buffer("bias", bias)
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor, bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16) -> "Fp8Linear":
+        """Quantises an fp32/bf16 weight [out_features, in_features] once, on whatever device it lives."""
+        wq, ws = quant.quantize_weight_block(weight.detach().to(torch.float32), dtype=torch.float8_e4m3fn)
+        return cls(wq, ws, bias, out_dtype)
+
+    @property
+    def in_features(self) -> int:
+        return self.weight_q.shape[1]
+
+    @property
+    def out_features(self) -> int:
+        return self.weight_q.shape[0]
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        if x2.dtype not in (torch.float32, torch.bfloat16):
+            x2 = x2.to(torch.bfloat16 if x2.dtype == torch.float16 else torch.float32)
+        weight, bias = self.weight_q, self.bias
+        fused = bias  # (where Int8Linear fuses it)
+        if bias is not None and (bias.shape != weight.shape[:1] or (bias.requires_grad and torch.is_grad_enabled())
+                                 or weight.shape[1] == 0 or forward_ad._current_level >= 0):
+            fused = None
+        out = torch.ops.gemm_int8_CUDA.fp8_linear(x2, weight, self.weight_scale, fused)
+        if bias is not None and fused is None:
+            out = out + bias.to(out.dtype)
+        if out.dtype != self.out_dtype:
+            out = out.to(self.out_dtype)
+        return out if x.dim() == 2 else out.reshape(*x.shape[:-1], weight.shape[0])

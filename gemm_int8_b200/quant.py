@@ -4,6 +4,8 @@ These are the callers' side of the GEMM (the reference ships none; its benchmark
 benchmark.py:17-18).  Plain torch ops, device-agnostic, used to build the synthetic workloads and by
 users who do not have a fused quantiser of their own.  Rule everywhere:
     s = amax / 127   (s = 1 where the block is all zero),   q = clamp(round_half_even(v / s), -127, 127)
+and with dtype=torch.float8_e4m3fn, for the products in 8-bit floating point:
+    s = amax / 448   (s = 1 where the block is all zero),   q = v / s rounded half to even
 """
 from __future__ import annotations
 
@@ -17,24 +19,38 @@ def _quant(v: torch.Tensor, amax: torch.Tensor):
     return s
 
 
-def quantize_per_token_block(a: torch.Tensor, block: int = KBLOCK):
-    """a fp32 [M, K] -> (q int8 [M, K], s fp32 [M, ceil(K/block)]), one scale per row per K block."""
+def _quant_fp8(v: torch.Tensor, amax: torch.Tensor, dtype: torch.dtype):
+    """(q, s) of blocks v whose largest magnitudes are amax (of v's dimensions).  A NaN or infinity makes its block's scale NaN or infinite."""
+    if dtype != torch.float8_e4m3fn:
+        raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
+    s = torch.where(amax == 0, torch.ones_like(amax), amax / amax.new_full((), 448.0))  # (a division: by a number, torch multiplies on a GPU)
+    return (v / s).clamp_(-448, 448).to(dtype), s
+
+
+def quantize_per_token_block(a: torch.Tensor, block: int = KBLOCK, dtype: torch.dtype = torch.int8):
+    """a fp32 [M, K] -> (q [M, K], s fp32 [M, ceil(K/block)]), one scale per row per K block; q in int8 or float8_e4m3fn."""
     M, K = a.shape
     KB = -(-K // block)
     pad = KB * block - K
     ap = torch.nn.functional.pad(a, (0, pad)) if pad else a
     blk = ap.reshape(M, KB, block)
+    if dtype != torch.int8:
+        q, s = _quant_fp8(blk, blk.abs().amax(dim=2, keepdim=True), dtype)
+        return q.reshape(M, KB * block)[:, :K].contiguous(), s[:, :, 0].contiguous()
     s = _quant(blk, blk.abs().amax(dim=2))
     q = torch.round(blk / s.unsqueeze(2)).clamp_(-127, 127).to(torch.int8).reshape(M, KB * block)
     return q[:, :K].contiguous(), s.contiguous()
 
 
-def quantize_weight_block(w: torch.Tensor, block: int = KBLOCK):
-    """w fp32 [N, K] -> (q int8 [N, K], s fp32 [ceil(N/block), ceil(K/block)]), one scale per block x block tile."""
+def quantize_weight_block(w: torch.Tensor, block: int = KBLOCK, dtype: torch.dtype = torch.int8):
+    """w fp32 [N, K] -> (q [N, K], s fp32 [ceil(N/block), ceil(K/block)]), one scale per block x block tile; q in int8 or float8_e4m3fn."""
     N, K = w.shape
     NB, KB = -(-N // block), -(-K // block)
     wp = torch.nn.functional.pad(w, (0, KB * block - K, 0, NB * block - N))
     blk = wp.reshape(NB, block, KB, block)
+    if dtype != torch.int8:
+        q, s = _quant_fp8(blk, blk.abs().amax(dim=(1, 3), keepdim=True), dtype)
+        return q.reshape(NB * block, KB * block)[:N, :K].contiguous(), s[:, 0, :, 0].contiguous()
     s = _quant(blk, blk.abs().amax(dim=(1, 3)))
     q = torch.round(blk / s[:, None, :, None]).clamp_(-127, 127).to(torch.int8).reshape(NB * block, KB * block)
     return q[:N, :K].contiguous(), s.contiguous()

@@ -284,6 +284,41 @@ int gi8_experts_add_f32(const void* x, int x_dtype, const void* logits, int logi
                         int64_t groups, int64_t top_groups, int group_top2, int renormalize, float scale, void* stream);
 
 /*
+ * The operators around the products of a feed-forward block, and the block-scaled product in 8-bit floating point (no reference counterpart).
+ * 8-bit results are int8 (q_type 0: s = amax / 127, q = clamp(round_half_even(v / s), -127, 127)) or e4m3 (q_type 1: s = amax / 448, q = v / s
+ * rounded half to even), s = 1 where all values are zero; with block_scales a scale per row and 128 columns, fp32 [M, ceil(K/128)], else one per
+ * row, fp32 [M] (int8 only).  A NaN or infinity makes the scale of its block or row NaN or infinite.  q is 8-byte aligned, and the features are a
+ * multiple of 16 below 131072.
+ *
+ * gi8_rms_norm_quantize: h = x + residual in fp32 (residual may be NULL);  total = h rounded to the residual's type;
+ *   v = h * (mean(h^2) + eps)^-1/2 * weight, all in fp32, from the sum before it is rounded;  q, scales of v.
+ *   x, residual, total [M,H] and weight [H] fp32 (dtype 0) or bf16 (1) each, total of the residual's type, all 16-byte aligned; H <= 32768;
+ *   1e-20 <= eps <= 1e20.  total is not touched without a residual, and may be the residual's or (of the same type) x's own memory.
+ */
+int gi8_rms_norm_quantize(const void* x, int x_dtype, const void* residual, int residual_dtype, const void* weight, int weight_dtype, float eps,
+                          void* total, void* q, int q_type, float* scales, int block_scales, int64_t M, int64_t H, void* stream);
+
+/* v = g / (1 + exp(-g)) * u in fp32 of the halves g (columns 0 .. N-1) and u of gate_up [M,2N], fp32 (dtype 0) or bf16 (1), 16-byte aligned. */
+int gi8_swiglu_quantize(const void* gate_up, int dtype, void* q, int q_type, float* scales, int block_scales, int64_t M, int64_t N, void* stream);
+
+/* gi8_quantize_token_block with e4m3 results (K % 8 == 0). */
+int gi8_fp8_quantize_token_block(const void* in, int in_dtype, void* q, float* scales, int64_t M, int64_t K, void* stream);
+
+/*
+ * gi8_matmul_blockwise for e4m3 operands: P is the fp32 dot product over a K block, on the tensor cores; accumulated with one fused multiply-add
+ * per K block and rounded to bf16 once.  Arguments and limits as there.
+ */
+int gi8_fp8_matmul_blockwise(const void* x, const void* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out_bf16, int64_t M,
+                             int64_t N, int64_t K, void* stream);
+
+/*
+ * gi8_linear with e4m3 weights (block scales): gi8_fp8_quantize_token_block and gi8_fp8_matmul_blockwise, with a bias (bf16 [N] or NULL) added to
+ * the fp32 sum before it is rounded.  xq e4m3 [M,K] (16-byte aligned) and xs fp32 [M, ceil(K/128)] are scratch.
+ */
+int gi8_fp8_linear(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const void* bias_bf16, void* xq, float* xs,
+                   void* out_bf16, int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
  * Forces a kernel variant for the calling process (tuning and tests); NULL or "" restores the fitted
  * per-shape dispatch that replaces the reference's shape table (csrc/kernels/gemm.cu:136-161).
  * Names: "dense_bn256", "dense_bn128", "dense_bn64" (tile width of the dense and of the blockwise kernel), "smallm"

@@ -1,0 +1,168 @@
+"""The operators as they are used: a feed-forward block in either 8-bit type, captured and replayed, on streams, two at once, in place through the C ABI."""
+import ctypes
+
+import pytest
+import torch
+
+import ffn_reference as R
+
+pytestmark = pytest.mark.gpu
+F8 = R.F8
+
+
+class _Block:
+    """norm -> gate and up product -> SwiGLU -> down product, the sum of the residual stream in the next norm."""
+
+    def __init__(self, H, I, dtype, seed=0):
+        from gemm_int8_b200 import quant
+
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        self.dtype, self.norm = dtype, (1 + 0.1 * torch.randn(H, generator=gen, device="cuda")).bfloat16()
+        self.w = [torch.randn(2 * I, H, generator=gen, device="cuda") * 0.03, torch.randn(H, I, generator=gen, device="cuda") * 0.03]
+        self.q = [quant.quantize_weight_block(w, dtype=dtype) for w in self.w]
+
+    def __call__(self, x, stream):
+        import gemm_int8_b200 as g
+
+        mm = g.matmul_blockwise_fp8 if self.dtype == F8 else g.matmul_blockwise
+        q, s, stream = g.rms_norm_quantize(x, self.norm, stream, 1e-5, dtype=self.dtype)
+        gate_up = mm(q, self.q[0][0], s, self.q[0][1])
+        q, s = g.swiglu_quantize(gate_up, dtype=self.dtype)
+        return mm(q, self.q[1][0], s, self.q[1][1]), stream
+
+    def exact(self, x, stream):
+        v, h = R.norm(x, self.norm, stream, 1e-5)
+        gate, up = (v @ self.w[0].double().t()).chunk(2, 1)
+        return (gate * torch.sigmoid(gate) * up) @ self.w[1].double().t(), h
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, F8])
+@pytest.mark.parametrize("M,H,I", [(1, 1024, 1408), (16, 512, 2048), (77, 1040, 2832), (600, 2048, 1408)])
+def test_block(M, H, I, dtype):
+    """Against the block in 64 bits with the weights before their quantisation.  Errors of independent roundings: activations and weights of either product are off by the rms of
+    their quantisation (int8: a step of amax/127 uniform, about 3.5/127/sqrt(12) = 0.8 %; e4m3: 2.6 %), so a product by sqrt(2) times that, the SwiGLU (two
+    factors, one with a slope up to 1.1) by 1.5 times that again, the down product adds its own: below 3.2 times 0.8 % and 2.6 %; twice that is allowed."""
+    import gemm_int8_b200 as g
+
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    block = _Block(H, I, dtype)
+    x = torch.randn(M, H, generator=gen, device="cuda").bfloat16()
+    stream = torch.randn(M, H, generator=gen, device="cuda").bfloat16()
+    out, total = block(x, stream)
+    want, h = block.exact(x, stream)
+    assert torch.equal(total, h.float().bfloat16())
+    rel = float((out.double() - want).norm() / want.norm())
+    assert rel < 2 * 3.2 * (0.008 if dtype == torch.int8 else 0.026), rel
+    g.check_device()
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, F8])
+def test_captured_block_replays_with_other_tokens(dtype):
+    block = _Block(512, 768, dtype)
+    x, stream = torch.zeros(24, 512, dtype=torch.bfloat16, device="cuda"), torch.zeros(24, 512, dtype=torch.float32, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block(x, stream)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):  # two graphs of the same layer
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(block(x, stream))
+        graphs.append(graph)
+    for seed in range(4):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        x.copy_(torch.randn(24, 512, generator=gen, device="cuda"))
+        stream.copy_(torch.randn(24, 512, generator=gen, device="cuda"))
+        for graph in graphs:
+            graph.replay()
+        want = block(x.clone(), stream.clone())
+        for got in outs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_streams_and_calls_at_once():
+    """Calls on two streams at once give what they give one after the other."""
+    import gemm_int8_b200 as g
+
+    blocks = [_Block(1024, 1408, d, seed=i) for i, d in enumerate((torch.int8, F8))]
+    data = [(R.outliers(torch.Generator(device="cuda").manual_seed(i), 300, 1024, torch.bfloat16), torch.randn(300, 1024, device="cuda")) for i in range(2)]
+    want = [b(*d) for b, d in zip(blocks, data)]
+    streams = [torch.cuda.Stream() for _ in blocks]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(blocks[i](*data[i]))
+    torch.cuda.synchronize()
+    for w, many in zip(want, got):
+        for o in many:
+            assert all(torch.equal(a, b) for a, b in zip(o, w))
+    g.check_device()
+
+
+def test_one_call_right_behind_the_other():
+    """Each operator is a programmatic dependent of the one in front: what it reads has been written, what it writes is read no more."""
+    import gemm_int8_b200 as g
+
+    block = _Block(512, 640, F8)
+    x, stream = torch.randn(9, 512, device="cuda").bfloat16(), torch.randn(9, 512, device="cuda").bfloat16()
+
+    def run(sync):
+        y, s = x, stream
+        for _ in range(40):
+            y, s = block(y, s)
+            if sync:
+                torch.cuda.synchronize()
+        return y, s
+
+    a, b = run(True), run(False)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    g.check_device()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_total_in_place(dtype):
+    """The C entry may write the sum over the residual, or over x of the same type."""
+    import gemm_int8_b200 as g
+
+    M, H = 300, 4096
+    x, r, w = torch.randn(M, H, device="cuda").to(dtype), torch.randn(M, H, device="cuda").to(dtype), torch.randn(H, device="cuda")
+    want = g.rms_norm_quantize(x, w, r)
+    p = lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+    for onto_x in (False, True):
+        a, b = x.clone(), r.clone()
+        q, s = torch.empty(M, H, dtype=torch.int8, device="cuda"), torch.empty(M, H // 128, device="cuda")
+        total = a if onto_x else b
+        code = 0 if dtype == torch.float32 else 1
+        assert g._C.gi8_rms_norm_quantize(p(a), code, p(b), code, p(w), 0, 1e-6, p(total), p(q), 0, p(s), 1, M, H, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        assert torch.equal(q, want[0]) and torch.equal(s, want[1]) and torch.equal(total, want[2])
+
+
+def test_nothing_behind_the_results_is_touched():
+    """Through the C ABI into the middle of larger buffers: the bytes around q, scales, total and out stay."""
+    import gemm_int8_b200 as g
+
+    M, H, N = 5, 1040, 200
+    KB = 9
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    x, w = torch.randn(M, H, device="cuda").bfloat16(), torch.randn(H, device="cuda").bfloat16()
+    p = lambda t, at: ctypes.c_void_p(t.data_ptr() + at)  # noqa: E731
+    for q_type in (0, 1):
+        q, s, t = (torch.full((n,), 0x5A, dtype=torch.uint8, device="cuda") for n in (M * H + 64, M * KB * 4 + 64, M * H * 2 + 64))
+        assert g._C.gi8_rms_norm_quantize(p(x, 0), 1, p(x, 0), 1, p(w, 0), 1, 1e-6, p(t, 32), p(q, 32), q_type, p(s, 32), 1, M, H, stream) == 0
+        for b in (q, s, t):
+            assert bool((b[:32] == 0x5A).all()) and bool((b[-32:] == 0x5A).all())
+        q, s = (torch.full((n,), 0x5A, dtype=torch.uint8, device="cuda") for n in (M * (H // 2 - 8) + 64, M * 4 * 5 + 64))
+        assert g._C.gi8_swiglu_quantize(p(x[:, : H - 16].contiguous(), 0), 1, p(q, 32), q_type, p(s, 32), 1, M, H // 2 - 8, stream) == 0
+        for b in (q, s):
+            assert bool((b[:32] == 0x5A).all()) and bool((b[-32:] == 0x5A).all())
+    x_q, w_q = torch.randn(M, H, device="cuda").to(F8), torch.randn(N, H, device="cuda").to(F8)
+    sx, sw = torch.rand(M, KB, device="cuda"), torch.rand(2, KB, device="cuda")
+    for rows in (M, 1):
+        out = torch.full((rows * N * 2 + 64,), 0x5A, dtype=torch.uint8, device="cuda")
+        assert g._C.gi8_fp8_matmul_blockwise(p(x_q, 0), p(w_q, 0), p(sx, 0), KB, p(sw, 0), KB, p(out, 32), rows, N, H, stream) == 0
+        assert bool((out[:32] == 0x5A).all()) and bool((out[-32:] == 0x5A).all())
