@@ -17,6 +17,7 @@ SOURCES = [os.path.join(_PKG, "csrc", "api.cu")]
 HEADERS = [os.path.join(_PKG, "csrc", f) for f in ("ptx.cuh", "k_dense.cuh", "k_dense_splitk.cuh", "k_blockwise.cuh", "k_blockwise_smallm.cuh", "k_smallm.cuh", "k_quant.cuh")]
 HEADERS += [os.path.join(_PKG, "csrc", "experts", f) for f in ("host.cuh", "k_route.cuh", "k_group.cuh", "k_experts_gemm.cuh", "k_combine.cuh")]
 HEADERS += [os.path.join(_PKG, "csrc", "ffn", f) for f in ("host.cuh", "out8.cuh", "k_norm.cuh", "k_act.cuh")]
+HEADERS += [os.path.join(_PKG, "csrc", "fp8", f) for f in ("host.cuh", "k_fp8_gemm.cuh")]
 HEADERS.append(os.path.join(os.path.dirname(_PKG), "include", "gemm_int8_b200.h"))
 
 OPS_NAME = "libgemm_int8_b200_torch.so"

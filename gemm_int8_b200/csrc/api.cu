@@ -1289,11 +1289,10 @@ int gi8_quantize_token(const void* in, int in_dtype, int8_t* q, float* scales, i
 // gather != nullptr: the N-sharded form.  This GEMM's [M,N] result is columns [col0, col0 + N) of an [M, n_total]
 // matrix, and the epilogue writes every block into all n_out such matrices (gather[i]: this rank's own and every
 // peer's, the latter through mapped peer memory) instead of `out`.
-// e4m3: both operands are in 8-bit floating point (the knobs that choose among forms of the int8 kernel do not apply).
 static int blockwise_impl(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw,
                           void* out, int64_t M, int64_t N, int64_t K, void* stream, void* const* gather, int n_out,
                           int64_t n_total, int64_t col0, bool out_f32 = false, int force_bn = 0, int pdl_role = 0,
-                          int scatter_me = -1, const uint16_t* bias = nullptr, bool after_quant = false, bool e4m3 = false)
+                          int scatter_me = -1, const uint16_t* bias = nullptr, bool after_quant = false)
 {
     // scatter_me >= 0: `gather` holds the n_out ranks' receive areas of the K-sharded reduce-scatter form
     const bool scatter = scatter_me >= 0;
@@ -1372,14 +1371,13 @@ static int blockwise_impl(const int8_t* x, const int8_t* y, const float* sa, int
         if (p.tma_store)
             if (int rc = make_output_map(&mo.m[0], out, M, N, N, box_cols)) return rc;
     }
-#define GI8_LAUNCH_BW_OF(E4M3_, BN_, ST_, SPLIT_, NISS_, PAIR_, BIAS_, AHEAD_, SLOT_)         \
+#define GI8_LAUNCH_BW(BN_, ST_, SPLIT_, NISS_, PAIR_, BIAS_, AHEAD_, SLOT_)                   \
     do {                                                                                      \
         constexpr size_t smem = blockwise_smem_bytes(BN_, ST_, PAIR_);                        \
-        auto kernel = blockwise_gemm_kernel<BN_, ST_, SPLIT_, NISS_, PAIR_, BIAS_, AHEAD_, E4M3_>; \
+        auto kernel = blockwise_gemm_kernel<BN_, ST_, SPLIT_, NISS_, PAIR_, BIAS_, AHEAD_>;   \
         if (int rc = ensure_smem(st, SLOT_, kernel, smem)) return rc;                         \
         return launch(kernel, dim3(grid), kBlockwiseThreads, smem, s, dim3(PAIR_ ? 2 : 1), pdl, mx, my, mo, p); \
     } while (0)
-#define GI8_LAUNCH_BW(...) GI8_LAUNCH_BW_OF(false, __VA_ARGS__)
     // Every launch is a programmatic dependent: its set-up (and the launch itself) overlaps the tail of the kernel in front.  Back
     // to back, before and after: 1024 x 4096 x 4096 dense 19.1 -> 16.7 us a call, 777 x 5003 x 3088 24.3 -> 22.1.
     // (Launches that write into peers' memory stay ordinary ones.)
@@ -1387,19 +1385,6 @@ static int blockwise_impl(const int8_t* x, const int8_t* y, const float* sa, int
     const bool two = knobs().bw_issuers == 2 || (knobs().bw_issuers == 0 && bn < 256);
     const bool halves = knobs().bw_halves != 1;
     const bool ahead = tiles > 2 * static_cast<int64_t>(st->sm_count);  // one-CTA column halves; both sides stand in the kernel's header
-    if (e4m3) {
-#define GI8_LAUNCH_E4M3(BIAS_, SLOT_)                                                        \
-    do {                                                                                     \
-        if (pair) GI8_LAUNCH_BW_OF(true, 256, 6, 2, 2, true, BIAS_, true, SLOT_);            \
-        if (bn == 256 && ahead) GI8_LAUNCH_BW_OF(true, 256, 4, 2, 2, false, BIAS_, true, SLOT_ + 1); \
-        if (bn == 256) GI8_LAUNCH_BW_OF(true, 256, 4, 2, 2, false, BIAS_, false, SLOT_ + 2); \
-        if (bn == 128) GI8_LAUNCH_BW_OF(true, 128, 6, 1, 2, false, BIAS_, false, SLOT_ + 3); \
-        GI8_LAUNCH_BW_OF(true, 64, 8, 1, 2, false, BIAS_, false, SLOT_ + 4);                 \
-    } while (0)
-        if (bias) GI8_LAUNCH_E4M3(true, 64);
-        GI8_LAUNCH_E4M3(false, 69);
-#undef GI8_LAUNCH_E4M3
-    }
     if (bias) {  // (the knobs below choose among forms without one)
         if (pair) GI8_LAUNCH_BW(256, 6, 2, 2, true, true, true, 28);
         if (bn == 256 && ahead) GI8_LAUNCH_BW(256, 4, 2, 2, false, true, true, 35);
@@ -1424,12 +1409,11 @@ static int blockwise_impl(const int8_t* x, const int8_t* y, const float* sa, int
         else GI8_LAUNCH_BW(64, 8, 1, 1, false, false, false, 20);
     }
 #undef GI8_LAUNCH_BW
-#undef GI8_LAUNCH_BW_OF
 }
 
 // (bias, after_quant: see scaled_impl)
 static int blockwise_dispatch(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out,
-                              int64_t M, int64_t N, int64_t K, void* stream, const uint16_t* bias, bool after_quant, bool e4m3 = false)
+                              int64_t M, int64_t N, int64_t K, void* stream, const uint16_t* bias, bool after_quant)
 {
     if (g_forced_variant == VAR_AUTO && use_blockwise_smallm(M, N, K)) {
         if (int rc = check_common(x, y, out, M, N, K, 2)) return rc;
@@ -1441,9 +1425,8 @@ static int blockwise_dispatch(const int8_t* x, const int8_t* y, const float* sa,
         q.ldo = N, q.ld_sa = ld_sa, q.ld_sw = ld_sw, q.M = (int)M, q.N = (int)N, q.K = (int)K;
         q.after_quant = after_quant && knobs().pdl;
         cudaStream_t s = static_cast<cudaStream_t>(stream);
-        const bool six = blockwise_smallm_six_stages(N, K, q.after_quant, st->sm_count);
-        if (e4m3) return six ? launch_blockwise_smallm<6, E4m3>(st, 75, x, y, q, s) : launch_blockwise_smallm<4, E4m3>(st, 74, x, y, q, s);
-        return six ? launch_blockwise_smallm<6>(st, 33, x, y, q, s) : launch_blockwise_smallm<4>(st, 32, x, y, q, s);
+        if (blockwise_smallm_six_stages(N, K, q.after_quant, st->sm_count)) return launch_blockwise_smallm<6>(st, 33, x, y, q, s);
+        return launch_blockwise_smallm<4>(st, 32, x, y, q, s);
     }
     if (g_forced_variant == VAR_AUTO && M > 0 && N > 0 && K > 0 && out && reinterpret_cast<uintptr_t>(out) % 16 == 0 && N % 8 == 0) {
         DeviceState* st;
@@ -1453,13 +1436,13 @@ static int blockwise_dispatch(const int8_t* x, const int8_t* y, const float* sa,
             // both launches write through a tensor map of the whole [M, N] matrix, each its own columns
             void* outs[1] = {out};
             const bool pdl = knobs().pdl;  // GEMM_INT8_PDL=0: two ordinary launches, one after the other
-            if (int rc = blockwise_impl(x, y, sa, ld_sa, sw, ld_sw, nullptr, M, c.n1, K, stream, outs, 1, N, 0, false, 256, 0, -1, bias, after_quant, e4m3))
+            if (int rc = blockwise_impl(x, y, sa, ld_sa, sw, ld_sw, nullptr, M, c.n1, K, stream, outs, 1, N, 0, false, 256, 0, -1, bias, after_quant))
                 return rc;
             return blockwise_impl(x, y + c.n1 * K, sa, ld_sa, sw ? sw + (c.n1 / 128) * ld_sw : sw, ld_sw, nullptr, M, N - c.n1, K,
-                                  stream, outs, 1, N, c.n1, false, c.bn_tail, pdl ? 2 : 0, -1, bias ? bias + c.n1 : nullptr, false, e4m3);
+                                  stream, outs, 1, N, c.n1, false, c.bn_tail, pdl ? 2 : 0, -1, bias ? bias + c.n1 : nullptr, false);
         }
     }
-    return blockwise_impl(x, y, sa, ld_sa, sw, ld_sw, out, M, N, K, stream, nullptr, 1, N, 0, false, 0, 0, -1, bias, after_quant, e4m3);
+    return blockwise_impl(x, y, sa, ld_sa, sw, ld_sw, out, M, N, K, stream, nullptr, 1, N, 0, false, 0, 0, -1, bias, after_quant);
 }
 
 int gi8_matmul_blockwise(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa, const float* sw,
@@ -1613,3 +1596,4 @@ int gi8_peer_release(void* ptr)
 
 #include "experts/host.cuh"
 #include "ffn/host.cuh"
+#include "fp8/host.cuh"

@@ -22,9 +22,11 @@ int check_out8(const void* q, int q_type, const float* scales, int block_scales,
     return GI8_OK;
 }
 
-// Threads of a row: as many loads of eight values a thread as keep its warps few.
+// Values a thread: 32, which wants the fewest warps a row and the most rows on an SM (16384 x 8192 bf16 with a residual, 8 / 16 / 32 / 64 values: 179 / 176 /
+// 141 / 163 us; 16384 x 4096 without one 71 / 64 / 54); 16 where there is no second row for an SM to work on beside (148 x 8192: 4.5 us for 6.3; level from
+// 592 rows on), 64 where 512 threads of 32 would not hold the row.
 template <typename TX, typename TR, typename TW, Out8 OUT, bool BLOCK>
-int launch_norm(NormParams p, cudaStream_t s)
+int launch_norm(NormParams p, int sms, cudaStream_t s)
 {
     const int vectors = (p.H + 7) / 8;
     auto go = [&](auto kernel, int loads) {
@@ -32,54 +34,53 @@ int launch_norm(NormParams p, cudaStream_t s)
         const int rows = p.row_warps == 1 ? 8 : 1;
         return launch(kernel, dim3(static_cast<unsigned>((p.M + rows - 1) / rows)), p.row_warps * rows * 32, 0, s, dim3(1), knobs().pdl, p);
     };
-    if (vectors <= 512) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 1>, 1);
-    if (vectors <= 1024) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 2>, 2);
-    if (vectors <= 2048) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 4>, 4);
+    if (p.M <= 2 * sms && vectors <= 2 * kNormThreads) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 2>, 2);
+    if (vectors <= 4 * kNormThreads) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 4>, 4);
     return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 8>, 8);
 }
 
 template <typename TX, typename TR, typename TW>
-int launch_norm(const NormParams& p, int q_type, int block_scales, cudaStream_t s)
+int launch_norm(const NormParams& p, int q_type, int block_scales, int sms, cudaStream_t s)
 {
-    if (q_type == 1) return launch_norm<TX, TR, TW, Out8::kE4m3, true>(p, s);
-    if (block_scales) return launch_norm<TX, TR, TW, Out8::kInt8, true>(p, s);
-    return launch_norm<TX, TR, TW, Out8::kInt8, false>(p, s);
+    if (q_type == 1) return launch_norm<TX, TR, TW, Out8::kE4m3, true>(p, sms, s);
+    if (block_scales) return launch_norm<TX, TR, TW, Out8::kInt8, true>(p, sms, s);
+    return launch_norm<TX, TR, TW, Out8::kInt8, false>(p, sms, s);
 }
 
 template <typename TX, typename TR>
-int launch_norm(const NormParams& p, int weight_dtype, int q_type, int block_scales, cudaStream_t s)
+int launch_norm(const NormParams& p, int weight_dtype, int q_type, int block_scales, int sms, cudaStream_t s)
 {
-    return weight_dtype == 0 ? launch_norm<TX, TR, float>(p, q_type, block_scales, s) : launch_norm<TX, TR, __nv_bfloat16>(p, q_type, block_scales, s);
+    return weight_dtype == 0 ? launch_norm<TX, TR, float>(p, q_type, block_scales, sms, s) : launch_norm<TX, TR, __nv_bfloat16>(p, q_type, block_scales, sms, s);
 }
 
 template <typename TX>
-int launch_norm(const NormParams& p, int residual_dtype, int weight_dtype, int q_type, int block_scales, cudaStream_t s)
+int launch_norm(const NormParams& p, int residual_dtype, int weight_dtype, int q_type, int block_scales, int sms, cudaStream_t s)
 {
-    if (!p.residual) return launch_norm<TX, void>(p, weight_dtype, q_type, block_scales, s);
-    return residual_dtype == 0 ? launch_norm<TX, float>(p, weight_dtype, q_type, block_scales, s) : launch_norm<TX, __nv_bfloat16>(p, weight_dtype, q_type, block_scales, s);
+    if (!p.residual) return launch_norm<TX, void>(p, weight_dtype, q_type, block_scales, sms, s);
+    return residual_dtype == 0 ? launch_norm<TX, float>(p, weight_dtype, q_type, block_scales, sms, s) : launch_norm<TX, __nv_bfloat16>(p, weight_dtype, q_type, block_scales, sms, s);
 }
 
-// Block scales: eight 16-byte loads a lane (four of the plain bf16 quantiser's).
+// Block scales: 32 values a lane, of the two fp32 halves 16, each item on a warp of its own (4096 x 14336 bf16 SwiGLU with 8 / 16 / 32 values 66 / 58 / 49 us;
+// a grid of as many CTAs as are resident, whose warps take item after item, 53; e4m3 quantiser of 16384 x 8192 fp32 98, resident CTAs 104).
 template <typename T, bool SWIGLU, Out8 OUT>
-int launch_act_block(ActParams p, int sms, cudaStream_t s)
+int launch_act_block(const ActParams& p, cudaStream_t s)
 {
     constexpr int LOADS = SWIGLU && sizeof(T) == 4 ? 2 : 4;
     const int64_t items = p.M * ((p.KB + 2 * LOADS - 1) / (2 * LOADS));
     if (items >= (int64_t(1) << 31)) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "too many quantisation blocks");
-    const int64_t ctas = std::min<int64_t>((items + kActThreads / 32 - 1) / (kActThreads / 32), static_cast<int64_t>(sms) * 16);
-    return launch(act_quantize_block_kernel<T, SWIGLU, OUT, LOADS>, dim3(static_cast<unsigned>(ctas)), kActThreads, 0, s, dim3(1), knobs().pdl, p);
+    return launch(act_quantize_block_kernel<T, SWIGLU, OUT, LOADS>, dim3(static_cast<unsigned>((items + kActThreads / 32 - 1) / (kActThreads / 32))), kActThreads, 0, s,
+                  dim3(1), knobs().pdl, p);
 }
 
+// A scale per row: 32 values a thread (4096 x 14336 bf16 with 16 / 32 / 64 values 79 / 62 / 78 us, 8192 x 4096 39 / 35 / 57).
 template <typename T>
-int launch_swiglu_row(ActParams p, int sms, cudaStream_t s)
+int launch_swiglu_row(const ActParams& p, int sms, cudaStream_t s)
 {
+    constexpr int LOADS = 4;
     const int vectors = (p.K + 7) / 8;
-    const unsigned ctas = static_cast<unsigned>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8));
-    auto go = [&](auto kernel, int loads) {
-        const int threads = std::min(1024, (vectors + 32 * loads - 1) / (32 * loads) * 32);
-        return launch(kernel, dim3(ctas), threads, 0, s, dim3(1), knobs().pdl, p);
-    };
-    return vectors <= 1024 ? go(swiglu_quantize_row_kernel<T, Out8::kInt8, 1>, 1) : go(swiglu_quantize_row_kernel<T, Out8::kInt8, 2>, 2);
+    const int threads = std::min(1024, (vectors + 32 * LOADS - 1) / (32 * LOADS) * 32);
+    return launch(swiglu_quantize_row_kernel<T, Out8::kInt8, LOADS>, dim3(static_cast<unsigned>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8))), threads, 0, s, dim3(1),
+                  knobs().pdl, p);
 }
 
 }  // namespace
@@ -105,8 +106,9 @@ int gi8_rms_norm_quantize(const void* x, int x_dtype, const void* residual, int 
     p.x = x, p.residual = residual, p.weight = weight, p.total = total, p.q = static_cast<uint8_t*>(q), p.s = scales, p.M = M, p.H = static_cast<int>(H);
     p.KB = static_cast<int>((H + 127) / 128), p.eps = eps, p.inv_h = 1.0f / static_cast<float>(H);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return x_dtype == 0 ? launch_norm<float>(p, residual_dtype, weight_dtype, q_type, block_scales, s)
-                        : launch_norm<__nv_bfloat16>(p, residual_dtype, weight_dtype, q_type, block_scales, s);
+    const int sms = st->sm_count;
+    return x_dtype == 0 ? launch_norm<float>(p, residual_dtype, weight_dtype, q_type, block_scales, sms, s)
+                        : launch_norm<__nv_bfloat16>(p, residual_dtype, weight_dtype, q_type, block_scales, sms, s);
 }
 
 int gi8_swiglu_quantize(const void* gate_up, int dtype, void* q, int q_type, float* scales, int block_scales, int64_t M, int64_t N, void* stream)
@@ -123,46 +125,8 @@ int gi8_swiglu_quantize(const void* gate_up, int dtype, void* q, int q_type, flo
     const int sms = st->sm_count;
     if (!block_scales) return dtype == 0 ? launch_swiglu_row<float>(p, sms, s) : launch_swiglu_row<__nv_bfloat16>(p, sms, s);
     if (q_type == 1)
-        return dtype == 0 ? launch_act_block<float, true, Out8::kE4m3>(p, sms, s) : launch_act_block<__nv_bfloat16, true, Out8::kE4m3>(p, sms, s);
-    return dtype == 0 ? launch_act_block<float, true, Out8::kInt8>(p, sms, s) : launch_act_block<__nv_bfloat16, true, Out8::kInt8>(p, sms, s);
-}
-
-int gi8_fp8_quantize_token_block(const void* in, int in_dtype, void* q, float* scales, int64_t M, int64_t K, void* stream)
-{
-    if (int rc = check_quant(in, in_dtype, static_cast<const int8_t*>(q), scales, M, K)) return rc;
-    if (K % 8) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "K=%lld must be a multiple of 8", (long long)K);
-    if (M == 0 || K == 0) return GI8_OK;
-    DeviceState* st;
-    if (int rc = get_device_state(&st)) return rc;
-    ActParams p{in, static_cast<uint8_t*>(q), scales, M, static_cast<int>(K), static_cast<int>((K + 127) / 128)};
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return in_dtype == 0 ? launch_act_block<float, false, Out8::kE4m3>(p, st->sm_count, s) : launch_act_block<__nv_bfloat16, false, Out8::kE4m3>(p, st->sm_count, s);
-}
-
-int gi8_fp8_matmul_blockwise(const void* x, const void* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out, int64_t M, int64_t N,
-                             int64_t K, void* stream)
-{
-    if (int rc = check_common(x, y, out, M, N, K, 2)) return rc;
-    if (M > 0 && N > 0 && K > 0)
-        if (int rc = check_block_scales(sa, ld_sa, sw, ld_sw, M, N, K)) return rc;
-    return blockwise_dispatch(static_cast<const int8_t*>(x), static_cast<const int8_t*>(y), sa, ld_sa, sw, ld_sw, out, M, N, K, stream, nullptr, false, true);
-}
-
-int gi8_fp8_linear(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const void* bias, void* xq, float* xs, void* out,
-                   int64_t M, int64_t N, int64_t K, void* stream)
-{
-    // Everything that the quantiser or the product refuses is refused before the quantiser is launched (as in gi8_linear).
-    if (int rc = check_common(xq, w, out, M, N, K, 2)) return rc;
-    if (int rc = check_quant(x, x_dtype, static_cast<const int8_t*>(xq), xs, M, K)) return rc;
-    if (misaligned(bias, 2)) return fail(GI8_ERR_MISALIGNED, "bias must be 2-byte aligned");
-    if (M == 0 || N == 0) return GI8_OK;
-    if (K == 0 && bias) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "K must be positive for a product with a bias");
-    const int64_t ld_xs = (K + kBK - 1) / kBK;
-    if (K > 0)
-        if (int rc = check_block_scales(xs, ld_xs, w_scale, ld_sw, M, N, K)) return rc;
-    if (int rc = gi8_fp8_quantize_token_block(x, x_dtype, xq, xs, M, K, stream)) return rc;
-    return blockwise_dispatch(static_cast<const int8_t*>(xq), static_cast<const int8_t*>(w), xs, ld_xs, w_scale, ld_sw, out, M, N, K, stream,
-                              static_cast<const uint16_t*>(bias), K > 0, true);
+        return dtype == 0 ? launch_act_block<float, true, Out8::kE4m3>(p, s) : launch_act_block<__nv_bfloat16, true, Out8::kE4m3>(p, s);
+    return dtype == 0 ? launch_act_block<float, true, Out8::kInt8>(p, s) : launch_act_block<__nv_bfloat16, true, Out8::kInt8>(p, s);
 }
 
 }  // extern "C"

@@ -15,9 +15,18 @@ struct ActParams {
     int K, KB;
 };
 
-// (an overflowing exponential gives -0, the limit; the quick exponential and division are good to about 1e-6, next to the half step of
-// 1/254 or 2^-4 that the result is rounded by)
-GI8_DEVICE float silu_times(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// g u / (1 + 2^(-g log2 e)) for a pair, in packed steps but for the exponentials and reciprocals, which the special-function unit takes one by one
+// (subnormal results flushed: next to 1 they are nothing, and a reciprocal of 2^126 and more, or of an overflowed exponential, is the limit 0).
+// Good to (5 + |g|) units in the last place, next to the half step of 1/254 or 2^-4 that the result is rounded by.
+GI8_DEVICE uint64_t swiglu2(uint64_t g, uint64_t u)
+{
+    float a, b;
+    f32x2_split(mul2(g, f32x2(-1.44269504f, -1.44269504f)), a, b);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
+    f32x2_split(add2(f32x2(a, b), f32x2(1.0f, 1.0f)), a, b);
+    return mul2(mul2(g, f32x2(approx_reciprocal(a), approx_reciprocal(b))), u);
+}
 
 template <typename T, bool SWIGLU>
 struct ActRaw {
@@ -47,11 +56,7 @@ GI8_DEVICE void act_values(const ActRaw<T, SWIGLU>& r, uint64_t (&v)[4])
         uint64_t w[4];
         unpack8<T>(r.b, w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float g0, g1, u0, u1;
-            f32x2_split(v[i], g0, g1), f32x2_split(w[i], u0, u1);
-            v[i] = f32x2(silu_times(g0, u0), silu_times(g1, u1));
-        }
+        for (int i = 0; i < 4; ++i) v[i] = swiglu2(v[i], w[i]);
     }
 }
 
@@ -64,24 +69,28 @@ __global__ void __launch_bounds__(kActThreads) act_quantize_block_kernel(const A
     quant_dependency();
     const int lane = threadIdx.x & 31;
     const uint32_t groups = static_cast<uint32_t>((p.KB + 2 * LOADS - 1) / (2 * LOADS));
-    const uint32_t items = static_cast<uint32_t>(p.M) * groups;  // the host checks that this fits
-    const uint32_t step = gridDim.x * (kActThreads / 32);
-    for (uint32_t item = blockIdx.x * (kActThreads / 32) + (threadIdx.x >> 5); item < items; item += step) {
-        const uint32_t row = item / groups;
-        const int col0 = static_cast<int>(item - row * groups) * (2 * LOADS * 128) + lane * 8;
-        ActRaw<T, SWIGLU> raw[LOADS];
+    const uint32_t item = blockIdx.x * (kActThreads / 32) + (threadIdx.x >> 5);  // the host checks that this fits
+    const uint32_t row = item / groups;
+    if (row >= p.M) return;  // (a whole warp)
+    const int col0 = static_cast<int>(item - row * groups) * (2 * LOADS * 128) + lane * 8;
+    ActRaw<T, SWIGLU> raw[LOADS];
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) raw[u] = act_load<T, SWIGLU>(p, row, col0 + u * 256, col0 + u * 256 < p.K);
+    for (int u = 0; u < LOADS; ++u) raw[u] = act_load<T, SWIGLU>(p, row, col0 + u * 256, col0 + u * 256 < p.K);
+    uint64_t v[LOADS][4];
+    float m[LOADS];
 #pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
-            const int col = col0 + u * 256;
-            uint64_t v[4];
-            act_values<T, SWIGLU>(raw[u], v);
-            const QuantScale qs = make_out_scale<OUT>(lanes_max_nan<16>(amax8_nan(v)));
-            if (col < p.K) {
-                if ((lane & 15) == 0) p.s[static_cast<int64_t>(row) * p.KB + (col >> 7)] = qs.s;
-                *reinterpret_cast<uint2*>(p.q + static_cast<int64_t>(row) * p.K + col) = out8_pack8<OUT>(v, qs);
-            }
+    for (int u = 0; u < LOADS; ++u) {
+        act_values<T, SWIGLU>(raw[u], v[u]);
+        m[u] = amax8_nan(v[u]);
+    }
+    QuantScale qs[LOADS];
+    block_scales<OUT, LOADS>(m, qs);
+#pragma unroll
+    for (int u = 0; u < LOADS; ++u) {
+        const int col = col0 + u * 256;
+        if (col < p.K) {
+            if ((lane & 15) == 0) p.s[static_cast<int64_t>(row) * p.KB + (col >> 7)] = qs[u].s;
+            *reinterpret_cast<uint2*>(p.q + static_cast<int64_t>(row) * p.K + col) = out8_pack8<OUT>(v[u], qs[u]);
         }
     }
 }

@@ -70,76 +70,86 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_quantize_kernel(const N
         raw[u] = in ? load8(static_cast<const TX*>(p.x) + base + col) : zero8<TX>();
         if constexpr (RESIDUAL) raw_r[u] = in ? load8(static_cast<const TS*>(p.residual) + base + col) : zero8<TS>();
     }
-    uint64_t h[LOADS][4];
+    // A bf16 weight is requested with the row, not behind the reduction (the registers of an fp32 one would cost resident CTAs).
+    constexpr bool EARLY = sizeof(TW) == 2 && !RESIDUAL;
+    [[maybe_unused]] Raw8<TW> raw_w[LOADS];
+    auto load_weight = [&](int u) {
+        const int col = (u * row_threads + t) * 8;
+        return col < p.H ? load8(static_cast<const TW*>(p.weight) + col) : zero8<TW>();
+    };
+    if constexpr (EARLY) {
+#pragma unroll
+        for (int u = 0; u < LOADS; ++u) raw_w[u] = load_weight(u);
+    }
+    uint64_t kept[LOADS][4];  // the sums, then the values
     uint64_t sum2 = 0ull;
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
-        unpack8<TX>(raw[u], h[u]);
+        uint64_t (&h)[4] = kept[u];
+        unpack8<TX>(raw[u], h);
         if constexpr (RESIDUAL) {
             uint64_t w[4];
             unpack8<TS>(raw_r[u], w);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[u][i] = add2(h[u][i], w[i]);
+            for (int i = 0; i < 4; ++i) h[i] = add2(h[i], w[i]);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum2 = fma2(h[u][i], h[u][i], sum2);
+        for (int i = 0; i < 4; ++i) sum2 = fma2(h[i], h[i], sum2);
     }
     if constexpr (RESIDUAL) {
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
             const int col = (u * row_threads + t) * 8;
-            if (live && col < p.H) store8(static_cast<TS*>(p.total) + base + col, h[u]);
+            if (live && col < p.H) store8(static_cast<TS*>(p.total) + base + col, kept[u]);
         }
     }
     float lo, hi;
     f32x2_split(sum2, lo, hi);
     float sum = row_reduce<false>(lo + hi, slots[0], p.row_warps);
-    float eps = p.eps;
-    // Squares that fp32 cannot hold (values from about 1e17 on): once more with values 2^80 times smaller, next to which eps is nothing.
+    float r = rsqrtf(fmaf(sum, p.inv_h, p.eps));
+    // Squares that fp32 cannot hold (values from about 1e17 on): once more from values 2^80 times smaller, next to which eps is nothing.
     // (All threads that meet at the reduction's barrier hold the same sum.)
     if (sum > 1e37f) {
+        const uint64_t down = f32x2(0x1p-80f, 0x1p-80f);
         sum2 = 0ull;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[u][i] = mul2(h[u][i], f32x2(0x1p-80f, 0x1p-80f)), sum2 = fma2(h[u][i], h[u][i], sum2);
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t h = mul2(kept[u][i], down);
+                sum2 = fma2(h, h, sum2);
+            }
         }
         f32x2_split(sum2, lo, hi);
-        sum = row_reduce<false>(lo + hi, slots[2], p.row_warps);
-        eps = 0.0f;
+        r = rsqrtf(row_reduce<false>(lo + hi, slots[2], p.row_warps) * p.inv_h) * 0x1p-80f;
     }
-    const float r = rsqrtf(fmaf(sum, p.inv_h, eps));
     const uint64_t r2 = f32x2(r, r);
-
     float m[LOADS];
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
-        const int col = (u * row_threads + t) * 8;
-        uint64_t w[4] = {0ull, 0ull, 0ull, 0ull};
-        if (col < p.H) unpack8<TW>(load8(static_cast<const TW*>(p.weight) + col), w);
+        uint64_t w[4];
+        if constexpr (EARLY) unpack8<TW>(raw_w[u], w);
+        else unpack8<TW>(load_weight(u), w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[u][i] = mul2(mul2(h[u][i], r2), w[i]);
-        m[u] = amax8_nan(h[u]);
+        for (int i = 0; i < 4; ++i) kept[u][i] = mul2(mul2(kept[u][i], r2), w[i]);
+        m[u] = amax8_nan(kept[u]);
     }
     QuantScale qs[LOADS];
     if constexpr (BLOCK) {
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) qs[u] = make_out_scale<OUT>(lanes_max_nan<16>(m[u]));
+        block_scales<OUT, LOADS>(m, qs);
     } else {
         float top = m[0];
 #pragma unroll
         for (int u = 1; u < LOADS; ++u) top = max_nan(top, m[u]);
-        const QuantScale all = make_out_scale<OUT>(row_reduce<true>(top, slots[1], p.row_warps));
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) qs[u] = all;
-        if (live && t == 0) p.s[row] = all.s;
+        qs[0] = make_out_scale<OUT>(row_reduce<true>(top, slots[1], p.row_warps));
+        if (live && t == 0) p.s[row] = qs[0].s;
     }
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
         const int col = (u * row_threads + t) * 8;
         if (live && col < p.H) {
             if (BLOCK && (t & 15) == 0) p.s[row * p.KB + (col >> 7)] = qs[u].s;
-            *reinterpret_cast<uint2*>(p.q + base + col) = out8_pack8<OUT>(h[u], qs[u]);
+            *reinterpret_cast<uint2*>(p.q + base + col) = out8_pack8<OUT>(kept[u], qs[BLOCK ? u : 0]);
         }
     }
 }

@@ -47,6 +47,42 @@ GI8_DEVICE QuantScale make_out_scale(float amax)
     return q;
 }
 
+// Scales of U values a lane over runs of sixteen lanes (128-wide blocks), one division a lane instead of U: while a butterfly doubles the lanes
+// that a value has been reduced over it halves the values that a lane is in charge of, so that in the end each lane holds the maximum of one of them,
+// makes its scale, and fetches the others'.  (As group_scales of k_quant.cuh, for either type, and with NaN.)
+template <Out8 OUT, int U>
+GI8_DEVICE void block_scales(float (&m)[U], QuantScale (&qs)[U])
+{
+    static_assert(U == 1 || U == 2 || U == 4 || U == 8, "values a lane");
+    const int lane = threadIdx.x & 31;
+    int n = U;
+#pragma unroll
+    for (int o = 1; o < U; o <<= 1) {
+        n >>= 1;
+        const bool up = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < U / 2; ++i) {
+            if (i < n) {
+                const float keep = up ? m[i + n] : m[i], give = up ? m[i] : m[i + n];
+                m[i] = max_nan(keep, __shfl_xor_sync(0xffffffffu, give, o));
+            }
+        }
+    }
+#pragma unroll
+    for (int o = U; o < 16; o <<= 1) m[0] = max_nan(m[0], __shfl_xor_sync(0xffffffffu, m[0], o));
+    const QuantScale mine = make_out_scale<OUT>(m[0]);
+    const int first = lane & ~15;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        // the lane whose lowest bits are those of u from the highest down
+        int src = first;
+#pragma unroll
+        for (int b = 1, h = U / 2; b < U; b <<= 1, h >>= 1) src += u & h ? b : 0;
+        qs[u].s = U == 1 ? mine.s : __shfl_sync(0xffffffffu, mine.s, src);
+        qs[u].r = U == 1 ? mine.r : __shfl_sync(0xffffffffu, mine.r, src);
+    }
+}
+
 // Two floats -> two packed e4m3 (lo in the low byte).
 GI8_DEVICE uint32_t cvt_e4m3x2(float lo, float hi)
 {

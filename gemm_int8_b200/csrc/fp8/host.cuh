@@ -1,0 +1,146 @@
+// C ABI of the product in 8-bit floating point and its layer: argument checks, the choice of a tile, launches.  Included at the end of api.cu,
+// behind ffn/host.cuh, whose helpers it uses.
+#pragma once
+
+#include "k_fp8_gemm.cuh"
+
+namespace {
+
+// Tile forms and what a wave of them costs per K block, in ns (back to back; of one full wave and of many, which run at lower clocks: two-CTA 0.46 - 0.51 us, 128 x 256
+// 0.44 - 0.53, 128 x 128 0.27 - 0.31, 128 x 64 0.23 - 0.26).
+constexpr TileForm kFp8Forms[] = {{256, true, 480.0, 0, 0}, {256, false, 495.0, 0, 0}, {128, false, 300.0, 0, 0}, {64, false, 245.0, 0, 0}};
+
+struct Fp8Choice {
+    int bn;
+    bool pair;
+};
+
+// The form whose waves take the fewest cycles.
+Fp8Choice choose_fp8(int64_t M, int64_t N, int sms)
+{
+    Fp8Choice best{};
+    double best_cost = 1e300;
+    for (const TileForm& f : kFp8Forms) {
+        const int tile_m = f.pair ? 2 * kBM : kBM;
+        const int64_t tiles = ((M + tile_m - 1) / tile_m) * ((N + f.bn - 1) / f.bn);
+        const int64_t slots = f.pair ? sms / 2 : sms;
+        const double cost = static_cast<double>((tiles + slots - 1) / slots) * f.kblock_cycles;
+        if (cost < best_cost) best_cost = cost, best = {f.bn, f.pair};
+    }
+    return best;
+}
+
+template <int BN, int STAGES, bool PAIR, bool BIAS>
+int launch_fp8(DeviceState* st, int slot, const int8_t* x, const int8_t* y, Fp8GemmParams p, cudaStream_t s)
+{
+    constexpr size_t smem = fp8_smem_bytes(BN, STAGES, PAIR);
+    static_assert(smem <= 227 * 1024 - 512, "shared memory per CTA");
+    auto kernel = fp8_gemm_kernel<BN, STAGES, PAIR, BIAS>;
+    if (int rc = ensure_smem(st, slot, kernel, smem)) return rc;
+    CUtensorMap mx, my, mo{};
+    if (int rc = make_operand_map(&mx, x, p.M, p.K, kBM)) return rc;
+    if (int rc = make_operand_map(&my, y, p.N, p.K, PAIR ? BN / 4 : BN)) return rc;
+    if (p.tma_store)
+        if (int rc = make_output_map(&mo, p.out, p.M, p.N, p.ldo, kFp8StoreCols)) return rc;
+    constexpr int kTileM = PAIR ? 2 * kBM : kBM;
+    p.tiles_m = (p.M + kTileM - 1) / kTileM, p.tiles_n = (p.N + BN - 1) / BN;
+    p.group_m = pick_group_m(p.K);
+    if (PAIR) p.group_m = std::max(1, p.group_m / 2);
+    const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
+    const int slots = PAIR ? st->sm_count / 2 : st->sm_count;
+    const int grid = static_cast<int>(std::min<int64_t>(tiles, slots)) * (PAIR ? 2 : 1);
+    p.release_late = !PAIR && !(p.after_quant && BN < 256) && (tiles <= st->sm_count || p.K % 32 != 0) && release_late(tiles, st->sm_count);
+    return launch(kernel, dim3(grid), kBlockwiseThreads, smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mx, my, mo, p);
+}
+
+template <bool BIAS>
+int launch_fp8(DeviceState* st, Fp8Choice c, const int8_t* x, const int8_t* y, const Fp8GemmParams& p, cudaStream_t s)
+{
+    constexpr int slot = BIAS ? 64 : 70;
+    if (c.pair) return launch_fp8<256, 6, true, BIAS>(st, slot, x, y, p, s);
+    if (c.bn == 256) return launch_fp8<256, 4, false, BIAS>(st, slot + 1, x, y, p, s);
+    if (c.bn == 128) return launch_fp8<128, 6, false, BIAS>(st, slot + 2, x, y, p, s);
+    return launch_fp8<64, 8, false, BIAS>(st, slot + 3, x, y, p, s);
+}
+
+// (bias, after_quant: see scaled_impl)
+int fp8_matmul(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out, int64_t M, int64_t N, int64_t K,
+               void* stream, const uint16_t* bias, bool after_quant)
+{
+    if (int rc = check_common(x, y, out, M, N, K, 2)) return rc;
+    if (M == 0 || N == 0) return GI8_OK;
+    if (K > 0)
+        if (int rc = check_block_scales(sa, ld_sa, sw, ld_sw, M, N, K)) return rc;
+    DeviceState* st;
+    if (int rc = get_device_state(&st)) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (K == 0) return zero_output(out, M * N * 2, s);
+    after_quant = after_quant && knobs().pdl;
+    const int forced = g_forced_variant;
+    if (forced == VAR_AUTO && use_blockwise_smallm(M, N, K)) {
+        BlockwiseSmallMParams q{};
+        q.out = static_cast<uint16_t*>(out), q.sa = sa, q.sw = sw, q.bias = bias, q.status = st->status;
+        q.ldo = N, q.ld_sa = ld_sa, q.ld_sw = ld_sw, q.M = (int)M, q.N = (int)N, q.K = (int)K;
+        q.after_quant = after_quant;
+        if (blockwise_smallm_six_stages(N, K, q.after_quant, st->sm_count)) return launch_blockwise_smallm<6, E4m3>(st, 77, x, y, q, s);
+        return launch_blockwise_smallm<4, E4m3>(st, 76, x, y, q, s);
+    }
+    Fp8GemmParams p{};
+    p.out = out, p.sa = sa, p.sw = sw, p.bias = bias, p.status = st->status, p.ldo = N, p.ld_sa = ld_sa, p.ld_sw = ld_sw;
+    p.M = (int)M, p.N = (int)N, p.K = (int)K;
+    p.tma_store = !misaligned(out, 16) && N % 8 == 0 && knobs().tma_store;
+    p.pair_ok = !misaligned(out, 4) && N % 2 == 0;
+    p.bias_vec = !misaligned(bias, 16);
+    p.after_quant = after_quant;
+    p.scale_vec = (K + kBK - 1) / kBK % 4 == 0 && ld_sa % 4 == 0 && !misaligned(sa, 16);
+    Fp8Choice c;
+    switch (forced) {
+        case VAR_DENSE_BN256: c = {256, false}; break;
+        case VAR_DENSE_BN128: c = {128, false}; break;
+        case VAR_DENSE_BN64: c = {64, false}; break;
+        case VAR_PAIR: c = {256, true}; break;
+        default: c = choose_fp8(M, N, st->sm_count);
+    }
+    return bias ? launch_fp8<true>(st, c, x, y, p, s) : launch_fp8<false>(st, c, x, y, p, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int gi8_fp8_quantize_token_block(const void* in, int in_dtype, void* q, float* scales, int64_t M, int64_t K, void* stream)
+{
+    if (int rc = check_quant(in, in_dtype, static_cast<const int8_t*>(q), scales, M, K)) return rc;
+    if (K % 8) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "K=%lld must be a multiple of 8", (long long)K);
+    if (M == 0 || K == 0) return GI8_OK;
+    DeviceState* st;
+    if (int rc = get_device_state(&st)) return rc;
+    ActParams p{in, static_cast<uint8_t*>(q), scales, M, static_cast<int>(K), static_cast<int>((K + 127) / 128)};
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return in_dtype == 0 ? launch_act_block<float, false, Out8::kE4m3>(p, s) : launch_act_block<__nv_bfloat16, false, Out8::kE4m3>(p, s);
+}
+
+int gi8_fp8_matmul_blockwise(const void* x, const void* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out, int64_t M, int64_t N,
+                             int64_t K, void* stream)
+{
+    return fp8_matmul(static_cast<const int8_t*>(x), static_cast<const int8_t*>(y), sa, ld_sa, sw, ld_sw, out, M, N, K, stream, nullptr, false);
+}
+
+int gi8_fp8_linear(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const void* bias, void* xq, float* xs, void* out,
+                   int64_t M, int64_t N, int64_t K, void* stream)
+{
+    // Everything that the quantiser or the product refuses is refused before the quantiser is launched (as in gi8_linear).
+    if (int rc = check_common(xq, w, out, M, N, K, 2)) return rc;
+    if (int rc = check_quant(x, x_dtype, static_cast<const int8_t*>(xq), xs, M, K)) return rc;
+    if (misaligned(bias, 2)) return fail(GI8_ERR_MISALIGNED, "bias must be 2-byte aligned");
+    if (M == 0 || N == 0) return GI8_OK;
+    if (K == 0 && bias) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "K must be positive for a product with a bias");
+    const int64_t ld_xs = (K + kBK - 1) / kBK;
+    if (K > 0)
+        if (int rc = check_block_scales(xs, ld_xs, w_scale, ld_sw, M, N, K)) return rc;
+    if (int rc = gi8_fp8_quantize_token_block(x, x_dtype, xq, xs, M, K, stream)) return rc;
+    return fp8_matmul(static_cast<const int8_t*>(xq), static_cast<const int8_t*>(w), xs, ld_xs, w_scale, ld_sw, out, M, N, K, stream,
+                      static_cast<const uint16_t*>(bias), K > 0);
+}
+
+}  // extern "C"

@@ -202,19 +202,6 @@ GI8_DEVICE void promote_pair_biased(uint64_t& acc, uint32_t v0, uint32_t v1, uin
         : "r"(v0), "r"(v1), "l"(c2), "l"(b2), "l"(ts2));
 }
 
-// The same for a partial that is fp32 already (e4m3 operands).
-GI8_DEVICE void promote_pair_f32(uint64_t& acc, uint32_t v0, uint32_t v1, uint64_t t2)
-{
-    asm volatile(
-        "{\n\t"
-        ".reg .b64 pv;\n\t"
-        "mov.b64 pv, {%1, %2};\n\t"
-        "fma.rn.f32x2 %0, pv, %3, %0;\n\t"
-        "}\n"
-        : "+l"(acc)
-        : "r"(v0), "r"(v1), "l"(t2));
-}
-
 // One accumulator the slow way, for scale products that promote_pair_biased does not cover: the sum over K blocks of one
 // output element, from the operands in global memory (K a multiple of 16, rows 16-byte aligned).
 GI8_DEVICE float chain_from_global(const int8_t* x, const int8_t* y, const float* sa, const float* sw, int K)
@@ -267,14 +254,6 @@ GI8_DEVICE uint32_t pack_bf16x2_of(uint64_t pair)
     return pack_bf16x2(lo, hi);
 }
 
-// A packed fp32 pair plus a packed bf16 pair.
-GI8_DEVICE uint64_t plus_bf16x2(uint64_t pair, uint32_t b)
-{
-    float lo, hi;
-    f32x2_split(pair, lo, hi);
-    return f32x2(lo + __uint_as_float(b << 16), hi + __uint_as_float(b & 0xffff0000u));
-}
-
 // Position `tile` of the sequence that starts at tile `rot` and wraps at `n` (rot < n).
 GI8_DEVICE int rotate_tile(int tile, int rot, int n)
 {
@@ -311,9 +290,7 @@ GI8_DEVICE void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(
 // tile columns cg * 128 + h * 64 .. (still contiguous and inside one weight-scale block).
 // BIAS: a bf16 vector is added to the rounded result.  A template parameter, not a branch: with the branch in the epilogue
 // the K loop of the 256-wide forms was compiled 6 % slower (2048 x 11008 x 4096: 97 -> 103 us).
-// E4M3: operands in 8-bit floating point.  A partial is then an fp32 sum, which needs neither bias nor conversion: one multiply-add per
-// pair of columns (promote_pair_f32).  A bias is added before the only rounding.
-template <int BN, int STAGES, int SPLIT, int NISS, bool PAIR, bool BIAS, bool DECOUPLED, bool E4M3 = false>
+template <int BN, int STAGES, int SPLIT, int NISS, bool PAIR, bool BIAS, bool DECOUPLED>
 __global__ void __launch_bounds__(kBlockwiseThreads, 1)
 blockwise_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                       const __grid_constant__ OutputMaps outs, const BlockwiseParams p)
@@ -339,14 +316,14 @@ blockwise_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     // same warp hands back after the awaited K block (see the protocol above).
     static_assert(DECOUPLED || STAGES >= NBUF, "the stage ring must be at least as deep as the partial-buffer ring");
     static_assert(!PAIR || BN == 256, "two-CTA tiles are 256 wide");
-    constexpr bool BIASED = SPLIT == 2 && !E4M3;
+    constexpr bool BIASED = SPLIT == 2;
     constexpr int kTileM = PAIR ? 2 * kBM : kBM;  // rows of the (pair's) tile
     constexpr int kRowsB = PAIR ? BN / 2 : BN;    // rows of y this CTA loads
     constexpr uint32_t kBytesA = kBM * kBK;
     constexpr uint32_t kBytesB = kRowsB * kBK;
     constexpr uint32_t kStageBytes = kBytesA + kBytesB;
     constexpr uint32_t kTmemCols = 512;
-    constexpr uint32_t kIdesc = E4M3 ? make_idesc_e4m3(kTileM, NSUB) : make_idesc_i8(kTileM, NSUB, false);
+    constexpr uint32_t kIdesc = make_idesc_i8(kTileM, NSUB, false);
     // Tile column of the first column of segment (half h, column group cg), see above.
     constexpr int kSegStrideH = (PAIR && SPLIT == 2) ? SEGW : NSUB;
     constexpr int kSegStrideCg = (PAIR && SPLIT == 2) ? NSUB : SEGW;
@@ -519,9 +496,7 @@ blockwise_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                     // The first K step overwrites the buffer.
 #pragma unroll
                     for (int k = 0; k < kBK / kUmmaK; ++k) {
-                        if constexpr (E4M3 && PAIR) umma_f8_pair(tmem_d, smem_desc_k128_of(da + 2 * k), smem_desc_k128_of(db + 2 * k), kIdesc, k != 0 ? 1u : 0u);
-                        else if constexpr (E4M3) umma_f8(tmem_d, smem_desc_k128_of(da + 2 * k), smem_desc_k128_of(db + 2 * k), kIdesc, k != 0 ? 1u : 0u);
-                        else if constexpr (PAIR) umma_i8_pair(tmem_d, smem_desc_k128_of(da + 2 * k), smem_desc_k128_of(db + 2 * k), kIdesc, k != 0 ? 1u : 0u);
+                        if constexpr (PAIR) umma_i8_pair(tmem_d, smem_desc_k128_of(da + 2 * k), smem_desc_k128_of(db + 2 * k), kIdesc, k != 0 ? 1u : 0u);
                         else umma_i8(tmem_d, smem_desc_k128_of(da + 2 * k), smem_desc_k128_of(db + 2 * k), kIdesc, k != 0 ? 1u : 0u);
                     }
                     if constexpr (BIASED) {
@@ -665,7 +640,6 @@ blockwise_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                         for (int q = 0; q < CHW / 2; ++q) {
                             uint64_t& a = acc[h * (SEGW / 2) + c * (CHW / 2) + q];
                             if constexpr (BIASED) promote_pair_biased(a, v[2 * q], v[2 * q + 1], unbias_c2, unbias_b2, t2);
-                            else if constexpr (E4M3) promote_pair_f32(a, v[2 * q], v[2 * q + 1], t2);
                             else promote_pair(a, v[2 * q], v[2 * q + 1], t2);
                         }
                     }
@@ -694,7 +668,7 @@ blockwise_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                     constexpr int B = decltype(jc)::value;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float ts = BIASED ? t[h] * 0x1p22f : t[h];
+                        const float ts = t[h] * 0x1p22f;
                         const uint64_t t2 = f32x2(ts, ts);
 #pragma unroll
                         for (int c = 0; c < NC; ++c) {
@@ -715,11 +689,8 @@ blockwise_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                                 polled = mbar_test_wait_addr(bar_part_0 + (hn * NBUF + bn) * 8, (buf_par >> bn) & 1u);
                             }
 #pragma unroll
-                            for (int q = 0; q < CHW / 2; ++q) {
-                                uint64_t& a = acc[h * (SEGW / 2) + c * (CHW / 2) + q];
-                                if constexpr (BIASED) promote_pair_biased(a, v[cur][2 * q], v[cur][2 * q + 1], unbias_c2, unbias_b2, t2);
-                                else promote_pair_f32(a, v[cur][2 * q], v[cur][2 * q + 1], t2);
-                            }
+                            for (int q = 0; q < CHW / 2; ++q)
+                                promote_pair_biased(acc[h * (SEGW / 2) + c * (CHW / 2) + q], v[cur][2 * q], v[cur][2 * q + 1], unbias_c2, unbias_b2, t2);
                         }
                     }
                     return true;
@@ -908,14 +879,10 @@ blockwise_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
                         for (int q = 0; q < STORE_W / 8; ++q) {
                             const int cq = STORE_W == 64 ? (q ^ (lane & 7)) : (q ^ ((lane >> 1) & 3));
                             const int a0 = b * (STORE_W / 2) + 4 * q;
-                            uint4 bv;
-                            if constexpr (BIAS) bv = load_bias8(p.bias, col0 + 8 * q, p.N, p.bias_vec);
-                            if constexpr (BIAS && E4M3)
-                                acc[a0] = plus_bf16x2(acc[a0], bv.x), acc[a0 + 1] = plus_bf16x2(acc[a0 + 1], bv.y), acc[a0 + 2] = plus_bf16x2(acc[a0 + 2], bv.z),
-                                acc[a0 + 3] = plus_bf16x2(acc[a0 + 3], bv.w);
                             uint4 w = make_uint4(pack_bf16x2_of(acc[a0]), pack_bf16x2_of(acc[a0 + 1]), pack_bf16x2_of(acc[a0 + 2]),
                                                  pack_bf16x2_of(acc[a0 + 3]));
-                            if constexpr (BIAS && !E4M3) {
+                            if constexpr (BIAS) {
+                                const uint4 bv = load_bias8(p.bias, col0 + 8 * q, p.N, p.bias_vec);
                                 w = make_uint4(add_bf16x2(w.x, bv.x), add_bf16x2(w.y, bv.y), add_bf16x2(w.z, bv.z), add_bf16x2(w.w, bv.w));
                             }
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stg + lane * (STORE_W * 2) + cq * 16),

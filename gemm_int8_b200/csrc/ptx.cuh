@@ -461,6 +461,27 @@ GI8_DEVICE uint64_t f32x2(float lo, float hi)
 }
 GI8_DEVICE void f32x2_split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
 
+// acc{lo,hi} += {v0,v1} * t2 for a pair of fp32 partials that a tensor-memory load left in two consecutive registers.
+GI8_DEVICE void promote_pair_f32(uint64_t& acc, uint32_t v0, uint32_t v1, uint64_t t2)
+{
+    asm volatile(
+        "{\n\t"
+        ".reg .b64 pv;\n\t"
+        "mov.b64 pv, {%1, %2};\n\t"
+        "fma.rn.f32x2 %0, pv, %3, %0;\n\t"
+        "}\n"
+        : "+l"(acc)
+        : "r"(v0), "r"(v1), "l"(t2));
+}
+
+// A packed fp32 pair plus a packed bf16 pair.
+GI8_DEVICE uint64_t plus_bf16x2(uint64_t pair, uint32_t b)
+{
+    float lo, hi;
+    f32x2_split(pair, lo, hi);
+    return f32x2(lo + __uint_as_float(b << 16), hi + __uint_as_float(b & 0xffff0000u));
+}
+
 // max(|a|, |b|, |c|): ignoring NaN, and propagating it.
 GI8_DEVICE float max3_abs(float a, float b, float c)
 {
@@ -605,6 +626,13 @@ GI8_DEVICE void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, 
 GI8_DEVICE void umma_commit_pair(uint32_t bar_cluster_addr)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar_cluster_addr)
+                 : "memory");
+}
+
+// The same onto the barriers at one shared-memory address of both CTAs of the pair.
+GI8_DEVICE void umma_commit_both(uint32_t bar_addr)
+{
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar_addr), "h"(static_cast<uint16_t>(3))
                  : "memory");
 }
 

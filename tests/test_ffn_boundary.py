@@ -129,3 +129,28 @@ def test_torch_quantisers_in_e4m3():
     assert float(s[3, 0]) == 1.0 and not q[3, :128].float().any()
     with pytest.raises(ValueError):
         quant.quantize_weight_block(a, dtype=torch.float16)
+
+
+# The rules on waits that hold for the kernels of the package, read from the source of the e4m3 product.
+def _kernels():
+    import os
+
+    import test_kernel_waits as W
+
+    csrc, W.CSRC = W.CSRC, os.path.join(W.CSRC, "fp8")
+    try:
+        return W._kernels()
+    finally:
+        W.CSRC = csrc
+
+
+def test_waits_of_the_e4m3_product():
+    import test_kernel_waits as W
+
+    kernels = _kernels()
+    assert {p.id for p in kernels} == {"fp8_gemm_kernel"}
+    W.test_last_commits_are_awaited(kernels[0].values[0])
+    W.test_lanes_of_a_warp_decide_together(kernels[0].values[0])
+    # copies that the warps issue themselves have landed before the CTA ends
+    body = kernels[0].values[0]
+    assert body.rindex("cp_async_wait_all()") > body.rindex("cp_async_arrive(")
