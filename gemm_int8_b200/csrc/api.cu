@@ -782,7 +782,8 @@ int launch_blockwise_smallm(DeviceState* st, int slot, const int8_t* x, const in
     CUtensorMap mw, mx;
     if (int rc = make_operand_map(&mw, w, p.N, p.K, kBwSmallTileN)) return rc;
     if (int rc = make_operand_map(&mx, x, p.M, p.K, kBwSmallTokens)) return rc;
-    return launch(kernel, dim3((p.N + kBwSmallTileN - 1) / kBwSmallTileN), S::THREADS, S::SMEM, stream, dim3(1), knobs().pdl, mw, mx, p);
+    const unsigned splits = sizeof...(OPERAND) != 0 ? p.splits : 1;
+    return launch(kernel, dim3((p.N + kBwSmallTileN - 1) / kBwSmallTileN, splits), S::THREADS, S::SMEM, stream, dim3(1, splits), knobs().pdl, mw, mx, p);
 }
 
 template <int MT, int STAGES>

@@ -13,29 +13,64 @@ constexpr TileForm kFp8Forms[] = {{256, true, 480.0, 0, 0}, {256, false, 495.0, 
 struct Fp8Choice {
     int bn;
     bool pair;
+    int splits;  // CTAs that share a tile's K blocks
 };
 
-// The form whose waves take the fewest cycles.
-Fp8Choice choose_fp8(int64_t M, int64_t N, int sms)
+// ns that a split costs beside its K blocks: two barriers of the cluster and the sums that its CTAs send each other (rows: of the tile that are stored).  Fitted to
+// 32 to 256 tokens x 1024 to 8192 columns, K = 4096 to 28672, us without / with two / with four CTAs a tile: 64 x 4096 x 14336 28.7 / 19.0 (64-wide) and 17.0 (128-wide, four),
+// 64 x 4096 x 4096 11.3 / 10.0 / 10.4, 40 x 2048 x 8192 18.0 / 13.3 / 11.7, 256 x 4096 x 14336 29.8 / 23.6 / 24.4, 1024 x 1024 x 8192 19.0 / 16.3 / 17.8, 100 x 1001 x 6992
+// 22.0 / 16.4 / 14.9; not 300 x 300 x 1024 6.3 / 7.2, 200 x 640 x 2048 7.3 / 8.0.
+double fp8_split_fixed(int bn, int splits, int64_t rows)
+{
+    const double part = static_cast<double>(std::min<int64_t>(4, (rows + 31) / 32)) / 4.0;
+    if (bn == 64) return 2000.0 + 1000.0 * part;
+    if (bn == 128) return splits == 2 ? 2500.0 + 1600.0 * part : 3900.0 + 2400.0 * part;
+    return splits == 2 ? 3500.0 + 2800.0 * part : 5000.0 + 3600.0 * part;
+}
+
+// K blocks of each CTA of a split tile: a multiple of four, so that 16-byte copies of the row scales stay aligned.
+int fp8_kb_per_split(int64_t kb, int splits) { return static_cast<int>((kb + 4 * splits - 1) / (4 * splits)) * 4; }
+
+// CTAs that share a tile's K blocks in the kernel for few tokens: as many as one CTA an SM leaves room for, with eight K blocks each at least (us with 1 / 2 / 4 / 8: 16 x
+// 4096 x 4096 8.6 / 7.9 / 8.0 / 12.7, 16 x 4096 x 14336 21.9 / 15.0 / 14.1 / 19.8, 16 x 2048 x 8192 13.6 / 9.7 / 8.1 / 9.2, 1 x 1024 x 4096 8.0 / 6.3 / 5.8 / 5.6, 16 x 8192 x 8192,
+// which has 128 CTAs, 15.1 / 20.9; 1 x 4096 x 1024 5.4 / 5.5).
+int fp8_smallm_splits(int64_t N, int64_t K, int sms)
+{
+    const int64_t ctas = (N + kBwSmallTileN - 1) / kBwSmallTileN, kb = (K + kBK - 1) / kBK;
+    int splits = 1;
+    while (splits < 8 && ctas * splits * 2 <= sms && kb >= 8 * 2 * splits) splits *= 2;
+    return splits;
+}
+
+// The form whose waves take the least time; grids that leave SMs idle are also weighed with every tile's K blocks split over the CTAs of a cluster.
+Fp8Choice choose_fp8(int64_t M, int64_t N, int64_t K, int sms)
 {
     Fp8Choice best{};
     double best_cost = 1e300;
+    const int64_t kb = (K + kBK - 1) / kBK;
     for (const TileForm& f : kFp8Forms) {
         const int tile_m = f.pair ? 2 * kBM : kBM;
         const int64_t tiles = ((M + tile_m - 1) / tile_m) * ((N + f.bn - 1) / f.bn);
         const int64_t slots = f.pair ? sms / 2 : sms;
-        const double cost = static_cast<double>((tiles + slots - 1) / slots) * f.kblock_cycles;
-        if (cost < best_cost) best_cost = cost, best = {f.bn, f.pair};
+        const double cost = static_cast<double>((tiles + slots - 1) / slots) * f.kblock_cycles * kb;
+        if (cost < best_cost) best_cost = cost, best = {f.bn, f.pair, 1};
+        if (f.pair) continue;
+        for (int splits = 2; splits <= std::min(4, f.bn / 32) && tiles * splits <= sms; splits *= 2) {
+            const int each = fp8_kb_per_split(kb, splits);
+            if (each * (splits - 1) >= kb) break;  // (no CTA without K blocks)
+            const double split = each * f.kblock_cycles + fp8_split_fixed(f.bn, splits, M);
+            if (split < best_cost) best_cost = split, best = {f.bn, false, splits};
+        }
     }
     return best;
 }
 
-template <int BN, int STAGES, bool PAIR, bool BIAS>
+template <int BN, int STAGES, bool PAIR, bool BIAS, bool SPLITK = false>
 int launch_fp8(DeviceState* st, int slot, const int8_t* x, const int8_t* y, Fp8GemmParams p, cudaStream_t s)
 {
     constexpr size_t smem = fp8_smem_bytes(BN, STAGES, PAIR);
     static_assert(smem <= 227 * 1024 - 512, "shared memory per CTA");
-    auto kernel = fp8_gemm_kernel<BN, STAGES, PAIR, BIAS>;
+    auto kernel = fp8_gemm_kernel<BN, STAGES, PAIR, BIAS, SPLITK>;
     if (int rc = ensure_smem(st, slot, kernel, smem)) return rc;
     CUtensorMap mx, my, mo{};
     if (int rc = make_operand_map(&mx, x, p.M, p.K, kBM)) return rc;
@@ -50,13 +85,21 @@ int launch_fp8(DeviceState* st, int slot, const int8_t* x, const int8_t* y, Fp8G
     const int slots = PAIR ? st->sm_count / 2 : st->sm_count;
     const int grid = static_cast<int>(std::min<int64_t>(tiles, slots)) * (PAIR ? 2 : 1);
     p.release_late = !PAIR && !(p.after_quant && BN < 256) && (tiles <= st->sm_count || p.K % 32 != 0) && release_late(tiles, st->sm_count);
+    if constexpr (SPLITK) return launch(kernel, dim3(static_cast<unsigned>(tiles), p.splits), kBlockwiseThreads, smem, s, dim3(1, p.splits), knobs().pdl, mx, my, mo, p);
     return launch(kernel, dim3(grid), kBlockwiseThreads, smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mx, my, mo, p);
 }
 
 template <bool BIAS>
 int launch_fp8(DeviceState* st, Fp8Choice c, const int8_t* x, const int8_t* y, const Fp8GemmParams& p, cudaStream_t s)
 {
-    constexpr int slot = BIAS ? 64 : 70;
+    constexpr int slot = BIAS ? 64 : 71;
+    if (c.splits > 1) {
+        Fp8GemmParams q = p;
+        q.splits = c.splits, q.kb_per_split = fp8_kb_per_split((p.K + kBK - 1) / kBK, c.splits);
+        if (c.bn == 256) return launch_fp8<256, 4, false, BIAS, true>(st, slot + 4, x, y, q, s);
+        if (c.bn == 128) return launch_fp8<128, 6, false, BIAS, true>(st, slot + 5, x, y, q, s);
+        return launch_fp8<64, 8, false, BIAS, true>(st, slot + 6, x, y, q, s);
+    }
     if (c.pair) return launch_fp8<256, 6, true, BIAS>(st, slot, x, y, p, s);
     if (c.bn == 256) return launch_fp8<256, 4, false, BIAS>(st, slot + 1, x, y, p, s);
     if (c.bn == 128) return launch_fp8<128, 6, false, BIAS>(st, slot + 2, x, y, p, s);
@@ -82,8 +125,10 @@ int fp8_matmul(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa,
         q.out = static_cast<uint16_t*>(out), q.sa = sa, q.sw = sw, q.bias = bias, q.status = st->status;
         q.ldo = N, q.ld_sa = ld_sa, q.ld_sw = ld_sw, q.M = (int)M, q.N = (int)N, q.K = (int)K;
         q.after_quant = after_quant;
-        if (blockwise_smallm_six_stages(N, K, q.after_quant, st->sm_count)) return launch_blockwise_smallm<6, E4m3>(st, 77, x, y, q, s);
-        return launch_blockwise_smallm<4, E4m3>(st, 76, x, y, q, s);
+        q.splits = fp8_smallm_splits(N, K, st->sm_count);
+        q.kb_per_split = static_cast<int>(((K + kBK - 1) / kBK + q.splits - 1) / q.splits);
+        if (q.splits == 1 && blockwise_smallm_six_stages(N, K, q.after_quant, st->sm_count)) return launch_blockwise_smallm<6, E4m3>(st, 79, x, y, q, s);
+        return launch_blockwise_smallm<4, E4m3>(st, 78, x, y, q, s);
     }
     Fp8GemmParams p{};
     p.out = out, p.sa = sa, p.sw = sw, p.bias = bias, p.status = st->status, p.ldo = N, p.ld_sa = ld_sa, p.ld_sw = ld_sw;
@@ -95,11 +140,11 @@ int fp8_matmul(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa,
     p.scale_vec = (K + kBK - 1) / kBK % 4 == 0 && ld_sa % 4 == 0 && !misaligned(sa, 16);
     Fp8Choice c;
     switch (forced) {
-        case VAR_DENSE_BN256: c = {256, false}; break;
-        case VAR_DENSE_BN128: c = {128, false}; break;
-        case VAR_DENSE_BN64: c = {64, false}; break;
-        case VAR_PAIR: c = {256, true}; break;
-        default: c = choose_fp8(M, N, st->sm_count);
+        case VAR_DENSE_BN256: c = {256, false, 1}; break;
+        case VAR_DENSE_BN128: c = {128, false, 1}; break;
+        case VAR_DENSE_BN64: c = {64, false, 1}; break;
+        case VAR_PAIR: c = {256, true, 1}; break;
+        default: c = choose_fp8(M, N, K, st->sm_count);
     }
     return bias ? launch_fp8<true>(st, c, x, y, p, s) : launch_fp8<false>(st, c, x, y, p, s);
 }

@@ -4,6 +4,7 @@
 #pragma once
 
 #include "../k_blockwise.cuh"
+#include "../k_quant.cuh"  // packed arithmetic
 
 namespace gi8 {
 
@@ -22,6 +23,7 @@ struct Fp8GemmParams {
     int bias_vec;      // bias is 16-byte aligned
     int after_quant;   // launched as the programmatic dependent of the quantiser that writes x and sa (and of nothing else)
     int scale_vec;     // ceil(K/128) % 4 == 0 and the rows of sa are 16-byte aligned: scales are copied four at a time
+    int splits, kb_per_split;  // SPLITK: CTAs of a cluster (BN / splits a multiple of 32), K blocks of each (a multiple of 4; the last has the rest)
     int release_late;  // do not let the next launch start before the CTAs have ended (see the host's release_late)
 };
 
@@ -47,11 +49,14 @@ GI8_DEVICE void cp_async_4(uint32_t smem_dst, const void* src, uint32_t src_byte
 // Where the four scales c (of four) of row r lie in a group: eight neighbouring rows' 16 bytes take different banks.
 GI8_DEVICE uint32_t fp8_scale_at(int r, int c) { return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) * 16)); }
 
-template <int BN, int STAGES, bool PAIR, bool BIAS>
+// SPLITK: the CTAs of a cluster share one tile, each over K blocks of its own (ranges of kb_per_split in rank order); at the end every CTA is
+// sent the other ones' sums of its share of the columns, adds them up in rank order and stores them.
+template <int BN, int STAGES, bool PAIR, bool BIAS, bool SPLITK = false>
 __global__ void __launch_bounds__(kBlockwiseThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y, const __grid_constant__ CUtensorMap map_out,
                 const Fp8GemmParams p)
 {
+    static_assert(!(PAIR && SPLITK), "a cluster is a pair or a split");
     static_assert(BN == 256 || (!PAIR && (BN == 128 || BN == 64)), "tile widths");
     constexpr int NBUF = 512 / BN;            // partial buffers in tensor memory ...
     constexpr int SPLIT = BN == 256 ? 2 : 1;  // ... each in as many parts with an issuer and barriers of their own
@@ -84,8 +89,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int num_tiles = p.tiles_m * p.tiles_n;
-    const int num_kb = (p.K + kBK - 1) / kBK;
+    const int kb_all = (p.K + kBK - 1) / kBK;
     const uint32_t rank = PAIR ? cluster_cta_rank() : 0u;
+    // K blocks kb_0 .. kb_0 + num_kb - 1 are this CTA's
+    const uint32_t share = SPLITK ? cluster_cta_rank() : 0u;
+    const int kb_0 = SPLITK ? static_cast<int>(share) * p.kb_per_split : 0;
+    const int num_kb = SPLITK ? min(p.kb_per_split, kb_all - kb_0) : kb_all;
     const int first_tile = PAIR ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
     const int tile_step = PAIR ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
 
@@ -139,13 +148,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     if (elect_one()) {
                         for (int kb = 0; kb < kb_early; ++kb) {
                             mbar_arrive_expect_tx(&bar_full[kb], kStageBytes);
-                            tma_load_2d(smem + kb * kStageBytes + kBytesA, &map_y, &bar_full[kb], kb * kBK, nb * BN);
+                            tma_load_2d(smem + kb * kStageBytes + kBytesA, &map_y, &bar_full[kb], (kb_0 + kb) * kBK, nb * BN);
                         }
                     }
                     __syncwarp();
                     pdl_wait();
                     if (elect_one()) {
-                        for (int kb = 0; kb < kb_early; ++kb) tma_load_2d(smem + kb * kStageBytes, &map_x, &bar_full[kb], kb * kBK, mb * kBM);
+                        for (int kb = 0; kb < kb_early; ++kb) tma_load_2d(smem + kb * kStageBytes, &map_x, &bar_full[kb], (kb_0 + kb) * kBK, mb * kBM);
                     }
                     __syncwarp();
                     armed = static_cast<uint32_t>(kb_early);
@@ -176,8 +185,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                                                  nb * BN + h * NSUB + static_cast<int>(rank) * (NSUB / 2));
                         } else {
                             mbar_arrive_expect_tx(&bar_full[s], kStageBytes);
-                            tma_load_2d(a_tile, &map_x, &bar_full[s], kb * kBK, mb * kBM);
-                            tma_load_2d(a_tile + kBytesA, &map_y, &bar_full[s], kb * kBK, nb * BN);
+                            tma_load_2d(a_tile, &map_x, &bar_full[s], (kb_0 + kb) * kBK, mb * kBM);
+                            tma_load_2d(a_tile + kBytesA, &map_y, &bar_full[s], (kb_0 + kb) * kBK, nb * BN);
                         }
                     }
                     __syncwarp();
@@ -249,14 +258,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 #pragma unroll 4
                         for (int r = lane >> 2; r < kBM; r += 8) {
                             const bool in = row0 + r < p.M && kb + 4 * c < num_kb;
-                            cp_async_16(dst + fp8_scale_at(r, c), in ? p.sa + static_cast<int64_t>(row0 + r) * p.ld_sa + kb + 4 * c : p.sa, in ? 16u : 0u);
+                            cp_async_16(dst + fp8_scale_at(r, c), in ? p.sa + static_cast<int64_t>(row0 + r) * p.ld_sa + kb_0 + kb + 4 * c : p.sa, in ? 16u : 0u);
                         }
                     } else {
                         const int k = lane & 15;
 #pragma unroll 4
                         for (int r = lane >> 4; r < kBM; r += 2) {
                             const bool in = row0 + r < p.M && kb + k < num_kb;
-                            cp_async_4(dst + fp8_scale_at(r, k >> 2) + (k & 3) * 4, in ? p.sa + static_cast<int64_t>(row0 + r) * p.ld_sa + kb + k : p.sa, in ? 4u : 0u);
+                            cp_async_4(dst + fp8_scale_at(r, k >> 2) + (k & 3) * 4, in ? p.sa + static_cast<int64_t>(row0 + r) * p.ld_sa + kb_0 + kb + k : p.sa, in ? 4u : 0u);
                         }
                     }
                     cp_async_arrive(&bar_scale_full[s]);
@@ -265,6 +274,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 }
             }
             cp_async_wait_all();  // (no copy is under way when the CTA ends, whatever has failed)
+        }
+        if constexpr (SPLITK) {  // the two barriers of the split's exchange (a warp's lanes come together for them)
+            __syncwarp();
+            cluster_sync_all();
+            cluster_sync_all();
         }
     } else {
         // ------------------------------------------------------------------ promotion + epilogue warps
@@ -310,7 +324,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             tile_coords(tile, p.tiles_m, p.tiles_n, mb, nb, p.group_m);
             const int col_base = nb * BN + cg * CW;  // (inside one 128-wide weight-scale block)
             // 32-bit element offset (the host checks the array's size)
-            uint32_t sw = static_cast<uint32_t>(col_base < p.N ? col_base / 128 : 0) * static_cast<uint32_t>(p.ld_sw);
+            uint32_t sw = static_cast<uint32_t>(col_base < p.N ? col_base / 128 : 0) * static_cast<uint32_t>(p.ld_sw) + static_cast<uint32_t>(kb_0);
             GI8_PIN(sw);
             // The row's scales of this K block and those behind it in its four; the weight block's: a lane each, for 32 K blocks.
             float a[4];
@@ -371,7 +385,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                 }
                 accumulate(v[1], NC - 1);
             }
-            if (!ok) break;
+            if (!SPLITK && !ok) break;  // (a split tile's CTAs meet below whatever has failed)
 
             // Blocks of 32 rows x STORE_W columns through swizzled shared memory and TMA stores, or row by row where TMA cannot address the rows.
             // (The tile's coordinates again, from an opaque copy, so that they occupy no registers across the loop.)
@@ -379,8 +393,71 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
             asm volatile("" : "+r"(tile_again));
             tile_coords(tile_again, p.tiles_m, p.tiles_n, mb2, nb2, p.group_m);
             const int row0 = mb2 * kTileM + static_cast<int>(rank) * kBM + quarter * 32;
-            if (row0 < p.M) {
-                const uint32_t stg = stage_end + (warp - 4) * kFp8StoreBytes;
+            const uint32_t stg = stage_end + (warp - 4) * kFp8StoreBytes;
+            // A staged block (32 rows x 32 columns, written by this warp) to the output.
+            auto store_block = [&](int col0) {
+                if (!p.tma_store) {
+                    __syncwarp();
+                    store_staged_rows<STORE_W>(stg, static_cast<uint16_t*>(p.out), p.ldo, row0, p.M, col0, p.N, p.pair_ok);
+                    return;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    tma_store_2d(&map_out, reinterpret_cast<const void*>(__cvta_shared_to_generic(stg)), col0, row0);
+                    tma_store_commit();
+                }
+            };
+            if constexpr (SPLITK) {
+                // The sums meet in the stages, which no CTA of the cluster uses any more behind the first barrier: for each sender and 32 columns of the
+                // receiver's share, four columns of all rows after each other, so that a warp's store is one run of 512 bytes.  They are added up in a loop
+                // that is not unrolled: this code runs once, and what it costs is fetching it (unrolled, with the own sums from registers, 64 columns took
+                // 8000 cycles).
+                const int share_cols = BN / p.splits;
+                const uint32_t recv = smem_u32(smem), r = static_cast<uint32_t>(quarter * 32 + lane);
+                cluster_sync_all();
+#pragma unroll
+                for (int b = 0; b < CW / 32; ++b) {
+                    if (row0 >= p.M) break;  // (rows that nobody stores)
+                    const int c = cg * CW + b * 32, owner = c / share_cols;
+                    const uint32_t at = map_to_cta(recv + ((share * share_cols + (c - owner * share_cols)) / 4 * kBM + r) * 16, owner);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(at + q * (kBM * 16)), "l"(acc[b * 16 + 2 * q]), "l"(acc[b * 16 + 2 * q + 1]) : "memory");
+                }
+                cluster_sync_all();
+                if (row0 < p.M) {
+#pragma unroll 1
+                    for (int c = cg * 32; c < share_cols; c += 64) {
+                        const int col0 = nb2 * BN + static_cast<int>(share) * share_cols + c;
+                        if (col0 >= p.N) break;
+                        if (p.tma_store && lane == 0) tma_store_wait_read<0>();
+                        __syncwarp();
+#pragma unroll 1
+                        for (int q = 0; q < 8; ++q) {
+                            uint64_t sum[2] = {0ull, 0ull};
+                            uint32_t at = recv + ((c / 4 + q) * kBM + r) * 16;
+#pragma unroll 1
+                            for (int src = 0; src < p.splits; ++src, at += share_cols / 4 * kBM * 16) {  // in the order of the K blocks
+                                uint64_t v0, v1;
+                                asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v0), "=l"(v1) : "r"(at) : "memory");
+                                sum[0] = add2(sum[0], v0), sum[1] = add2(sum[1], v1);
+                            }
+                            if constexpr (BIAS) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) w[j] = col0 + 4 * q + j < p.N ? __ldg(p.bias + col0 + 4 * q + j) : 0u;
+                                sum[0] = plus_bf16x2(sum[0], w[0] | (w[1] << 16)), sum[1] = plus_bf16x2(sum[1], w[2] | (w[3] << 16));
+                            }
+                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(stg + lane * (STORE_W * 2) + (((q >> 1) ^ ((lane >> 1) & 3)) * 16) + (q & 1) * 8),
+                                         "r"(pack_bf16x2_of(sum[0])), "r"(pack_bf16x2_of(sum[1]))
+                                         : "memory");
+                        }
+                        store_block(col0);
+                    }
+                }
+            }
+            if (!SPLITK && row0 < p.M) {
 #pragma unroll
                 for (int b = 0; b < CW / STORE_W; ++b) {
                     const int col0 = nb2 * BN + cg * CW + b * STORE_W;
@@ -400,19 +477,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                                      "r"(pack_bf16x2_of(acc[a0 + 1])), "r"(pack_bf16x2_of(acc[a0 + 2])), "r"(pack_bf16x2_of(acc[a0 + 3]))
                                      : "memory");
                     }
-                    if (!p.tma_store) {
-                        __syncwarp();
-                        store_staged_rows<STORE_W>(stg, static_cast<uint16_t*>(p.out), p.ldo, row0, p.M, col0, p.N, p.pair_ok);
-                        continue;
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(reinterpret_cast<uint64_t>(&map_out)),
-                                     "r"(stg), "r"(col0), "r"(row0)
-                                     : "memory");
-                        tma_store_commit();
-                    }
+                    store_block(col0);
                 }
             }
             __syncwarp();

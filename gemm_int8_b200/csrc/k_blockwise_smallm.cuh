@@ -28,6 +28,7 @@
 #pragma once
 
 #include "k_blockwise.cuh"
+#include "k_quant.cuh"  // packed arithmetic
 
 namespace gi8 {
 
@@ -43,6 +44,7 @@ struct BlockwiseSmallMParams {
     int64_t ldo, ld_sa, ld_sw;
     int M, N, K;
     int after_quant;      // launched as the programmatic dependent of the quantiser that writes x and sa (and of nothing else)
+    int splits, kb_per_split;  // E4m3: CTAs of a cluster that share a tile's K blocks, and how many each takes (the last has the rest)
 };
 
 template <int STAGES_>
@@ -60,7 +62,8 @@ struct BlockwiseSmallM {
     static constexpr uint32_t SMEM = STAGES * STAGE + BYTES_W + 1024;
 };
 
-// OPERAND: nothing for int8, E4m3 for operands in 8-bit floating point with partials in fp32 (see k_blockwise.cuh).
+// OPERAND: nothing for int8, E4m3 for operands in 8-bit floating point with partials in fp32.  Those need no chain over all K blocks: where the
+// weight rows do not fill the machine the CTAs of a cluster take a range of K blocks each, and the first adds up their sums in the order of the ranges.
 struct E4m3 {};
 template <int STAGES_, typename... OPERAND>
 __global__ void __launch_bounds__(BlockwiseSmallM<STAGES_>::THREADS)
@@ -92,7 +95,9 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     const int tile = blockIdx.x;
-    const int num_kb = (p.K + kBK - 1) / kBK;
+    const uint32_t share = E4M3 ? cluster_cta_rank() : 0u;
+    const int kb_0 = E4M3 ? static_cast<int>(share) * p.kb_per_split : 0;  // this CTA's first K block
+    const int num_kb = E4M3 ? min(p.kb_per_split, (p.K + kBK - 1) / kBK - kb_0) : (p.K + kBK - 1) / kBK;
     const int num_st = (num_kb + 1) / 2;
 
     if (warp == 2) {
@@ -132,12 +137,12 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             const int n = min(2, num_kb - 2 * i);
             mbar_arrive_expect_tx(&bar_full[s], n * (S::BYTES_W + S::BYTES_X));
             for (int j = 0; j < n; ++j)
-                tma_load_2d_hint(smem + s * S::STAGE + j * S::BYTES_W, &map_w, &bar_full[s], (2 * i + j) * kBK, tile * kBwSmallTileN, pol_w);
+                tma_load_2d_hint(smem + s * S::STAGE + j * S::BYTES_W, &map_w, &bar_full[s], (kb_0 + 2 * i + j) * kBK, tile * kBwSmallTileN, pol_w);
         };
         auto load_x = [&](int i, uint32_t s) {
             const int n = min(2, num_kb - 2 * i);
             for (int j = 0; j < n; ++j)
-                tma_load_2d_hint(smem + s * S::STAGE + 2 * S::BYTES_W + j * S::BYTES_X, &map_x, &bar_full[s], (2 * i + j) * kBK, 0, pol_x);
+                tma_load_2d_hint(smem + s * S::STAGE + 2 * S::BYTES_W + j * S::BYTES_X, &map_x, &bar_full[s], (kb_0 + 2 * i + j) * kBK, 0, pol_x);
         };
         const int first = min(num_st, STAGES);
         if (elect_one())
@@ -198,8 +203,8 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
         const uint32_t tm_warp = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + cg * 8;
         // Scale products of a stage: lane l forms that of token 8 cg + l % 8 and K block l / 8 of the stage (the upper half-warp the
         // same once more); shared memory turns them into broadcast operands.  The loads run three stages ahead of their use.
-        const float* sw_row = p.sw + static_cast<int64_t>(tile * kBwSmallTileN / 128) * p.ld_sw;
-        const float* sa_row = p.sa + static_cast<int64_t>(min(cg * 8 + (lane & 7), p.M - 1)) * p.ld_sa;
+        const float* sw_row = p.sw + static_cast<int64_t>(tile * kBwSmallTileN / 128) * p.ld_sw + kb_0;
+        const float* sa_row = p.sa + static_cast<int64_t>(min(cg * 8 + (lane & 7), p.M - 1)) * p.ld_sa + kb_0;
         auto scale_kb = [&](int i) { return min(2 * i + ((lane >> 3) & 1), num_kb - 1); };
         float* const my_t = t_s[cg * 2 + quarter][0];
         const uint32_t t_addr = smem_u32(my_t);
@@ -255,7 +260,32 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             stage(i, std::integral_constant<int, 0>{});
             if (ok && i + 1 < num_st) stage(i + 1, std::integral_constant<int, 1>{});
         }
-        if (n < p.N) {
+        if constexpr (E4M3) {
+            if (p.splits > 1) {
+                // Into the first CTA's stages, which nobody uses any more behind the first barrier: 16 bytes (four tokens) of all weight rows after each other.
+                const uint32_t at = smem_u32(smem) + ((cg * 2 * 64) + quarter * 32 + lane) * 16;
+                __syncwarp();
+                cluster_sync_all();
+                if (share != 0) {
+                    const uint32_t to = map_to_cta(at + share * (S::GROUPS * 2 * 64 * 16), 0);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) asm volatile("st.shared::cluster.v2.b64 [%0], {%1, %2};" ::"r"(to + h * (64 * 16)), "l"(acc[2 * h]), "l"(acc[2 * h + 1]) : "memory");
+                }
+                cluster_sync_all();
+                if (share == 0) {
+#pragma unroll 1
+                    for (int src = 1; src < p.splits; ++src) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint64_t v0, v1;
+                            asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v0), "=l"(v1) : "r"(at + src * (S::GROUPS * 2 * 64 * 16) + h * (64 * 16)) : "memory");
+                            acc[2 * h] = add2(acc[2 * h], v0), acc[2 * h + 1] = add2(acc[2 * h + 1], v1);
+                        }
+                    }
+                }
+            }
+        }
+        if (n < p.N && !(E4M3 && share != 0)) {
             const uint16_t b = p.bias ? __ldg(p.bias + n) : uint16_t(0);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -273,6 +303,12 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
     }
 
     __syncwarp();
+    if constexpr (E4M3) {  // the other warps at the two barriers of the exchange
+        if (p.splits > 1 && !((warp & 3) < 2)) {
+            cluster_sync_all();
+            cluster_sync_all();
+        }
+    }
     tcgen05_fence_before_sync();
     __syncthreads();
     if (warp == 3) {

@@ -71,6 +71,34 @@ def test_exact_sums(M, N, K, variant):
     assert torch.equal(out, want.float().bfloat16())
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 64, 28672), (16, 200, 2064), (9, 4096, 14336), (5, 1000, 4112), (16, 2048, 8192), (40, 2048, 8192), (64, 4096, 14336), (100, 1001, 6992),
+                                   (33, 5003, 4096), (256, 512, 14336), (17, 100, 28672), (130, 1030, 8208), (1024, 1024, 8192), (64, 8192, 28672), (128, 8192, 8192)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_split_k_blocks(M, N, K, bias):
+    """Few tiles with long sums: the K blocks of a tile are shared out.  Exact sums, as above, so the result is the same whoever adds them up; the layer's bias is a whole number."""
+    import gemm_int8_b200 as g
+
+    gen = torch.Generator(device="cuda").manual_seed(K + N)
+    KB = -(-K // 128)
+    x_q = torch.randint(-7, 8, (M, K), generator=gen, device="cuda").float().to(F8)
+    w_q = torch.randint(-7, 8, (N, K), generator=gen, device="cuda").float().to(F8)
+    sx, sw = torch.randint(0, 2, (M, KB), generator=gen, device="cuda").float().exp2(), torch.randint(-1, 1, (-(-N // 128), KB), generator=gen, device="cuda").float().exp2()
+    want = R.product(x_q, w_q, sx, sw)[0]
+    assert float(want.abs().max()) < 2 ** 22
+    if not bias:
+        assert torch.equal(g.matmul_blockwise_fp8(x_q, w_q, sx, sw), want.float().bfloat16())
+    else:  # the layer quantises what dequantises exactly: blocks whose largest magnitude is 448 times a power of two
+        a = x_q.float()
+        a[:, ::128] = 448.0
+        b = torch.randint(-8, 9, (N,), generator=gen, device="cuda").float()
+        q, s = g.quantize_per_token_block(a, dtype=F8)
+        assert torch.equal(s, torch.ones_like(s)) and torch.equal(q.float(), a)
+        want = R.product(q, w_q, s, sw)[0] + b.double()
+        assert float(want.abs().max()) < 2 ** 23
+        assert torch.equal(g.Fp8Linear(w_q, sw, b.bfloat16())(a), want.float().bfloat16())
+    g.check_device()
+
+
 @pytest.mark.parametrize("M,N", [(8, 64), (64, 256), (300, 512)])
 def test_large_and_small_products_in_one_block(M, N):
     """Products of 448 x 448 that cancel and products of 1 beside them in the same K block: what is left is what fp32 sums keep."""
