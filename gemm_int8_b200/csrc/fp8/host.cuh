@@ -84,7 +84,8 @@ int launch_fp8(DeviceState* st, int slot, const int8_t* x, const int8_t* y, Fp8G
     const int64_t tiles = static_cast<int64_t>(p.tiles_m) * p.tiles_n;
     const int slots = PAIR ? st->sm_count / 2 : st->sm_count;
     const int grid = static_cast<int>(std::min<int64_t>(tiles, slots)) * (PAIR ? 2 : 1);
-    p.release_late = !PAIR && !(p.after_quant && BN < 256) && (tiles <= st->sm_count || p.K % 32 != 0) && release_late(tiles, st->sm_count);
+    const int64_t ctas = tiles * (SPLITK ? p.splits : 1);
+    p.release_late = !PAIR && !(p.after_quant && BN < 256) && (ctas <= st->sm_count || p.K % 32 != 0) && release_late(ctas, st->sm_count);
     if constexpr (SPLITK) return launch(kernel, dim3(static_cast<unsigned>(tiles), p.splits), kBlockwiseThreads, smem, s, dim3(1, p.splits), knobs().pdl, mx, my, mo, p);
     return launch(kernel, dim3(grid), kBlockwiseThreads, smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mx, my, mo, p);
 }

@@ -71,6 +71,21 @@ def test_exact_sums(M, N, K, variant):
     assert torch.equal(out, want.float().bfloat16())
 
 
+@pytest.mark.parametrize("M,N,K", [(7, 136, 272), (200, 264, 512)])
+def test_subnormal_codes(M, N, K):
+    """Multiples of 2^-9, among them all of e4m3's subnormal numbers, which must not be flushed: exact sums of multiples of 2^-18."""
+    import gemm_int8_b200 as g
+
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.randint(-15, 16, (M, K), generator=gen, device="cuda").float() * 2.0 ** -9
+    w = torch.randint(-7, 8, (N, K), generator=gen, device="cuda").float() * 2.0 ** -9
+    x_q, w_q = x.to(F8), w.to(F8)
+    assert torch.equal(x_q.float(), x) and torch.equal(w_q.float(), w)
+    one = torch.ones(max(M, -(-N // 128)), -(-K // 128), device="cuda")
+    want = R.product(x_q, w_q, one[:M], one[: -(-N // 128)])[0]
+    assert torch.equal(g.matmul_blockwise_fp8(x_q, w_q, one[:M], one[: -(-N // 128)]), want.float().bfloat16())
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 64, 28672), (16, 200, 2064), (9, 4096, 14336), (5, 1000, 4112), (16, 2048, 8192), (40, 2048, 8192), (64, 4096, 14336), (100, 1001, 6992),
                                    (33, 5003, 4096), (256, 512, 14336), (17, 100, 28672), (130, 1030, 8208), (1024, 1024, 8192), (64, 8192, 28672), (128, 8192, 8192)])
 @pytest.mark.parametrize("bias", [False, True])
