@@ -79,7 +79,7 @@ int launch_swiglu_row(const ActParams& p, int sms, cudaStream_t s)
     constexpr int LOADS = 4;
     const int vectors = (p.K + 7) / 8;
     const int threads = std::min(1024, (vectors + 32 * LOADS - 1) / (32 * LOADS) * 32);
-    return launch(swiglu_quantize_row_kernel<T, Out8::kInt8, LOADS>, dim3(static_cast<unsigned>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8))), threads, 0, s, dim3(1),
+    return launch(swiglu_quantize_row_kernel<T, LOADS>, dim3(static_cast<unsigned>(std::min<int64_t>(p.M, static_cast<int64_t>(sms) * 8))), threads, 0, s, dim3(1),
                   knobs().pdl, p);
 }
 

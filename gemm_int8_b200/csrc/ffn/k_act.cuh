@@ -85,19 +85,18 @@ __global__ void __launch_bounds__(kActThreads) act_quantize_block_kernel(const A
     }
     QuantScale qs[LOADS];
     block_scales<OUT, LOADS>(m, qs);
-#pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
+    out8_store<OUT>(v, qs, [&](int u, uint2 w) {
         const int col = col0 + u * 256;
         if (col < p.K) {
             if ((lane & 15) == 0) p.s[static_cast<int64_t>(row) * p.KB + (col >> 7)] = qs[u].s;
-            *reinterpret_cast<uint2*>(p.q + static_cast<int64_t>(row) * p.K + col) = out8_pack8<OUT>(v[u], qs[u]);
+            *reinterpret_cast<uint2*>(p.q + static_cast<int64_t>(row) * p.K + col) = w;
         }
-    }
+    });
 }
 
-// SwiGLU with a scale per row: a CTA per row.  LOADS x 8 values a thread stay in registers between the maximum and the quantisation;
+// SwiGLU in int8 with a scale per row: a CTA per row.  LOADS x 8 values a thread stay in registers between the maximum and the quantisation;
 // what lies beyond them is read and computed twice (it hits L2).
-template <typename T, Out8 OUT, int LOADS>
+template <typename T, int LOADS>
 __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActParams p)
 {
     quant_dependency();
@@ -128,18 +127,17 @@ __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActPara
         if ((threadIdx.x & 31) == 0) slots[parity][threadIdx.x >> 5] = m;
         __syncthreads();
         m = (threadIdx.x & 31) < warps ? slots[parity][threadIdx.x & 31] : 0.0f;
-        const QuantScale qs = make_out_scale<OUT>(lanes_max_nan<32>(m));
-        if (threadIdx.x == 0) p.s[row] = qs.s;
+        const QuantScale qs[1] = {make_out_scale<Out8::kInt8>(lanes_max_nan<32>(m))};
+        if (threadIdx.x == 0) p.s[row] = qs[0].s;
         uint8_t* q = p.q + row * p.K;
-#pragma unroll
-        for (int u = 0; u < LOADS; ++u) {
+        out8_store<Out8::kInt8>(v, qs, [&](int u, uint2 w) {
             const int col = u * span + threadIdx.x * 8;
-            if (col < p.K) *reinterpret_cast<uint2*>(q + col) = out8_pack8<OUT>(v[u], qs);
-        }
+            if (col < p.K) *reinterpret_cast<uint2*>(q + col) = w;
+        });
         for (int col = LOADS * span + threadIdx.x * 8; col < p.K; col += span) {
             uint64_t w[4];
             act_values<T, true>(act_load<T, true>(p, row, col, true), w);
-            *reinterpret_cast<uint2*>(q + col) = out8_pack8<OUT>(w, qs);
+            *reinterpret_cast<uint2*>(q + col) = make_uint2(quant_pack4(w[0], w[1], qs[0]), quant_pack4(w[2], w[3], qs[0]));
         }
     }
 }

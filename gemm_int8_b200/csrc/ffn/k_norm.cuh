@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_quantize_kernel(const N
         for (int i = 0; i < 4; ++i) kept[u][i] = mul2(mul2(kept[u][i], r2), w[i]);
         m[u] = amax8_nan(kept[u]);
     }
-    QuantScale qs[LOADS];
+    QuantScale qs[BLOCK ? LOADS : 1];
     if constexpr (BLOCK) {
         block_scales<OUT, LOADS>(m, qs);
     } else {
@@ -144,14 +144,13 @@ __global__ void __launch_bounds__(kNormThreads) rms_norm_quantize_kernel(const N
         qs[0] = make_out_scale<OUT>(row_reduce<true>(top, slots[1], p.row_warps));
         if (live && t == 0) p.s[row] = qs[0].s;
     }
-#pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
+    out8_store<OUT>(kept, qs, [&](int u, uint2 w) {
         const int col = (u * row_threads + t) * 8;
         if (live && col < p.H) {
-            if (BLOCK && (t & 15) == 0) p.s[row * p.KB + (col >> 7)] = qs[u].s;
-            *reinterpret_cast<uint2*>(p.q + base + col) = out8_pack8<OUT>(kept[u], qs[BLOCK ? u : 0]);
+            if (BLOCK && (t & 15) == 0) p.s[row * p.KB + (col >> 7)] = qs[BLOCK ? u : 0].s;
+            *reinterpret_cast<uint2*>(p.q + base + col) = w;
         }
-    }
+    });
 }
 
 }  // namespace gi8
