@@ -1,7 +1,7 @@
 // What the operators around the products share: eight values a lane in, 8-bit values and their scale out.
 //   int8   s = amax / 127,  q = clamp(rint(v / s), -127, 127)
 //   e4m3   s = amax / 448,  q = v / s rounded to e4m3 (half to even)
-// with s = 1 where all values are zero.  A NaN or infinity among the values makes the scale NaN or infinite, so that every product with
+// with s = 1 where all values are zero, or so small that s would be.  A NaN or infinity among the values makes the scale NaN or infinite, so that every product with
 // them shows it (an int8 has no value of its own for it).
 #pragma once
 
@@ -26,12 +26,10 @@ GI8_DEVICE float max_nan(float a, float b)
     return r;
 }
 
-// Over runs of LANES consecutive lanes (16: a 128-wide block of eight values a lane; 32: a warp).
-template <int LANES>
-GI8_DEVICE float lanes_max_nan(float m)
+GI8_DEVICE float warp_max_nan(float m)
 {
 #pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 1; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
 }
 
@@ -40,7 +38,8 @@ template <Out8 OUT>
 GI8_DEVICE QuantScale make_out_scale(float amax)
 {
     QuantScale q;
-    q.s = amax == 0.0f ? 1.0f : __fdiv_rn(amax, OUT == Out8::kInt8 ? 127.0f : 448.0f);
+    q.s = __fdiv_rn(amax, OUT == Out8::kInt8 ? 127.0f : 448.0f);
+    if (q.s == 0.0f) q.s = 1.0f;
     if constexpr (OUT == Out8::kInt8) asm("rcp.approx.f32 %0, %1;" : "=f"(q.r) : "f"(q.s));
     else q.r = __frcp_rn(q.s);
     if (!(q.s > (OUT == Out8::kInt8 ? 1e-30f : 1e-20f) && q.s < 1e30f)) q.r = __int_as_float(0x7fffffff);

@@ -1,6 +1,31 @@
 // Block-scaled product of e4m3 operands for sm_100a:
 //   out[m,n] = bf16( sum_kb P[m,n,kb] * (sa[m,kb] * sw[n/128,kb]) (+ bias[n]) ),  kb ascending, one fused multiply-add in fp32 per K block
 //   (128 wide), P the block's fp32 dot product on the tensor cores, one rounding at the end.
+//
+// Structure, as in k_blockwise.cuh (one persistent CTA per SM, or two CTAs on one 256 x 256 tile): warp 0 loads operand tiles by TMA, warps 1 and 3 issue the MMAs,
+// whose partials of a K block lie in tensor memory, warps 4..11 promote them: tensor-memory loads and one fma.rn.f32x2 per pair of columns into fp32 accumulators in
+// registers, then the epilogue.  Partials are fp32 as they come, so there is no bias MMA and no conversion.  What is done otherwise than there:
+//   - A half of the wide tile (128 columns) belongs to ONE of the two column groups of promotion warps, with an issuer, buffers and barriers of its own.  A warp has one
+//     hand-over a K block, not two, and while the warps of one half wait for theirs those of the other work: 8192^3 495 -> 453 us, 2048 x 11008 x 4096 90 -> 82.
+//     In the two-CTA form each CTA loads 64 weight rows of either half, so that a half is 128 neighbouring columns, one weight block.
+//   - The barrier that frees a stage also says that its partial is there: one commit a half and K block.
+//   - Row scales come through shared memory, 64 bytes of a row at a time, by asynchronous copies of warp 2; as 16-byte loads of the promotion warps, each touching
+//     32 rows, they cost 80 - 100 of 800 cycles.  The weight block's scales are held by the lanes of a warp and broadcast by shuffles.
+//   - Packed multiply-adds: scalar ones, with the register banks they get, took 760 cycles a K block for 705.
+//   - No branch leaves the loop over the K blocks: with early exits it spilled accumulators (205 us for 136).
+//
+// Bound (two-CTA form, 2048 x 9472 x 8192, cycles a K block, copies of the kernel with parts left out): all 705; without scale loads 612; without multiply-adds 567; with
+// neither multiply-adds nor tensor-memory loads 570: the MMAs with their operands, 512 at the nominal rate; without MMAs 620.  So the promotion loop, a chain of
+// four loads and their arithmetic and one hand-over for each warp, binds, not far in front of the MMAs; tensor pipe 70 % of the active cycles.  For a second on end the chip
+// holds 1.1 GHz at 1000 W (8192^3 561 us with random codes) and takes as long as it needs energy: N = 256 MMAs, which fetch the rows of x once, took 806 cycles at
+// 1.24 GHz, 581 us.  The one-CTA 256-wide form is bound by its operand bytes (48 KB a K block at 67 bytes a cycle, the most an SM drew from L2: 719 cycles without any
+// MMA).  An epilogue takes 3000 cycles a tile, half of them its TMA stores (with three staging blocks a warp 2800, with one fence a tile 2500, as plain 16-byte stores 4100;
+// nothing of it showed in the times).  Stages of the two-CTA form: six, five and four level, level and 5 % slower.
+//
+// Barrier protocol: see k_blockwise.cuh.  bar_full[s]: TMA bytes; waiters: the issuers.  bar_done[h][s]: the commit of half h; waiters: the producer, whose refill the
+// next completion needs, and half h's promotion warps, whose hand-back the next completion needs (STAGES >= NBUF).  bar_part_empty[h][b]: the arrivals of half h's promotion
+// warps, of both CTAs of a pair; waiter: the half's issuer.  bar_scale_full[g]: arrivals of warp 2's lanes behind their copies; waiters: the promotion warps, whose
+// arrivals on bar_scale_empty[g] the next completion needs.  Narrow tiles have one part, whose K blocks the issuers take in turn.
 #pragma once
 
 #include "../k_blockwise.cuh"
@@ -27,6 +52,7 @@ struct Fp8GemmParams {
     int release_late;  // do not let the next launch start before the CTAs have ended (see the host's release_late)
 };
 
+// (224 and 48, 240 and 24: the same)
 constexpr int kFp8PromoRegs = 232, kFp8ControlRegs = 40;
 static_assert(kPromoWarps * (kFp8PromoRegs - kLaunchRegs) <= 4 * (kLaunchRegs - kFp8ControlRegs), "setmaxnreg pool unbalanced");
 
@@ -73,6 +99,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     constexpr uint32_t kBytesA = kBM * kBK, kBytesB = kRowsB * kBK, kStageBytes = kBytesA + kBytesB;
     constexpr uint32_t kTmemCols = 512;
     constexpr uint32_t kIdesc = make_idesc_e4m3(kTileM, NSUB);
+    static_assert(STAGES >= NBUF, "a partial's barrier completes again only after its buffer has been handed back");
     static_assert(STAGES % 2 == 0 && NBUF % 2 == 0, "two issuers on alternate K blocks own their stages and buffers");
 
     extern __shared__ uint8_t smem_raw[];
@@ -222,12 +249,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                         else umma_f8(tmem_d, smem_desc_k128_of(da + 2 * k), smem_desc_k128_of(db + 2 * k), kIdesc, k != 0 ? 1u : 0u);
                     }
                     if constexpr (PAIR) {
-#ifdef P_BOTH
-                        umma_commit_both(done_0 + 8 * s);
-#else
                         umma_commit_pair(map_to_cta(done_0 + 8 * s, 0));
                         umma_commit_pair(map_to_cta(done_0 + 8 * s, 1));
-#endif
                     } else {
                         umma_commit(&bar_done[h][s]);
                     }

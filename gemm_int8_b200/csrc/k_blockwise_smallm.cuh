@@ -63,7 +63,8 @@ struct BlockwiseSmallM {
 };
 
 // OPERAND: nothing for int8, E4m3 for operands in 8-bit floating point with partials in fp32.  Those need no chain over all K blocks: where the
-// weight rows do not fill the machine the CTAs of a cluster take a range of K blocks each, and the first adds up their sums in the order of the ranges.
+// weight rows do not fill the machine the CTAs of a cluster take a range of K blocks each, and the first adds up their sums in the order of the ranges (16 x 4096 x 14336
+// 21.9 -> 15.0 us with two, 16 x 2048 x 8192 13.6 -> 8.1 with four).
 struct E4m3 {};
 template <int STAGES_, typename... OPERAND>
 __global__ void __launch_bounds__(BlockwiseSmallM<STAGES_>::THREADS)

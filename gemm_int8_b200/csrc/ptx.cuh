@@ -629,13 +629,6 @@ GI8_DEVICE void umma_commit_pair(uint32_t bar_cluster_addr)
                  : "memory");
 }
 
-// The same onto the barriers at one shared-memory address of both CTAs of the pair.
-GI8_DEVICE void umma_commit_both(uint32_t bar_addr)
-{
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar_addr), "h"(static_cast<uint16_t>(3))
-                 : "memory");
-}
-
 // Arrival on a barrier in (possibly) another CTA of the cluster, default semantics (release at CTA scope): what orders
 // the tensor-memory accesses around it is the tcgen05 fence the caller issues, and a cluster-scope release costs a
 // cluster-wide memory fence per arrival.

@@ -394,7 +394,9 @@ at::Tensor int8_experts(const at::Tensor& x, const at::Tensor& logits, const std
 std::tuple<at::Tensor, at::Tensor> new_out8(int64_t rows, int64_t cols, bool blockwise, bool e4m3, const at::Tensor& like)
 {
     at::Tensor q = new_tensor({rows, cols}, e4m3 ? at::kFloat8_e4m3fn : at::kChar, like);
-    return {q, blockwise ? new_tensor({rows, blocks_of(cols)}, at::kFloat, like) : new_tensor({rows}, at::kFloat, like)};
+    at::Tensor s = blockwise ? new_tensor({rows, blocks_of(cols)}, at::kFloat, like) : new_tensor({rows}, at::kFloat, like);
+    if (cols == 0) s.fill_(1.0);  // (nothing is launched: the scale of rows without values)
+    return {q, s};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_quantize(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& residual,

@@ -64,8 +64,9 @@ def matmul_blockwise_fp8(x_q: torch.Tensor, w_q: torch.Tensor, x_scale: torch.Te
     """`matmul_blockwise` in 8-bit floating point -> bf16 [M, N].
 
     ``out[m, n] = bf16( sum_kb P[m, n, kb] * (x_scale[m, kb] * w_scale[n // 128, kb]) )`` where ``P`` is the fp32 dot product over the kb-th
-    128-wide K block, accumulated in fp32 in ascending kb order.  x_q (M, K) and w_q (N, K) float8_e4m3fn, x_scale (M, ceil(K/128)) and
-    w_scale (ceil(N/128), ceil(K/128)) fp32; K a multiple of 16 below 131072.
+    128-wide K block, accumulated in fp32 in ascending kb order (where few tiles have long sums, in up to eight ranges of K blocks whose sums are
+    added up in order).  x_q (M, K) and w_q (N, K) float8_e4m3fn, x_scale (M, ceil(K/128)) and w_scale (ceil(N/128), ceil(K/128)) fp32; K a
+    multiple of 16 below 131072.
     """
     return _matmul(x_q, w_q, x_scale, w_scale)
 

@@ -5,7 +5,7 @@ benchmark.py:17-18).  Plain torch ops, device-agnostic, used to build the synthe
 users who do not have a fused quantiser of their own.  Rule everywhere:
     s = amax / 127   (s = 1 where the block is all zero),   q = clamp(round_half_even(v / s), -127, 127)
 and with dtype=torch.float8_e4m3fn, for the products in 8-bit floating point:
-    s = amax / 448   (s = 1 where the block is all zero),   q = v / s rounded half to even
+    s = amax / 448   (s = 1 where the block is all zero, or so small that s would be),   q = v / s rounded half to even
 """
 from __future__ import annotations
 
@@ -23,7 +23,8 @@ def _quant_fp8(v: torch.Tensor, amax: torch.Tensor, dtype: torch.dtype):
     """(q, s) of blocks v whose largest magnitudes are amax (of v's dimensions).  A NaN or infinity makes its block's scale NaN or infinite."""
     if dtype != torch.float8_e4m3fn:
         raise ValueError("dtype must be torch.int8 or torch.float8_e4m3fn")
-    s = torch.where(amax == 0, torch.ones_like(amax), amax / amax.new_full((), 448.0))  # (a division: by a number, torch multiplies on a GPU)
+    s = amax / amax.new_full((), 448.0)  # (a division: by a number, torch multiplies on a GPU)
+    s = torch.where(s == 0, torch.ones_like(s), s)
     return (v / s).clamp_(-448, 448).to(dtype), s
 
 

@@ -286,9 +286,9 @@ int gi8_experts_add_f32(const void* x, int x_dtype, const void* logits, int logi
 /*
  * The operators around the products of a feed-forward block, and the block-scaled product in 8-bit floating point (no reference counterpart).
  * 8-bit results are int8 (q_type 0: s = amax / 127, q = clamp(round_half_even(v / s), -127, 127)) or e4m3 (q_type 1: s = amax / 448, q = v / s
- * rounded half to even), s = 1 where all values are zero; with block_scales a scale per row and 128 columns, fp32 [M, ceil(K/128)], else one per
- * row, fp32 [M] (int8 only).  A NaN or infinity makes the scale of its block or row NaN or infinite.  q is 8-byte aligned, and the features are a
- * multiple of 16 below 131072.
+ * rounded half to even), s = 1 where all values are zero, or so small that s would be; with block_scales a scale per row and 128 columns,
+ * fp32 [M, ceil(K/128)], else one per row, fp32 [M] (int8 only).  A NaN or infinity makes the scale of its block or row NaN or infinite.  q is
+ * 8-byte aligned, and the features are a multiple of 16 below 131072.
  *
  * gi8_rms_norm_quantize: h = x + residual in fp32 (residual may be NULL);  total = h rounded to the residual's type;
  *   v = h * (mean(h^2) + eps)^-1/2 * weight, all in fp32, from the sum before it is rounded;  q, scales of v.
@@ -306,7 +306,9 @@ int gi8_fp8_quantize_token_block(const void* in, int in_dtype, void* q, float* s
 
 /*
  * gi8_matmul_blockwise for e4m3 operands: P is the fp32 dot product over a K block, on the tensor cores; accumulated with one fused multiply-add
- * per K block and rounded to bf16 once.  Arguments and limits as there.
+ * per K block, kb ascending, and rounded to bf16 once.  Where the tiles do not fill the machine a tile's K blocks are shared out in up to eight
+ * ranges, whose sums are added up in order: a row's result may differ in the last bits of the fp32 sum with M, never from call to call.
+ * Arguments and limits as there.
  */
 int gi8_fp8_matmul_blockwise(const void* x, const void* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out_bf16, int64_t M,
                              int64_t N, int64_t K, void* stream);

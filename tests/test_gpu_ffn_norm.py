@@ -44,6 +44,13 @@ def test_sizes(M, H, scales, dtype):
 
 
 @pytest.mark.parametrize("scales,dtype", FORMS)
+@pytest.mark.parametrize("M,H", [(2, 16400), (2, 28672), (1, 32768), (400, 16384)])
+def test_wide_fp32(M, H, scales, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(H)
+    _check(R.outliers(gen, M, H, torch.float32), torch.randn(H, generator=gen, device="cuda"), R.outliers(gen, M, H, torch.float32), 1e-6, scales, dtype)
+
+
+@pytest.mark.parametrize("scales,dtype", FORMS)
 @pytest.mark.parametrize("H", [256, 4096])
 def test_padding_and_magnitudes(H, scales, dtype):
     """Rows of zeros, of fp32's largest values, of small ones next to eps, side by side."""
@@ -104,6 +111,8 @@ def test_empty():
         assert got[0].shape == (0, 256) and got[1].shape == (0, 2) and (residual is None or got[2].shape == (0, 256))
     q, s = g.rms_norm_quantize(torch.empty(4, 0, device="cuda"), torch.empty(0, device="cuda"))
     assert q.shape == (4, 0) and s.shape == (4, 0)
+    q, s = g.rms_norm_quantize(torch.empty(4, 0, device="cuda"), torch.empty(0, device="cuda"), scales="token")
+    assert q.shape == (4, 0) and torch.equal(s, torch.ones(4, device="cuda"))
 
 
 def test_refusals():

@@ -112,12 +112,19 @@ def test_e4m3_quantiser_nan_infinity_zeros():
     import gemm_int8_b200 as g
     from gemm_int8_b200 import quant
 
-    a = torch.randn(4, 512, device="cuda")
+    a = torch.randn(8, 512, device="cuda")
     a[0, 130], a[1, 130], a[2, 128:256], a[3] = float("nan"), float("inf"), 0.0, -0.0
+    for row, top in ((4, 1e-44), (5, 2e-43), (6, 1e-40), (7, 3e38)):  # scales of zero, subnormal scales, the largest
+        a[row] = top
+        a[row, ::3] = 0.0
     q, s = g.quantize_per_token_block(a, dtype=F8)
     want_q, want_s = quant.quantize_per_token_block(a, dtype=F8)
     assert torch.equal(torch.nan_to_num(s, -1.0, -2.0), torch.nan_to_num(want_s, -1.0, -2.0)) and torch.equal(torch.isnan(q.float()), torch.isnan(want_q.float()))
     assert torch.equal(torch.nan_to_num(q.float()), torch.nan_to_num(want_q.float()))
+    assert torch.isfinite(q[2:].float()).all() and torch.equal(s[4], torch.ones_like(s[4])) and not q[4].float().any()
+    for dtype in (torch.int8, F8):
+        q, s = g.swiglu_quantize(torch.cat([torch.full((1, 128), 1e-22, device="cuda"), torch.full((1, 128), 1e-22, device="cuda")], 1), dtype=dtype)
+        assert torch.equal(s, torch.ones_like(s)) and not q.float().any()
     with pytest.raises(ValueError):
         g.quantize_per_token_block(a, dtype=torch.float8_e5m2)
     with pytest.raises(RuntimeError):

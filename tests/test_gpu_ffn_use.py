@@ -124,6 +124,26 @@ def test_one_call_right_behind_the_other():
     g.check_device()
 
 
+@pytest.mark.parametrize("M,N,K", [(4, 2048, 2048), (16, 4096, 512), (40, 1024, 4096), (150, 600, 1040), (600, 4096, 512)])
+def test_weights_written_right_in_front_of_the_layer(M, N, K):
+    """The product requests weights while the layer's quantiser still runs: they were written before that was let start, by the copy in front."""
+    import gemm_int8_b200 as g
+
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    layers = [g.Fp8Linear.from_float(torch.randn(N, K, generator=gen, device="cuda") * 0.03) for _ in range(2)]
+    x = torch.randn(M, K, generator=gen, device="cuda").bfloat16()
+    want = [layer(x) for layer in layers]
+    changing = g.Fp8Linear(layers[0].weight_q.clone(), layers[0].weight_scale.clone())
+    torch.cuda.synchronize()
+    got = []
+    for i in range(20):
+        changing.weight_q.view(torch.uint8).copy_(layers[i % 2].weight_q.view(torch.uint8))
+        changing.weight_scale.copy_(layers[i % 2].weight_scale)
+        got.append(changing(x))
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2]), i
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_total_in_place(dtype):
     """The C entry may write the sum over the residual, or over x of the same type."""
@@ -166,3 +186,28 @@ def test_nothing_behind_the_results_is_touched():
         out = torch.full((rows * N * 2 + 64,), 0x5A, dtype=torch.uint8, device="cuda")
         assert g._C.gi8_fp8_matmul_blockwise(p(x_q, 0), p(w_q, 0), p(sx, 0), KB, p(sw, 0), KB, p(out, 32), rows, N, H, stream) == 0
         assert bool((out[:32] == 0x5A).all()) and bool((out[-32:] == 0x5A).all())
+
+
+def test_offsets_beyond_32_bits():
+    """Tensors of more than 2^31 elements: the last rows are what they are by themselves."""
+    import gemm_int8_b200 as g
+
+    def same(many, few, rows):
+        for a, b in zip(many, few):
+            assert torch.equal(a[-rows:].contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+
+    M, H = 132000, 16400
+    x, w = torch.empty(M, H, dtype=torch.bfloat16, device="cuda"), torch.ones(H, device="cuda")
+    x.view(torch.int16).copy_((torch.arange(M * 16, device="cuda", dtype=torch.int32).reshape(M, 16) % 16000).to(torch.int16).repeat(1, H // 16))
+    for kw in ({"dtype": F8}, {"scales": "token"}):
+        same(g.rms_norm_quantize(x, w, x, **kw), g.rms_norm_quantize(x[-300:], w, x[-300:], **kw), 300)
+        same(g.swiglu_quantize(x[:, :16384], **kw), g.swiglu_quantize(x[-300:, :16384], **kw), 300)
+    same(g.quantize_per_token_block(x, F8), g.quantize_per_token_block(x[-300:], F8), 300)
+    del x
+    M, N, K = 66000, 32784, 256
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x_q, w_q = (torch.randint(-7, 8, (r, K), generator=gen, device="cuda").to(F8) for r in (M, N))
+    sx, sw = torch.ones(M, 2, device="cuda"), torch.ones(-(-N // 128), 2, device="cuda")
+    out = g.matmul_blockwise_fp8(x_q, w_q, sx, sw)
+    assert torch.equal(out[-500:], (x_q[-500:].double() @ w_q.double().t()).float().bfloat16())
+    g.check_device()
