@@ -87,6 +87,7 @@ class Fp8Linear(torch.nn.Module):
     The counterpart of `Int8Linear(mode="blockwise")`: activations are quantised on the fly, the product is `matmul_blockwise_fp8`, and a bias is
     added to its fp32 sums before they are rounded to bf16 (one that broadcasts or is differentiated, to the rounded result).  weight_q
     float8_e4m3fn [out_features, in_features], weight_scale fp32 [ceil(out/128), ceil(in/128)].  Inference only.
+    A module's `.to(dtype)` converts every floating-point buffer, both of these among them: the layer is made behind it (a call refuses other types).
     """
 
     def __init__(self, weight_q: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16):

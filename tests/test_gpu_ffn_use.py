@@ -211,3 +211,34 @@ def test_offsets_beyond_32_bits():
     out = g.matmul_blockwise_fp8(x_q, w_q, sx, sw)
     assert torch.equal(out[-500:], (x_q[-500:].double() @ w_q.double().t()).float().bfloat16())
     g.check_device()
+
+
+def test_opcheck_and_compile():
+    import gemm_int8_b200 as g
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    ops = torch.ops.gemm_int8_CUDA
+    x, residual, weight = torch.randn(5, 272, generator=gen, device="cuda").bfloat16(), torch.randn(5, 272, generator=gen, device="cuda"), torch.ones(272, device="cuda")
+    q, s = g.quantize_per_token_block(x, F8)
+    layer = g.Fp8Linear.from_float(torch.randn(544, 272, generator=gen, device="cuda"), torch.randn(544, generator=gen, device="cuda"))
+    every = ("test_schema", "test_autograd_registration", "test_faketensor")
+    for blockwise, e4m3 in ((True, True), (True, False), (False, False)):
+        checks = every[e4m3:]  # (the check of the schema multiplies what comes back, which torch cannot do in 8-bit floating point)
+        torch.library.opcheck(ops.rms_norm_quantize.default, (x, weight, residual, 1e-6, blockwise, e4m3), test_utils=checks)
+        torch.library.opcheck(ops.rms_norm_quantize.default, (x, weight, None, 1e-6, blockwise, e4m3), test_utils=checks)
+        torch.library.opcheck(ops.swiglu_quantize.default, (x[:, :256], blockwise, e4m3), test_utils=checks)
+    checks = every[1:]
+    torch.library.opcheck(ops.fp8_quantize_token_block.default, (x,), test_utils=checks)
+    torch.library.opcheck(ops.fp8_matmul_blockwise.default, (q, layer.weight_q, s, layer.weight_scale), test_utils=checks)
+    for bias in (layer.bias, None):
+        torch.library.opcheck(ops.fp8_linear.default, (x, layer.weight_q, layer.weight_scale, bias), test_utils=checks)
+
+    def block(x, residual):
+        q, s, total = g.rms_norm_quantize(x, weight, residual, dtype=F8)
+        gate_up = g.matmul_blockwise_fp8(q, layer.weight_q, s, layer.weight_scale)
+        return (*g.swiglu_quantize(gate_up, dtype=F8), total, layer(x))
+
+    compiled = torch.compile(block, fullgraph=True, backend="aot_eager")
+    for rows in (5, 1, 3):
+        for a, b in zip(compiled(x[:rows], residual[:rows]), block(x[:rows], residual[:rows])):
+            assert a.dtype == b.dtype and torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
