@@ -112,6 +112,7 @@ struct DeviceState {
     int sm_count = 0;
     uint32_t* status = nullptr;
     bool attr_set[96] = {};
+    int quads = 0;  // clusters of four CTAs that take an SM each and run at the same time (0: not asked yet)
 };
 
 std::mutex g_mutex;

@@ -9,6 +9,9 @@ namespace {
 // Tile forms and what a wave of them costs per K block, in ns (back to back; of one full wave and of many, which run at lower clocks: two-CTA 0.46 - 0.51 us, 128 x 256
 // 0.44 - 0.53, 128 x 128 0.27 - 0.31, 128 x 64 0.23 - 0.26).
 constexpr TileForm kFp8Forms[] = {{256, true, 480.0, 0, 0}, {256, false, 495.0, 0, 0}, {128, false, 300.0, 0, 0}, {64, false, 245.0, 0, 0}};
+// What a K block takes where K is not a multiple of 32, so that rows begin inside a 32-byte sector, over what it takes where it is (1024 x 4736 x 6992 next to
+// K = 6912, us: 50.6 / 48.1, 64.6 / 47.6, 50.9 / 34.0, 71.9 / 55.4; without this rule 1024 x 5003 x 6992 took 128 columns and 73 us, not the pair's 53).
+constexpr double kFp8OddRows[] = {1.06, 1.42, 1.47, 1.31};
 
 struct Fp8Choice {
     int bn;
@@ -43,26 +46,54 @@ int fp8_smallm_splits(int64_t N, int64_t K, int sms)
 }
 
 // The form whose waves take the least time; grids that leave SMs idle are also weighed with every tile's K blocks split over the CTAs of a cluster.
-Fp8Choice choose_fp8(int64_t M, int64_t N, int64_t K, int sms)
+// (quads: clusters of four that run at once, 33 of the 37 that 148 SMs have room for, as a cluster lies in one group of SMs: 777 x 640 x 28672 in 35 of them ran as two
+// waves, 44.6 us, and takes 32.9 in pairs.)
+Fp8Choice choose_fp8(int64_t M, int64_t N, int64_t K, int sms, int quads)
 {
     Fp8Choice best{};
     double best_cost = 1e300;
     const int64_t kb = (K + kBK - 1) / kBK;
-    for (const TileForm& f : kFp8Forms) {
+    for (size_t i = 0; i < sizeof(kFp8Forms) / sizeof(kFp8Forms[0]); ++i) {
+        const TileForm& f = kFp8Forms[i];
+        const double ns = f.kblock_cycles * (K % 32 ? kFp8OddRows[i] : 1.0);
         const int tile_m = f.pair ? 2 * kBM : kBM;
         const int64_t tiles = ((M + tile_m - 1) / tile_m) * ((N + f.bn - 1) / f.bn);
         const int64_t slots = f.pair ? sms / 2 : sms;
-        const double cost = static_cast<double>((tiles + slots - 1) / slots) * f.kblock_cycles * kb;
+        const double cost = static_cast<double>((tiles + slots - 1) / slots) * ns * kb;
         if (cost < best_cost) best_cost = cost, best = {f.bn, f.pair, 1};
         if (f.pair) continue;
-        for (int splits = 2; splits <= std::min(4, f.bn / 32) && tiles * splits <= sms; splits *= 2) {
+        for (int splits = 2; splits <= std::min(4, f.bn / 32) && tiles <= (splits == 2 ? sms / 2 : quads); splits *= 2) {
             const int each = fp8_kb_per_split(kb, splits);
             if (each * (splits - 1) >= kb) break;  // (no CTA without K blocks)
-            const double split = each * f.kblock_cycles + fp8_split_fixed(f.bn, splits, M);
+            const double split = each * ns + fp8_split_fixed(f.bn, splits, M);
             if (split < best_cost) best_cost = split, best = {f.bn, false, splits};
         }
     }
     return best;
+}
+
+// (the split kernels take an SM each; asked once per device)
+int resident_quads(DeviceState* st, int* out)
+{
+    {
+        std::lock_guard<std::mutex> lock(g_mutex);
+        *out = st->quads;
+    }
+    if (*out) return GI8_OK;
+    constexpr size_t smem = fp8_smem_bytes(256, 4, false);
+    auto kernel = fp8_gemm_kernel<256, 4, false, false, true>;
+    if (int rc = ensure_smem(st, 75, kernel, smem)) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(1, 4), cfg.blockDim = dim3(kBlockwiseThreads), cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1, attr.val.clusterDim.y = 4, attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr, cfg.numAttrs = 1;
+    GI8_CUDA(cudaOccupancyMaxActiveClusters(out, kernel, &cfg));
+    *out = std::max(*out, 1);
+    std::lock_guard<std::mutex> lock(g_mutex);
+    st->quads = *out;
+    return GI8_OK;
 }
 
 template <int BN, int STAGES, bool PAIR, bool BIAS, bool SPLITK = false>
@@ -145,7 +176,11 @@ int fp8_matmul(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa,
         case VAR_DENSE_BN128: c = {128, false, 1}; break;
         case VAR_DENSE_BN64: c = {64, false, 1}; break;
         case VAR_PAIR: c = {256, true, 1}; break;
-        default: c = choose_fp8(M, N, K, st->sm_count);
+        default: {
+            int quads;
+            if (int rc = resident_quads(st, &quads)) return rc;
+            c = choose_fp8(M, N, K, st->sm_count, quads);
+        }
     }
     return bias ? launch_fp8<true>(st, c, x, y, p, s) : launch_fp8<false>(st, c, x, y, p, s);
 }

@@ -66,10 +66,10 @@ __host__ __device__ constexpr size_t fp8_smem_bytes(int bn, int stages, bool pai
     return static_cast<size_t>(stages) * (kBM + (pair ? bn / 2 : bn)) * kBK + kPromoWarps * kFp8StoreBytes + 2 * kFp8ScaleBytes + 1024;
 }
 
-// global -> shared copy of 4 bytes (src_bytes 0: zeros), see cp_async_16.
-GI8_DEVICE void cp_async_4(uint32_t smem_dst, const void* src, uint32_t src_bytes)
+// global -> shared copy of 4 bytes, see cp_async_16.
+GI8_DEVICE void cp_async_4(uint32_t smem_dst, const void* src)
 {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_dst), "l"(src), "r"(src_bytes) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_dst), "l"(src) : "memory");
 }
 
 // Where the four scales c (of four) of row r lie in a group: eight neighbouring rows' 16 bytes take different banks.
@@ -284,12 +284,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                             cp_async_16(dst + fp8_scale_at(r, c), in ? p.sa + static_cast<int64_t>(row0 + r) * p.ld_sa + kb_0 + kb + 4 * c : p.sa, in ? 16u : 0u);
                         }
                     } else {
-                        const int k = lane & 15;
+                        // Four times as many copies; scales that nobody uses (rows behind the last, columns behind num_kb) are read from the last row or column
+                        // instead of being tested for at every copy (a K block of the 128-wide tile 369 -> 275 ns, of the 64-wide one 350 -> 230, next to 265 and 225
+                        // with copies of 16 bytes; 1024 x 4736 x 6912 46.1 -> 34.2 us).
+                        const int k = lane & 15, last = p.M - 1 - row0;
+                        const float* src = p.sa + static_cast<int64_t>(row0) * p.ld_sa + kb_0 + min(kb + k, num_kb - 1);
 #pragma unroll 4
-                        for (int r = lane >> 4; r < kBM; r += 2) {
-                            const bool in = row0 + r < p.M && kb + k < num_kb;
-                            cp_async_4(dst + fp8_scale_at(r, k >> 2) + (k & 3) * 4, in ? p.sa + static_cast<int64_t>(row0 + r) * p.ld_sa + kb_0 + kb + k : p.sa, in ? 4u : 0u);
-                        }
+                        for (int r = lane >> 4; r < kBM; r += 2)
+                            cp_async_4(dst + fp8_scale_at(r, k >> 2) + (k & 3) * 4, src + static_cast<int64_t>(min(r, last)) * p.ld_sa);
                     }
                     cp_async_arrive(&bar_scale_full[s]);
                     s ^= 1;

@@ -222,3 +222,21 @@ def test_linear_shapes_types_and_refusals():
     for f in (lambda: layer(x.cpu()), lambda: layer(x[..., :128]), lambda: g.Fp8Linear(layer.weight_q, layer.weight_scale[:2])(x)):
         with pytest.raises(RuntimeError):
             f()
+
+
+@pytest.mark.parametrize("M,N,K", [(20, 300, 272), (130, 520, 2064), (777, 640, 28672), (1024, 5003, 6992), (300, 9472, 6912), (40, 1024, 8320), (600, 4736, 4224)])
+def test_scales_inside_a_wider_buffer(M, N, K):
+    """Any number of K blocks, rows of scales at any stride: what lies behind the last row and the last column is NaN and reaches nothing."""
+    import gemm_int8_b200 as g
+
+    ops = _operands(M, N, K)
+    want = g.matmul_blockwise_fp8(*ops)
+    R.check_bf16(want, *R.product(*ops))
+    for extra in (1, 3, 4):
+        wide = []
+        for s in ops[2:]:
+            buf = torch.full((s.shape[0] + 3, s.shape[1] + extra), float("nan"), device="cuda")
+            buf[: s.shape[0], : s.shape[1]] = s
+            wide.append(buf[: s.shape[0], : s.shape[1]])
+        assert torch.equal(g.matmul_blockwise_fp8(ops[0], ops[1], *wide), want)
+    g.check_device()
