@@ -21,6 +21,8 @@ struct ActParams {
 // g u / (1 + 2^(-g log2 e)) for a pair, in packed steps but for the exponentials and reciprocals, which the special-function unit takes one by one
 // (subnormal results flushed: next to 1 they are nothing, and a reciprocal of 2^126 and more, or of an overflowed exponential, is the limit 0).
 // Good to (5 + |g|) units in the last place, next to the half step of 1/254 or 2^-4 that the result is rounded by.
+// (Of 63 million e4m3 results of fp32 input 47 lay on the other side of a rounding step than the exact ones; of the same sum with expf and a division 43, of torch's silu
+// 52.  Those took 129 us for 96 with a scale per row, 4096 x 14336, and the same with block scales.)
 GI8_DEVICE uint64_t swiglu2(uint64_t g, uint64_t u)
 {
     float a, b;

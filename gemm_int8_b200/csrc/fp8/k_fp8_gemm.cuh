@@ -49,6 +49,7 @@ struct Fp8GemmParams {
     int after_quant;   // launched as the programmatic dependent of the quantiser that writes x and sa (and of nothing else)
     int scale_vec;     // ceil(K/128) % 4 == 0 and the rows of sa are 16-byte aligned: scales are copied four at a time
     int splits, kb_per_split;  // SPLITK: CTAs of a cluster (BN / splits a multiple of 32), K blocks of each (a multiple of 4; the last has the rest)
+    int box_rows;      // rows of x that a load brings: all 128, or as many as there are (the tile's other rows are whatever lies there, and stored by nobody)
     int release_late;  // do not let the next launch start before the CTAs have ended (see the host's release_late)
 };
 
@@ -174,7 +175,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                     kb_early = min(num_kb, STAGES);
                     if (elect_one()) {
                         for (int kb = 0; kb < kb_early; ++kb) {
-                            mbar_arrive_expect_tx(&bar_full[kb], kStageBytes);
+                            mbar_arrive_expect_tx(&bar_full[kb], kBytesB + p.box_rows * kBK);
                             tma_load_2d(smem + kb * kStageBytes + kBytesA, &map_y, &bar_full[kb], (kb_0 + kb) * kBK, nb * BN);
                         }
                     }
@@ -211,7 +212,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                                 tma_load_2d_pair(a_tile + kBytesA + h * (kBytesB / SPLIT), &map_y, leader_full, kb * kBK,
                                                  nb * BN + h * NSUB + static_cast<int>(rank) * (NSUB / 2));
                         } else {
-                            mbar_arrive_expect_tx(&bar_full[s], kStageBytes);
+                            mbar_arrive_expect_tx(&bar_full[s], kBytesB + p.box_rows * kBK);
                             tma_load_2d(a_tile, &map_x, &bar_full[s], (kb_0 + kb) * kBK, mb * kBM);
                             tma_load_2d(a_tile + kBytesA, &map_y, &bar_full[s], (kb_0 + kb) * kBK, nb * BN);
                         }

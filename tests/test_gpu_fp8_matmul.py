@@ -240,3 +240,25 @@ def test_scales_inside_a_wider_buffer(M, N, K):
             wide.append(buf[: s.shape[0], : s.shape[1]])
         assert torch.equal(g.matmul_blockwise_fp8(ops[0], ops[1], *wide), want)
     g.check_device()
+
+
+@pytest.mark.parametrize("N,K", [(14336, 512), (4096, 4096), (9472, 640), (1000, 8320)])
+def test_fewer_rows_than_a_tile(N, K):
+    """Every number of rows up to a tile's gives the rows of the largest: bit for bit where the same tiles are taken, and right where K blocks are shared out otherwise."""
+    import gemm_int8_b200 as g
+
+    x_q, w_q, x_s, w_s = _operands(128, N, K)
+    full = torch.full_like(x_q.view(torch.uint8), 0x7F).view(F8)  # NaN behind the rows that a call is given
+    for M in (17, 18, 23, 24, 25, 31, 33, 40, 63, 65, 97, 121, 127, 128):
+        full.view(torch.uint8)[:M] = x_q.view(torch.uint8)[:M]
+        out = g.matmul_blockwise_fp8(full[:M], w_q, x_s[:M], w_s)
+        R.check_bf16(out, *R.product(x_q[:M], w_q, x_s[:M], w_s))
+    for variant in ("dense_bn128", "dense_bn64", "dense_bn256", "pair"):
+        g.force_variant(variant)
+        try:
+            want = g.matmul_blockwise_fp8(x_q, w_q, x_s, w_s)
+            for M in (1, 7, 17, 24, 100):
+                assert torch.equal(g.matmul_blockwise_fp8(x_q[:M], w_q, x_s[:M], w_s), want[:M]), (variant, M)
+        finally:
+            g.force_variant(None)
+    g.check_device()
