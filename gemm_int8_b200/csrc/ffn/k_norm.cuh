@@ -4,7 +4,7 @@
 // The norm is of the sum in fp32, not of the total that is stored: one rounding less on the way to q.
 //
 // One pass: a row is read once, stays in registers (8 LOADS values a thread) while its squares are summed up across its warps (and with per-row scales its largest
-// magnitude found), and is written once.  Bound: HBM: 16384 x 8192 bf16 with a residual 141 - 145 us, 6.5 - 6.7 TB/s, the copy rate; 8191 x 4096 bf16 onto an fp32 residual
+// magnitude found), and is written once.  Bound: HBM: 16384 x 8192 bf16 with a residual 141 - 150 us by machine, 6.3 - 6.7 TB/s, the copy rate; 8191 x 4096 bf16 onto an fp32 residual
 // 60 us, 6.1 TB/s; without a residual, 3 bytes an element, the latency of a row's steps: 16384 x 4096 50 us, 4 TB/s.  Persistent CTAs that request the next row
 // before they work on this one were no faster (150, 65, 58 us): registers for two rows halve the rows on an SM.
 #pragma once
