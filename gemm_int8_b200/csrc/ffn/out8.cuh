@@ -94,13 +94,15 @@ GI8_DEVICE uint32_t cvt_e4m3x2(float lo, float hi)
 // remainder v - t s corrects t (P. Markstein, IBM J. Res. Dev. 34, 1990), two multiply-adds on packed pairs; a quotient that lies
 // between two e4m3 numbers comes out exactly there.  Scales from 1e-20 on keep the remainder of every quotient that does not round to
 // zero in range; the others (r is NaN) take the division itself.
+// What is computed is -v / s, whose sign bits one XOR turns round: from v = -0 the sums above would give +0, as (-0)(-s) - 0 = +0; from t = +0 they keep the
+// sign that division gives.
 GI8_DEVICE uint32_t e4m3_pack4(uint64_t v0, uint64_t v1, const QuantScale& qs)
 {
-    const uint64_t r2 = f32x2(qs.r, qs.r), ns2 = f32x2(-qs.s, -qs.s);
-    const uint64_t t0 = mul2(v0, r2), t1 = mul2(v1, r2);
+    const uint64_t nr2 = f32x2(-qs.r, -qs.r), s2 = f32x2(qs.s, qs.s);
+    const uint64_t t0 = mul2(v0, nr2), t1 = mul2(v1, nr2);
     float a, b, c, d;
-    f32x2_split(fma2(fma2(t0, ns2, v0), r2, t0), a, b), f32x2_split(fma2(fma2(t1, ns2, v1), r2, t1), c, d);
-    return cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16);
+    f32x2_split(fma2(fma2(t0, s2, v0), nr2, t0), a, b), f32x2_split(fma2(fma2(t1, s2, v1), nr2, t1), c, d);
+    return (cvt_e4m3x2(a, b) | (cvt_e4m3x2(c, d) << 16)) ^ 0x80808080u;
 }
 
 GI8_DEVICE uint32_t e4m3_pack4_exact(uint64_t v0, uint64_t v1, float s)
