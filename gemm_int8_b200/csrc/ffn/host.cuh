@@ -29,12 +29,13 @@ template <typename TX, typename TR, typename TW, Out8 OUT, bool BLOCK>
 int launch_norm(NormParams p, int sms, cudaStream_t s)
 {
     const int vectors = (p.H + 7) / 8;
+    // (two loads a thread: two warps for each of the form of four, whose order of summing up they keep; rows that one warp of that form holds stay with it)
     auto go = [&](auto kernel, int loads) {
-        p.row_warps = (vectors + 32 * loads - 1) / (32 * loads);
+        p.row_warps = loads == 2 ? (vectors + 127) / 128 * 2 : (vectors + 32 * loads - 1) / (32 * loads);
         const int rows = p.row_warps == 1 ? 8 : 1;
         return launch(kernel, dim3(static_cast<unsigned>((p.M + rows - 1) / rows)), p.row_warps * rows * 32, 0, s, dim3(1), knobs().pdl, p);
     };
-    if (p.M <= 2 * sms && vectors <= 2 * kNormThreads) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 2>, 2);
+    if (p.M <= 2 * sms && vectors > 128 && vectors <= 2 * kNormThreads) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 2>, 2);
     if (vectors <= 4 * kNormThreads) return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 4>, 4);
     return go(rms_norm_quantize_kernel<TX, TR, TW, OUT, BLOCK, 8>, 8);
 }

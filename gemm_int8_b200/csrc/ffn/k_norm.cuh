@@ -30,24 +30,47 @@ struct NormParams {
     float eps, inv_h;
 };
 
-// The sum of the row's values over its warps' lanes, in a fixed order (MAX: their maximum).
-template <bool MAX>
-GI8_DEVICE float row_reduce(float v, float* slots, int row_warps)
+GI8_DEVICE float warp_sum(float v)
 {
-    auto warp_all = [](float x) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float w = __shfl_xor_sync(0xffffffffu, x, o);
-            x = MAX ? max_nan(x, w) : x + w;
-        }
-        return x;
-    };
-    v = warp_all(v);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// The sum over a row, in an order that is the same in the forms of two and four loads, so that a row's result does not depend on its batch (the form of eight is
+// the only one for its widths).  A thread of four loads adds up two parts, its loads 0 and 2, and 1 and 3; of the form of two loads, which has twice the threads, the
+// first half of the threads have the first part and are sent the second by the others.  Then over the lanes of a warp, and over the warps.
+GI8_DEVICE float row_sum(const float (&part)[2], float*, float* slots, int row_warps)
+{
+    const int lane = threadIdx.x & 31;
+    float v = warp_sum(part[0] + part[1]);
+    if (row_warps == 1) return v;
+    if (lane == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp_sum(lane < row_warps ? slots[lane] : 0.0f);
+}
+
+GI8_DEVICE float row_sum(const float (&part)[1], float* sent, float* slots, int row_warps)
+{
+    const int lane = threadIdx.x & 31, warps = row_warps / 2, t = threadIdx.x - warps * 32;
+    if (t >= 0) sent[t] = part[0];
+    __syncthreads();
+    if (t < 0) {  // (a whole warp)
+        const float v = warp_sum(part[0] + sent[threadIdx.x]);
+        if (lane == 0) slots[threadIdx.x >> 5] = v;
+    }
+    __syncthreads();
+    return warp_sum(lane < warps ? slots[lane] : 0.0f);
+}
+
+GI8_DEVICE float row_max(float v, float* slots, int row_warps)
+{
+    v = warp_max_nan(v);
     if (row_warps == 1) return v;
     const int lane = threadIdx.x & 31;
     if (lane == 0) slots[threadIdx.x >> 5] = v;
     __syncthreads();
-    return warp_all(lane < row_warps ? slots[lane] : 0.0f);
+    return warp_max_nan(lane < row_warps ? slots[lane] : 0.0f);
 }
 
 // (At most 64 registers where a thread has 32 values, so that two CTAs of 512 threads fit on an SM; e4m3 spills 4 to 12 bytes for it.  With 70 and 76: 16384 x 16384 with a
@@ -58,7 +81,8 @@ __global__ void __launch_bounds__(kNormThreads, LOADS == 4 ? 2 : 0) rms_norm_qua
     quant_dependency();
     constexpr bool RESIDUAL = !std::is_same<TR, void>::value;
     using TS = typename std::conditional<RESIDUAL, TR, TX>::type;
-    __shared__ float slots[3][32];
+    constexpr int PARTS = LOADS == 2 ? 1 : 2;
+    __shared__ float slots[3][32], sent[PARTS == 1 ? kNormThreads / 2 : 1];
     const int row_threads = p.row_warps * 32;
     const int t = p.row_warps == 1 ? threadIdx.x & 31 : threadIdx.x;
     const int64_t row = p.row_warps == 1 ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
@@ -86,7 +110,22 @@ __global__ void __launch_bounds__(kNormThreads, LOADS == 4 ? 2 : 0) rms_norm_qua
         for (int u = 0; u < LOADS; ++u) raw_w[u] = load_weight(u);
     }
     uint64_t kept[LOADS][4];  // the sums, then the values
-    uint64_t sum2 = 0ull;
+    uint64_t sum2[PARTS];     // of squares
+    auto add_squares = [&](int u, const uint64_t (&h)[4]) {
+        uint64_t& sum = sum2[u % PARTS];
+        sum = u < PARTS ? mul2(h[0], h[0]) : fma2(h[0], h[0], sum);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) sum = fma2(h[i], h[i], sum);
+    };
+    auto row_total = [&](float* at) {
+        float part[PARTS], lo, hi;
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) {
+            f32x2_split(sum2[i], lo, hi);
+            part[i] = lo + hi;
+        }
+        return row_sum(part, sent, at, p.row_warps);
+    };
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
         uint64_t (&h)[4] = kept[u];
@@ -97,8 +136,7 @@ __global__ void __launch_bounds__(kNormThreads, LOADS == 4 ? 2 : 0) rms_norm_qua
 #pragma unroll
             for (int i = 0; i < 4; ++i) h[i] = add2(h[i], w[i]);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sum2 = fma2(h[i], h[i], sum2);
+        add_squares(u, h);
     }
     if constexpr (RESIDUAL) {
 #pragma unroll
@@ -107,25 +145,18 @@ __global__ void __launch_bounds__(kNormThreads, LOADS == 4 ? 2 : 0) rms_norm_qua
             if (live && col < p.H) store8(static_cast<TS*>(p.total) + base + col, kept[u]);
         }
     }
-    float lo, hi;
-    f32x2_split(sum2, lo, hi);
-    float sum = row_reduce<false>(lo + hi, slots[0], p.row_warps);
+    const float sum = row_total(slots[0]);
     float r = rsqrtf(fmaf(sum, p.inv_h, p.eps));
     // Squares that fp32 cannot hold (values from about 1e17 on): once more from values 2^80 times smaller, next to which eps is nothing.
     // (All threads that meet at the reduction's barrier hold the same sum.)
     if (sum > 1e37f) {
         const uint64_t down = f32x2(0x1p-80f, 0x1p-80f);
-        sum2 = 0ull;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint64_t h = mul2(kept[u][i], down);
-                sum2 = fma2(h, h, sum2);
-            }
+            const uint64_t h[4] = {mul2(kept[u][0], down), mul2(kept[u][1], down), mul2(kept[u][2], down), mul2(kept[u][3], down)};
+            add_squares(u, h);
         }
-        f32x2_split(sum2, lo, hi);
-        r = rsqrtf(row_reduce<false>(lo + hi, slots[2], p.row_warps) * p.inv_h) * 0x1p-80f;
+        r = rsqrtf(row_total(slots[1]) * p.inv_h) * 0x1p-80f;
     }
     const uint64_t r2 = f32x2(r, r);
     float m[LOADS];
@@ -145,7 +176,7 @@ __global__ void __launch_bounds__(kNormThreads, LOADS == 4 ? 2 : 0) rms_norm_qua
         float top = m[0];
 #pragma unroll
         for (int u = 1; u < LOADS; ++u) top = max_nan(top, m[u]);
-        qs[0] = make_out_scale<OUT>(row_reduce<true>(top, slots[1], p.row_warps));
+        qs[0] = make_out_scale<OUT>(row_max(top, slots[2], p.row_warps));
         if (live && t == 0) p.s[row] = qs[0].s;
     }
     out8_store<OUT>(kept, qs, [&](int u, uint2 w) {

@@ -46,6 +46,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor, residual: torch.Ten
     scales="token" one per token (fp32 [M], int8 only, for `matmul_scaled`).  The sum comes back in the residual's type; the norm is of the
     sum in fp32, before it is rounded to that type.  weight [H] and residual [M, H] are fp32 or bf16, each independently; H is a multiple of 16,
     at most 32768, and eps lies between 1e-20 and 1e20.  A NaN or infinity in a token makes the scales it reaches NaN or infinite.
+    A token's results do not depend on the other tokens or their number.
     """
     blockwise, e4m3 = _form(scales, dtype)
     q, s, total = _norm(x, weight, residual, eps, blockwise, e4m3)

@@ -293,7 +293,7 @@ int gi8_experts_add_f32(const void* x, int x_dtype, const void* logits, int logi
  * gi8_rms_norm_quantize: h = x + residual in fp32 (residual may be NULL);  total = h rounded to the residual's type;
  *   v = h * (mean(h^2) + eps)^-1/2 * weight, all in fp32, from the sum before it is rounded;  q, scales of v.
  *   x, residual, total [M,H] and weight [H] fp32 (dtype 0) or bf16 (1) each, total of the residual's type, all 16-byte aligned; H <= 32768;
- *   1e-20 <= eps <= 1e20.  total is not touched without a residual, and may be the residual's or (of the same type) x's own memory.
+ *   1e-20 <= eps <= 1e20.  A row's results do not depend on the other rows or their number.  total is not touched without a residual, and may be the residual's or (of the same type) x's own memory.
  */
 int gi8_rms_norm_quantize(const void* x, int x_dtype, const void* residual, int residual_dtype, const void* weight, int weight_dtype, float eps,
                           void* total, void* q, int q_type, float* scales, int block_scales, int64_t M, int64_t H, void* stream);
