@@ -18,19 +18,44 @@ struct ActParams {
     int K, KB;
 };
 
-// g u / (1 + 2^(-g log2 e)) for a pair, in packed steps but for the exponentials and reciprocals, which the special-function unit takes one by one
-// (subnormal results flushed: next to 1 they are nothing, and a reciprocal of 2^126 and more, or of an overflowed exponential, is the limit 0).
-// Good to (5 + |g|) units in the last place, next to the half step of 1/254 or 2^-4 that the result is rounded by.
-// (Of 63 million e4m3 results of fp32 input 47 lay on the other side of a rounding step than the exact ones; of the same sum with expf and a division 43, of torch's silu
-// 52.  Those took 129 us for 96 with a scale per row, 4096 x 14336, and the same with block scales.)
-GI8_DEVICE uint64_t swiglu2(uint64_t g, uint64_t u)
+// g u / (1 + exp(-g)) for a pair, in packed steps but for the exponentials and reciprocals, which the special-function unit takes one by one.
+// (Subnormal exponentials are flushed: next to 1 they are nothing.)  Good to (5 + |g|) units in the last place, next to the half step of 1/254 or 2^-4 that the result is
+// rounded by.
+// sums: what 1 + exp(-g) adds up to, for act_far.
+template <typename T>
+GI8_DEVICE uint64_t swiglu2(uint64_t g, uint64_t u, uint64_t& sums)
 {
+    constexpr float kLog2e = 1.44269504f;
+    const uint64_t one = f32x2(1.0f, 1.0f), t = mul2(g, f32x2(-kLog2e, -kLog2e));
     float a, b;
-    f32x2_split(mul2(g, f32x2(-1.44269504f, -1.44269504f)), a, b);
+    f32x2_split(t, a, b);
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(a));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(b));
-    f32x2_split(add2(f32x2(a, b), f32x2(1.0f, 1.0f)), a, b);
+    const uint64_t e = f32x2(a, b);
+    const uint64_t s = add2(e, one);  // 1 + exp(-g)
+    sums = add2(sums, s);
+    f32x2_split(s, a, b);
     return mul2(mul2(g, f32x2(approx_reciprocal(a), approx_reciprocal(b))), u);
+}
+
+// Gates for which that does not hold: the lowest, whose reciprocals would be subnormal and flushed, or whose exponentials overflow while g exp(g) u is still a number
+// (-64 is well inside), infinities and NaN.  (From 1e38 on v is g u either way.)
+GI8_DEVICE bool far_gate(float g) { return !(g > -64.0f && g < 1e38f); }
+
+// A lane's sums tell whether it may have met one: each adds 2^92 at least, or NaN.
+GI8_DEVICE bool act_far(uint64_t sums)
+{
+    float a, b;
+    f32x2_split(sums, a, b);
+    return !(a + b <= 0x1p90f);
+}
+
+// For them: with y = exp(g/2) for negative g, g u exp(g) / (1 + exp(g)) as (g y) (u y) / (1 + y^2), no part of which underflows before the result does
+// (down to -174, from where on y is subnormal and the result below 1e-35 for every u).
+GI8_DEVICE float swiglu_far(float g, float u)
+{
+    const float h = expf(-0.5f * fabsf(g)), y = g < 0.0f ? h : 1.0f;
+    return __fdiv_rn(g * y, fmaf(h, h, 1.0f)) * (u * y);
 }
 
 template <typename T, bool SWIGLU>
@@ -54,18 +79,53 @@ GI8_DEVICE ActRaw<T, SWIGLU> act_load(const ActParams& p, int64_t row, int col, 
 }
 
 template <typename T, bool SWIGLU>
-GI8_DEVICE void act_values(const ActRaw<T, SWIGLU>& r, uint64_t (&v)[4])
+GI8_DEVICE void act_values(const ActRaw<T, SWIGLU>& r, uint64_t (&v)[4], uint64_t& sums)
 {
     unpack8<T>(r.a, v);
     if constexpr (SWIGLU) {
         uint64_t w[4];
         unpack8<T>(r.b, w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = swiglu2(v[i], w[i]);
+        for (int i = 0; i < 4; ++i) v[i] = swiglu2<T>(v[i], w[i], sums);
+    }
+}
+
+// The same with far gates right.  The others' values are the same to the bit, so that a value depends on nothing beside it.
+template <typename T>
+GI8_DEVICE void act_values_far(const ActRaw<T, true>& r, uint64_t (&v)[4])
+{
+    uint64_t g[4], w[4], sums = 0ull;
+    unpack8<T>(r.a, g), unpack8<T>(r.b, w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float g0, g1, u0, u1, v0, v1;
+        f32x2_split(g[i], g0, g1), f32x2_split(w[i], u0, u1), f32x2_split(swiglu2<T>(g[i], w[i], sums), v0, v1);
+        v[i] = f32x2(far_gate(g0) ? swiglu_far(g0, u0) : v0, far_gate(g1) ? swiglu_far(g1, u1) : v1);
     }
 }
 
 constexpr int kActThreads = 64;  // (small CTAs: 4096 x 14336 SwiGLU 51.5 us with 256 threads, 49.3 with 64; e4m3 quantiser of 16384 x 8192 bf16 77.7 and 71.9)
+
+// The work item of a warp whose lanes have met far gates, from its inputs on, two blocks at a time.  (A function of its own, so that it costs the kernel no registers.)
+template <typename T, Out8 OUT>
+__device__ __noinline__ void act_block_far(const ActParams p, int64_t row, int col0, int loads)
+{
+#pragma unroll 1
+    for (int u = 0; u < loads; ++u) {
+        const int col = col0 + u * 256;
+        uint64_t v[1][4];
+        act_values_far<T>(act_load<T, true>(p, row, col, col < p.K), v[0]);
+        float m[1] = {amax8_nan(v[0])};
+        QuantScale qs[1];
+        block_scales<OUT, 1>(m, qs);
+        out8_store<OUT>(v, qs, [&](int, uint2 w) {
+            if (col < p.K) {
+                if ((threadIdx.x & 15) == 0) p.s[row * p.KB + (col >> 7)] = qs[0].s;
+                *reinterpret_cast<uint2*>(p.q + row * p.K + col) = w;
+            }
+        });
+    }
+}
 
 // A scale per 128 columns: sixteen lanes of eight values each.  A work item is 2 LOADS consecutive blocks of a row, for one warp.
 template <typename T, bool SWIGLU, Out8 OUT, int LOADS>
@@ -81,12 +141,18 @@ __global__ void __launch_bounds__(kActThreads) act_quantize_block_kernel(const A
     ActRaw<T, SWIGLU> raw[LOADS];
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) raw[u] = act_load<T, SWIGLU>(p, row, col0 + u * 256, col0 + u * 256 < p.K);
-    uint64_t v[LOADS][4];
+    uint64_t v[LOADS][4], sums = 0ull;
     float m[LOADS];
 #pragma unroll
     for (int u = 0; u < LOADS; ++u) {
-        act_values<T, SWIGLU>(raw[u], v[u]);
+        act_values<T, SWIGLU>(raw[u], v[u], sums);
         m[u] = amax8_nan(v[u]);
+    }
+    if constexpr (SWIGLU) {
+        if (__any_sync(0xffffffffu, act_far(sums))) {
+            act_block_far<T, OUT>(p, row, col0, LOADS);
+            return;
+        }
     }
     QuantScale qs[LOADS];
     block_scales<OUT, LOADS>(m, qs);
@@ -99,15 +165,44 @@ __global__ void __launch_bounds__(kActThreads) act_quantize_block_kernel(const A
     });
 }
 
-// SwiGLU in int8 with a scale per row: a CTA per row.  LOADS x 8 values a thread stay in registers between the maximum and the quantisation;
-// what lies beyond them is read and computed twice (it hits L2).
+// A row with far gates (or a NaN), from its inputs on, by all threads of the CTA.
+template <typename T>
+__device__ __noinline__ void swiglu_row_far(const ActParams p, int64_t row, float* slots)
+{
+    const int span = blockDim.x * 8;
+    float m = 0.0f;
+    uint64_t v[4];
+#pragma unroll 1
+    for (int col = threadIdx.x * 8; col < p.K; col += span) {
+        act_values_far<T>(act_load<T, true>(p, row, col, true), v);
+        m = max_nan(m, amax8_nan(v));
+    }
+    __syncwarp();
+    m = warp_max_nan(m);
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = (threadIdx.x & 31) < blockDim.x >> 5 ? slots[threadIdx.x & 31] : 0.0f;
+    const QuantScale qs = make_out_scale<Out8::kInt8>(warp_max_nan(m));
+    if (threadIdx.x == 0) p.s[row] = qs.s;
+#pragma unroll 1
+    for (int col = threadIdx.x * 8; col < p.K; col += span) {
+        act_values_far<T>(act_load<T, true>(p, row, col, true), v);
+        *reinterpret_cast<uint2*>(p.q + row * p.K + col) = make_uint2(quant_pack4(v[0], v[1], qs), quant_pack4(v[2], v[3], qs));
+    }
+    __syncthreads();  // (the slots are free again)
+}
+
+// SwiGLU in int8 with a scale per row: a CTA per row.  A lane that may have met a far gate reports NaN for its maximum, and the rows whose scale is NaN are done once
+// more behind the others: a call inside the loop over the rows costs its registers (4096 x 14336 fp32 99 us for 87, bf16 66 for 64).
+// LOADS x 8 values a thread stay in registers between the maximum and the quantisation; what lies beyond them is read and computed twice (it hits L2).
 template <typename T, int LOADS>
 __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActParams p)
 {
     quant_dependency();
-    __shared__ float slots[2][32];
+    __shared__ float slots[3][32];
     const int span = blockDim.x * 8, warps = blockDim.x >> 5;
     int parity = 0;
+    bool again = false;
     for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x, parity ^= 1) {
         ActRaw<T, true> raw[LOADS];
 #pragma unroll
@@ -115,24 +210,27 @@ __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActPara
             const int col = u * span + threadIdx.x * 8;
             raw[u] = act_load<T, true>(p, row, col, col < p.K);
         }
-        uint64_t v[LOADS][4];
+        uint64_t v[LOADS][4], sums = 0ull;
         float m = 0.0f;
 #pragma unroll
         for (int u = 0; u < LOADS; ++u) {
-            act_values<T, true>(raw[u], v[u]);
+            act_values<T, true>(raw[u], v[u], sums);
             m = max_nan(m, amax8_nan(v[u]));
         }
         for (int col = LOADS * span + threadIdx.x * 8; col < p.K; col += span) {
             uint64_t w[4];
-            act_values<T, true>(act_load<T, true>(p, row, col, true), w);
+            act_values<T, true>(act_load<T, true>(p, row, col, true), w, sums);
             m = max_nan(m, amax8_nan(w));
         }
+        if (act_far(sums)) m = __int_as_float(0x7fffffff);
         m = warp_max_nan(m);
         // (two sets of slots in turn: one barrier per row is enough)
         if ((threadIdx.x & 31) == 0) slots[parity][threadIdx.x >> 5] = m;
         __syncthreads();
         m = (threadIdx.x & 31) < warps ? slots[parity][threadIdx.x & 31] : 0.0f;
-        const QuantScale qs[1] = {make_out_scale<Out8::kInt8>(warp_max_nan(m))};
+        m = warp_max_nan(m);
+        const QuantScale qs[1] = {make_out_scale<Out8::kInt8>(m)};
+        again |= !(m == m);
         if (threadIdx.x == 0) p.s[row] = qs[0].s;
         uint8_t* q = p.q + row * p.K;
         out8_store<Out8::kInt8>(v, qs, [&](int u, uint2 w) {
@@ -141,9 +239,14 @@ __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActPara
         });
         for (int col = LOADS * span + threadIdx.x * 8; col < p.K; col += span) {
             uint64_t w[4];
-            act_values<T, true>(act_load<T, true>(p, row, col, true), w);
+            act_values<T, true>(act_load<T, true>(p, row, col, true), w, sums);
             *reinterpret_cast<uint2*>(q + col) = make_uint2(quant_pack4(w[0], w[1], qs[0]), quant_pack4(w[2], w[3], qs[0]));
         }
+    }
+    if (again) {
+        __syncthreads();
+        for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x)
+            if (!(p.s[row] == p.s[row])) swiglu_row_far<T>(p, row, slots[2]);
     }
 }
 
