@@ -81,7 +81,7 @@ int resident_quads(DeviceState* st, int* out)
     }
     if (*out) return GI8_OK;
     constexpr size_t smem = fp8_smem_bytes(256, 4, false);
-    auto kernel = fp8_gemm_kernel<256, 4, false, false, true>;
+    auto kernel = fp8_gemm_kernel<256, 4, false, Fp8Bias::kNone, true>;
     if (int rc = ensure_smem(st, 75, kernel, smem)) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(1, 4), cfg.blockDim = dim3(kBlockwiseThreads), cfg.dynamicSmemBytes = smem;
@@ -96,7 +96,7 @@ int resident_quads(DeviceState* st, int* out)
     return GI8_OK;
 }
 
-template <int BN, int STAGES, bool PAIR, bool BIAS, bool SPLITK = false>
+template <int BN, int STAGES, bool PAIR, Fp8Bias BIAS, bool SPLITK = false>
 int launch_fp8(DeviceState* st, int slot, const int8_t* x, const int8_t* y, Fp8GemmParams p, cudaStream_t s)
 {
     constexpr size_t smem = fp8_smem_bytes(BN, STAGES, PAIR);
@@ -124,10 +124,10 @@ int launch_fp8(DeviceState* st, int slot, const int8_t* x, const int8_t* y, Fp8G
     return launch(kernel, dim3(grid), kBlockwiseThreads, smem, s, dim3(PAIR ? 2 : 1), knobs().pdl, mx, my, mo, p);
 }
 
-template <bool BIAS>
+template <Fp8Bias BIAS>
 int launch_fp8(DeviceState* st, Fp8Choice c, const int8_t* x, const int8_t* y, const Fp8GemmParams& p, cudaStream_t s)
 {
-    constexpr int slot = BIAS ? 64 : 71;
+    constexpr int slot = BIAS == Fp8Bias::kBf16 ? 64 : BIAS == Fp8Bias::kNone ? 71 : 80;
     if (c.splits > 1) {
         Fp8GemmParams q = p;
         q.splits = c.splits, q.kb_per_split = fp8_kb_per_split((p.K + kBK - 1) / kBK, c.splits);
@@ -141,9 +141,9 @@ int launch_fp8(DeviceState* st, Fp8Choice c, const int8_t* x, const int8_t* y, c
     return launch_fp8<64, 8, false, BIAS>(st, slot + 3, x, y, p, s);
 }
 
-// (bias, after_quant: see scaled_impl)
+// (bias bf16 or fp32, or null; after_quant: see scaled_impl)
 int fp8_matmul(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out, int64_t M, int64_t N, int64_t K,
-               void* stream, const uint16_t* bias, bool after_quant)
+               void* stream, const void* bias, bool bias_f32, bool after_quant)
 {
     if (int rc = check_common(x, y, out, M, N, K, 2)) return rc;
     if (M == 0 || N == 0) return GI8_OK;
@@ -157,7 +157,7 @@ int fp8_matmul(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa,
     const int forced = g_forced_variant;
     if (forced == VAR_AUTO && use_blockwise_smallm(M, N, K)) {
         BlockwiseSmallMParams q{};
-        q.out = static_cast<uint16_t*>(out), q.sa = sa, q.sw = sw, q.bias = bias, q.status = st->status;
+        q.out = static_cast<uint16_t*>(out), q.sa = sa, q.sw = sw, q.bias = static_cast<const uint16_t*>(bias), q.bias_f32 = bias_f32, q.status = st->status;
         q.ldo = N, q.ld_sa = ld_sa, q.ld_sw = ld_sw, q.M = (int)M, q.N = (int)N, q.K = (int)K;
         q.after_quant = after_quant;
         q.splits = fp8_smallm_splits(N, K, st->sm_count);
@@ -185,7 +185,25 @@ int fp8_matmul(const int8_t* x, const int8_t* y, const float* sa, int64_t ld_sa,
             c = choose_fp8(M, N, K, st->sm_count, quads);
         }
     }
-    return bias ? launch_fp8<true>(st, c, x, y, p, s) : launch_fp8<false>(st, c, x, y, p, s);
+    if (!bias) return launch_fp8<Fp8Bias::kNone>(st, c, x, y, p, s);
+    return bias_f32 ? launch_fp8<Fp8Bias::kF32>(st, c, x, y, p, s) : launch_fp8<Fp8Bias::kBf16>(st, c, x, y, p, s);
+}
+
+int fp8_linear(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const void* bias, bool bias_f32, void* xq, float* xs, void* out,
+               int64_t M, int64_t N, int64_t K, void* stream)
+{
+    // Everything that the quantiser or the product refuses is refused before the quantiser is launched (as in gi8_linear).
+    if (int rc = check_common(xq, w, out, M, N, K, 2)) return rc;
+    if (int rc = check_quant(x, x_dtype, static_cast<const int8_t*>(xq), xs, M, K)) return rc;
+    if (misaligned(bias, bias_f32 ? 4 : 2)) return fail(GI8_ERR_MISALIGNED, "bias must be aligned to its type");
+    if (M == 0 || N == 0) return GI8_OK;
+    if (K == 0 && bias) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "K must be positive for a product with a bias");
+    const int64_t ld_xs = (K + kBK - 1) / kBK;
+    if (K > 0)
+        if (int rc = check_block_scales(xs, ld_xs, w_scale, ld_sw, M, N, K)) return rc;
+    if (int rc = gi8_fp8_quantize_token_block(x, x_dtype, xq, xs, M, K, stream)) return rc;
+    return fp8_matmul(static_cast<const int8_t*>(xq), static_cast<const int8_t*>(w), xs, ld_xs, w_scale, ld_sw, out, M, N, K, stream,
+                      bias, bias_f32, K > 0);
 }
 
 }  // namespace
@@ -207,24 +225,19 @@ int gi8_fp8_quantize_token_block(const void* in, int in_dtype, void* q, float* s
 int gi8_fp8_matmul_blockwise(const void* x, const void* y, const float* sa, int64_t ld_sa, const float* sw, int64_t ld_sw, void* out, int64_t M, int64_t N,
                              int64_t K, void* stream)
 {
-    return fp8_matmul(static_cast<const int8_t*>(x), static_cast<const int8_t*>(y), sa, ld_sa, sw, ld_sw, out, M, N, K, stream, nullptr, false);
+    return fp8_matmul(static_cast<const int8_t*>(x), static_cast<const int8_t*>(y), sa, ld_sa, sw, ld_sw, out, M, N, K, stream, nullptr, false, false);
 }
 
 int gi8_fp8_linear(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const void* bias, void* xq, float* xs, void* out,
                    int64_t M, int64_t N, int64_t K, void* stream)
 {
-    // Everything that the quantiser or the product refuses is refused before the quantiser is launched (as in gi8_linear).
-    if (int rc = check_common(xq, w, out, M, N, K, 2)) return rc;
-    if (int rc = check_quant(x, x_dtype, static_cast<const int8_t*>(xq), xs, M, K)) return rc;
-    if (misaligned(bias, 2)) return fail(GI8_ERR_MISALIGNED, "bias must be 2-byte aligned");
-    if (M == 0 || N == 0) return GI8_OK;
-    if (K == 0 && bias) return fail(GI8_ERR_UNSUPPORTED_SHAPE, "K must be positive for a product with a bias");
-    const int64_t ld_xs = (K + kBK - 1) / kBK;
-    if (K > 0)
-        if (int rc = check_block_scales(xs, ld_xs, w_scale, ld_sw, M, N, K)) return rc;
-    if (int rc = gi8_fp8_quantize_token_block(x, x_dtype, xq, xs, M, K, stream)) return rc;
-    return fp8_matmul(static_cast<const int8_t*>(xq), static_cast<const int8_t*>(w), xs, ld_xs, w_scale, ld_sw, out, M, N, K, stream,
-                      static_cast<const uint16_t*>(bias), K > 0);
+    return fp8_linear(x, x_dtype, w, w_scale, ld_sw, bias, false, xq, xs, out, M, N, K, stream);
+}
+
+int gi8_fp8_linear_bias_f32(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const float* bias, void* xq, float* xs,
+                            void* out, int64_t M, int64_t N, int64_t K, void* stream)
+{
+    return fp8_linear(x, x_dtype, w, w_scale, ld_sw, bias, true, xq, xs, out, M, N, K, stream);
 }
 
 }  // extern "C"

@@ -39,11 +39,12 @@ struct BlockwiseSmallMParams {
     uint16_t* out;        // bf16 [M, N], leading dimension ldo
     const float* sa;      // [M, KB], row stride ld_sa
     const float* sw;      // [ceil(N/128), KB], row stride ld_sw
-    const uint16_t* bias; // bf16 [N] added to the rounded result, or null
+    const uint16_t* bias; // bf16 [N] added to the rounded result, or null; E4m3: bf16, or fp32 where bias_f32, added to the sum
     uint32_t* status;
     int64_t ldo, ld_sa, ld_sw;
     int M, N, K;
     int after_quant;      // launched as the programmatic dependent of the quantiser that writes x and sa (and of nothing else)
+    int bias_f32;
     int splits, kb_per_split;  // E4m3: CTAs of a cluster that share a tile's K blocks, and how many each takes (the last has the rest)
 };
 
@@ -287,7 +288,8 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
             }
         }
         if (n < p.N && !(E4M3 && share != 0)) {
-            const uint16_t b = p.bias ? __ldg(p.bias + n) : uint16_t(0);
+            const uint16_t b = p.bias && !(E4M3 && p.bias_f32) ? __ldg(p.bias + n) : uint16_t(0);
+            [[maybe_unused]] const float bf = E4M3 && p.bias && p.bias_f32 ? __ldg(reinterpret_cast<const float*>(p.bias) + n) : __uint_as_float(static_cast<uint32_t>(b) << 16);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 if (cg * 8 + j < p.M) {
@@ -295,7 +297,7 @@ blockwise_smallm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_
                     f32x2_split(acc[j / 2], lo, hi);
                     const float a = j & 1 ? hi : lo;
                     uint16_t r;
-                    if constexpr (E4M3) r = to_bf16_bits(p.bias ? a + __uint_as_float(static_cast<uint32_t>(b) << 16) : a);
+                    if constexpr (E4M3) r = to_bf16_bits(p.bias ? a + bf : a);
                     else r = p.bias ? add_bf16(to_bf16_bits(a), b) : to_bf16_bits(a);
                     p.out[static_cast<int64_t>(cg * 8 + j) * p.ldo + n] = r;
                 }

@@ -474,14 +474,6 @@ GI8_DEVICE void promote_pair_f32(uint64_t& acc, uint32_t v0, uint32_t v1, uint64
         : "r"(v0), "r"(v1), "l"(t2));
 }
 
-// A packed fp32 pair plus a packed bf16 pair.
-GI8_DEVICE uint64_t plus_bf16x2(uint64_t pair, uint32_t b)
-{
-    float lo, hi;
-    f32x2_split(pair, lo, hi);
-    return f32x2(lo + __uint_as_float(b << 16), hi + __uint_as_float(b & 0xffff0000u));
-}
-
 // max(|a|, |b|, |c|): ignoring NaN, and propagating it.
 GI8_DEVICE float max3_abs(float a, float b, float c)
 {

@@ -488,15 +488,19 @@ at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& w, const at::Tensor
     at::Tensor b;
     if (bias.has_value()) {
         TORCH_CHECK(bias->device() == x.device() && bias->dim() == 1 && bias->size(0) == N, name, ": bias must have shape [", N, "] on ", x.device());
-        b = bias->to(at::kBFloat16).contiguous();
+        b = (bias->scalar_type() == at::kBFloat16 ? *bias : bias->to(at::kFloat)).contiguous();
     }
     const at::Tensor c = aligned(x);
     at::Tensor out = new_tensor({M, N}, at::kBFloat16, x);
     const int64_t q_bytes = (M * K + 255) / 256 * 256;
     at::Tensor scratch = new_tensor({q_bytes + 4 * M * blocks_of(K)}, at::kByte, x);
     uint8_t* q = static_cast<uint8_t*>(scratch.data_ptr());
-    check(gi8_fp8_linear(c.data_ptr(), c.scalar_type() == at::kFloat ? 0 : 1, w.data_ptr(), f32(ws), ld, b.defined() ? b.data_ptr() : nullptr, q,
-                         reinterpret_cast<float*>(q + q_bytes), out.data_ptr(), M, N, K, stream_of(x)));
+    const int x_dtype = c.scalar_type() == at::kFloat ? 0 : 1;
+    float* s = reinterpret_cast<float*>(q + q_bytes);
+    if (b.defined() && b.scalar_type() == at::kFloat)
+        check(gi8_fp8_linear_bias_f32(c.data_ptr(), x_dtype, w.data_ptr(), f32(ws), ld, f32(b), q, s, out.data_ptr(), M, N, K, stream_of(x)));
+    else
+        check(gi8_fp8_linear(c.data_ptr(), x_dtype, w.data_ptr(), f32(ws), ld, b.defined() ? b.data_ptr() : nullptr, q, s, out.data_ptr(), M, N, K, stream_of(x)));
     return out;
 }
 

@@ -85,7 +85,7 @@ class Fp8Linear(torch.nn.Module):
     """y = x @ W.T (+ bias) with W and x in 8-bit floating point (float8_e4m3fn): per-128x128 weight scales, per-token-per-128-K activation scales.
 
     The counterpart of `Int8Linear(mode="blockwise")`: activations are quantised on the fly, the product is `matmul_blockwise_fp8`, and a bias is
-    added to its fp32 sums before they are rounded to bf16 (one that broadcasts or is differentiated, to the rounded result).  weight_q
+    added in fp32 to its sums before they are rounded to bf16 (one that broadcasts or is differentiated, in fp32 to the rounded result).  weight_q
     float8_e4m3fn [out_features, in_features], weight_scale fp32 [ceil(out/128), ceil(in/128)].  Inference only.
     A module's `.to(dtype)` converts every floating-point buffer, both of these among them: the layer is made behind it (a call refuses other types).
     """
@@ -124,7 +124,7 @@ class Fp8Linear(torch.nn.Module):
             fused = None
         out = torch.ops.gemm_int8_CUDA.fp8_linear(x2, weight, self.weight_scale, fused)
         if bias is not None and fused is None:
-            out = out + bias.to(out.dtype)
+            out = (out.float() + bias.float()).to(self.out_dtype)
         if out.dtype != self.out_dtype:
             out = out.to(self.out_dtype)
         return out if x.dim() == 2 else out.reshape(*x.shape[:-1], weight.shape[0])

@@ -293,7 +293,8 @@ int gi8_experts_add_f32(const void* x, int x_dtype, const void* logits, int logi
  * gi8_rms_norm_quantize: h = x + residual in fp32 (residual may be NULL);  total = h rounded to the residual's type;
  *   v = h * (mean(h^2) + eps)^-1/2 * weight, all in fp32, from the sum before it is rounded;  q, scales of v.
  *   x, residual, total [M,H] and weight [H] fp32 (dtype 0) or bf16 (1) each, total of the residual's type, all 16-byte aligned; H <= 32768;
- *   1e-20 <= eps <= 1e20.  A row's results do not depend on the other rows or their number.  total is not touched without a residual, and may be the residual's or (of the same type) x's own memory.
+ *   1e-20 <= eps <= 1e20.  A row's results do not depend on the other rows or their number.  total is not touched without a residual, and may be
+ *   the residual's or (of the same type) x's own memory.
  */
 int gi8_rms_norm_quantize(const void* x, int x_dtype, const void* residual, int residual_dtype, const void* weight, int weight_dtype, float eps,
                           void* total, void* q, int q_type, float* scales, int block_scales, int64_t M, int64_t H, void* stream);
@@ -319,6 +320,10 @@ int gi8_fp8_matmul_blockwise(const void* x, const void* y, const float* sa, int6
  */
 int gi8_fp8_linear(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const void* bias_bf16, void* xq, float* xs,
                    void* out_bf16, int64_t M, int64_t N, int64_t K, void* stream);
+
+/* The same with a bias in fp32, added as it is. */
+int gi8_fp8_linear_bias_f32(const void* x, int x_dtype, const void* w, const float* w_scale, int64_t ld_sw, const float* bias, void* xq, float* xs,
+                            void* out_bf16, int64_t M, int64_t N, int64_t K, void* stream);
 
 /*
  * Forces a kernel variant for the calling process (tuning and tests); NULL or "" restores the fitted
