@@ -87,6 +87,9 @@ class Fp8Linear(torch.nn.Module):
     The counterpart of `Int8Linear(mode="blockwise")`: activations are quantised on the fly, the product is `matmul_blockwise_fp8`, and a bias is
     added in fp32 to its sums before they are rounded to bf16 (one that broadcasts or is differentiated, in fp32 to the rounded result).  weight_q
     float8_e4m3fn [out_features, in_features], weight_scale fp32 [ceil(out/128), ceil(in/128)].  Inference only.
+    fp32 and bf16 activations are quantised as they are.  fp16 ones are rounded to bf16 first, as `Int8Linear` rounds them, so that the two layers see the same
+    activations: 2^-8 of a value, next to the half step of 2^-4 that e4m3 rounds it by; `layer(x.float())` keeps all of their bits.  The product's results are bf16, as
+    `matmul_blockwise_fp8` gives them; out_dtype is what they are cast to.
     A module's `.to(dtype)` converts every floating-point buffer, both of these among them: the layer is made behind it (a call refuses other types).
     """
 
