@@ -20,9 +20,9 @@ struct ActParams {
 
 // g u / (1 + exp(-g)) for a pair, in packed steps but for the exponentials and reciprocals, which the special-function unit takes one by one.
 // A product with log2 e that is rounded, by up to |g| / 2^24, would cost the exponential |g| / 2 units in the last place.  So
-//   bf16   exp(-g) = 2^t (1 - g d),  t = -g l, l = log2 e to 16 bits, so that t is exact, and d = ln 2 (log2 e - l);  (g d)^2 / 2 is below 2^-24 where exp(-g) counts
+//   bf16   exp(-g) = 2^t (1 - g d),  t = -g l, l = log2 e to 16 bits, so that t is exact, and d = ln 2 (log2 e - l);  (g d)^2 / 2 is below 1.6 / 2^24
 //   fp32   exp(-g) = 2^t (1 - r),    t = -g log2 e rounded, r = g + t ln 2 in one fused step
-// and v is good to 13 / 2^24 of itself, next to the half step of 1/254 or 2^-4 that it is rounded by.  (Subnormal exponentials are flushed: next to 1 they are nothing.)
+// and v is good to 14 / 2^24 of itself, next to the half step of 1/254 or 2^-4 that it is rounded by.  (Subnormal exponentials are flushed: next to 1 they are nothing.)
 // Without the correction: 4096 x 14336 bf16 47.3 us for 49.8 in e4m3, in int8 level; fp32 level.
 // sums: what 1 + exp(-g) adds up to, for act_far.
 template <typename T>
@@ -43,16 +43,16 @@ GI8_DEVICE uint64_t swiglu2(uint64_t g, uint64_t u, uint64_t& sums)
     return mul2(mul2(g, f32x2(approx_reciprocal(a), approx_reciprocal(b))), u);
 }
 
-// Gates for which that does not hold: the lowest, whose reciprocals would be subnormal and flushed, or whose exponentials overflow while g exp(g) u is still a number
-// (-64 is well inside), infinities and NaN.  (From 1e38 on v is g u either way.)
-GI8_DEVICE bool far_gate(float g) { return !(g > -64.0f && g < 1e38f); }
+// Gates for which that does not hold: the lowest, whose reciprocals would be subnormal and flushed (from -87.3 on), or whose exponentials overflow while g exp(g) u is
+// still a number, infinities and NaN.  (From 1e38 on v is g u either way.)
+GI8_DEVICE bool far_gate(float g) { return !(g > -87.0f && g < 1e38f); }
 
-// A lane's sums tell whether it may have met one: each adds 2^92 at least, or NaN.
+// A lane's sums tell whether it may have met one: exp(87) = 2^125.5, an infinity of either sign (1 - r is rounded), or NaN.
 GI8_DEVICE bool act_far(uint64_t sums)
 {
     float a, b;
     f32x2_split(sums, a, b);
-    return !(a + b <= 0x1p90f);
+    return !(fabsf(a + b) <= 0x1p125f);
 }
 
 // For them: with y = exp(g/2) for negative g, g u exp(g) / (1 + exp(g)) as (g y) (u y) / (1 + y^2), no part of which underflows before the result does
@@ -100,11 +100,13 @@ template <typename T>
 GI8_DEVICE void act_values_far(const ActRaw<T, true>& r, uint64_t (&v)[4])
 {
     uint64_t g[4], w[4], sums = 0ull;
+    act_values<T, true>(r, v, sums);
+    if (!act_far(sums)) return;
     unpack8<T>(r.a, g), unpack8<T>(r.b, w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float g0, g1, u0, u1, v0, v1;
-        f32x2_split(g[i], g0, g1), f32x2_split(w[i], u0, u1), f32x2_split(swiglu2<T>(g[i], w[i], sums), v0, v1);
+        f32x2_split(g[i], g0, g1), f32x2_split(w[i], u0, u1), f32x2_split(v[i], v0, v1);
         v[i] = f32x2(far_gate(g0) ? swiglu_far(g0, u0) : v0, far_gate(g1) ? swiglu_far(g1, u1) : v1);
     }
 }
@@ -170,35 +172,73 @@ __global__ void __launch_bounds__(kActThreads) act_quantize_block_kernel(const A
     });
 }
 
-// A row with far gates (or a NaN), from its inputs on, by all threads of the CTA.
+// What a thread of a row with far gates puts right: their values, which the kernel has taken for zeros.  Where one of them may be the row's largest, so that the scale is
+// another, or is NaN, the scale becomes NaN, and the row is done again.
+template <typename T>
+__device__ __noinline__ void swiglu_row_patch(const ActParams p, int64_t row)
+{
+    const float s = *static_cast<volatile float*>(p.s + row);  // (another thread may be at that)
+    bool fits = true;
+#pragma unroll 1
+    for (int col = threadIdx.x * 8; col < p.K; col += blockDim.x * 8) {
+        const T* at = static_cast<const T*>(p.in) + row * 2 * p.K + col;
+        uint64_t g[4];
+        unpack8<T>(load8(at), g);
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a, b;
+            f32x2_split(g[i], a, b);
+            any |= far_gate(a) || far_gate(b);
+        }
+        if (!any) continue;
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            const float gate = static_cast<float>(at[i]);
+            if (!far_gate(gate)) continue;
+            const float v = swiglu_far(gate, static_cast<float>(at[p.K + i]));
+            if (v == 0.0f) continue;
+            // (s is 1 where all other values are zero)
+            if (s != 1.0f && fabsf(v) < 126.9f * s) p.q[row * p.K + col + i] = static_cast<uint8_t>(quant_exact(v, s));
+            else fits = false;
+        }
+    }
+    if (!fits) *static_cast<volatile float*>(p.s + row) = __int_as_float(0x7fffffff);
+}
+
+// A row from its inputs on, by all threads of the CTA, its far gates like the others.
 template <typename T>
 __device__ __noinline__ void swiglu_row_far(const ActParams p, int64_t row, float* slots)
 {
     const int span = blockDim.x * 8;
     float m = 0.0f;
-    uint64_t v[4];
+    QuantScale qs{};
 #pragma unroll 1
-    for (int col = threadIdx.x * 8; col < p.K; col += span) {
-        act_values_far<T>(act_load<T, true>(p, row, col, true), v);
-        m = max_nan(m, amax8_nan(v));
-    }
-    __syncwarp();
-    m = warp_max_nan(m);
-    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = m;
-    __syncthreads();
-    m = (threadIdx.x & 31) < blockDim.x >> 5 ? slots[threadIdx.x & 31] : 0.0f;
-    const QuantScale qs = make_out_scale<Out8::kInt8>(warp_max_nan(m));
-    if (threadIdx.x == 0) p.s[row] = qs.s;
+    for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll 1
-    for (int col = threadIdx.x * 8; col < p.K; col += span) {
-        act_values_far<T>(act_load<T, true>(p, row, col, true), v);
-        *reinterpret_cast<uint2*>(p.q + row * p.K + col) = make_uint2(quant_pack4(v[0], v[1], qs), quant_pack4(v[2], v[3], qs));
+        for (int col = threadIdx.x * 8; col < p.K; col += span) {
+            uint64_t v[4];
+            act_values_far<T>(act_load<T, true>(p, row, col, true), v);
+            if (pass == 0) m = max_nan(m, amax8_nan(v));
+            else *reinterpret_cast<uint2*>(p.q + row * p.K + col) = make_uint2(quant_pack4(v[0], v[1], qs), quant_pack4(v[2], v[3], qs));
+        }
+        if (pass == 0) {
+            __syncwarp();
+            m = warp_max_nan(m);
+            if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = m;
+        }
+        __syncthreads();  // (behind the second pass: the slots are free again)
+        if (pass == 0) {
+            m = (threadIdx.x & 31) < blockDim.x >> 5 ? slots[threadIdx.x & 31] : 0.0f;
+            qs = make_out_scale<Out8::kInt8>(warp_max_nan(m));
+            if (threadIdx.x == 0) p.s[row] = qs.s;
+        }
     }
-    __syncthreads();  // (the slots are free again)
 }
 
-// SwiGLU in int8 with a scale per row: a CTA per row.  A lane that may have met a far gate reports NaN for its maximum, and the rows whose scale is NaN are done once
-// more behind the others: a call inside the loop over the rows costs its registers (4096 x 14336 fp32 99 us for 87, bf16 66 for 64).
+// SwiGLU in int8 with a scale per row: a CTA per row.  Far gates come out as zeros or NaN; rows that have them are put right behind the others, by the threads that
+// have met them or, where the scale is NaN or may change, by the CTA.  (A call inside the loop over the rows costs its registers: 4096 x 14336 fp32 99 us for 87,
+// bf16 66 for 64.  A call of 16 x 14336 with one such row takes 3 us more, 10 if it is done from its inputs on.)
 // LOADS x 8 values a thread stay in registers between the maximum and the quantisation; what lies beyond them is read and computed twice (it hits L2).
 template <typename T, int LOADS>
 __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActParams p)
@@ -207,7 +247,7 @@ __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActPara
     __shared__ float slots[3][32];
     const int span = blockDim.x * 8, warps = blockDim.x >> 5;
     int parity = 0;
-    bool again = false;
+    bool again = false;  // (one flag for all rows: a bit for each is a register more)
     for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x, parity ^= 1) {
         ActRaw<T, true> raw[LOADS];
 #pragma unroll
@@ -227,7 +267,7 @@ __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActPara
             act_values<T, true>(act_load<T, true>(p, row, col, true), w, sums);
             m = max_nan(m, amax8_nan(w));
         }
-        if (act_far(sums)) m = __int_as_float(0x7fffffff);
+        again |= act_far(sums);
         m = warp_max_nan(m);
         // (two sets of slots in turn: one barrier per row is enough)
         if ((threadIdx.x & 31) == 0) slots[parity][threadIdx.x >> 5] = m;
@@ -248,7 +288,10 @@ __global__ void __launch_bounds__(1024) swiglu_quantize_row_kernel(const ActPara
             *reinterpret_cast<uint2*>(q + col) = make_uint2(quant_pack4(w[0], w[1], qs[0]), quant_pack4(w[2], w[3], qs[0]));
         }
     }
-    if (again) {
+    if (__syncthreads_or(again)) {
+        if (again) {
+            for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x) swiglu_row_patch<T>(p, row);
+        }
         __syncthreads();
         for (int64_t row = blockIdx.x; row < p.M; row += gridDim.x)
             if (!(p.s[row] == p.s[row])) swiglu_row_far<T>(p, row, slots[2]);

@@ -8,8 +8,10 @@ import ffn_reference as R
 pytestmark = pytest.mark.gpu
 FORMS = [("block", torch.int8), ("token", torch.int8), ("block", R.F8)]
 
-# Units of 2^-24 of the value: expf twice 8 (two units in the last place each), four products, the sum and the division 5, the scale's division 1.
-UNITS = 14
+# Units of 2^-24 of the value.  Gates from -87 on, fp32: ex2.approx 4 (two units in the last place), ln 2 in fp32 4 (its rounding, 1.9e-9, times an exponent of at most 126), 1 - r and
+# 1 + e 2, the reciprocal 2 (one unit in the last place), two products 2, the scale's division 1; bf16: 1.6 for the square left out, not 4.
+# Below: expf twice 8, four products, the sum and the division 5, the scale's division 1.
+UNITS = 15
 
 
 def _rel(gates, ups, scales, dtype, x, N=None):
@@ -101,3 +103,53 @@ def test_infinite_and_largest_gates(scales, dtype):
         top = float(torch.finfo(x).max)
         assert abs(float(s[1]) / top - 1) <= UNITS * 2.0 ** -24 and abs(float(s[4]) / (0.5 * top) - 1) <= UNITS * 2.0 ** -24
         assert float(s[5]) > 0.7
+
+
+@pytest.mark.parametrize("scales,dtype", FORMS)
+@pytest.mark.parametrize("x", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N", [(3, 640), (2500, 256), (5, 40016), (1300, 2064)])
+def test_low_gates_among_ordinary_ones(M, N, x, scales, dtype):
+    """Gates below -87 here and there, whose ups make their values too small to count, ones among the others, or the largest, in more rows than a CTA has and beside NaN: each
+    q and scale against 64 bits, and rows without them as they are by themselves."""
+    import gemm_int8_b200 as g
+
+    gen = torch.Generator(device="cuda").manual_seed(M + N)
+    gate, up = torch.randn(M, N, generator=gen, device="cuda"), torch.randn(M, N, generator=gen, device="cuda")
+    kind = torch.randint(0, 5, (M,), generator=gen, device="cuda")  # 0 none, 1 too small, 2 among the others, 3 the largest, 4 NaN too
+    for c in (7, N // 2 + 3, N - 1):
+        low = -87.5 - 12 * torch.rand(M, generator=gen, device="cuda")
+        size = torch.tensor([0.0, 1e-4, 0.3, 20.0, 0.3], device="cuda")[kind].double()
+        u = (size / (low.double() * torch.sigmoid(low.double())).abs()).clamp(max=3e38).float()
+        some = (kind > 0) & (torch.rand(M, generator=gen, device="cuda") < 0.7)
+        gate[some, c], up[some, c] = low[some], u[some]
+    gu = torch.cat([gate, up], 1).to(x)
+    gu[kind == 4, 50] = float("nan")
+    q, s = g.swiglu_quantize(gu, scales=scales, dtype=dtype)
+    assert torch.isnan(s.reshape(M, -1)[kind == 4][:, 0]).all()
+    fine = kind != 4
+    v, _ = R.swiglu(gu[fine])
+    R.check_quantised(q[fine], s[fine], v, v.abs() * UNITS * 2.0 ** -24 + 2.0 ** -140, dtype, scales == "block")
+    plain = kind == 0
+    alone = g.swiglu_quantize(gu[plain], scales=scales, dtype=dtype)
+    assert torch.equal(alone[0].view(torch.uint8), q[plain].view(torch.uint8)) and torch.equal(alone[1], s[plain])
+
+
+@pytest.mark.parametrize("scales,dtype", FORMS)
+@pytest.mark.parametrize("x", [torch.bfloat16, torch.float32])
+def test_lowest_gates_hide_no_other(x, scales, dtype):
+    """Gates of the type's lowest value, as a mask would leave, give zeros and do not keep a low gate beside them, of one with a large up, from counting."""
+    import gemm_int8_b200 as g
+
+    N = 256
+    for lowest in (torch.finfo(x).min, -1e38, -1e9):
+        gu = torch.ones(4, 2 * N, device="cuda", dtype=x)
+        gu[:, :N] = 0.25
+        gu[0, 8:16] = lowest
+        gu[1, 8:12], gu[1, 12], gu[1, N + 12] = lowest, -88.0, 1e37
+        gu[2, 12], gu[2, N + 12] = -88.0, 1e37
+        gu[3, 8:N:2] = lowest
+        q, s = g.swiglu_quantize(gu, scales=scales, dtype=dtype)
+        v, _ = R.swiglu(gu)
+        assert float(v[1].abs().max()) > 3
+        R.check_quantised(q, s, v, v.abs() * UNITS * 2.0 ** -24, dtype, scales == "block")
+        assert not q[0, 8:16].float().any()
