@@ -23,7 +23,7 @@ int check_out8(const void* q, int q_type, const float* scales, int block_scales,
 }
 
 // Values a thread: 32, which wants the fewest warps a row and the most rows on an SM (16384 x 8192 bf16 with a residual, 8 / 16 / 32 / 64 values: 179 / 176 /
-// 141 / 163 us; 16384 x 4096 without one 71 / 64 / 54); 16 where there is no second row for an SM to work on beside (148 x 8192: 4.5 us for 6.3; level from
+// 141 / 163 us; 16384 x 4096 without one 71 / 64 / 54, and 50 since 32 values have at most 64 registers); 16 where there is no second row for an SM to work on beside (148 x 8192: 4.5 us for 6.3; level from
 // 592 rows on), 64 where 512 threads of 32 would not hold the row.
 template <typename TX, typename TR, typename TW, Out8 OUT, bool BLOCK>
 int launch_norm(NormParams p, int sms, cudaStream_t s)

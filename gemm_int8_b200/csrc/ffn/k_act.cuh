@@ -1,9 +1,9 @@
 // Elementwise activations in 8 bits: the e4m3 quantiser, and SwiGLU behind the product of gate and up rows,
 //   v = g / (1 + exp(-g)) u   of the two halves of a row,   in fp32 from fp32 or bf16,
 // with a scale per row and 128 columns, or (SwiGLU in int8) one per row.  Every element is read and written once.  Bound: HBM, with instruction issue close behind for
-// bf16 input: SwiGLU 4096 x 14336 48 us, 6.15 TB/s (0.94 of the copy rate; 17.7 instructions an element issued on 65 % of the cycles), fp32 78 us, 6.8 TB/s; e4m3
-// quantiser 16384 x 8192 bf16 72 us, 5.7 TB/s, fp32 98 us, 6.9 TB/s; per row 4096 x 14336 62 us, 4.7 TB/s (a CTA's loads, maximum and stores follow each other; two
-// CTAs of 448 threads share an SM).
+// bf16 input: SwiGLU 4096 x 14336 in e4m3 50 - 55 us by machine, 5.4 - 5.9 TB/s (0.82 - 0.9 of the copy rate; 17 instructions an element issued on 62 % of the cycles), fp32
+// 76 - 78 us, 6.8 TB/s; e4m3 quantiser 16384 x 8192 bf16 72 us, 5.7 TB/s, fp32 98 us, 6.9 TB/s; per row 4096 x 14336 60 - 64 us, 4.6 - 4.9 TB/s, fp32 84 - 87 us, 6.1 TB/s
+// (a CTA's loads, maximum and stores follow each other; two CTAs of 448 threads share an SM).
 #pragma once
 
 #include "out8.cuh"

@@ -4,8 +4,8 @@
 // The norm is of the sum in fp32, not of the total that is stored: one rounding less on the way to q.
 //
 // One pass: a row is read once, stays in registers (8 LOADS values a thread) while its squares are summed up across its warps (and with per-row scales its largest
-// magnitude found), and is written once.  Bound: HBM: 16384 x 8192 bf16 with a residual 141 - 150 us by machine, 6.3 - 6.7 TB/s, the copy rate; 8191 x 4096 bf16 onto an fp32 residual
-// 60 us, 6.1 TB/s; without a residual, 3 bytes an element, the latency of a row's steps: 16384 x 4096 50 us, 4 TB/s.  Persistent CTAs that request the next row
+// magnitude found), and is written once.  Bound: HBM: 16384 x 8192 bf16 with a residual 141 - 150 us by machine, 6.3 - 6.7 TB/s (a copy: 6.55); 8191 x 4096 bf16 onto an
+// fp32 residual 60 us, 6.1 TB/s; without a residual, 3 bytes an element, the latency of a row's steps: 16384 x 4096 50 us, 4 TB/s.  Persistent CTAs that request the next row
 // before they work on this one were no faster (150, 65, 58 us): registers for two rows halve the rows on an SM.
 #pragma once
 
@@ -73,7 +73,7 @@ GI8_DEVICE float row_max(float v, float* slots, int row_warps)
     return warp_max_nan(lane < row_warps ? slots[lane] : 0.0f);
 }
 
-// (At most 64 registers where a thread has 32 values, so that two CTAs of 512 threads fit on an SM; e4m3 spills 4 to 12 bytes for it.  With 70 and 76: 16384 x 16384 with a
+// (At most 64 registers where a thread has 32 values, so that two CTAs of 512 threads fit on an SM; most e4m3 forms spill 4 to 12 bytes for it.  With 70 and 76: 16384 x 16384 with a
 // residual 371 us for 281, without one 297 for 202, x 8192 without one 108 for 96, x 4096 55 for 50; narrower rows with a residual within 2 %, either way.)
 template <typename TX, typename TR, typename TW, Out8 OUT, bool BLOCK, int LOADS>
 __global__ void __launch_bounds__(kNormThreads, LOADS == 4 ? 2 : 0) rms_norm_quantize_kernel(const NormParams p)

@@ -9,8 +9,9 @@ namespace {
 // Tile forms and what a wave of them costs per K block, in ns (back to back; of one full wave and of many, which run at lower clocks: two-CTA 0.46 - 0.51 us, 128 x 256
 // 0.44 - 0.53, 128 x 128 0.27 - 0.31, 128 x 64 0.23 - 0.26).
 constexpr TileForm kFp8Forms[] = {{256, true, 480.0, 0, 0}, {256, false, 495.0, 0, 0}, {128, false, 300.0, 0, 0}, {64, false, 245.0, 0, 0}};
-// What a K block takes where K is not a multiple of 32, so that rows begin inside a 32-byte sector, over what it takes where it is (1024 x 4736 x 6992 next to
-// K = 6912, us: 50.6 / 48.1, 64.6 / 47.6, 50.9 / 34.0, 71.9 / 55.4; without this rule 1024 x 5003 x 6992 took 128 columns and 73 us, not the pair's 53).
+// What a K block takes where K is not a multiple of 32, so that rows begin inside a 32-byte sector, over what it takes where it is: for the forms in turn 0.96 - 1.06,
+// 1.25 - 1.49, 1.31 - 1.52 and 1.18 - 1.38 (512 and 1024 x 4736, K = 2064, 4112, 4240, 6992 and 14352 next to the multiple of 128 below; 1024 x 4736 x 4112, us: 33.3 / 30.8,
+// 40.8 / 30.2, 31.3 / 20.5, 43.0 / 33.4).  (Without this rule 1024 x 5003 x 6992 took 128 columns and 73 us, not the pair's 53.)
 constexpr double kFp8OddRows[] = {1.06, 1.42, 1.47, 1.31};
 
 struct Fp8Choice {
@@ -35,8 +36,8 @@ double fp8_split_fixed(int bn, int splits, int64_t rows)
 int fp8_kb_per_split(int64_t kb, int splits) { return static_cast<int>((kb + 4 * splits - 1) / (4 * splits)) * 4; }
 
 // CTAs that share a tile's K blocks in the kernel for few tokens: as many as one CTA an SM leaves room for, with eight K blocks each at least (us with 1 / 2 / 4 / 8: 16 x
-// 4096 x 4096 8.6 / 7.9 / 8.0 / 12.7, 16 x 4096 x 14336 21.9 / 15.0 / 14.1 / 19.8, 16 x 2048 x 8192 13.6 / 9.7 / 8.1 / 9.2, 1 x 1024 x 4096 8.0 / 6.3 / 5.8 / 5.6, 16 x 8192 x 8192,
-// which has 128 CTAs, 15.1 / 20.9; 1 x 4096 x 1024 5.4 / 5.5).
+// 4096 x 4096 8.6 / 7.9 / 8.0 / 12.7, 16 x 2048 x 8192 13.6 / 9.7 / 8.1 / 9.2, 1 x 1024 x 4096 8.0 / 6.3 / 5.8 / 5.6, 16 x 8192 x 8192, which has 128 CTAs, 15.1 / 20.9;
+// 1 x 4096 x 1024 5.4 / 5.5).  Two CTAs an SM would fit, which long sums can use: 16 x 4096 x 14336 21.9 / 15.0 / 14.1 / 19.8, where the rule takes two.
 int fp8_smallm_splits(int64_t N, int64_t K, int sms)
 {
     const int64_t ctas = (N + kBwSmallTileN - 1) / kBwSmallTileN, kb = (K + kBK - 1) / kBK;

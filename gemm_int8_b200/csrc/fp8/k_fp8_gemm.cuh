@@ -12,7 +12,8 @@
 //   - Row scales come through shared memory, 64 bytes of a row at a time, by asynchronous copies of warp 2; as 16-byte loads of the promotion warps, each touching
 //     32 rows, they cost 80 - 100 of 800 cycles.  The weight block's scales are held by the lanes of a warp and broadcast by shuffles.
 //   - Packed multiply-adds: scalar ones, with the register banks they get, took 760 cycles a K block for 705.
-//   - No branch leaves the loop over the K blocks: with early exits it spilled accumulators (205 us for 136).
+//   - No branch leaves the loop over the K blocks: with early exits it spilled accumulators (205 us for 136).  The split forms of 256 and 128 columns still spill 12 and 16
+//     bytes, reloaded at 11 and 32 places: 265 ns a K block of 128 columns in four splits of sixteen tiles, next to 230 - 300 of the form without splits.
 //
 // Bound (two-CTA form, 2048 x 9472 x 8192, cycles a K block, copies of the kernel with parts left out): all 705; without scale loads 612; without multiply-adds 567; with
 // neither multiply-adds nor tensor-memory loads 570: the MMAs with their operands, 512 at the nominal rate; without MMAs 620.  So the promotion loop, a chain of
