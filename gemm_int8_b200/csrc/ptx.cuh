@@ -527,7 +527,7 @@ GI8_DEVICE uint4 load_bias8(const uint16_t* bias, int col, int N, bool vec)
 // Thread-block clusters and two-CTA (cta_group::2) forms
 // ---------------------------------------------------------------------------------------------
 // Cluster barrier: a hardware barrier without a time limit -- every thread of every CTA of the cluster must reach
-// it unconditionally.
+// it, under no condition or one that is the same for the whole cluster.
 GI8_DEVICE void cluster_sync_all()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
